@@ -248,7 +248,7 @@ def paged(s, table, lengths, score):
     c = s.case
     kv = F.GhKv(handle(s.kc), handle(s.vc), F.KV_F16, c.get("layers", 1), s.slots, c["kv_heads"], HEAD_DIM, HEAD_DIM)
     return F.GhKvPaged(kv, handle(table), handle(lengths), F.GhBuf() if score is None else handle(score),
-                       c["page"], table.shape[1])
+                       c["page"], table.shape[1], c["rows"])
 
 
 def prepare(case, seed):
@@ -290,22 +290,21 @@ def run(s):
 
 def attn_own(s):
     c = s.case
-    backend().attention_decode_paged(s.buf["out"], s.buf["q"], s.kv, c["kv_heads"] * c["group"], c["rows"],
-                                     c["length"], 0)
+    backend().attention_decode_paged(s.buf["out"], s.buf["q"], s.kv, c["kv_heads"] * c["group"], c["length"], 0)
 
 
 def append_own(s):
     c, b = s.case, s.buf
     if c["rope"]:
         backend().rope_kv_write_paged(s.kv, b["out"], b["q"], b["k"], b["v"], c["kv_heads"] * c["group"],
-                                      b["positions"], c["tokens"], c["rows"], s.most, s.yarn, 0)
+                                      b["positions"], c["tokens"], s.most, s.yarn, 0)
     else:
-        backend().kv_write_paged(s.kv, b["k"], b["v"], c["tokens"], c["rows"], 0)
+        backend().kv_write_paged(s.kv, b["k"], b["v"], c["tokens"], 0)
 
 
 def evict_own(s):
     c = s.case
-    backend().kv_evict_paged(s.to_kv, s.kv, s.buf["kept"], c["rows"], c["budget"], c["recent"])
+    backend().kv_evict_paged(s.to_kv, s.kv, s.buf["kept"], c["budget"], c["recent"])
 
 
 def slots_of(table, page, at):
