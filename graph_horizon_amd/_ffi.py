@@ -55,6 +55,11 @@ class GhKv(C.Structure):
                 ("value_dim", C.c_uint32)]
 
 
+class GhKvPaged(C.Structure):
+    _fields_ = [("kv", GhKv), ("table", GhBuf), ("lengths", GhBuf), ("score", GhBuf),
+                ("page_size", C.c_uint32), ("table_width", C.c_uint32), ("rows", C.c_uint32)]
+
+
 class GhSampling(C.Structure):
     _fields_ = [("temperature", C.c_float), ("top_p", C.c_float), ("top_k", C.c_uint32),
                 ("min_p", C.c_float), ("repeat_penalty", C.c_float), ("seed", C.c_uint64)]
@@ -116,6 +121,11 @@ SIGNATURES = {
     "gh_attention_decode": (I32, [P, P, BUFP, BUFP, C.POINTER(GhKv), U32, U32, U32]),
     "gh_attention_decode_noalloc": (I32, [P, P, BUFP, BUFP, C.POINTER(GhKv), U32, U32, U32]),
     "gh_attention_prefill": (I32, [P, P, BUFP, BUFP, C.POINTER(GhKv), U32, U32, U32, U32]),
+    "gh_kv_write_paged": (I32, [P, P, C.POINTER(GhKvPaged), BUFP, BUFP, U32, U32]),
+    "gh_rope_kv_write_paged": (I32, [P, P, C.POINTER(GhKvPaged), BUFP, BUFP, BUFP, BUFP, U32, BUFP, U32,
+                                     U32, C.POINTER(GhYarn), U32]),
+    "gh_attention_decode_paged": (I32, [P, P, BUFP, BUFP, C.POINTER(GhKvPaged), U32, U32, U32]),
+    "gh_kv_evict_paged": (I32, [P, P, C.POINTER(GhKvPaged), C.POINTER(GhKvPaged), BUFP, U32, U32]),
     "gh_read_logits": (I32, [P, BUFP, U64, P]),
     "gh_read_argmax": (I32, [P, BUFP, U64, C.POINTER(U32)]),
     "gh_read_topk": (I32, [P, BUFP, U64, U64, P, P, C.POINTER(U64)]),

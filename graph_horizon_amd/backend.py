@@ -13,7 +13,7 @@ from dataclasses import dataclass
 import numpy as np
 
 from . import _ffi as F
-from ._ffi import GhBuf, GhKv, GhModelConfig, GhSampling, GhYarn
+from ._ffi import GhBuf, GhKv, GhKvPaged, GhModelConfig, GhSampling, GhYarn
 
 
 class GhError(RuntimeError):
@@ -182,6 +182,27 @@ class HipBackend:
     def attention_prefill(self, out, q, kv: GhKv, q_heads, base, n, layer):
         self._run("gh_attention_prefill", C.byref(out), C.byref(q), C.byref(kv), q_heads, base,
                   n, layer)
+
+    # ---- a batch of sequences over paged caches (GhKvPaged) ----
+    def kv_write_paged(self, kv: GhKvPaged, k, v, tokens, layer):
+        """Append `tokens` K/V vectors per row at the end of its positions."""
+        self._run("gh_kv_write_paged", C.byref(kv), C.byref(k), C.byref(v), tokens, layer)
+
+    def rope_kv_write_paged(self, kv: GhKvPaged, q_out, q, k, v, q_heads, positions, tokens, max_pos,
+                            yarn: Yarn, layer):
+        """RoPE of q (into q_out) and k at the rows' own positions, and the append, in one launch."""
+        self._run("gh_rope_kv_write_paged", C.byref(kv), C.byref(q_out), C.byref(q), C.byref(k), C.byref(v),
+                  q_heads, C.byref(positions), tokens, max_pos, C.byref(yarn.c()), layer)
+
+    def attention_decode_paged(self, out, q, kv: GhKvPaged, q_heads, max_len, layer):
+        """One token per row over its cached positions; adds the attention weights to kv.score if kept."""
+        self._run("gh_attention_decode_paged", C.byref(out), C.byref(q), C.byref(kv), q_heads, max_len, layer)
+
+    def kv_evict_paged(self, dst: GhKvPaged, src: GhKvPaged, kept, budget, recent):
+        """Rows longer than `budget` keep their last `recent` and best-scored positions, in dst's pages;
+        kept: a buffer for the kept positions, or None."""
+        self._run("gh_kv_evict_paged", C.byref(dst), C.byref(src), None if kept is None else C.byref(kept),
+                  budget, recent)
 
     # ---- read-back ----
     def read_logits(self, logits, vocab) -> np.ndarray:

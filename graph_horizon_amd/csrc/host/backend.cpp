@@ -85,9 +85,15 @@ const KernelName kKernels[] = {
     {K_GEMM_FEW_MIXED_T32, "gh_gemm_few_mixed_t32"},
     {K_GEMM_FEW_Q4K_T48, "gh_gemm_few_q4k_t48"}, {K_GEMM_FEW_Q6K_T48, "gh_gemm_few_q6k_t48"},
     {K_GEMM_FEW_MIXED_T48, "gh_gemm_few_mixed_t48"},
+    {K_PAGED_WRITE, "gh_paged_write"},
+    {K_PAGED_ATTN_G4, "gh_paged_attn_g4"}, {K_PAGED_ATTN_G4_S, "gh_paged_attn_g4_s"},
+    {K_PAGED_ATTN_G8, "gh_paged_attn_g8"}, {K_PAGED_ATTN_G8_S, "gh_paged_attn_g8_s"},
+    {K_PAGED_ATTN_G16, "gh_paged_attn_g16"}, {K_PAGED_ATTN_G16_S, "gh_paged_attn_g16_s"},
+    {K_PAGED_JOIN, "gh_paged_join"},
+    {K_PAGED_SELECT, "gh_paged_select"}, {K_PAGED_MOVE, "gh_paged_move"},
 };
 
-const char* kModules[] = {"gh_quant", "gh_gemv", "gh_glue", "gh_attention", "gh_gemm", "gh_gemm_few"};
+const char* kModules[] = {"gh_quant", "gh_gemv", "gh_glue", "gh_attention", "gh_gemm", "gh_gemm_few", "gh_paged"};
 
 constexpr uint32_t kArgmaxBlocks = 256;
 // argmax scratch at the front of the workspace: f32[256] values, u32[256] indices
@@ -233,6 +239,12 @@ int ensure_workspace(gh_backend* b, size_t bytes) {
     if (b->ws_bytes >= bytes) return GH_OK;
     if (b->capturing) return fail(b, GH_E_STATE, "workspace growth during graph capture");
     return regrow(b, &b->ws, &b->ws_bytes, std::max(bytes, (size_t)(4u << 20)), "hipMalloc(workspace)");
+}
+
+int workspace_at(gh_backend* b, size_t bytes, char** at) {
+    const int rc = ensure_workspace(b, bytes);
+    *at = (char*)b->ws + kArgmaxBytes;
+    return rc;
 }
 
 // Workspace for a launch that has a form with less: *room = false, and no error, where it cannot be had.
@@ -842,6 +854,8 @@ int gh_create(const gh_config* cfg, gh_backend** out) {
     (void)hipGetLastError();
     if (!rc) rc = ensure_workspace(b, 0);
     if (!rc) rc = hip_check(b, hipHostMalloc((void**)&b->result, kResultBytes, hipHostMallocDefault), "hipHostMalloc");
+    if (!rc) rc = hip_check(b, hipHostMalloc((void**)&b->paged_fault, 64, hipHostMallocDefault), "hipHostMalloc");
+    if (!rc) *b->paged_fault = 0;
     if (!rc) rc = noalloc_init(b);
     if (!rc) {
         b->xcds = probe_xcds(b);
@@ -861,6 +875,7 @@ void gh_destroy(gh_backend* b) {
     if (b->ws) (void)hipFree(b->ws);
     if (b->counters) (void)hipFree(b->counters);
     if (b->result) (void)hipHostFree(b->result);
+    if (b->paged_fault) (void)hipHostFree((void*)b->paged_fault);
     free_rope(b->rope);
     for (hipModule_t m : b->modules) (void)hipModuleUnload(m);
     if (b->ev_start) (void)hipEventDestroy(b->ev_start);
@@ -1011,6 +1026,14 @@ int gh_submit(gh_backend* b, gh_encoder* enc) {
     if (rc) return rc;
     b->enc_open = false;
     rc = hip_check(b, hipStreamSynchronize(b->stream), "submit");
+    if (const uint32_t what = *b->paged_fault) {
+        *b->paged_fault = 0;
+        if (enc->latched == GH_OK)
+            enc->latched = fail(b, GH_E_RANGE,
+                                what == GH_PAGED_LENGTH ? "paged cache: a row longer than its table or max_len"
+                                : what == GH_PAGED_PAGE ? "paged cache: a page number beyond the pool"
+                                                        : "paged cache: a position beyond max_pos");
+    }
     return enc->latched != GH_OK ? enc->latched : rc;
 }
 

@@ -131,6 +131,17 @@ enum GhKernel : int {
     K_GEMM5_Q4K,
     K_GEMM5_Q6K,
     K_GEMM5_MIXED,
+    K_PAGED_WRITE,
+    // decode attention of up to 4, 8 and 16 query heads per kv head, each followed by its scoring form
+    K_PAGED_ATTN_G4,
+    K_PAGED_ATTN_G4_S,
+    K_PAGED_ATTN_G8,
+    K_PAGED_ATTN_G8_S,
+    K_PAGED_ATTN_G16,
+    K_PAGED_ATTN_G16_S,
+    K_PAGED_JOIN,
+    K_PAGED_SELECT,
+    K_PAGED_MOVE,
     K_COUNT
 };
 
@@ -165,6 +176,8 @@ struct gh_backend {
     // growable device workspace (attention partials, argmax partials)
     void* ws = nullptr;
     uint32_t* result = nullptr;  // pinned host memory that the read-back kernels write
+    // pinned host word in which the paged kernels leave what they found wrong (GH_PAGED_*), 0: nothing
+    volatile uint32_t* paged_fault = nullptr;
     size_t ws_bytes = 0;
     void* counters = nullptr;  // attention merge counters, zero between launches
     size_t counter_slots = 0;
@@ -206,6 +219,8 @@ int hip_check(gh_backend* b, hipError_t e, const char* what);
 int launch(gh_backend* b, GhKernel k, uint32_t gx, uint32_t gy, uint32_t gz, uint32_t bx,
            const void* args, uint32_t shmem = 0);
 int ensure_workspace(gh_backend* b, size_t bytes);
+// `bytes` of the workspace for one call's launches, 16-byte aligned, behind the argmax scratch.
+int workspace_at(gh_backend* b, size_t bytes, char** at);
 // Workgroups of `block` threads and `shmem` bytes of LDS resident on the whole device at once.
 uint32_t resident_wgs(gh_backend* b, GhKernel k, uint32_t block, uint32_t shmem);
 // Builds (or rebuilds, for other parameters or more positions) table t for `positions`

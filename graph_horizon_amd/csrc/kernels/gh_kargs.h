@@ -249,5 +249,72 @@ struct GhArgmaxArgs {
     uint32_t blocks;
 };
 
+// ---- paged caches (kernels/paged.hip) ----
+// What a kernel found that the host cannot check, left in pinned host memory for gh_submit.
+#define GH_PAGED_LENGTH 1u    // a row longer than its table, or than the call's max_len
+#define GH_PAGED_PAGE 2u      // a page number beyond the pool
+#define GH_PAGED_POSITION 3u  // a position beyond the call's max_pos
+
+// The rows' view of one layer of a page pool.
+struct GhPages {
+    uint64_t kc;       // f16 [slots][kv_heads][128] of the layer (all layers: of layer 0)
+    uint64_t vc;
+    uint64_t table;    // u32 [rows][width]
+    uint64_t lengths;  // u32 [rows]
+    uint64_t score;    // f32 [rows][kv_heads][width << shift] of the layer (0: not kept)
+    uint64_t fault;    // u32, pinned host memory
+    uint32_t width;
+    uint32_t shift;    // page_size = 1 << shift
+    uint32_t pages;    // pages of the pool
+    uint32_t kv_heads;
+};
+
+struct GhPagedWriteArgs {
+    GhPages p;
+    uint64_t q;        // f16 [rows][tokens][q_heads][128] (rotated into q_out), 0: none
+    uint64_t q_out;
+    uint64_t k;        // f16 [rows][tokens][kv_heads][128]
+    uint64_t v;
+    uint64_t positions;  // u32 [rows], 0: no rotation
+    uint64_t table;    // float2 [positions][pairs]
+    uint64_t post;     // float [positions]
+    uint32_t q_heads;  // 0 without q
+    uint32_t pairs;    // rotated pairs of a head
+    uint32_t tokens;
+    uint32_t max_pos;
+    uint32_t groups;   // workgroups per token
+};
+
+// Decode attention. Partials of (row, kv head, split): acc f32 [group][128] and (m, l) float2 [group].
+struct GhPagedAttnArgs {
+    GhPages p;
+    uint64_t q;        // f16 [rows][q_heads][128]
+    uint64_t out;
+    uint64_t part_acc;
+    uint64_t part_ml;
+    uint64_t raw;      // f32 [rows][kv_heads][group][raw_len] scores, base 2 (0: not kept)
+    uint32_t q_heads;
+    uint32_t group;
+    uint32_t max_len;
+    uint32_t span;     // positions per split, a multiple of 64, at most 4096
+    uint32_t splits;   // ceil(max_len / span)
+    uint32_t raw_len;  // max_len rounded up to 16
+    float scale;       // log2(e) / sqrt(128)
+    uint32_t chunks;   // gh_paged_join: workgroups per kv head that add scores
+};
+
+// Eviction. Strides of a layer: slots of the pools, rows for the scores.
+struct GhPagedEvictArgs {
+    GhPages src;
+    GhPages dst;
+    uint64_t src_layer;  // bytes of a layer of src's k and v
+    uint64_t dst_layer;
+    uint64_t kept;     // u32 [layers][rows][kv_heads][budget]
+    uint64_t act;      // u32 [rows]: the rows that are evicted
+    uint32_t rows;
+    uint32_t budget;
+    uint32_t recent;
+    uint32_t pad;
+};
 
 #endif

@@ -91,6 +91,28 @@ typedef struct gh_kv {
     uint32_t value_dim;
 } gh_kv;
 
+/* A pool of KV cache pages shared by a batch of sequences (no counterpart in the reference, whose
+ * requests run one at a time over a cache of their own). `kv` is the pool: an ordinary cache
+ * [layer][slot][kv_heads][dim] whose `context` counts slots, a multiple of page_size; page p is the
+ * slots p·page_size .. + page_size of every layer. Sequence r is row r of the batch: its position j
+ * lives at slot j mod page_size of page table[r][j / page_size]. Rows may share pages (a common
+ * prompt) as long as nothing is written to them. Table and lengths live on the device and are the
+ * caller's to fill (gh_upload); places of the table past a row's length are never read for an
+ * address. A row of length 0 is free: nothing is read, written or scored for it.
+ * Kernels check what the host cannot: a length beyond table_width·page_size (or the call's max_len),
+ * a page number beyond the pool or a position beyond max_pos touches no memory, and the next
+ * gh_submit returns GH_E_RANGE; that row's results are unspecified then, other rows' are not touched. */
+typedef struct gh_kv_paged {
+    gh_kv kv;            /* f16 scheme, head_dim = value_dim = 128; k, v on 16 bytes */
+    gh_buf table;        /* u32 [rows][table_width] page numbers */
+    gh_buf lengths;      /* u32 [rows] cached positions of each row */
+    gh_buf score;        /* FP32 [block_count][rows][kv_heads][table_width·page_size] accumulated attention
+                            weights, by the row's position, on 16 bytes; addr 0: not kept */
+    uint32_t page_size;  /* a power of two, 16..32768 */
+    uint32_t table_width;
+    uint32_t rows;       /* 1..65535 */
+} gh_kv_paged;
+
 typedef struct gh_backend gh_backend;
 typedef struct gh_encoder gh_encoder;
 
@@ -188,6 +210,40 @@ int gh_attention_prefill(gh_backend* b, gh_encoder* enc, const gh_buf* out, cons
 int gh_attention_decode_noalloc(gh_backend* b, gh_encoder* enc, const gh_buf* out,
                                 const gh_buf* q, const gh_kv* kv, uint32_t q_heads, uint32_t pos,
                                 uint32_t layer);
+
+/* ---- a batch of sequences over paged caches (gh_kv_paged; no counterpart in the reference) ---- */
+/* Append: `tokens` new K and V vectors per row, FP16 [rows][tokens][kv_heads][128], to the positions
+ * lengths[r] - tokens .. lengths[r] - 1 of `layer` (the lengths already count them); their scores, where
+ * kept, become 0. Vectors before a row's first position (lengths[r] < tokens) are skipped. The bytes of
+ * gh_kv_write. Rows must not share the pages that they append to. */
+int gh_kv_write_paged(gh_backend* b, gh_encoder* enc, const gh_kv_paged* kv, const gh_buf* k,
+                      const gh_buf* v, uint32_t tokens, uint32_t layer);
+/* RoPE and append in one launch: token t of row r is rotated for position positions[r] + t (u32 [rows] on
+ * the device; after an eviction a row stands further on than its length says), queries FP16
+ * [rows][tokens][q_heads][128] from q to q_out (may be the same buffer) with the query's post-scale, keys on
+ * their way into the cache. The values of gh_rope_yarn and gh_kv_write. max_pos: the largest of the positions
+ * positions[r] + t of this call, at most 262143 (it sizes the rotation table). */
+int gh_rope_kv_write_paged(gh_backend* b, gh_encoder* enc, const gh_kv_paged* kv, const gh_buf* q_out,
+                           const gh_buf* q, const gh_buf* k, const gh_buf* v, uint32_t q_heads,
+                           const gh_buf* positions, uint32_t tokens, uint32_t max_pos, const gh_yarn* yarn,
+                           uint32_t layer);
+/* Attention of one new token per row over its lengths[r] positions: q, out FP16 [rows][q_heads][128], 1 to 16
+ * query heads per kv head. Free rows get zeros. max_len: no row is longer (0: table_width·page_size); it
+ * sizes the launch. Where scores are kept, each position's attention weight, summed over the query heads of
+ * a kv head, is added to its score. */
+int gh_attention_decode_paged(gh_backend* b, gh_encoder* enc, const gh_buf* out, const gh_buf* q,
+                              const gh_kv_paged* kv, uint32_t q_heads, uint32_t max_len, uint32_t layer);
+/* Eviction by accumulated attention weight: of every row longer than `budget`, for each layer and kv head by
+ * itself, the last `recent` positions and the budget - recent others with the largest scores (f32 total
+ * order, equal scores: the lowest positions) are kept, in their order: their K, V and scores are copied from
+ * `src`'s pages to positions 0 .. budget - 1 of the same row of `dst`, and its length becomes budget. `kept`
+ * (u32 [block_count][rows][kv_heads][budget], or NULL) receives their former positions. Shorter rows stay as
+ * they are: nothing of theirs is written. src's pages are only read, so other rows may share them; dst's
+ * pages of the evicted rows must be no page that src's rows use, and none of them twice. dst has src's rows,
+ * page_size, block_count and heads, and the scores; its lengths and, with the same table_width, its scores may
+ * be src's own buffers. */
+int gh_kv_evict_paged(gh_backend* b, gh_encoder* enc, const gh_kv_paged* dst, const gh_kv_paged* src,
+                      const gh_buf* kept, uint32_t budget, uint32_t recent);
 
 /* ---- read-back, contract.rs:300-318 (synchronous) ---- */
 int gh_read_logits(gh_backend* b, const gh_buf* logits, uint64_t vocab, float* dst);

@@ -1,0 +1,547 @@
+"""The operators over paged caches (gh_*_paged): append with RoPE, decode attention with and without the
+accumulation of weights, eviction, and a run of all of them, against 64-bit definitions (tests/paged.py)."""
+import numpy as np
+import pytest
+
+from graph_horizon_amd import GhError, GhKvPaged, HipBackend, Yarn
+from graph_horizon_amd import _ffi as F
+from paged import D, Paged, attend, check_attention, keep, pages_of
+
+pytestmark = pytest.mark.gpu
+YARN = Yarn(128, 16384, 1e6, 16.0, 32.0, 1.0, 1.0, 0.1)
+
+
+def run_attention(hip, p, q_heads, rng, layer=0, max_len=0, q=None):
+    if q is None:
+        q = rng.standard_normal((p.rows, q_heads, D)).astype(np.float16)
+    qb, ob = hip.from_host(q), hip.from_host(np.full_like(q, np.nan))
+    try:
+        hip.attention_decode_paged(ob, qb, p.handle(), q_heads, max_len, layer)
+        out = hip.download(ob, np.float16, q.size).reshape(q.shape)
+    finally:
+        hip.free_buffer(qb)
+        hip.free_buffer(ob)
+    return q, out
+
+
+# ---- attention ----
+
+LENGTHS = {
+    "one": [1],
+    "tile_edges": [15, 16, 17, 0, 63, 64, 65, 1],
+    "empty": [0, 0],
+    "ragged": [1000, 3, 0, 257, 640, 129, 1],
+    "long": [9001, 100],
+}
+
+
+@pytest.mark.parametrize("scored", [False, True])
+@pytest.mark.parametrize("name", list(LENGTHS))
+@pytest.mark.parametrize("page,heads,group", [(16, 8, 4), (64, 2, 8), (32, 1, 1), (128, 5, 3), (16, 3, 16), (256, 1, 7)])
+def test_attention(hip, rng, name, page, heads, group, scored):
+    p = Paged(hip, rng, LENGTHS[name], page, heads, layers=2, scored=scored)
+    before = None if not scored else p.read("score")
+    q, out = run_attention(hip, p, heads * group, rng, layer=1)
+    check_attention(p, 1, q, out, before, p.read("score") if scored else None)
+    for name in ("k", "v", "table", "lengths"):
+        assert np.array_equal(p.read(name).view(np.uint8), getattr(p, name).view(np.uint8)), name
+    p.free()
+
+
+@pytest.mark.parametrize("max_len", [300, 320, 1000, 4096])
+@pytest.mark.parametrize("group", [2, 4])
+def test_attention_launch_longer_than_rows(hip, rng, max_len, group):
+    """A table with room: the launch is sized by max_len, the rows end before it."""
+    p = Paged(hip, rng, [300, 0, 17], 16, 4, width=256, scored=True)
+    before = p.read("score")
+    q, out = run_attention(hip, p, 4 * group, rng, max_len=max_len)
+    check_attention(p, 0, q, out, before, p.read("score"))
+    p.free()
+
+
+def test_attention_row_groups(hip, rng):
+    """More scratch than one group of rows may take: 300 rows of 16 heads over up to 32768 positions."""
+    lengths = [int(n) for n in rng.integers(0, 40, 300)]
+    lengths[-1] = 700
+    p = Paged(hip, rng, lengths, 16, 1, width=2048, scored=True)
+    before = p.read("score")
+    q, out = run_attention(hip, p, 16, rng)
+    check_attention(p, 0, q, out, before, p.read("score"))
+    p.free()
+
+
+def test_attention_repeats_bit_for_bit(hip, rng):
+    p = Paged(hip, rng, [3000, 40, 1111], 32, 8)
+    q, first = run_attention(hip, p, 32, rng)
+    for _ in range(3):
+        assert np.array_equal(run_attention(hip, p, 32, rng, q=q)[1].view(np.uint16), first.view(np.uint16))
+    p.free()
+
+
+def test_attention_equals_contiguous_decode(hip, rng):
+    """Pages in order are the contiguous cache: both operators within twice the bound of each."""
+    n, heads, group = 777, 8, 4
+    p = Paged(hip, rng, [n], 16, heads, layers=2)
+    q, out = run_attention(hip, p, heads * group, rng, layer=1)
+    c = np.zeros((2, 800, heads, D), np.float16), np.zeros((2, 800, heads, D), np.float16)
+    c[0][:, :n], c[1][:, :n] = p.k[:, p.cells(0, n)], p.v[:, p.cells(0, n)]
+    kb, vb, qb, ob = hip.from_host(c[0]), hip.from_host(c[1]), hip.from_host(q), hip.alloc_buffer(q.nbytes)
+    hip.attention_decode(ob, qb, F.GhKv(kb, vb, F.KV_F16, 2, 800, heads, D, D), heads * group, n - 1, 1)
+    other = hip.download(ob, np.float16, q.size).reshape(q.shape).astype(np.float64)
+    for h in range(heads):
+        hs = slice(h * group, h * group + group)
+        bound = attend(q[0, hs], c[0][1, :n, h], c[1][1, :n, h])[2]
+        assert np.all(np.abs(other[0, hs] - out[0, hs]) <= 2 * bound)
+    for b in (kb, vb, qb, ob):
+        hip.free_buffer(b)
+    p.free()
+
+
+def test_attention_shared_and_repeated_pages(hip, rng):
+    """Two rows over one prompt's pages, and a row that has the same page twice."""
+    p = Paged(hip, rng, [200, 200, 64], 16, 2)
+    p.table[1, :8] = p.table[0, :8]
+    p.table[2, :4] = p.table[2, [0, 1, 0, 1]]
+    p.upload()
+    q, out = run_attention(hip, p, 8, rng)
+    check_attention(p, 0, q, out)
+    p.free()
+
+
+@pytest.mark.parametrize("heads", [8, 1])
+def test_attention_pool_past_4_gib(hip, rng, heads):
+    """Pages whose byte offsets pass 32 bits (a pool of 4.5 GiB each for K and V)."""
+    page, slots = 64, (9 << 29) // (256 * heads) // 64 * 64
+    lengths = [130, 70]
+    small = Paged(hip, rng, lengths, page, heads)
+    kv = [hip.alloc_buffer(slots * heads * 256) for _ in range(2)]
+    last = slots // page - 1
+    table = small.table.copy()
+    for r in range(2):
+        for i in range(pages_of(lengths[r], page)):
+            table[r, i] = last
+            for b, x in zip(kv, (small.k, small.v)):
+                at = int(small.table[r, i]) * page
+                hip.upload(b, x[0, at:at + page], last * page * heads * 256)
+            last -= 3 if i else slots // page // 2
+            last %= slots // page
+    tb, q = hip.from_host(table), rng.standard_normal((2, 4 * heads, D)).astype(np.float16)
+    h = small.handle()
+    h.kv = F.GhKv(kv[0], kv[1], F.KV_F16, 1, slots, heads, D, D)
+    h.table = tb
+    qb, ob = hip.from_host(q), hip.alloc_buffer(q.nbytes)
+    hip.attention_decode_paged(ob, qb, h, 4 * heads, 0, 0)
+    check_attention(small, 0, q, hip.download(ob, np.float16, q.size).reshape(q.shape))
+    for b in (*kv, tb, qb, ob):
+        hip.free_buffer(b)
+    small.free()
+
+
+def test_attention_peaked_and_flat_weights(hip, rng):
+    """One key far above all others; 30000 keys of 2^-26 of the largest each, which together are 2^-11 of
+    it; and a row of equal scores."""
+    n = 30000
+    p = Paged(hip, rng, [n, n, 500], 64, 1)
+    q = np.zeros((3, 1, D), np.float16)
+    q[:, 0, 0] = 8
+    p.k[:] = 0
+    p.v[:] = np.where(np.isnan(p.v), 0, p.v)
+    a, b = p.cells(0, n), p.cells(1, n)
+    p.k[0, a[1234], 0, 0] = 60
+    p.k[0, b, 0, 0] = -25.5  # 8 * 25.5 / sqrt(128) = 18.03 = 26.01 ln 2
+    p.k[0, b[77], 0, 0] = 0
+    p.v[0, b, 0, 1] = 1000
+    p.v[0, b[77], 0] = 0
+    p.upload()
+    q, out = run_attention(hip, p, 1, rng, q=q)
+    check_attention(p, 0, q, out)
+    assert 0.2 < out[1, 0, 1] < 0.7  # 30000 * 2^-26 * 1000
+    p.free()
+
+
+def test_attention_infinities_and_nan_stay_where_they_are_seen(hip, rng):
+    """An infinite V, an infinite and a NaN K: the outputs of the definition, in their head and row alone; NaN
+    and infinities behind the last position do not show (the pool is full of NaN elsewhere)."""
+    p = Paged(hip, rng, [100, 100, 100, 100], 16, 2)
+    cells = [p.cells(r, 100) for r in range(4)]
+    p.v[0, cells[0][40], 1, 5] = np.inf
+    p.v[0, cells[0][3], 1, 6] = -np.inf
+    p.v[0, cells[0][40], 1, 7] = np.nan
+    p.k[0, cells[1][50], 0] = np.nan
+    p.k[0, cells[2][50], 0, 0] = np.inf
+    p.upload()
+    q = np.abs(rng.standard_normal((4, 8, D))).astype(np.float16)
+    q[2, :, 0] = -1  # a score of -inf: weight 0
+    q, out = run_attention(hip, p, 8, rng, q=q)
+    assert np.all(out[0, 4:, 5] == np.inf) and np.all(out[0, 4:, 6] == -np.inf) and np.isnan(out[0, 4:, 7]).all()
+    assert np.isnan(out[1, :4]).all()
+    p.v[0, cells[0][[40, 40, 3]], 1, [5, 7, 6]] = 0
+    p.k[0, cells[1][50], 0] = 0
+    with np.errstate(invalid="ignore"):
+        for r, h, dims in ((0, 0, slice(None)), (0, 1, slice(8, None)), (1, 1, slice(None)), (3, 0, slice(None)),
+                           (3, 1, slice(None))):
+            want, _, bound, _ = attend(q[r, 4 * h:4 * h + 4], p.k[0, cells[r], h], p.v[0, cells[r], h])
+            assert np.all(np.abs(out[r, 4 * h:4 * h + 4] - want)[:, dims] <= bound[:, dims]), (r, h)
+    rest = np.delete(cells[2], 50)
+    want, _, bound, _ = attend(q[2, :4], p.k[0, rest, 0], p.v[0, rest, 0])
+    assert np.all(np.abs(out[2, :4] - want) <= bound)
+    p.free()
+
+
+def test_attention_without_scratch(rng):
+    """Scratch that cannot be had is an error, and the next call works."""
+    with HipBackend(0) as hip:
+        p = Paged(hip, rng, [60000], 64, 8, scored=True)
+        hip.set_scratch_limit(1 << 20)
+        with pytest.raises(GhError) as e:
+            run_attention(hip, p, 32, rng)
+        assert e.value.code == -4
+        hip.set_scratch_limit(0)
+        before = p.read("score")
+        q, out = run_attention(hip, p, 32, rng)
+        check_attention(p, 0, q, out, before, p.read("score"))
+        p.free()
+
+
+# ---- append ----
+
+@pytest.mark.parametrize("scored", [False, True])
+@pytest.mark.parametrize("page,heads,tokens,lengths", [
+    (16, 8, 1, [1, 16, 17, 0, 500]), (64, 2, 1, [64, 65]), (32, 1, 40, [40, 100, 0, 33, 7]), (16, 3, 300, [300]),
+])
+def test_write(hip, rng, page, heads, tokens, lengths, scored):
+    p = Paged(hip, rng, lengths, page, heads, layers=3, scored=scored)
+    k, v = (rng.standard_normal((p.rows, tokens, heads, D)).astype(np.float16) for _ in range(2))
+    kb, vb = hip.from_host(k), hip.from_host(v)
+    hip.kv_write_paged(p.handle(), kb, vb, tokens, 1)
+    for r, n in enumerate(lengths):
+        t = min(tokens, n)  # what lies before the row's first position is skipped
+        at = p.cells(r, n)[n - t:]
+        p.k[1, at], p.v[1, at] = k[r, tokens - t:], v[r, tokens - t:]
+        if scored:
+            p.score[1, r, :, n - t:n] = 0
+    for name in ("k", "v") + (("score",) if scored else ()):
+        assert np.array_equal(p.read(name).view(np.uint8), getattr(p, name).view(np.uint8)), name
+    hip.free_buffer(kb)
+    hip.free_buffer(vb)
+    p.free()
+
+
+@pytest.mark.parametrize("rope_dim", [128, 64, 6])
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("heads,group,tokens", [(8, 4, 1), (2, 3, 5)])
+def test_rope_write_has_the_bits_of_the_single_operations(hip, rng, rope_dim, in_place, heads, group, tokens):
+    yarn = Yarn(rope_dim, 16384, 1e6, 16.0, 32.0, 1.0, 1.0, 0.1)
+    lengths, q_heads = [20, 0, 6, 33], heads * group
+    positions = np.array([0, 5, 20000, 700], np.uint32)
+    p = Paged(hip, rng, lengths, 16, heads, layers=2)
+    q = rng.standard_normal((4, tokens, q_heads, D)).astype(np.float16)
+    k, v = (rng.standard_normal((4, tokens, heads, D)).astype(np.float16) for _ in range(2))
+    qb, kb, vb, pb = (hip.from_host(x) for x in (q, k, v, positions))
+    ob = qb if in_place else hip.from_host(np.full_like(q, 7))
+    hip.rope_kv_write_paged(p.handle(), ob, qb, kb, vb, q_heads, pb, tokens, 20000 + tokens - 1, yarn, 1)
+    got = hip.download(ob, np.float16, q.size).reshape(q.shape)
+    want_q = (q if in_place else np.full_like(q, 7)).copy()
+    for r, n in enumerate(lengths):
+        for t in range(tokens) if n else ():
+            row = {}
+            for name, x, role in (("q", q[r, t], F.ROPE_QUERY), ("k", k[r, t], F.ROPE_KEY)):
+                b = hip.from_host(x)
+                hip.rope_yarn(b, len(x), D, int(positions[r]) + t, yarn, role)
+                row[name] = hip.download(b, np.float16, x.size).reshape(x.shape)
+                hip.free_buffer(b)
+            want_q[r, t] = row["q"]
+            at = p.cells(r, n)[n - tokens + t]
+            p.k[1, at], p.v[1, at] = row["k"], v[r, t]
+    assert np.array_equal(got.view(np.uint16), want_q.view(np.uint16))
+    for name in ("k", "v"):
+        assert np.array_equal(p.read(name).view(np.uint16), getattr(p, name).view(np.uint16)), name
+    for b in (qb, kb, vb, pb) + (() if in_place else (ob,)):
+        hip.free_buffer(b)
+    p.free()
+
+
+# ---- eviction ----
+
+def evict_case(hip, rng, lengths, page, heads, layers, budget, recent, score=None, use_kept=True, alias=False):
+    src = Paged(hip, rng, lengths, page, heads, layers, scored=True, score=score)
+    dst = Paged(hip, rng, [budget if n > budget else 0 for n in lengths], page, heads, layers, scored=True,
+                width=src.width if alias else pages_of(budget, page))
+    dst.lengths = src.lengths.copy() if alias else np.arange(90, 90 + len(lengths), dtype=np.uint32)
+    dst.upload()
+    if alias:
+        dst.score = src.score.copy()
+        hip.free_buffer(dst.bufs["score"])
+        hip.free_buffer(dst.bufs["lengths"])
+        dst.bufs["score"], dst.bufs["lengths"] = src.bufs["score"], src.bufs["lengths"]
+    kept = np.full((layers, len(lengths), heads, budget), 0xABCD, np.uint32)
+    kb = hip.from_host(kept) if use_kept else None
+    hip.kv_evict_paged(dst.handle(), src.handle(), kb, budget, recent)
+    for r, n in enumerate(lengths):
+        if n <= budget:
+            continue
+        dst.lengths[r] = budget
+        old, new = src.cells(r, n), dst.cells(r, budget)
+        for layer in range(layers):
+            for h in range(heads):
+                best = keep(src.score[layer, r, h, :n], budget, recent)
+                kept[layer, r, h] = best
+                dst.score[layer, r, h, :budget] = src.score[layer, r, h, best]
+                dst.k[layer, new, h], dst.v[layer, new, h] = src.k[layer, old[best], h], src.v[layer, old[best], h]
+    if use_kept:
+        assert np.array_equal(hip.download(kb, np.uint32, kept.size).reshape(kept.shape), kept)
+        hip.free_buffer(kb)
+    for name in ("score", "lengths", "k", "v"):
+        assert np.array_equal(dst.read(name).view(np.uint8), getattr(dst, name).view(np.uint8)), name
+    for name in ("k", "v", "table") + (() if alias else ("lengths", "score")):
+        assert np.array_equal(src.read(name).view(np.uint8), getattr(src, name).view(np.uint8)), "source " + name
+    if alias:
+        dst.bufs.pop("score"), dst.bufs.pop("lengths")
+    src.free()
+    dst.free()
+
+
+@pytest.mark.parametrize("lengths,page,heads,layers,budget,recent", [
+    ([2], 16, 1, 1, 1, 0), ([2], 16, 1, 1, 1, 1), ([17, 16, 0, 40], 16, 2, 2, 16, 3), ([600, 601, 64], 32, 8, 3, 560, 64),
+    ([5000, 4097, 2049], 64, 2, 2, 2048, 256), ([300], 128, 3, 1, 299, 0), ([300], 16, 3, 1, 200, 200),
+    ([20001], 256, 1, 1, 7001, 1), ([100, 50], 16, 5, 2, 200, 10),
+])
+@pytest.mark.parametrize("alias", [False, True])
+def test_evict(hip, rng, lengths, page, heads, layers, budget, recent, alias):
+    evict_case(hip, rng, lengths, page, heads, layers, budget, recent, use_kept=not alias,
+               alias=alias and budget <= pages_of(max(lengths), page) * page)
+
+
+@pytest.mark.parametrize("kind", ["zeros", "few_values", "signs", "not_finite", "denormal"])
+@pytest.mark.parametrize("budget,recent", [(1000, 0), (1000, 100), (2900, 500)])
+def test_evict_order_of_scores(hip, rng, kind, budget, recent):
+    """Equal scores keep the first; the order is f32's total order (-NaN < -inf < ... -0 < +0 ... < NaN)."""
+    n = 3003
+    if kind == "zeros":
+        s = np.zeros(n)
+    elif kind == "few_values":
+        s = rng.integers(0, 4, n)
+    elif kind == "signs":
+        s = np.where(rng.random(n) < 0.5, -0.0, rng.standard_normal(n))
+    elif kind == "denormal":
+        s = rng.integers(0, 50, n) * np.float64(np.finfo(np.float32).smallest_subnormal)
+    else:
+        s = rng.choice(np.array([np.nan, -np.nan, np.inf, -np.inf, 0.0, -0.0, 1.0]), n)
+    s = np.resize(s.astype(np.float32), pages_of(n, 16) * 16)
+    evict_case(hip, rng, [n, n - 1], 16, 2, 1, budget, recent, score=s)
+
+
+def test_evict_leaves_shared_pages_alone(hip, rng):
+    """Two rows over one prompt: the longer is evicted, the other's cache keeps its bytes (evict_case checks
+    that of the whole source)."""
+    src = Paged(hip, rng, [400, 200], 16, 2, scored=True)
+    src.table[1, :12] = src.table[0, :12]
+    src.upload()
+    dst = Paged(hip, rng, [250, 0], 16, 2, scored=True)
+    hip.kv_evict_paged(dst.handle(), src.handle(), None, 250, 50)
+    assert np.array_equal(src.read("k").view(np.uint16), src.k.view(np.uint16))
+    best = keep(src.score[0, 0, 1, :400], 250, 50)
+    assert np.array_equal(dst.read("v")[0, dst.cells(0, 250), 1], src.v[0, src.cells(0, 400)[best], 1])
+    assert list(dst.read("lengths")) == [250, 0]
+    src.free()
+    dst.free()
+
+
+# ---- what the host cannot check ----
+
+def test_bad_device_data_is_an_error_of_its_row(hip, rng):
+    """A length beyond the table, a page beyond the pool, a position beyond max_pos: GH_E_RANGE at the submit,
+    other rows as ever, and the next call works."""
+    p = Paged(hip, rng, [100, 90, 300], 16, 2, scored=True)
+    good_lengths, good_table = p.lengths.copy(), p.table.copy()
+    q = rng.standard_normal((3, 8, D)).astype(np.float16)
+    k = rng.standard_normal((3, 1, 2, D)).astype(np.float16)
+    qb, ob, kb = hip.from_host(q), hip.alloc_buffer(q.nbytes), hip.from_host(k)
+    pb = hip.from_host(np.array([3, 9, 5], np.uint32))
+    dst = Paged(hip, rng, [50, 50, 50], 16, 2, scored=True)
+
+    def calls():
+        yield "write", lambda: hip.kv_write_paged(p.handle(), kb, kb, 1, 0)
+        yield "attend", lambda: hip.attention_decode_paged(ob, qb, p.handle(), 8, 0, 0)
+        yield "evict", lambda: hip.kv_evict_paged(dst.handle(), p.handle(), None, 50, 10)
+
+    for bad in ("length", "page"):
+        p.lengths, p.table = good_lengths.copy(), good_table.copy()
+        if bad == "length":
+            p.lengths[1] = p.width * 16 + 1
+        else:
+            p.table[1, :6] = p.slots // 16  # the first page beyond the pool
+        p.upload()
+        for name, call in calls():
+            with pytest.raises(GhError) as e:
+                call()
+            assert e.value.code == -5, (bad, name)
+            if name == "attend":
+                out = hip.download(ob, np.float16, q.size).reshape(q.shape)
+                now = p.read("k"), p.read("v")
+                for r in (0, 2):
+                    s = p.cells(r, int(good_lengths[r]))
+                    want, _, bound, _ = attend(q[r, :4], now[0][0, s, 0], now[1][0, s, 0])
+                    assert np.all(np.abs(out[r, :4] - want) <= bound)
+            if name == "evict":
+                assert dst.read("lengths")[0] == 50 and dst.read("lengths")[2] == 50
+    p.lengths, p.table = good_lengths, good_table
+    p.upload()
+    with pytest.raises(GhError) as e:
+        hip.rope_kv_write_paged(p.handle(), ob, qb, kb, kb, 8, pb, 1, 8, YARN, 0)
+    assert e.value.code == -5
+    hip.rope_kv_write_paged(p.handle(), ob, qb, kb, kb, 8, pb, 1, 9, YARN, 0)
+    for _, call in calls():
+        call()
+    for b in (qb, ob, kb, pb):
+        hip.free_buffer(b)
+    p.free()
+    dst.free()
+
+
+# ---- together ----
+
+def test_serving_run(hip, rng):
+    """Prompts go into pages, then steps of append and attention over two layers in one encoder each, an
+    eviction in between (rows go on in their new pages), against a restatement that holds every row's
+    vectors in lists."""
+    heads, group, page, layers, width, budget, recent = 2, 4, 16, 2, 12, 40, 8
+    prompts = [50, 0, 17, 90]
+    rows, q_heads, slots = len(prompts), heads * group, page * 64
+    kc, vc = (hip.from_host(np.full((layers, slots, heads, D), np.nan, np.float16)) for _ in range(2))
+    free = list(rng.permutation(slots // page))
+    tables = [[free.pop() for _ in range(width)] for _ in range(rows)]
+    table = hip.from_host(np.array(tables, np.uint32))
+    lengths_b, pos_b = hip.alloc_buffer(4 * rows), hip.alloc_buffer(4 * rows)
+    score = hip.from_host(np.zeros((layers, rows, heads, width * page), np.float32))
+    pool = F.GhKv(kc, vc, F.KV_F16, layers, slots, heads, D, D)
+    kv = GhKvPaged(pool, table, lengths_b, score, page, width, rows)
+    lengths = np.array(prompts, np.uint32)
+    position = lengths.copy()
+    # per layer and row: K, V [n][heads][128] and scores [heads][n]
+    state = [[(np.zeros((0, heads, D), np.float16),) * 2 + (np.zeros((heads, 0)),) for _ in range(rows)]
+             for _ in range(layers)]
+
+    def append(layer, r, k, v):
+        a, b, s = state[layer][r]
+        state[layer][r] = np.concatenate([a, k]), np.concatenate([b, v]), np.pad(s, ((0, 0), (0, len(k))))
+
+    # the prompts: prefilled elsewhere (as random vectors), moved in by rows
+    for r, n in enumerate(prompts):
+        if n == 0:
+            continue
+        only = np.where(np.arange(rows) == r, lengths, 0).astype(np.uint32)
+        hip.upload(lengths_b, only)
+        for layer in range(layers):
+            k, v = (rng.standard_normal((rows, n, heads, D)).astype(np.float16) for _ in range(2))
+            kb, vb = hip.from_host(k), hip.from_host(v)
+            hip.kv_write_paged(kv, kb, vb, n, layer)
+            append(layer, r, k[r], v[r])
+            hip.free_buffer(kb)
+            hip.free_buffer(vb)
+
+    def rope(x, pos, role):
+        b = hip.from_host(x)
+        hip.rope_yarn(b, len(x), D, int(pos), YARN, role)
+        y = hip.download(b, np.float16, x.size).reshape(x.shape)
+        hip.free_buffer(b)
+        return y
+
+    shape = (rows, q_heads, D)
+    for step in range(12):
+        if step == 4:
+            lengths[1], position[1] = 0, 0  # a new sequence takes the free row
+        live = np.array([r != 1 or step >= 4 for r in range(rows)])
+        lengths[live] += 1
+        hip.upload(lengths_b, np.where(live, lengths, 0).astype(np.uint32))
+        hip.upload(pos_b, position)
+        data = [(rng.standard_normal(shape).astype(np.float16), *(rng.standard_normal((rows, heads, D)).astype(np.float16)
+                 for _ in range(2))) for _ in range(layers)]
+        bufs = [[hip.from_host(x) for x in d] + [hip.alloc_buffer(2 * rows * q_heads * D) for _ in range(2)] for d in data]
+        hip.begin()
+        for layer, (qb, kb, vb, rb, ob) in enumerate(bufs):
+            hip.rope_kv_write_paged(kv, rb, qb, kb, vb, q_heads, pos_b, 1, 300, YARN, layer)
+            hip.attention_decode_paged(ob, rb, kv, q_heads, 0, layer)
+        hip.submit()
+        got_score = hip.download(score, np.float32, layers * rows * heads * width * page)
+        got_score = got_score.reshape(layers, rows, heads, width * page)
+        for layer, (q, k, v) in enumerate(data):
+            out = hip.download(bufs[layer][4], np.float16, q.size).reshape(shape)
+            for r in range(rows):
+                if not live[r]:
+                    assert not out[r].any()
+                    continue
+                append(layer, r, rope(k[r], position[r], F.ROPE_KEY)[None], v[r][None])
+                a, b, s = state[layer][r]
+                assert len(a) == lengths[r]
+                turned = rope(q[r], position[r], F.ROPE_QUERY)
+                for h in range(heads):
+                    want, w, bound, wb = attend(turned[h * group:(h + 1) * group], a[:, h], b[:, h])
+                    assert np.all(np.abs(out[r, h * group:(h + 1) * group] - want) <= bound), (step, layer, r, h)
+                    got = got_score[layer, r, h, :len(a)].astype(np.float64)
+                    s[h] += w.sum(0)
+                    assert np.all(np.abs(got - s[h]) <= wb.sum(0) + 1e-6 * s[h] + 1e-7), (step, layer, r, h)
+                    s[h] = got  # the operator's own sums decide an eviction
+        for bs in bufs:
+            for x in bs:
+                hip.free_buffer(x)
+        position[live] += 1
+        if step in (5, 9):
+            out_of = [r for r in range(rows) if live[r] and lengths[r] > budget]
+            fresh = [list(t) for t in tables]
+            for r in out_of:
+                fresh[r] = [free.pop() for _ in range(pages_of(budget, page))]
+            new_table = np.full((rows, width), 0xFFFFFFFF, np.uint32)
+            for r in out_of:
+                new_table[r, :len(fresh[r])] = fresh[r]
+            tb = hip.from_host(new_table)
+            hip.kv_evict_paged(GhKvPaged(pool, tb, lengths_b, score, page, width, rows), kv, None, budget, recent)
+            now = hip.download(lengths_b, np.uint32, rows)
+            for r in out_of:
+                assert now[r] == budget
+                lengths[r] = budget
+                free.extend(tables[r])
+                fresh[r] += [free.pop(0) for _ in range(width - len(fresh[r]))]
+                tables[r] = fresh[r]
+                for layer in range(layers):
+                    a, b, s = state[layer][r]
+                    best = [keep(s[h].astype(np.float32), budget, recent) for h in range(heads)]
+                    state[layer][r] = (np.stack([a[best[h], h] for h in range(heads)], 1),
+                                       np.stack([b[best[h], h] for h in range(heads)], 1),
+                                       np.stack([s[h, best[h]] for h in range(heads)]))
+            hip.upload(table, np.array(tables, np.uint32))
+            hip.free_buffer(tb)
+    for b in (kc, vc, table, lengths_b, pos_b, score):
+        hip.free_buffer(b)
+
+
+def test_prefill_into_a_run_of_pages(hip, rng):
+    """A prompt whose pages lie in a row is written and prefilled by the contiguous operators through a view of
+    the pool; decode goes on over the same pages."""
+    heads, group, page, n, slots = 2, 4, 16, 75, 16 * 20
+    q_heads, row = heads * group, heads * 256
+    kc, vc = (hip.from_host(np.full((2, slots, heads, D), np.nan, np.float16)) for _ in range(2))
+    layer, first, count = 1, 7, pages_of(n + 1, page)
+    at = (layer * slots + first * page) * row
+    part = F.GhKv(hip.view(kc, at, count * page * row), hip.view(vc, at, count * page * row), F.KV_F16, 1, count * page, heads, D, D)
+    k, v = (rng.standard_normal((n + 1, heads, D)).astype(np.float16) for _ in range(2))
+    q = rng.standard_normal((n + 1, q_heads, D)).astype(np.float16)
+    kb, vb, qb = hip.from_host(k[:n]), hip.from_host(v[:n]), hip.from_host(q[:n])
+    ob = hip.alloc_buffer(q.nbytes)
+    hip.begin()
+    hip.kv_write(part, kb, vb, 0, 0, n * heads)
+    hip.attention_prefill(ob, qb, part, q_heads, 0, n, 0)
+    hip.submit()
+    table, lengths = hip.from_host(np.arange(first, first + count, dtype=np.uint32)), hip.from_host(np.array([n + 1], np.uint32))
+    kv = GhKvPaged(F.GhKv(kc, vc, F.KV_F16, 2, slots, heads, D, D), table, lengths, F.GhBuf(), page, count, 1)
+    k1, v1, q1 = hip.from_host(k[n:]), hip.from_host(v[n:]), hip.from_host(q[n:])
+    hip.begin()
+    hip.kv_write_paged(kv, k1, v1, 1, layer)
+    hip.attention_decode_paged(ob, q1, kv, q_heads, 0, layer)
+    hip.submit()
+    out = hip.download(ob, np.float16, q_heads * D).reshape(q_heads, D)
+    for h in range(heads):
+        want, _, bound, _ = attend(q[n, h * group:(h + 1) * group], k[:, h], v[:, h])
+        assert np.all(np.abs(out[h * group:(h + 1) * group] - want) <= bound)
+    for b in (kc, vc, kb, vb, qb, ob, table, lengths, k1, v1, q1):
+        hip.free_buffer(b)
