@@ -1,0 +1,250 @@
+"""The checks and launch plans of the operators over paged caches, without a device: host/paged.cpp built
+with recorded launches (tests/paged_host.cpp). Every refused call launches nothing and is latched; every
+accepted one stays within its buffers and scratch."""
+import ctypes as C
+import os
+import random
+import subprocess
+
+import pytest
+
+from graph_horizon_amd import _ffi as F
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+SCRATCH = 1 << 50
+INVALID, OOM, RANGE, STATE, UNSUPPORTED = -1, -4, -5, -7, -8
+
+
+class Pages(C.Structure):
+    _fields_ = [(n, C.c_uint64) for n in ("kc", "vc", "table", "lengths", "score", "fault")] + \
+               [(n, C.c_uint32) for n in ("width", "shift", "pages", "kv_heads")]
+
+
+class AttnArgs(C.Structure):
+    _fields_ = [("p", Pages)] + [(n, C.c_uint64) for n in ("q", "out", "part_acc", "part_ml", "raw")] + \
+               [(n, C.c_uint32) for n in ("q_heads", "group", "max_len", "span", "splits", "raw_len")] + \
+               [("scale", C.c_float), ("chunks", C.c_uint32)]
+
+
+class Launch(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("kernel", "gx", "gy", "gz", "block")] + [("args", C.c_ubyte * 512)]
+
+
+@pytest.fixture(scope="module")
+def lib(tmp_path_factory):
+    out = str(tmp_path_factory.mktemp("paged") / "paged_host.so")
+    subprocess.run(["g++", "-O1", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include",
+                    "-Wall", "-Werror", "-o", out, os.path.join(ROOT, "tests", "paged_host.cpp"),
+                    os.path.join(ROOT, "graph_horizon_amd", "csrc", "host", "paged.cpp")], check=True)
+    h = C.CDLL(out)
+    for name in ("gh_kv_write_paged", "gh_rope_kv_write_paged", "gh_attention_decode_paged", "gh_kv_evict_paged"):
+        getattr(h, name).argtypes = F.SIGNATURES[name][1]
+    h.host_backend.restype = h.host_encoder.restype = h.host_launch.restype = C.c_void_p
+    h.host_encoder.argtypes = h.host_latched.argtypes = h.host_error.argtypes = [C.c_void_p]
+    h.host_reset.argtypes = [C.c_void_p, C.c_uint64]
+    h.host_scratch.restype = C.c_uint64
+    h.host_error.restype = C.c_char_p
+    return h
+
+
+class Host:
+    def __init__(self, lib, cus=256):
+        self.lib, self.b = lib, lib.host_backend(cus)
+        self.enc = lib.host_encoder(self.b)
+        self.at = 1 << 40
+        ids = (C.c_uint32 * 5)()
+        lib.host_kernels(ids)
+        self.ids = dict(zip(("write", "attn", "join", "select", "move"), ids))
+
+    def buf(self, nbytes, off=0):
+        b = F.GhBuf(self.at + off, nbytes, 0, F.BUF_ALLOC, 0, 0)
+        self.at += (nbytes + 4095 + off) // 4096 * 4096
+        return b
+
+    def kv(self, layers=2, slots=1024, heads=2, page=16, width=8, rows=3, scored=False):
+        cache = layers * slots * heads * 256
+        pool = F.GhKv(self.buf(cache), self.buf(cache), F.KV_F16, layers, slots, heads, 128, 128)
+        score = self.buf(layers * rows * heads * width * page * 4) if scored else F.GhBuf()
+        return F.GhKvPaged(pool, self.buf(rows * width * 4), self.buf(rows * 4), score, page, width, rows)
+
+    def call(self, name, *args, limit=0):
+        """(status, launches) of a call; a refused one has launched nothing and is latched."""
+        self.lib.host_reset(self.b, limit)
+        args = [C.byref(a) if isinstance(a, C.Structure) else a for a in args]
+        rc = getattr(self.lib, name)(self.b, self.enc, *args)
+        got = [Launch.from_buffer_copy(C.string_at(self.lib.host_launch(i), C.sizeof(Launch)))
+               for i in range(self.lib.host_launches())]
+        assert rc == self.lib.host_latched(self.b)
+        if rc:
+            assert not got and self.lib.host_error(self.b)
+        return rc, got
+
+
+@pytest.fixture
+def host(lib):
+    return Host(lib)
+
+
+def shift_buf(b, off):
+    return F.GhBuf(b.addr + off, b.bytes, b.format, b.kind, 0, 0)
+
+
+def shorter(b, by=1):
+    return F.GhBuf(b.addr, b.bytes - by, b.format, b.kind, 0, 0)
+
+
+def handles(host):
+    """(what is wrong, status, handle): the handle checks that every entry point makes."""
+    def change(status, what, **fields):
+        kv = host.kv(scored=True)
+        for k, v in fields.items():
+            target = kv.kv if k in ("scheme", "head_dim", "value_dim", "kv_heads", "context", "k", "v") else kv
+            setattr(target, k, v(getattr(target, k)) if callable(v) else v)
+        return what, status, kv
+
+    yield change(UNSUPPORTED, "scheme", scheme=1)
+    yield change(UNSUPPORTED, "head_dim", head_dim=64)
+    yield change(UNSUPPORTED, "value_dim", value_dim=256)
+    yield change(INVALID, "no kv heads", kv_heads=0)
+    for page in (0, 1, 8, 24, 48, 65536):
+        yield change(INVALID, "page_size %d" % page, page_size=page)
+    yield change(INVALID, "no slots", context=0)
+    yield change(INVALID, "part of a page", context=1023)
+    yield change(RANGE, "more slots than memory", context=2048)
+    yield change(RANGE, "context overflows", context=0xFFFFFFF0)
+    yield change(INVALID, "no rows", rows=0)
+    yield change(INVALID, "too many rows", rows=65536)
+    yield change(INVALID, "no table", table_width=0)
+    yield change(INVALID, "positions past 31 bits", table_width=1 << 27)
+    for name in ("k", "v", "table", "lengths", "score"):
+        yield change(RANGE, name + " too small", **{name: shorter})
+        yield change(RANGE, name + " not aligned", **{name: lambda b: shift_buf(b, 2)})
+    for name in ("k", "v", "table", "lengths"):
+        yield change(RANGE, name + " missing", **{name: F.GhBuf()})
+
+
+def test_handles_are_checked_by_every_entry_point(host):
+    big = host.buf(1 << 30)
+    yarn = F.GhYarn(128, 16384, 1e6, 16.0, 32.0, 1.0, 1.0, 0.1)
+    count = 0
+    for what, status, kv in handles(host):
+        good = host.kv(scored=True)
+        for name, args in (("gh_kv_write_paged", (kv, big, big, 1, 0)),
+                           ("gh_rope_kv_write_paged", (kv, big, big, big, big, 8, big, 1, 100, yarn, 0)),
+                           ("gh_attention_decode_paged", (big, big, kv, 8, 0, 0)),
+                           ("gh_kv_evict_paged", (good, kv, None, 8, 1)), ("gh_kv_evict_paged", (kv, good, None, 8, 1))):
+            assert host.call(name, *args)[0] == status, (what, name)
+            count += 1
+    assert count > 150
+    assert host.lib.gh_kv_write_paged(host.b, None, None, None, None, 1, 0) == STATE
+    assert host.call("gh_kv_write_paged", None, big, big, 1, 0)[0] == INVALID
+
+
+def test_write_refusals(host):
+    kv = host.kv()
+    n = 3 * 5 * 2 * 256
+    k, v = host.buf(n), host.buf(n)
+    assert host.call("gh_kv_write_paged", kv, k, v, 5, 1)[0] == 0
+    for args, status in (((kv, k, v, 0, 0), INVALID), ((kv, k, v, 6, 0), RANGE), ((kv, shorter(k), v, 5, 0), RANGE),
+                         ((kv, k, shorter(v), 5, 0), RANGE), ((kv, shift_buf(k, 8), v, 5, 0), RANGE),
+                         ((kv, k, None, 5, 0), RANGE), ((kv, k, v, 5, 2), RANGE), ((kv, k, v, 0xFFFFFFFF, 0), INVALID)):
+        assert host.call("gh_kv_write_paged", *args)[0] == status
+
+
+def test_rope_write_refusals(host):
+    kv = host.kv()
+    q, o, k, v = host.buf(3 * 8 * 256), host.buf(3 * 8 * 256), host.buf(3 * 2 * 256), host.buf(3 * 2 * 256)
+    pos, yarn = host.buf(12), F.GhYarn(128, 16384, 1e6, 16.0, 32.0, 1.0, 1.0, 0.1)
+    name = "gh_rope_kv_write_paged"
+    assert host.call(name, kv, o, q, k, v, 8, pos, 1, 262143, yarn, 0)[0] == 0
+    assert host.lib.host_rope_positions(C.c_void_p(host.b)) == 262144
+    assert host.call(name, kv, q, q, k, v, 8, pos, 1, 0, yarn, 0)[0] == 0  # in place
+    wide = F.GhYarn(130, 16384, 1e6, 16.0, 32.0, 1.0, 1.0, 0.1)
+    for args, status in (((kv, o, q, k, v, 8, pos, 1, 262144, yarn, 0), RANGE), ((kv, o, q, k, v, 8, pos, 1, 9, None, 0), INVALID),
+                         ((kv, o, q, k, v, 8, pos, 1, 9, wide, 0), INVALID), ((kv, o, q, k, v, 0, pos, 1, 9, yarn, 0), INVALID),
+                         ((kv, o, q, k, v, 9, pos, 1, 9, yarn, 0), RANGE), ((kv, shorter(o), q, k, v, 8, pos, 1, 9, yarn, 0), RANGE),
+                         ((kv, o, q, k, v, 8, shorter(pos), 1, 9, yarn, 0), RANGE), ((kv, o, q, k, v, 8, None, 1, 9, yarn, 0), RANGE),
+                         ((kv, o, None, k, v, 8, pos, 1, 9, yarn, 0), RANGE), ((kv, o, q, k, v, 8, pos, 0, 9, yarn, 0), INVALID),
+                         ((kv, F.GhBuf(q.addr + 256, 3 * 8 * 256, 0, 1, 0, 0), q, k, v, 8, pos, 1, 9, yarn, 0), INVALID)):
+        assert host.call(name, *args)[0] == status, args
+
+
+def test_attention_refusals(host):
+    kv = host.kv(scored=True)
+    q, o = host.buf(3 * 8 * 256), host.buf(3 * 8 * 256)
+    name = "gh_attention_decode_paged"
+    assert host.call(name, o, q, kv, 8, 128, 1)[0] == 0
+    for args, status in (((o, q, kv, 0, 0, 0), INVALID), ((o, q, kv, 7, 0, 0), INVALID), ((o, q, kv, 34, 0, 0), UNSUPPORTED),
+                         ((o, q, kv, 8, 129, 0), RANGE), ((o, q, kv, 8, 0, 2), RANGE), ((o, q, kv, 10, 0, 0), RANGE),
+                         ((shorter(o), q, kv, 8, 0, 0), RANGE), ((o, shift_buf(q, 4), kv, 8, 0, 0), RANGE),
+                         ((None, q, kv, 8, 0, 0), RANGE)):
+        assert host.call(name, *args)[0] == status, args
+    assert host.call(name, o, q, kv, 8, 0, 0, limit=1000)[0] == OOM
+
+
+def test_evict_refusals(host):
+    name = "gh_kv_evict_paged"
+    src, dst = host.kv(scored=True), host.kv(scored=True, width=3)
+    kept = host.buf(2 * 3 * 2 * 40 * 4)
+    rc, got = host.call(name, dst, src, kept, 40, 40)
+    assert rc == 0 and [g.kernel for g in got] == [host.ids["select"], host.ids["move"]]
+    same = F.GhKvPaged.from_buffer_copy(src)  # scores and lengths in place, another table
+    same.table = host.buf(src.table.bytes)
+    assert host.call(name, same, src, None, 40, 0)[0] == 0
+    narrow = F.GhKvPaged.from_buffer_copy(dst)
+    narrow.score = src.score
+    part = F.GhKvPaged.from_buffer_copy(dst)
+    part.score = F.GhBuf(src.score.addr + 64, dst.score.bytes, 0, 1, 0, 0)
+    lengths = F.GhKvPaged.from_buffer_copy(dst)
+    lengths.lengths = F.GhBuf(src.lengths.addr + 4, 12, 0, 1, 0, 0)
+    for d, s, k, budget, recent, status in (
+            (dst, src, kept, 0, 0, INVALID), (dst, src, kept, 40, 41, INVALID), (dst, src, kept, 49, 1, RANGE),
+            (dst, src, shorter(kept), 40, 1, RANGE), (dst, src, shift_buf(kept, 2), 40, 1, RANGE),
+            (host.kv(width=3), src, kept, 40, 1, INVALID), (dst, host.kv(), kept, 40, 1, INVALID),
+            (host.kv(scored=True, rows=2), src, None, 8, 1, INVALID), (host.kv(scored=True, page=32), src, None, 8, 1, INVALID),
+            (host.kv(scored=True, layers=3), src, None, 8, 1, INVALID), (host.kv(scored=True, heads=1), src, None, 8, 1, INVALID),
+            (narrow, src, None, 8, 1, INVALID), (part, src, None, 8, 1, INVALID), (lengths, src, None, 8, 1, INVALID)):
+        assert host.call(name, d, s, k, budget, recent)[0] == status, (budget, recent, status)
+    assert host.call(name, dst, src, None, 40, 1, limit=100)[0] == OOM
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_attention_plans_stay_within_their_scratch(host, seed):
+    """Splits cover max_len; the regions of the partials, their (m, l) and the scores lie in the scratch and apart;
+    the groups of rows cover all rows once; the grid is one that the device takes."""
+    rng = random.Random(seed)
+    heads, group = rng.choice((1, 2, 3, 8, 64)), rng.randint(1, 16)
+    page, rows = rng.choice((16, 64, 1024)), int(2 ** rng.uniform(0, 9))
+    width, scored = max(1, int(2 ** rng.uniform(4, 18)) // page), rng.random() < 0.5
+    kv = host.kv(layers=1, slots=page * 4, heads=heads, page=page, width=width, rows=rows, scored=scored)
+    q = host.buf(rows * heads * group * 256)
+    max_len = rng.choice((0, rng.randint(1, width * page)))
+    rc, got = host.call("gh_attention_decode_paged", q, q, kv, heads * group, max_len, 0)
+    assert rc == 0
+    want, size, at = max_len or width * page, host.lib.host_scratch(), 0
+    for g in got:
+        a = AttnArgs.from_buffer_copy(bytes(g.args))
+        assert a.max_len == want and a.span % 64 == 0 and 64 <= a.span <= 4096
+        assert a.splits * a.span >= want > (a.splits - 1) * a.span and a.raw_len >= want and a.raw_len % 16 == 0
+        assert g.gy <= 65535 and g.gz <= 65535 and g.gx * g.gy * g.gz < 2 ** 32 and g.block == 256
+        row = (a.q - q.addr) // (heads * group * 256)
+        assert a.out - q.addr == a.q - q.addr and a.p.table - kv.table.addr == row * width * 4
+        assert a.p.lengths - kv.lengths.addr == row * 4
+        if scored:
+            assert a.p.score - kv.score.addr == row * heads * width * page * 4
+        if g.kernel != host.ids["join"]:
+            assert row == at and g.gx == heads and g.gy == a.splits
+            assert g.kernel - host.ids["attn"] == 2 * (0 if group <= 4 else 1 if group <= 8 else 2) + scored
+            at += g.gz
+        else:
+            assert row + g.gz == at
+        if scored or a.splits > 1:
+            n = g.gz * heads * group
+            regions = [(a.part_acc, n * a.splits * 512), (a.part_ml, n * a.splits * 8)]
+            regions += [(a.raw, n * a.raw_len * 4)] if scored else []
+            regions.sort()
+            assert all(x % 16 == 0 or x == a.part_ml and x % 8 == 0 for x, _ in regions)
+            assert regions[0][0] >= SCRATCH and regions[-1][0] + regions[-1][1] <= SCRATCH + size
+            assert all(x + nx <= y for (x, nx), (y, _) in zip(regions, regions[1:]))
+    assert at == rows
+    assert size <= 512 << 20 or got[0].gz == 1
