@@ -86,9 +86,8 @@ const KernelName kKernels[] = {
     {K_GEMM_FEW_Q4K_T48, "gh_gemm_few_q4k_t48"}, {K_GEMM_FEW_Q6K_T48, "gh_gemm_few_q6k_t48"},
     {K_GEMM_FEW_MIXED_T48, "gh_gemm_few_mixed_t48"},
     {K_PAGED_WRITE, "gh_paged_write"},
-    {K_PAGED_ATTN_G4, "gh_paged_attn_g4"}, {K_PAGED_ATTN_G4_S, "gh_paged_attn_g4_s"},
-    {K_PAGED_ATTN_G8, "gh_paged_attn_g8"}, {K_PAGED_ATTN_G8_S, "gh_paged_attn_g8_s"},
-    {K_PAGED_ATTN_G16, "gh_paged_attn_g16"}, {K_PAGED_ATTN_G16_S, "gh_paged_attn_g16_s"},
+    {K_PAGED_ATTN, "gh_paged_attn"}, {K_PAGED_ATTN_S, "gh_paged_attn_s"},
+    {K_PAGED_SPLIT, "gh_paged_split"}, {K_PAGED_SPLIT_S, "gh_paged_split_s"},
     {K_PAGED_JOIN, "gh_paged_join"},
     {K_PAGED_SELECT, "gh_paged_select"}, {K_PAGED_MOVE, "gh_paged_move"},
 };

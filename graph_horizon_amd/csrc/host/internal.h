@@ -132,13 +132,10 @@ enum GhKernel : int {
     K_GEMM5_Q6K,
     K_GEMM5_MIXED,
     K_PAGED_WRITE,
-    // decode attention of up to 4, 8 and 16 query heads per kv head, each followed by its scoring form
-    K_PAGED_ATTN_G4,
-    K_PAGED_ATTN_G4_S,
-    K_PAGED_ATTN_G8,
-    K_PAGED_ATTN_G8_S,
-    K_PAGED_ATTN_G16,
-    K_PAGED_ATTN_G16_S,
+    K_PAGED_ATTN,
+    K_PAGED_ATTN_S,  // keeps the scores for gh_paged_join
+    K_PAGED_SPLIT,
+    K_PAGED_SPLIT_S,
     K_PAGED_JOIN,
     K_PAGED_SELECT,
     K_PAGED_MOVE,

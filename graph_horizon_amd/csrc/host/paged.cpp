@@ -18,6 +18,9 @@ bool fits(const gh_buf* buf, uint64_t bytes, uint64_t align) {
 
 bool overlap(const gh_buf& a, const gh_buf& b) { return a.addr < b.addr + b.bytes && b.addr < a.addr + a.bytes; }
 
+constexpr uint32_t kPagedRows = 512;  // rows that one attention launch lays out
+constexpr uint32_t kSpanTiles = 32;   // tiles of a gh_paged_split workgroup at most (its waves hold 64 each)
+
 uint64_t capacity(const gh_kv_paged* kv) { return (uint64_t)kv->table_width * kv->page_size; }
 
 // Everything about the handle that the host can see. `layer`: the one the call uses.
@@ -106,18 +109,6 @@ int write(gh_backend* b, const gh_kv_paged* kv, const gh_buf* k, const gh_buf* v
     return launch(b, K_PAGED_WRITE, (uint32_t)(n * a.groups), 1, 1, 256, &a);
 }
 
-// Positions per split: small enough that `rows` full rows give every CU four workgroups and that a long
-// row among short ones is spread over many, large enough that the partials (520 bytes per query head and
-// split) stay small beside the span's K and V (512 bytes per position).
-uint32_t span_of(const gh_backend* b, uint64_t rows, uint32_t kv_heads, uint32_t max_len) {
-    const uint64_t pairs = rows * kv_heads;
-    const uint64_t want = std::max<uint64_t>(1, ceil_div(4ull * b->cus, pairs));
-    uint64_t span = (ceil_div(max_len, want) + 63) / 64 * 64;
-    span = std::min<uint64_t>(std::max<uint64_t>(span, 64), 1024);
-    if (ceil_div(max_len, span) > 0xFFFFu) span = 4096;  // the grid's y
-    return (uint32_t)span;
-}
-
 int attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv_paged* kv, uint32_t q_heads,
               uint32_t max_len, uint32_t layer) {
     const uint32_t hk = kv->kv.kv_heads;
@@ -135,38 +126,66 @@ int attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv_pag
     a.q_heads = q_heads;
     a.group = group;
     a.max_len = max_len;
-    a.span = span_of(b, kv->rows, hk, max_len);
-    a.splits = ceil_div(max_len, a.span);
-    if (a.splits > 0xFFFFu) return fail(b, GH_E_UNSUPPORTED, "attention_decode_paged: max_len beyond 2^28");
     a.scale = 1.4426950408889634f / std::sqrt(128.0f);
     const bool scored = kv->score.addr != 0;
     a.raw_len = (max_len + 15) / 16 * 16;
-    a.chunks = scored ? std::min(ceil_div(max_len, 1024), 64u) : 0;
-    const bool parts = scored || a.splits > 1;
-    // scratch of a row: the splits' sums, and with scores each query head's
-    const uint64_t acc = parts ? (uint64_t)q_heads * a.splits * 512 : 0, ml = acc / 64;
-    const uint64_t raw = scored ? (uint64_t)q_heads * a.raw_len * 4 : 0, per = acc + ml + raw;
-    // rows in groups whose scratch fits 512 MiB
-    const uint32_t step = per ? (uint32_t)std::min<uint64_t>(kv->rows, std::max<uint64_t>(1, (512ull << 20) / per)) : kv->rows;
-    char* ws = nullptr;
-    if (per) {
-        const int rc = workspace_at(b, per * step, &ws);
-        if (rc) return rc;
+    a.blocks = scored ? std::min(ceil_div(max_len, 1024), 64u) : 0;
+    // Tiles of 16 positions and kv heads (8 KiB of K and V) that the rows can hold. Rows of one span, or few
+    // tiles in all: each row by itself in fixed spans (gh_paged_split), which start sooner (no row needs the
+    // others' lengths) and need no join where a row has one span; else all rows together in equal chunks
+    // (gh_paged_attn), which balances ragged rows. us, spans / chunks: 1 row of 500 8.3 / 10.4, 3 of 3000 13.9 /
+    // 15.3, 256 of up to 300 40.8 / 54, 12 of up to 1000 15.1 / 15.0, 64 of up to 600 29.3 / 25.3, 8 of up to 8192
+    // 46.3 / 34.2, 32 of up to 4000 70.8 / 54.2.
+    const uint32_t tiles1 = ceil_div(max_len, 16);
+    const uint64_t most = (uint64_t)kv->rows * hk * tiles1;
+    const bool split = tiles1 <= kSpanTiles || most < 6144;
+    if (split) {
+        // about two workgroups per CU, each wave at most 8 tiles (1 row of 9000, in spans of 4 / 12 / 32 / 64 tiles:
+        // 16.5 / 14.3 / 16.7 / 23.8 us)
+        a.least = std::min(std::max(ceil_div(most, 8ull * b->cus) * 4, 4u), kSpanTiles);
+        a.chunks = ceil_div(tiles1, a.least);
+    } else {
+        // eight waves per CU, all of them at once: with more, the rows' streams disturb each other (64 rows of
+        // 8192 with 4 / 6 / 8 / 10 / 12 waves per CU: 394 / 377 / 326 / 381 / 344 us). Half of them where that
+        // gives a wave at most 12 tiles: a second workgroup on some CUs would only make those the last
+        // (16 rows of up to 2500: 31.8 / 26.9 us).
+        a.least = 4;
+        a.chunks = std::max(1u, 8 * b->cus / hk);
+        a.solo = 12;
     }
-    const GhKernel first = group <= 4 ? K_PAGED_ATTN_G4 : group <= 8 ? K_PAGED_ATTN_G8 : K_PAGED_ATTN_G16;
+    // From half the last-level cache on, the next call will not find this one's K and V there, and reads past
+    // it are faster (64 rows of 8192 368 / 346 us, 1 of 32768 36.0 / 34.0; 16 of up to 2500, 83 MB: 31.2 / 37.7).
+    a.stream = 128ull << 20;
+    // scratch of a row: its partials, and with scores each query head's
+    const uint64_t acc = (uint64_t)q_heads * 512, ml = acc / 64, raw = scored ? (uint64_t)q_heads * a.raw_len * 4 : 0;
+    // rows in groups that the kernel lays out at once and whose scratch fits 512 MiB
+    const uint64_t per = (acc + ml) * (split ? a.chunks : 1) + raw;
+    const uint64_t room = std::min<uint64_t>((512ull << 20) / per, (1u << 30) / tiles1);  // tiles count in 32 bits
+    const uint32_t step = (uint32_t)std::min<uint64_t>(std::min(kv->rows, kPagedRows), std::max<uint64_t>(1, room));
+    const uint64_t parts = split ? (uint64_t)a.chunks * step : a.chunks + step, layout = (kPagedRows + 4) * 4;
+    char* ws = nullptr;
+    int rc = workspace_at(b, layout + (acc + ml) * parts + raw * step, &ws);
+    if (rc) return rc;
+    a.layout = split ? 0 : (uint64_t)ws;
+    a.part_acc = (uint64_t)ws + layout;
+    a.raw = scored ? a.part_acc + acc * parts : 0;
+    a.part_ml = a.part_acc + acc * parts + raw * step;
     const GhPages p0 = a.p;
     for (uint32_t r = 0; r < kv->rows; r += step) {
-        const uint32_t rows = std::min(step, kv->rows - r);
+        a.rows = std::min(step, kv->rows - r);
         a.p.table = p0.table + (uint64_t)r * p0.width * 4;
         a.p.lengths = p0.lengths + (uint64_t)r * 4;
         a.p.score = scored ? p0.score + (uint64_t)r * hk * capacity(kv) * 4 : 0;
         a.q = q->addr + (uint64_t)r * q_heads * 256;
         a.out = out->addr + (uint64_t)r * q_heads * 256;
-        a.part_acc = (uint64_t)ws;
-        a.raw = scored ? (uint64_t)ws + acc * step : 0;
-        a.part_ml = (uint64_t)ws + (acc + raw) * step;
-        int rc = launch(b, (GhKernel)(first + (scored ? 1 : 0)), hk, a.splits, rows, 256, &a);
-        if (!rc && parts) rc = launch(b, K_PAGED_JOIN, q_heads + hk * a.chunks, 1, rows, 256, &a);
+        if (split) {
+            rc = launch(b, scored ? K_PAGED_SPLIT_S : K_PAGED_SPLIT, hk, a.chunks, a.rows, 256, &a, 4 * group * 134 * 4);
+        } else {
+            // no more chunks than the rows' tiles can fill
+            const uint64_t chunks = std::min<uint64_t>(a.chunks, ceil_div((uint64_t)a.rows * tiles1, a.least));
+            rc = launch(b, scored ? K_PAGED_ATTN_S : K_PAGED_ATTN, ceil_div(hk * chunks, 4), 1, 1, 256, &a);
+        }
+        if (!rc && (!split || a.chunks > 1)) rc = launch(b, K_PAGED_JOIN, q_heads + hk * a.blocks, a.rows, 2, 256, &a);
         if (rc) return rc;
     }
     return GH_OK;

@@ -285,7 +285,12 @@ struct GhPagedWriteArgs {
     uint32_t groups;   // workgroups per token
 };
 
-// Decode attention. Partials of (row, kv head, split): acc f32 [group][128] and (m, l) float2 [group].
+// Decode attention, in tiles of 16 positions. Partials (what one row has in one workgroup's or wave's share):
+// acc f32 [kv_heads][group][128] and (m, l) float2 [kv_heads][group].
+// gh_paged_attn: all rows' tiles, one row after the other, are cut into chunks of `per` tiles, the larger of
+// `least` and an equal share of `chunks` (of chunks / 2 where that is at most `solo`); the part of row r in chunk c
+// has partial c + r, a number that grows from each part to the next. gh_paged_split (layout 0): each row in `chunks`
+// spans of `least` tiles; span c of row r has partial r·chunks + c.
 struct GhPagedAttnArgs {
     GhPages p;
     uint64_t q;        // f16 [rows][q_heads][128]
@@ -293,14 +298,18 @@ struct GhPagedAttnArgs {
     uint64_t part_acc;
     uint64_t part_ml;
     uint64_t raw;      // f32 [rows][kv_heads][group][raw_len] scores, base 2 (0: not kept)
+    uint64_t stream;   // bytes of K and V from which they are read past the last-level cache
+    uint64_t layout;   // u32: per, then each row's first tile, [rows + 1], for gh_paged_join
     uint32_t q_heads;
     uint32_t group;
+    uint32_t rows;
     uint32_t max_len;
-    uint32_t span;     // positions per split, a multiple of 64, at most 4096
-    uint32_t splits;   // ceil(max_len / span)
+    uint32_t chunks;
+    uint32_t least;
+    uint32_t solo;
     uint32_t raw_len;  // max_len rounded up to 16
     float scale;       // log2(e) / sqrt(128)
-    uint32_t chunks;   // gh_paged_join: workgroups per kv head that add scores
+    uint32_t blocks;   // gh_paged_join: workgroups per kv head that add scores
 };
 
 // Eviction. Strides of a layer: slots of the pools, rows for the scores.

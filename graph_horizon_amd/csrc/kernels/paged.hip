@@ -87,10 +87,9 @@ GH_KERNEL __launch_bounds__(256) void gh_paged_write(GhPagedWriteArgs a) {
 }
 
 // ---- decode attention ---------------------------------------------------------------------------
-// Grid (kv heads, splits, rows), 256 threads: a workgroup takes the G query heads of one kv head over `span`
-// positions of one row. Wave w owns tiles of 16 positions w, w + 4, ... of the span, each within one page
-// (page_size >= 16): lane i holds the table entry of the wave's i-th tile, read once at the start, so a
-// tile's address is a readlane away. Per tile, with FP32 accumulators and scores in base 2:
+// Bound by the read of K and V. A wave takes the G <= 16 query heads of one kv head over tiles of 16 positions, each
+// within one page (page_size >= 16) and so at one address: lanes hold the next 64 tiles' slots, looked up
+// together, and a tile's is a readlane away. Per tile, with FP32 accumulators and scores in base 2:
 //   S^T = K·Q^T     4 x v_mfma_f32_16x16x32_f16: A = 16 K rows straight from memory (lane l: position l % 16,
 //                   dims 32 s + 8 (l / 16) .. + 8), B = the query, column n = l % 16 is head n (zero
 //                   past G); lane l receives head n's scores of positions 4 (l / 16) + i;
@@ -100,7 +99,12 @@ GH_KERNEL __launch_bounds__(256) void gh_paged_write(GhPagedWriteArgs a) {
 // Weights are 2^(s - m + 15), m the running maximum: hi + lo then reach 2^-39 of the largest weight. Both
 // parts are at least 2^-24, so that an infinite V gives an infinity and not infinity times 0.
 // K and V are read through buffer resources whose range ends at the row's last position: what a page holds
-// past it reads as zero, without a memory access, and has weight 0.
+// past it reads as zero, without a memory access, and has weight 0. The next tile's K is asked for as soon as
+// this one's products are made, its V behind the last use of this one's: one set of registers, 126 to 158
+// VGPRs. (A second and third set of registers, with 146 and 178 VGPRs, measured no different: 64 rows of 8192
+// 365 / 363 us, at 366 with one.)
+// Two divisions of the work over waves, paged_attn and paged_split (the host's rule says when), then
+// gh_paged_join where a row is in several parts.
 namespace {
 typedef _Float16 ph8 __attribute__((ext_vector_type(8)));
 typedef float pf4 __attribute__((ext_vector_type(4)));
@@ -152,261 +156,504 @@ __device__ __forceinline__ void weight_parts(float p0, float p1, uint32_t* hi, u
     *lo = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(pu2, l), one));
 }
 
-template <int GM>
-struct AttnLds {
-    float m[4][GM], l[4][GM];
-    float acc[4][GM][132];
-    float e[4][GM], M[GM], L[GM];
+// A tile's addresses: K and V of one head from the slot of the tile's first position, `count` positions long
+// (0: no range, and nothing is read). The widest row, 65535 heads, keeps offsets below 2^28.
+struct Where {
+    __amdgpu_buffer_rsrc_t k, v;
 };
+__device__ __forceinline__ Where tile_at(const GhPages& p, uint32_t slot, uint32_t count, uint32_t kvh) {
+    const uint32_t row_bytes = p.kv_heads * 256;
+    const uint64_t at = (uint64_t)slot * row_bytes + kvh * 256;
+    const int range = count ? (int)((count - 1) * row_bytes + 256) : 0;
+    return {__builtin_amdgcn_make_buffer_rsrc((void*)(p.kc + at), 0, range, kBufWord3),
+            __builtin_amdgcn_make_buffer_rsrc((void*)(p.vc + at), 0, range, kBufWord3)};
+}
+template <int CACHE>
+__device__ __forceinline__ void load_k(const Where& w, uint32_t row_bytes, Tile& r) {
+    const uint32_t lane = threadIdx.x & 63u, n = lane & 15u, g = lane >> 4;
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+        r.k[s] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(w.k, n * row_bytes + 16 * g + 64 * s, 0, CACHE));
+}
+template <int CACHE>
+__device__ __forceinline__ void load_v(const Where& w, uint32_t row_bytes, Tile& r) {
+    const uint32_t lane = threadIdx.x & 63u, n = lane & 15u, g = lane >> 4;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        r.v[j] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(w.v, (4 * g + j) * row_bytes + 16 * n, 0, CACHE));
+}
 
-template <int GM, bool SCORED>
-__device__ __forceinline__ void paged_attn(const GhPagedAttnArgs& a) {
-    __shared__ AttnLds<GM> sh;
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, n = lane & 15u, g = lane >> 4;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t kvh = blockIdx.x, split = blockIdx.y, row = blockIdx.z, G = a.group;
-    const uint32_t begin = split * a.span;  // < max_len
-    // the wave's table entries: tile i covers positions begin + 64 i + 16 wave .. + 16
-    const uint32_t mine = begin + 64 * lane + 16 * wave;
-    uint32_t entry = 0;
-    if (64 * lane < a.span && mine < a.max_len)
-        entry = gh_gp<uint32_t>(a.p.table)[(uint64_t)row * a.p.width + (mine >> a.p.shift)];
-    ph8 qf[4];
-    const GH_GLOBAL uint4* qp =
-        gh_gp<uint4>(a.q + (((uint64_t)row * a.q_heads + kvh * G + min(n, G - 1)) * 128 + 8 * g) * 2);
+// B fragments of the G queries of a kv head: head n = l % 16 (zero past G), dims 32 s + 8 (l / 16) .. + 8.
+__device__ __forceinline__ void load_q(const GhPagedAttnArgs& a, uint32_t row, uint32_t kvh, ph8 (&qf)[4]) {
+    const uint32_t lane = threadIdx.x & 63u, n = lane & 15u, g = lane >> 4, G = a.group;
+    const GH_GLOBAL uint4* qp = gh_gp<uint4>(a.q + (((uint64_t)row * a.q_heads + kvh * G + min(n, G - 1)) * 128 + 8 * g) * 2);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
         const uint4 x = qp[4 * s];
         qf[s] = __builtin_bit_cast(ph8, n < G ? x : make_uint4(0u, 0u, 0u, 0u));
     }
-    const uint32_t len = row_length(a.p, row, a.max_len, kvh == 0 && split == 0);
-    const uint64_t out0 = a.out + ((uint64_t)row * a.q_heads + kvh * G) * 256;
-    if (len == 0) {
-        if (split == 0)
-            for (uint32_t i = tid; i < G * 64; i += 256) gh_gpw<uint32_t>(out0)[i] = 0u;
+}
+
+// A wave's running sums: lane l holds head n = l % 16's maximum, its own part of Σ weights, and value dims
+// 32 (l / 16) + 8 j + t in acc[t][j].
+struct Sums {
+    float m, l;
+    pf4 acc[8];
+    __device__ __forceinline__ void clear() {
+        m = -__builtin_inff();
+        l = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) acc[t] = pf4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+};
+
+__device__ __forceinline__ pf4 tile_products(const Tile& r, const ph8 (&qf)[4]) {
+    pf4 st = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+        st = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ph8, r.k[s]), qf[s], st, 0, 0, 0);
+    return st;
+}
+// products -> scores in base 2, -inf past the tile's positions
+__device__ __forceinline__ pf4 tile_scores(pf4 st, uint32_t count, float scale) {
+    const uint32_t g = (threadIdx.x & 63u) >> 4;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) st[j] = 4 * g + (uint32_t)j < count ? st[j] * scale : -__builtin_inff();
+    return st;
+}
+__device__ __forceinline__ void tile_add(Sums& x, pf4 st, const Tile& r) {
+    const float mx = fmaxf(x.m, lanes4_max(fmaxf(fmaxf(st[0], st[1]), fmaxf(st[2], st[3]))));
+    const float f = share(x.m, mx);
+    // nothing but -inf so far: every weight 0
+    const float up = mx == -__builtin_inff() ? 0.0f : kUp - mx;
+    x.m = mx;
+    float p[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p[j] = __builtin_amdgcn_exp2f(st[j] + up);
+    x.l = x.l * f + ((p[0] + p[1]) + (p[2] + p[3]));
+    uint32_t h0, h1, l0, l1;
+    weight_parts(p[0], p[1], &h0, &l0);
+    weight_parts(p[2], p[3], &h1, &l1);
+    const ph8 pv = __builtin_bit_cast(ph8, make_uint4(h0, h1, l0, l1));
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+        x.acc[t] *= f;
+        x.acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v_column(r.v, t), pv, x.acc[t], 0, 0, 0);
+    }
+}
+
+// Adds the weights of positions from, from + step, ... (four each) to the scores of a row and kv head: 2^(s - M + 15) / L
+// per query head, summed over the G heads in order. Positions past the row keep their bits.
+__device__ __forceinline__ void add_scores(const GhPagedAttnArgs& a, uint32_t row, uint32_t kvh, const float* M, const float* L,
+                                           uint32_t from, uint32_t step, uint32_t len) {
+    const uint64_t raw = a.raw + ((uint64_t)row * a.p.kv_heads + kvh) * a.group * a.raw_len * 4;
+    const uint64_t to = a.p.score + ((uint64_t)row * a.p.kv_heads + kvh) * (a.p.width << a.p.shift) * 4;
+    for (uint32_t pos = from; pos < len; pos += step) {
+        pf4 w = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t h = 0; h < a.group; ++h) {
+            const pf4 s = *gh_gp<pf4>(raw + ((uint64_t)h * a.raw_len + pos) * 4);
+            const float up = kUp - M[h], inv = 1.0f / L[h];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] += __builtin_amdgcn_exp2f(s[j] + up) * inv;
+        }
+        GH_GLOBAL pf4* p = (GH_GLOBAL pf4*)gh_gpw<float>(to + (uint64_t)pos * 4);
+        const pf4 old = *p;
+        if (pos + 4 <= len) {
+            *p = old + w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 3; ++j)
+                if (pos + j < len) gh_gpw<float>(to)[pos + j] = old[j] + w[j];
+        }
+    }
+}
+
+constexpr uint32_t kRows = 512;  // rows of a launch at most
+
+// The rows' tiles one after the other: row r has tiles first[r] .. first[r + 1] of 16 positions.
+struct RowsLds {
+    uint32_t len[kRows], first[kRows + 1];
+    uint32_t sums[4];
+};
+
+// Fills sh from the rows' lengths (longer ones than max_len count 0); 256 threads.
+__device__ __forceinline__ void lay_out_rows(const GhPagedAttnArgs& a, RowsLds& sh, bool report) {
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+    if (a.rows <= 64) {  // each wave by itself, the same values
+        uint32_t n = lane < a.rows ? gh_gp<uint32_t>(a.p.lengths)[lane] : 0u;
+        if (n > a.max_len) {
+            if (report) fault(a.p, GH_PAGED_LENGTH);
+            n = 0;
+        }
+        uint32_t upto = (n + 15) >> 4;
+        for (uint32_t o = 1; o < a.rows; o <<= 1) {
+            const uint32_t x = __shfl_up(upto, o, 64);
+            if (lane >= o) upto += x;
+        }
+        sh.len[lane] = n;
+        if (lane == 0) sh.first[0] = 0;
+        sh.first[lane + 1] = upto;
         return;
     }
-    if (begin >= len) return;
-    const uint32_t end = min(len, begin + a.span);
-    const bool bad = 64 * lane < a.span && mine < end && entry >= a.p.pages;
-    if (bad) fault(a.p, GH_PAGED_PAGE);
-    const uint64_t bad_tiles = __ballot(bad);
-    const uint32_t first = begin + 16 * wave;
-    const uint32_t tiles = first < end ? (end - first + 63) / 64 : 0u;
-    const uint32_t row_bytes = a.p.kv_heads * 256;
+    uint32_t n[2], t[2];
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {  // rows 2 tid, 2 tid + 1
+        const uint32_t r = 2 * tid + i;
+        n[i] = r < a.rows ? gh_gp<uint32_t>(a.p.lengths)[r] : 0u;
+        if (n[i] > a.max_len) {
+            if (report) fault(a.p, GH_PAGED_LENGTH);
+            n[i] = 0;
+        }
+        t[i] = (n[i] + 15) >> 4;
+    }
+    uint32_t upto = t[0] + t[1];
+#pragma unroll
+    for (uint32_t o = 1; o < 64; o <<= 1) {
+        const uint32_t x = __shfl_up(upto, o, 64);
+        if (lane >= o) upto += x;
+    }
+    if (lane == 63) sh.sums[wave] = upto;
+    sh.len[2 * tid] = n[0];
+    sh.len[2 * tid + 1] = n[1];
+    __syncthreads();
+    for (uint32_t w = 0; w < wave; ++w) upto += sh.sums[w];
+    if (tid == 0) sh.first[0] = 0;
+    sh.first[2 * tid + 1] = upto - t[1];
+    sh.first[2 * tid + 2] = upto;
+    __syncthreads();
+}
 
-    auto load = [&](uint32_t i, Tile& r) __attribute__((always_inline)) {
-        const uint32_t pos = first + 64 * i;
-        const uint32_t page = __builtin_amdgcn_readlane(entry, i & 63u);
-        // a tile past the last or of a bad page has no range, and no address is formed from its entry
-        const bool none = i >= tiles || (bad_tiles >> i & 1);
-        const uint64_t slot = none ? 0 : ((uint64_t)page << a.p.shift) + (pos & ((1u << a.p.shift) - 1));
-        const uint64_t at = slot * row_bytes + kvh * 256;
-        const int range = none ? 0 : (int)((min(end - pos, 16u) - 1) * row_bytes + 256);
-        const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)(a.p.kc + at), 0, range, kBufWord3);
-        const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)(a.p.vc + at), 0, range, kBufWord3);
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-            r.k[s] = __builtin_bit_cast(
-                uint4, __builtin_amdgcn_raw_buffer_load_b128(rk, n * row_bytes + 16 * g + 64 * s, 0, 0));
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            r.v[j] = __builtin_bit_cast(
-                uint4, __builtin_amdgcn_raw_buffer_load_b128(rv, (4 * g + j) * row_bytes + 16 * n, 0, 0));
+// One chunk of the rows' tiles for one kv head by one wave.
+constexpr int kStream = 2;  // cache policy of reads that will not be wanted again soon (nt)
+
+template <bool SCORED, int CACHE>
+__device__ __forceinline__ void paged_chunk(const GhPagedAttnArgs& a, const RowsLds& sh, uint32_t total, uint32_t per,
+                                            uint32_t chunk, uint32_t kvh) {
+    const uint32_t lane = threadIdx.x & 63u, n = lane & 15u, g = lane >> 4, G = a.group;
+    const uint32_t begin = chunk * per, tiles = min(per, total - begin), row_bytes = a.p.kv_heads * 256;
+
+    // lane i: slot, first position, and row | positions << 16 of tile i of the current 64
+    uint32_t t_slot = 0, t_pos = 0, t_row = 0;
+    auto look_up = [&](uint32_t from) __attribute__((always_inline)) {
+        const uint32_t t = begin + from + lane;
+        t_slot = t_pos = t_row = 0;
+        if (from + lane >= tiles) return;
+        uint32_t lo = 0, hi = a.rows;  // first[lo] <= t < first[hi]
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) >> 1;
+            if (sh.first[mid] <= t) lo = mid;
+            else hi = mid;
+        }
+        t_pos = (t - sh.first[lo]) * 16;
+        const uint32_t page = gh_gp<uint32_t>(a.p.table)[(uint64_t)lo * a.p.width + (t_pos >> a.p.shift)];
+        const bool bad = page >= a.p.pages;
+        if (bad) fault(a.p, GH_PAGED_PAGE);
+        t_slot = bad ? 0u : (page << a.p.shift) + (t_pos & ((1u << a.p.shift) - 1));
+        t_row = lo | (bad ? 0u : min(sh.len[lo] - t_pos, 16u) << 16);
+    };
+    look_up(0);
+    auto where = [&](uint32_t i) __attribute__((always_inline)) {
+        const uint32_t count = i < tiles ? __builtin_amdgcn_readlane(t_row, i & 63u) >> 16 : 0u;
+        return tile_at(a.p, __builtin_amdgcn_readlane(t_slot, i & 63u), count, kvh);
     };
 
-    float m = -__builtin_inff(), l = 0.0f;
-    pf4 acc[8];
+    ph8 qf[4];
+    Sums x;
+    uint32_t row = 0xFFFFu, since = 0;  // the row at hand and the tile it began with
+    uint64_t raw = 0;
+    // the row's sums up to tile i: its output if they are whole, else a partial
+    auto flush = [&](uint32_t i) __attribute__((always_inline)) {
+        const float L = lanes4_sum(x.l);
+        if (n >= G) return;
+        if (!SCORED && begin + since == sh.first[row] && begin + i == sh.first[row + 1]) {
 #pragma unroll
-    for (int t = 0; t < 8; ++t) acc[t] = pf4{0.0f, 0.0f, 0.0f, 0.0f};
-    const uint64_t raw = a.raw + (((uint64_t)row * a.p.kv_heads + kvh) * G + n) * a.raw_len * 4;
-
-    auto step = [&](uint32_t i, const Tile& r) __attribute__((always_inline)) {
-        const uint32_t pos = first + 64 * i + 4 * g;  // this lane's first position
-        const uint32_t last = bad_tiles >> i & 1 ? 0u : end;
-        pf4 st = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int j = 0; j < 4; ++j) {
+                uint32_t w[4];
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
-            st = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ph8, r.k[s]), qf[s], st, 0, 0, 0);
-        float mx = -__builtin_inff();
+                for (int t = 0; t < 4; ++t)
+                    w[t] = (uint32_t)gh_f2h(x.acc[2 * t][j] / L) | (uint32_t)gh_f2h(x.acc[2 * t + 1][j] / L) << 16;
+                *gh_gpw<uint4>(a.out + ((uint64_t)row * a.q_heads + kvh * G + n) * 256 + 64 * g + 16 * j) =
+                    make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            return;
+        }
+        const uint64_t part = ((uint64_t)(chunk + row) * a.p.kv_heads + kvh) * G + n;
+        GH_GLOBAL float4* to = gh_gpw<float4>(a.part_acc + part * 512 + 128 * g);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            st[j] = pos + (uint32_t)j < last ? st[j] * a.scale : -__builtin_inff();
-            mx = fmaxf(mx, st[j]);
+            to[2 * j] = make_float4(x.acc[0][j], x.acc[1][j], x.acc[2][j], x.acc[3][j]);
+            to[2 * j + 1] = make_float4(x.acc[4][j], x.acc[5][j], x.acc[6][j], x.acc[7][j]);
         }
-        if (SCORED && n < G) *gh_gpw<float4>(raw + (uint64_t)pos * 4) = make_float4(st[0], st[1], st[2], st[3]);
-        mx = fmaxf(m, lanes4_max(mx));
-        const float f = share(m, mx);
-        // nothing but -inf so far: every weight 0
-        const float up = mx == -__builtin_inff() ? 0.0f : kUp - mx;
-        m = mx;
-        float p[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) p[j] = __builtin_amdgcn_exp2f(st[j] + up);
-        l = l * f + ((p[0] + p[1]) + (p[2] + p[3]));
-        uint32_t h0, h1, l0, l1;
-        weight_parts(p[0], p[1], &h0, &l0);
-        weight_parts(p[2], p[3], &h1, &l1);
-        const ph8 pv = __builtin_bit_cast(ph8, make_uint4(h0, h1, l0, l1));
-#pragma unroll
-        for (int t = 0; t < 8; ++t) {
-            acc[t] *= f;
-            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v_column(r.v, t), pv, acc[t], 0, 0, 0);
-        }
+        if (g == 0) gh_gpw<float2>(a.part_ml)[part] = make_float2(x.m, L);
     };
 
-    if (tiles) {
-        Tile ra, rb;
-        load(0, ra);
-        for (uint32_t i = 0; i < tiles; i += 2) {
-            load(i + 1, rb);
-            step(i, ra);
-            if (i + 1 >= tiles) break;
-            load(i + 2, ra);
-            step(i + 1, rb);
+    // K of the next tile is asked for as soon as this one's products are made, V behind its last use
+    Tile r;
+    Where w = where(0);
+    load_k<CACHE>(w, row_bytes, r);
+    load_v<CACHE>(w, row_bytes, r);
+    for (uint32_t i = 0; i < tiles; ++i) {
+        const uint32_t info = __builtin_amdgcn_readlane(t_row, i & 63u);
+        const uint32_t pos = SCORED ? __builtin_amdgcn_readlane(t_pos, i & 63u) : 0u;
+        if ((info & 0xFFFFu) != row) {
+            if (i) flush(i);
+            row = info & 0xFFFFu;
+            since = i;
+            x.clear();
+            load_q(a, row, kvh, qf);
+            if (SCORED) raw = a.raw + (((uint64_t)row * a.p.kv_heads + kvh) * G + n) * a.raw_len * 4;
         }
+        pf4 st = tile_products(r, qf);
+        if ((i & 63u) == 63) look_up(i + 1);
+        w = where(i + 1);
+        load_k<CACHE>(w, row_bytes, r);
+        st = tile_scores(st, info >> 16, a.scale);
+        if (SCORED && n < G)
+            *gh_gpw<float4>(raw + (uint64_t)(pos + 4 * g) * 4) = make_float4(st[0], st[1], st[2], st[3]);
+        tile_add(x, st, r);
+        load_v<CACHE>(w, row_bytes, r);
     }
+    flush(tiles);
+}
 
-    // the four waves: M = max m_w, L = Σ 2^(m_w - M) l_w, ACC likewise
-    const float lt = lanes4_sum(l);
-    if (n < G) {
-        if (g == 0) {
-            sh.m[wave][n] = m;
-            sh.l[wave][n] = lt;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int t = 0; t < 8; ++t) sh.acc[wave][n][32 * g + 8 * j + t] = acc[t][j];
+// All rows' tiles in equal chunks. Grid: a wave per (chunk, kv head), heads first, 256 threads. A workgroup's
+// four waves read four heads of the same positions, 1 KiB in a row per position (four chunks of one head
+// instead: 64 rows of 8192 346 -> 396 us). The number of tiles is known on the device alone: every workgroup
+// adds up the rows' lengths, workgroup 0 leaves the result for the join.
+template <bool SCORED>
+__device__ __forceinline__ void paged_attn(const GhPagedAttnArgs& a) {
+    __shared__ RowsLds sh;
+    const uint32_t unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t chunk = unit / a.p.kv_heads, kvh = unit % a.p.kv_heads;
+    lay_out_rows(a, sh, blockIdx.x == 0);
+    const uint32_t total = sh.first[a.rows];
+    const uint32_t half = (2 * total + a.chunks - 1) / a.chunks;
+    const uint32_t per = max(a.least, half <= a.solo ? half : (total + a.chunks - 1) / a.chunks);
+    if (blockIdx.x == 0) {  // for the join
+        for (uint32_t r = threadIdx.x; r <= a.rows; r += 256) gh_gpw<uint32_t>(a.layout)[1 + r] = sh.first[r];
+        if (threadIdx.x == 0) gh_gpw<uint32_t>(a.layout)[0] = per;
     }
-    __syncthreads();
-    if (tid < G) {
-        const float M = fmaxf(fmaxf(sh.m[0][tid], sh.m[1][tid]), fmaxf(sh.m[2][tid], sh.m[3][tid]));
-        float L = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float e = share(sh.m[w][tid], M);
-            sh.e[w][tid] = e;
-            L += e * sh.l[w][tid];
-        }
-        sh.M[tid] = M;
-        sh.L[tid] = L;
-    }
-    __syncthreads();
-    const bool whole = !SCORED && len <= a.span;  // one split: the output itself
-    const uint64_t part = ((uint64_t)row * a.p.kv_heads + kvh) * a.splits + split;
-    for (uint32_t i = tid; i < G * 64; i += 256) {
-        const uint32_t h = i >> 6, d = 2 * (i & 63u);
-        float2 v = make_float2(0.0f, 0.0f);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float e = sh.e[w][h];
-            v.x += e * sh.acc[w][h][d];
-            v.y += e * sh.acc[w][h][d + 1];
-        }
-        if (whole) {
-            const float L = sh.L[h];
-            gh_gpw<uint32_t>(out0)[i] = (uint32_t)gh_f2h(v.x / L) | (uint32_t)gh_f2h(v.y / L) << 16;
-        } else {
-            gh_gpw<float2>(a.part_acc)[part * G * 64 + i] = v;
-        }
-    }
-    if (!whole && tid < G) gh_gpw<float2>(a.part_ml)[part * G + tid] = make_float2(sh.M[tid], sh.L[tid]);
+    for (uint32_t r = blockIdx.x; r < a.rows; r += gridDim.x)
+        if (sh.len[r] == 0)
+            for (uint32_t i = threadIdx.x; i < a.q_heads * 64; i += 256)
+                gh_gpw<uint32_t>(a.out)[(uint64_t)r * a.q_heads * 64 + i] = 0u;
+    if (chunk >= a.chunks || chunk * per >= total) return;
+    if ((uint64_t)total * a.p.kv_heads * 8192 >= a.stream) paged_chunk<SCORED, kStream>(a, sh, total, per, chunk, kvh);
+    else paged_chunk<SCORED, 0>(a, sh, total, per, chunk, kvh);
 }
 }  // namespace
 
-#define GH_PAGED_ATTN(GM)                                                                                  \
-    GH_KERNEL __launch_bounds__(256) void gh_paged_attn_g##GM(GhPagedAttnArgs a) { paged_attn<GM, false>(a); } \
-    GH_KERNEL __launch_bounds__(256) void gh_paged_attn_g##GM##_s(GhPagedAttnArgs a) { paged_attn<GM, true>(a); }
-GH_PAGED_ATTN(4)
-GH_PAGED_ATTN(8)
-GH_PAGED_ATTN(16)
+GH_KERNEL __launch_bounds__(256, 3) void gh_paged_attn(GhPagedAttnArgs a) { paged_attn<false>(a); }
+GH_KERNEL __launch_bounds__(256, 3) void gh_paged_attn_s(GhPagedAttnArgs a) { paged_attn<true>(a); }
 
-// The splits joined. Grid (q_heads + kv_heads·chunks, 1, rows), 256 threads.
-// x < q_heads: the output of one query head: M = max m_s, out = Σ 2^(m_s - M) acc_s / Σ 2^(m_s - M) l_s; eight
-// groups of 32 threads take every eighth split, four dims per thread, and add up in group order.
-// Else: the scores of a kv head, every chunks-th 1024 positions: the weight of position j is
-// 2^(s_j - M + 15) / L per query head, summed over the G heads in order and added to the row's score.
-GH_KERNEL __launch_bounds__(256) void gh_paged_join(GhPagedAttnArgs a) {
-    __shared__ float sm[16], sl[16];
-    __shared__ float4 red[8][32];
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, row = blockIdx.z, G = a.group;
-    const uint32_t len = row_length(a.p, row, a.max_len, false);
-    if (len == 0) return;
-    const uint32_t ns = (len + a.span - 1) / a.span;
-    const bool score = blockIdx.x >= a.q_heads;
-    if (!score && ns == 1 && !a.raw) return;  // written by the attention launch
-    const uint32_t kvh = score ? (blockIdx.x - a.q_heads) / a.chunks : blockIdx.x / G;
-    const uint64_t part = ((uint64_t)row * a.p.kv_heads + kvh) * a.splits;
-    const GH_GLOBAL float2* ml = gh_gp<float2>(a.part_ml) + part * G;
-    const uint32_t h0 = score ? 0 : blockIdx.x % G, h1 = score ? G : h0 + 1;
-    for (uint32_t h = h0 + wave; h < h1; h += 4) {
-        float M = -__builtin_inff(), L = 0.0f;
-        for (uint32_t s = lane; s < ns; s += 64) M = fmaxf(M, ml[(uint64_t)s * G + h].x);
-        M = gh_wave_max(M);
-        for (uint32_t s = lane; s < ns; s += 64) {
-            const float2 x = ml[(uint64_t)s * G + h];
-            L += share(x.x, M) * x.y;
+namespace {
+// Each row in spans. Grid (kv heads, spans, rows), 256 threads: wave w takes tiles w, w + 4, ... of the span, then
+// the four waves' sums are joined in LDS. A row of one span is finished here, scores included.
+template <bool SCORED>
+__device__ __forceinline__ void paged_split(const GhPagedAttnArgs& a) {
+    extern __shared__ __align__(16) float dyn[];  // per wave and head: 132 floats of acc, then m and l
+    __shared__ float sM[16], sL[16];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, n = lane & 15u, g = lane >> 4, G = a.group;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t kvh = blockIdx.x, split = blockIdx.y, row = blockIdx.z;
+    const uint32_t span = a.least * 16, begin = split * span;  // < max_len
+    // the wave's tile i covers positions begin + 64 i + 16 wave .. + 16
+    const uint32_t first = begin + 16 * wave, mine = first + 64 * lane;
+    uint32_t entry = 0;
+    if (64 * lane + 16 * wave < span && mine < a.max_len)
+        entry = gh_gp<uint32_t>(a.p.table)[(uint64_t)row * a.p.width + (mine >> a.p.shift)];
+    const uint32_t len = row_length(a.p, row, a.max_len, kvh == 0 && split == 0);
+    const uint64_t out = a.out + ((uint64_t)row * a.q_heads + kvh * G) * 256;
+    if (len == 0) {
+        if (split == 0)
+            for (uint32_t i = tid; i < G * 64; i += 256) gh_gpw<uint32_t>(out)[i] = 0u;
+        return;
+    }
+    if (begin >= len) return;
+    ph8 qf[4];
+    load_q(a, row, kvh, qf);
+    const uint32_t end = min(len, begin + span);
+    const bool bad = mine < end && entry >= a.p.pages;
+    if (bad) fault(a.p, GH_PAGED_PAGE);
+    const uint32_t t_count = mine < end && !bad ? min(end - mine, 16u) : 0u;
+    const uint32_t t_slot = bad ? 0u : (entry << a.p.shift) + (mine & ((1u << a.p.shift) - 1));
+    const uint32_t tiles = first < end ? (end - first + 63) / 64 : 0u, row_bytes = a.p.kv_heads * 256;
+    auto where = [&](uint32_t i) __attribute__((always_inline)) {
+        const uint32_t count = i < tiles ? __builtin_amdgcn_readlane(t_count, i & 63u) : 0u;
+        return tile_at(a.p, __builtin_amdgcn_readlane(t_slot, i & 63u), count, kvh);
+    };
+    const uint64_t raw0 = a.raw + ((uint64_t)row * a.p.kv_heads + kvh) * G * a.raw_len * 4;
+    Sums x;
+    x.clear();
+    if (tiles) {
+        Tile r;
+        Where w = where(0);
+        load_k<0>(w, row_bytes, r);
+        load_v<0>(w, row_bytes, r);
+        for (uint32_t i = 0; i < tiles; ++i) {
+            pf4 st = tile_products(r, qf);
+            w = where(i + 1);
+            load_k<0>(w, row_bytes, r);
+            st = tile_scores(st, __builtin_amdgcn_readlane(t_count, i & 63u), a.scale);
+            if (SCORED && n < G)
+                *gh_gpw<float4>(raw0 + ((uint64_t)n * a.raw_len + first + 64 * i + 4 * g) * 4) =
+                    make_float4(st[0], st[1], st[2], st[3]);
+            tile_add(x, st, r);
+            load_v<0>(w, row_bytes, r);
         }
-        L = gh_wave_sum(L);
-        if (lane == 0) {
-            sm[h] = M;
-            sl[h] = L;
+    }
+    // the waves: M = max m_w, L = Σ 2^(m_w - M) l_w, ACC likewise
+    float* wm = dyn + 4 * G * 132;
+    float* wl = wm + 4 * G;
+    const float lt = lanes4_sum(x.l);
+    if (n < G) {
+        const uint32_t at = wave * G + n;
+        if (g == 0) {
+            wm[at] = x.m;
+            wl[at] = lt;
+        }
+        float4* to = (float4*)(dyn + at * 132 + 32 * g);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            to[2 * j] = make_float4(x.acc[0][j], x.acc[1][j], x.acc[2][j], x.acc[3][j]);
+            to[2 * j + 1] = make_float4(x.acc[4][j], x.acc[5][j], x.acc[6][j], x.acc[7][j]);
         }
     }
     __syncthreads();
-    if (!score) {
-        const uint32_t h = h0, grp = tid >> 5, d4 = tid & 31u;
-        const float M = sm[h];
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const GH_GLOBAL float4* acc = gh_gp<float4>(a.part_acc) + (part * G + h) * 32 + d4;
-#pragma unroll 4
-        for (uint32_t s = grp; s < ns; s += 8) {
-            const float e = share(ml[(uint64_t)s * G + h].x, M);
-            const float4 x = acc[(uint64_t)s * G * 32];
-            o.x += e * x.x;
-            o.y += e * x.y;
-            o.z += e * x.z;
-            o.w += e * x.w;
+    const bool whole = len <= span;  // one split: the output itself
+    const uint64_t part = ((uint64_t)row * a.chunks + split) * a.p.kv_heads * G + kvh * G;
+    for (uint32_t i = tid; i < G * 64; i += 256) {
+        const uint32_t h = i >> 6, d = 2 * (i & 63u);
+        float M = -__builtin_inff();
+#pragma unroll
+        for (int w = 0; w < 4; ++w) M = fmaxf(M, wm[w * G + h]);
+        float L = 0.0f;
+        float2 v = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float e = share(wm[w * G + h], M);
+            const float2 y = *(const float2*)(dyn + (w * G + h) * 132 + d);
+            L += e * wl[w * G + h];
+            v.x += e * y.x;
+            v.y += e * y.y;
         }
-        red[grp][d4] = o;
-        __syncthreads();
-        if (tid < 32) {
-            for (uint32_t i = 1; i < 8; ++i) {
-                const float4 x = red[i][tid];
-                o.x += x.x;
-                o.y += x.y;
-                o.z += x.z;
-                o.w += x.w;
+        if (whole) gh_gpw<uint32_t>(out)[i] = (uint32_t)gh_f2h(v.x / L) | (uint32_t)gh_f2h(v.y / L) << 16;
+        else gh_gpw<float2>(a.part_acc)[part * 64 + i] = v;
+        if (d == 0) {
+            sM[h] = M;
+            sL[h] = L;
+            if (!whole) gh_gpw<float2>(a.part_ml)[part + h] = make_float2(M, L);
+        }
+    }
+    if (!SCORED || !whole) return;
+    __syncthreads();
+    add_scores(a, row, kvh, sM, sL, 4 * tid, 1024, len);
+}
+}  // namespace
+GH_KERNEL __launch_bounds__(256) void gh_paged_split(GhPagedAttnArgs a) { paged_split<false>(a); }
+GH_KERNEL __launch_bounds__(256) void gh_paged_split_s(GhPagedAttnArgs a) { paged_split<true>(a); }
+
+// The chunks of a row joined. Grid (q_heads + kv_heads·blocks, rows, 2), 256 threads.
+// x < q_heads: 64 dims of the output of one query head: M = max m_s, out = Σ 2^(m_s - M) acc_s /
+// Σ 2^(m_s - M) l_s; sixteen groups of 16 threads take every sixteenth partial, four dims per thread, each with
+// a running maximum, and add up in group order.
+// Else: the scores of a kv head, every blocks-th 1024 positions: the weight of position j is
+// 2^(s_j - M + 15) / L per query head, summed over the G heads in order and added to the row's score.
+GH_KERNEL __launch_bounds__(256) void gh_paged_join(GhPagedAttnArgs a) {
+    __shared__ float sm[16], sl[16];
+    __shared__ pf4 red[16][16];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, row = blockIdx.y, half = blockIdx.z, G = a.group;
+    const bool score = blockIdx.x >= a.q_heads;
+    if (score && half) return;
+    // the row's first partial and their number
+    uint32_t p0, ns;
+    if (a.layout) {
+        const GH_GLOBAL uint32_t* lay = gh_gp<uint32_t>(a.layout);
+        const uint32_t per = lay[0], t0 = lay[1 + row], t1 = lay[2 + row];
+        if (t0 == t1) return;
+        p0 = t0 / per + row;
+        ns = (t1 - 1) / per - t0 / per + 1;
+        if (!score && ns == 1 && !a.raw) return;  // written by the attention launch
+    } else {
+        const uint32_t len = row_length(a.p, row, a.max_len, false);
+        p0 = row * a.chunks;
+        ns = (len + 16 * a.least - 1) / (16 * a.least);
+        if (ns <= 1) return;  // likewise, with its scores
+    }
+    const uint32_t kvh = score ? (blockIdx.x - a.q_heads) / a.blocks : blockIdx.x / G;
+    const uint32_t step = a.p.kv_heads * G;  // partials of a chunk and row
+    const uint64_t part = (uint64_t)p0 * step + kvh * G;
+    const GH_GLOBAL float2* ml = gh_gp<float2>(a.part_ml) + part;
+    if (!score) {
+        // thread: partials grp, grp + 16, ... , dims 64 half + 4 d4 .. + 4
+        const uint32_t h = blockIdx.x % G, grp = tid >> 4, d4 = 16 * half + (tid & 15u);
+        float M = -__builtin_inff(), L = 0.0f;
+        pf4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+        const GH_GLOBAL pf4* acc = gh_gp<pf4>(a.part_acc) + (part + h) * 32 + d4;
+        for (uint32_t s0 = grp; s0 < ns; s0 += 128) {
+            float2 x[8];
+            pf4 v[8];
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                const uint64_t at = min(s0 + 16 * i, ns - 1) * (uint64_t)step;
+                x[i] = ml[at + h];
+                v[i] = acc[at * 32];
             }
-            const float L = sl[h];
-            gh_gpw<uint2>(a.out)[((uint64_t)row * a.q_heads + blockIdx.x) * 32 + tid] =
+            float top = M;
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) top = fmaxf(top, x[i].x);
+            const float f = share(M, top);
+            M = top;
+            L *= f;
+            o *= f;
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i)
+                if (s0 + 16 * i < ns) {
+                    const float e = share(x[i].x, M);
+                    L += e * x[i].y;
+                    o += e * v[i];
+                }
+        }
+        red[grp][tid & 15u] = o;
+        if ((tid & 15u) == 0) {
+            sm[grp] = M;
+            sl[grp] = L;
+        }
+        __syncthreads();
+        if (tid < 16) {
+            M = sm[0];
+            for (uint32_t i = 1; i < 16; ++i) M = fmaxf(M, sm[i]);
+            L = 0.0f;
+            o = pf4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (uint32_t i = 0; i < 16; ++i) {
+                const float e = share(sm[i], M);
+                L += e * sl[i];
+                o += e * red[i][tid];
+            }
+            gh_gpw<uint2>(a.out)[((uint64_t)row * a.q_heads + blockIdx.x) * 32 + d4] =
                 make_uint2((uint32_t)gh_f2h(o.x / L) | (uint32_t)gh_f2h(o.y / L) << 16,
                            (uint32_t)gh_f2h(o.z / L) | (uint32_t)gh_f2h(o.w / L) << 16);
         }
         return;
     }
-    const uint64_t raw = a.raw + ((uint64_t)row * a.p.kv_heads + kvh) * G * a.raw_len * 4;
-    const uint64_t to = a.p.score + ((uint64_t)row * a.p.kv_heads + kvh) * (a.p.width << a.p.shift) * 4;
-    for (uint32_t c = (blockIdx.x - a.q_heads) % a.chunks; c * 1024 < len; c += a.chunks) {
-        const uint32_t pos = c * 1024 + 4 * tid;
-        if (pos >= len) continue;
-        float4 w = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (uint32_t h = 0; h < G; ++h) {
-            const float4 s = *gh_gp<float4>(raw + ((uint64_t)h * a.raw_len + pos) * 4);
-            const float up = kUp - sm[h], inv = 1.0f / sl[h];
-            w.x += __builtin_amdgcn_exp2f(s.x + up) * inv;
-            w.y += __builtin_amdgcn_exp2f(s.y + up) * inv;
-            w.z += __builtin_amdgcn_exp2f(s.z + up) * inv;
-            w.w += __builtin_amdgcn_exp2f(s.w + up) * inv;
+    for (uint32_t h = wave; h < G; h += 4) {
+        float M = -__builtin_inff(), L = 0.0f;
+        for (uint32_t s = lane; s < ns; s += 64) {
+            const float2 x = ml[(uint64_t)s * step + h];
+            const float top = fmaxf(M, x.x);
+            L = L * share(M, top) + share(x.x, top) * x.y;
+            M = top;
         }
-        // positions past the row keep their bits
-        GH_GLOBAL float* p = gh_gpw<float>(to) + pos;
-        const float v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (uint32_t j = 0; j < 4; ++j)
-            if (pos + j < len) p[j] += v[j];
+        const float top = gh_wave_max(M);
+        L = gh_wave_sum(L * share(M, top));
+        if (lane == 0) {
+            sm[h] = top;
+            sl[h] = L;
+        }
     }
+    __syncthreads();
+    add_scores(a, row, kvh, sm, sl, 1024 * ((blockIdx.x - a.q_heads) % a.blocks) + 4 * tid, 1024 * a.blocks,
+               gh_gp<uint32_t>(a.p.lengths)[row]);
 }
 
 // ---- eviction -----------------------------------------------------------------------------------

@@ -56,5 +56,5 @@ uint64_t host_scratch(void) { return scratch_bytes; }
 uint32_t host_launches(void) { return (uint32_t)launches.size(); }
 const void* host_launch(uint32_t i) { return &launches[i]; }
 // kernel ids: write, the first attention, join, select, move
-void host_kernels(uint32_t* k) { k[0] = K_PAGED_WRITE, k[1] = K_PAGED_ATTN_G4, k[2] = K_PAGED_JOIN, k[3] = K_PAGED_SELECT, k[4] = K_PAGED_MOVE; }
+void host_kernels(uint32_t* k) { k[0] = K_PAGED_WRITE, k[1] = K_PAGED_ATTN, k[2] = K_PAGED_JOIN, k[3] = K_PAGED_SELECT, k[4] = K_PAGED_MOVE; }
 }

@@ -21,9 +21,9 @@ class Pages(C.Structure):
 
 
 class AttnArgs(C.Structure):
-    _fields_ = [("p", Pages)] + [(n, C.c_uint64) for n in ("q", "out", "part_acc", "part_ml", "raw")] + \
-               [(n, C.c_uint32) for n in ("q_heads", "group", "max_len", "span", "splits", "raw_len")] + \
-               [("scale", C.c_float), ("chunks", C.c_uint32)]
+    _fields_ = [("p", Pages)] + [(n, C.c_uint64) for n in ("q", "out", "part_acc", "part_ml", "raw", "stream", "layout")] + \
+               [(n, C.c_uint32) for n in ("q_heads", "group", "rows", "max_len", "chunks", "least", "solo", "raw_len")] + \
+               [("scale", C.c_float), ("blocks", C.c_uint32)]
 
 
 class Launch(C.Structure):
@@ -208,13 +208,13 @@ def test_evict_refusals(host):
     assert host.call(name, dst, src, None, 40, 1, limit=100)[0] == OOM
 
 
-@pytest.mark.parametrize("seed", range(40))
+@pytest.mark.parametrize("seed", range(60))
 def test_attention_plans_stay_within_their_scratch(host, seed):
-    """Splits cover max_len; the regions of the partials, their (m, l) and the scores lie in the scratch and apart;
-    the groups of rows cover all rows once; the grid is one that the device takes."""
+    """The spans or chunks cover the rows; the regions of the partials, their (m, l), the scores and the layout
+    lie in the scratch and apart; the groups of rows cover all rows once; the grid is one that the device takes."""
     rng = random.Random(seed)
     heads, group = rng.choice((1, 2, 3, 8, 64)), rng.randint(1, 16)
-    page, rows = rng.choice((16, 64, 1024)), int(2 ** rng.uniform(0, 9))
+    page, rows = rng.choice((16, 64, 1024)), int(2 ** rng.uniform(0, 11))
     width, scored = max(1, int(2 ** rng.uniform(4, 18)) // page), rng.random() < 0.5
     kv = host.kv(layers=1, slots=page * 4, heads=heads, page=page, width=width, rows=rows, scored=scored)
     q = host.buf(rows * heads * group * 256)
@@ -224,27 +224,36 @@ def test_attention_plans_stay_within_their_scratch(host, seed):
     want, size, at = max_len or width * page, host.lib.host_scratch(), 0
     for g in got:
         a = AttnArgs.from_buffer_copy(bytes(g.args))
-        assert a.max_len == want and a.span % 64 == 0 and 64 <= a.span <= 4096
-        assert a.splits * a.span >= want > (a.splits - 1) * a.span and a.raw_len >= want and a.raw_len % 16 == 0
+        split = a.layout == 0
+        assert a.max_len == want and a.raw_len >= want and a.raw_len % 16 == 0 and a.rows <= 512
         assert g.gy <= 65535 and g.gz <= 65535 and g.gx * g.gy * g.gz < 2 ** 32 and g.block == 256
         row = (a.q - q.addr) // (heads * group * 256)
         assert a.out - q.addr == a.q - q.addr and a.p.table - kv.table.addr == row * width * 4
         assert a.p.lengths - kv.lengths.addr == row * 4
         if scored:
             assert a.p.score - kv.score.addr == row * heads * width * page * 4
-        if g.kernel != host.ids["join"]:
-            assert row == at and g.gx == heads and g.gy == a.splits
-            assert g.kernel - host.ids["attn"] == 2 * (0 if group <= 4 else 1 if group <= 8 else 2) + scored
-            at += g.gz
+        if g.kernel == host.ids["join"]:
+            assert row + a.rows == at and (g.gx, g.gy, g.gz) == (heads * group + heads * a.blocks, a.rows, 2)
         else:
-            assert row + g.gz == at
-        if scored or a.splits > 1:
-            n = g.gz * heads * group
-            regions = [(a.part_acc, n * a.splits * 512), (a.part_ml, n * a.splits * 8)]
-            regions += [(a.raw, n * a.raw_len * 4)] if scored else []
-            regions.sort()
-            assert all(x % 16 == 0 or x == a.part_ml and x % 8 == 0 for x, _ in regions)
-            assert regions[0][0] >= SCRATCH and regions[-1][0] + regions[-1][1] <= SCRATCH + size
-            assert all(x + nx <= y for (x, nx), (y, _) in zip(regions, regions[1:]))
+            assert row == at
+            at += a.rows
+            if split:
+                assert 4 <= a.least <= 32 and a.chunks * a.least * 16 >= want > (a.chunks - 1) * a.least * 16
+                assert g.kernel - host.ids["attn"] == 2 + scored and (g.gx, g.gy, g.gz) == (heads, a.chunks, a.rows)
+            else:
+                most = a.rows * -(-want // 16)
+                assert g.kernel - host.ids["attn"] == scored and most < 2 ** 30
+                # enough waves for every chunk that the rows can fill, whatever their lengths
+                for total in (1, most // 3 + 1, most):
+                    half = -(-2 * total // a.chunks)
+                    per = max(a.least, half if half <= a.solo else -(-total // a.chunks))
+                    assert -(-total // per) * heads <= 4 * g.gx and -(-total // per) <= a.chunks
+        parts = a.chunks * a.rows if split else a.chunks + a.rows
+        regions = [(a.part_acc, parts * heads * group * 512), (a.part_ml, parts * heads * group * 8)]
+        regions += [(a.raw, a.rows * heads * group * a.raw_len * 4)] if scored else []
+        regions += [] if split else [(a.layout, (a.rows + 2) * 4)]
+        regions.sort()
+        assert all(x % 16 == 0 or x == a.part_ml and x % 8 == 0 for x, _ in regions)
+        assert regions[0][0] >= SCRATCH and regions[-1][0] + regions[-1][1] <= SCRATCH + size
+        assert all(x + nx <= y for (x, nx), (y, _) in zip(regions, regions[1:]))
     assert at == rows
-    assert size <= 512 << 20 or got[0].gz == 1
