@@ -137,6 +137,7 @@ enum GhKernel : int {
     K_PAGED_SPLIT,
     K_PAGED_SPLIT_S,
     K_PAGED_JOIN,
+    K_PAGED_JOIN2,  // two workgroups per query head
     K_PAGED_SELECT,
     K_PAGED_MOVE,
     K_COUNT

@@ -115,6 +115,7 @@ int attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv_pag
     const uint32_t hk = kv->kv.kv_heads;
     if (q_heads == 0 || q_heads % hk) return fail(b, GH_E_INVALID, "attention_decode_paged: q_heads not a multiple of kv_heads");
     const uint32_t group = q_heads / hk;
+    if (q_heads > 0xFFFFu) return fail(b, GH_E_UNSUPPORTED, "attention_decode_paged: more than 65535 heads");
     if (group > 16) return fail(b, GH_E_UNSUPPORTED, "attention_decode_paged: at most 16 query heads per kv head");
     const uint64_t bytes = (uint64_t)kv->rows * q_heads * 256;
     if (!fits(q, bytes, 16) || !fits(out, bytes, 16))
@@ -186,7 +187,10 @@ int attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv_pag
             const uint64_t chunks = std::min<uint64_t>(a.chunks, ceil_div((uint64_t)a.rows * tiles1, a.least));
             rc = launch(b, scored ? K_PAGED_ATTN_S : K_PAGED_ATTN, ceil_div(hk * chunks, 4), 1, 1, 256, &a);
         }
-        if (!rc && (!split || a.chunks > 1)) rc = launch(b, K_PAGED_JOIN, q_heads + hk * a.blocks, a.rows, 2, 256, &a);
+        // the halves of the heads apart where a row may have more partials than one round of the join takes (64)
+        const uint32_t halves = a.chunks > 64 * a.rows ? 2 : 1;
+        if (!rc && (!split || a.chunks > 1))
+            rc = launch(b, halves == 2 ? K_PAGED_JOIN2 : K_PAGED_JOIN, q_heads + hk * a.blocks, a.rows, halves, 256, &a);
         if (rc) return rc;
     }
     return GH_OK;

@@ -34,7 +34,8 @@ __device__ __forceinline__ uint32_t slot_of(const GhPages& p, uint32_t row, uint
 // Thread = 8 values (16 bytes) of one head of one token: the token's query heads, then its key and value
 // heads; a.groups workgroups per token. Rotation as in gh_rope: adjacent pairs turned by the (position, pair)
 // table's (cos, sin) in FP32, queries times the post-scale, one rounding. Bound by launch latency at decode
-// sizes and by memory at prompt sizes.
+// sizes (256 tokens of 32 + 8 heads 3.9 us) and by memory at prompt sizes (2000 tokens of 8 heads, 16 MB, 4.6 us);
+// the vector, the row's length and its position are asked for at once.
 namespace {
 __device__ __forceinline__ uint32_t turn(uint32_t v, float2 c, float scale) {
 #pragma clang fp contract(off)
@@ -49,24 +50,20 @@ GH_KERNEL __launch_bounds__(256) void gh_paged_write(GhPagedWriteArgs a) {
     const uint32_t token = blockIdx.x / a.groups, row = token / a.tokens, t = token % a.tokens;
     const uint32_t item = (blockIdx.x % a.groups) * 256 + threadIdx.x;
     const uint32_t head = item >> 4, part = item & 15u;  // 8 dims each
-    const uint32_t n = row_length(a.p, row, a.p.width << a.p.shift, blockIdx.x % a.groups == 0);
-    if (n + t < a.tokens) return;  // a free row, or before its first position
-    const uint32_t at = n - a.tokens + t;
-    uint32_t pos = 0;
-    if (a.positions) {
-        const uint32_t from = gh_gp<uint32_t>(a.positions)[row];
-        if (from > a.max_pos || t > a.max_pos - from) {
-            if (item == 0) fault(a.p, GH_PAGED_POSITION);
-            return;
-        }
-        pos = from + t;
-    }
     if (head >= a.q_heads + 2 * a.p.kv_heads) return;
     const bool query = head < a.q_heads, value = head >= a.q_heads + a.p.kv_heads;
     const uint32_t h = query ? head : head - a.q_heads - (value ? a.p.kv_heads : 0u);
     const uint32_t heads = query ? a.q_heads : a.p.kv_heads;
     const uint64_t in = ((uint64_t)token * heads + h) * 256 + 16 * part;
     uint4 x = *gh_gp<uint4>((query ? a.q : value ? a.v : a.k) + in);
+    const uint32_t from = a.positions ? gh_gp<uint32_t>(a.positions)[row] : 0u;
+    const uint32_t n = row_length(a.p, row, a.p.width << a.p.shift, blockIdx.x % a.groups == 0);
+    if (n + t < a.tokens) return;  // a free row, or before its first position
+    const uint32_t at = n - a.tokens + t, pos = from + t;
+    if (a.positions && (from > a.max_pos || t > a.max_pos - from)) {
+        if (item == 0) fault(a.p, GH_PAGED_POSITION);
+        return;
+    }
     if (a.positions && !value && 4 * part < a.pairs) {
         const float scale = query ? gh_gp<float>(a.post)[pos] : 1.0f;
         const GH_GLOBAL float2* cs = gh_gp<float2>(a.table) + (uint64_t)pos * a.pairs + 4 * part;
@@ -242,22 +239,32 @@ __device__ __forceinline__ void tile_add(Sums& x, pf4 st, const Tile& r) {
     }
 }
 
-// Adds the weights of positions from, from + step, ... (four each) to the scores of a row and kv head: 2^(s - M + 15) / L
-// per query head, summed over the G heads in order. Positions past the row keep their bits.
-__device__ __forceinline__ void add_scores(const GhPagedAttnArgs& a, uint32_t row, uint32_t kvh, const float* M, const float* L,
-                                           uint32_t from, uint32_t step, uint32_t len) {
+// The scores of four query heads h0 .. h0 + 3 (the last of G again past G) at positions pos .. pos + 3.
+__device__ __forceinline__ void load_raw(const GhPagedAttnArgs& a, uint32_t row, uint32_t kvh, uint32_t h0, uint32_t pos, pf4 (&s)[4]) {
     const uint64_t raw = a.raw + ((uint64_t)row * a.p.kv_heads + kvh) * a.group * a.raw_len * 4;
-    const uint64_t to = a.p.score + ((uint64_t)row * a.p.kv_heads + kvh) * (a.p.width << a.p.shift) * 4;
-    for (uint32_t pos = from; pos < len; pos += step) {
-        pf4 w = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (uint32_t h = 0; h < a.group; ++h) {
-            const pf4 s = *gh_gp<pf4>(raw + ((uint64_t)h * a.raw_len + pos) * 4);
-            const float up = kUp - M[h], inv = 1.0f / L[h];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] += __builtin_amdgcn_exp2f(s[j] + up) * inv;
-        }
+    for (uint32_t i = 0; i < 4; ++i) s[i] = *gh_gp<pf4>(raw + ((uint64_t)min(h0 + i, a.group - 1) * a.raw_len + pos) * 4);
+}
+// Adds the weights of positions pos .. + 3, pos + step .. + 3, ... < len to the scores of a row and kv head:
+// 2^(s - M + 15) / L per query head, summed over the G heads in order. s: load_raw of the first four heads
+// at the first position, where that is below len. Positions past the row keep their bits.
+__device__ __forceinline__ void add_scores(const GhPagedAttnArgs& a, uint32_t row, uint32_t kvh, const float* M, const float* L,
+                                           uint32_t pos, uint32_t step, uint32_t len, pf4 (&s)[4]) {
+    const uint64_t to = a.p.score + ((uint64_t)row * a.p.kv_heads + kvh) * (a.p.width << a.p.shift) * 4;
+    for (bool first = true; pos < len; pos += step, first = false) {
         GH_GLOBAL pf4* p = (GH_GLOBAL pf4*)gh_gpw<float>(to + (uint64_t)pos * 4);
         const pf4 old = *p;
+        pf4 w = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t h0 = 0; h0 < a.group; h0 += 4) {
+            if (h0 || !first) load_raw(a, row, kvh, h0, pos, s);
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i)
+                if (h0 + i < a.group) {
+                    const float up = kUp - M[h0 + i], inv = 1.0f / L[h0 + i];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) w[j] += __builtin_amdgcn_exp2f(s[i][j] + up) * inv;
+                }
+        }
         if (pos + 4 <= len) {
             *p = old + w;
         } else {
@@ -547,24 +554,34 @@ __device__ __forceinline__ void paged_split(const GhPagedAttnArgs& a) {
     }
     if (!SCORED || !whole) return;
     __syncthreads();
-    add_scores(a, row, kvh, sM, sL, 4 * tid, 1024, len);
+    pf4 s[4];
+    if (4 * tid < len) load_raw(a, row, kvh, 0, 4 * tid, s);
+    add_scores(a, row, kvh, sM, sL, 4 * tid, 1024, len, s);
 }
 }  // namespace
 GH_KERNEL __launch_bounds__(256) void gh_paged_split(GhPagedAttnArgs a) { paged_split<false>(a); }
 GH_KERNEL __launch_bounds__(256) void gh_paged_split_s(GhPagedAttnArgs a) { paged_split<true>(a); }
 
-// The chunks of a row joined. Grid (q_heads + kv_heads·blocks, rows, 2), 256 threads.
-// x < q_heads: 64 dims of the output of one query head: M = max m_s, out = Σ 2^(m_s - M) acc_s /
-// Σ 2^(m_s - M) l_s; sixteen groups of 16 threads take every sixteenth partial, four dims per thread, each with
-// a running maximum, and add up in group order.
-// Else: the scores of a kv head, every blocks-th 1024 positions: the weight of position j is
-// 2^(s_j - M + 15) / L per query head, summed over the G heads in order and added to the row's score.
-GH_KERNEL __launch_bounds__(256) void gh_paged_join(GhPagedAttnArgs a) {
+// The parts of a row joined. Grid (q_heads + kv_heads·blocks, rows, HALVES), 256 threads.
+// x < q_heads: 128 / HALVES dims of the output of one query head: M = max m_s, out = Σ 2^(m_s - M) acc_s /
+// Σ 2^(m_s - M) l_s; 8·HALVES groups of threads take every so many-th partial, four dims per thread, each with a
+// running maximum, and add up in group order. Bound by its chain of loads; two halves where few rows have many
+// partials each (1 row of 32768, 256 partials: 7.6 us with one, 5.9 with two), one where many rows have few.
+// Else: the scores of a kv head, every blocks-th 1024 positions (add_scores).
+namespace {
+template <uint32_t HALVES>
+__device__ __forceinline__ void paged_join(const GhPagedAttnArgs& a) {
+    constexpr uint32_t kGroups = 8 * HALVES, kLanes = 32 / HALVES;
     __shared__ float sm[16], sl[16];
-    __shared__ pf4 red[16][16];
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, row = blockIdx.y, half = blockIdx.z, G = a.group;
+    __shared__ pf4 red[kGroups][kLanes];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, row = blockIdx.y, G = a.group;
     const bool score = blockIdx.x >= a.q_heads;
-    if (score && half) return;
+    if (score && blockIdx.z) return;
+    const uint32_t len = row_length(a.p, row, a.max_len, false);
+    const uint32_t kvh = score ? (blockIdx.x - a.q_heads) / a.blocks : blockIdx.x / G;
+    const uint32_t pos = score ? 1024 * ((blockIdx.x - a.q_heads) % a.blocks) + 4 * tid : 0u;
+    pf4 raw[4];
+    if (score && pos < len) load_raw(a, row, kvh, 0, pos, raw);  // on their way while M and L are found
     // the row's first partial and their number
     uint32_t p0, ns;
     if (a.layout) {
@@ -575,57 +592,62 @@ GH_KERNEL __launch_bounds__(256) void gh_paged_join(GhPagedAttnArgs a) {
         ns = (t1 - 1) / per - t0 / per + 1;
         if (!score && ns == 1 && !a.raw) return;  // written by the attention launch
     } else {
-        const uint32_t len = row_length(a.p, row, a.max_len, false);
         p0 = row * a.chunks;
         ns = (len + 16 * a.least - 1) / (16 * a.least);
         if (ns <= 1) return;  // likewise, with its scores
     }
-    const uint32_t kvh = score ? (blockIdx.x - a.q_heads) / a.blocks : blockIdx.x / G;
-    const uint32_t step = a.p.kv_heads * G;  // partials of a chunk and row
+    const uint32_t step = a.p.kv_heads * G;  // partials of a chunk or span
     const uint64_t part = (uint64_t)p0 * step + kvh * G;
-    const GH_GLOBAL float2* ml = gh_gp<float2>(a.part_ml) + part;
     if (!score) {
-        // thread: partials grp, grp + 16, ... , dims 64 half + 4 d4 .. + 4
-        const uint32_t h = blockIdx.x % G, grp = tid >> 4, d4 = 16 * half + (tid & 15u);
+        // what is asked past the row's last partial is not read (at most 2048 + 65535 partials of 512 bytes)
+        const uint32_t h = blockIdx.x % G, grp = tid / kLanes, d4 = kLanes * blockIdx.z + tid % kLanes;
+        const uint32_t most = (ns - 1) * step + 1;
+        const __amdgpu_buffer_rsrc_t ra =
+            __builtin_amdgcn_make_buffer_rsrc((void*)(a.part_acc + (part + h) * 512), 0, (int)(most * 512), kBufWord3);
+        const __amdgpu_buffer_rsrc_t rm =
+            __builtin_amdgcn_make_buffer_rsrc((void*)(a.part_ml + (part + h) * 8), 0, (int)(most * 8), kBufWord3);
         float M = -__builtin_inff(), L = 0.0f;
         pf4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-        const GH_GLOBAL pf4* acc = gh_gp<pf4>(a.part_acc) + (part + h) * 32 + d4;
-        for (uint32_t s0 = grp; s0 < ns; s0 += 128) {
+        for (uint32_t s0 = grp; s0 < ns; s0 += 8 * kGroups) {
             float2 x[8];
             pf4 v[8];
 #pragma unroll
             for (uint32_t i = 0; i < 8; ++i) {
-                const uint64_t at = min(s0 + 16 * i, ns - 1) * (uint64_t)step;
-                x[i] = ml[at + h];
-                v[i] = acc[at * 32];
+                const uint32_t at = (s0 + kGroups * i) * step;
+                x[i] = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(rm, at * 8, 0, 0));
+                v[i] = __builtin_bit_cast(pf4, __builtin_amdgcn_raw_buffer_load_b128(ra, at * 512 + 16 * d4, 0, 0));
             }
             float top = M;
 #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) top = fmaxf(top, x[i].x);
+            for (uint32_t i = 0; i < 8; ++i) {
+                if (s0 + kGroups * i >= ns) x[i].x = -__builtin_inff();
+                top = fmaxf(top, x[i].x);
+            }
             const float f = share(M, top);
             M = top;
             L *= f;
             o *= f;
 #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i)
-                if (s0 + 16 * i < ns) {
-                    const float e = share(x[i].x, M);
-                    L += e * x[i].y;
-                    o += e * v[i];
-                }
+            for (uint32_t i = 0; i < 8; ++i) {
+                const float e = share(x[i].x, M);
+                L += e * x[i].y;
+                o += e * v[i];
+            }
         }
-        red[grp][tid & 15u] = o;
-        if ((tid & 15u) == 0) {
+        red[grp][tid % kLanes] = o;
+        if (tid % kLanes == 0) {
             sm[grp] = M;
             sl[grp] = L;
         }
         __syncthreads();
-        if (tid < 16) {
+        if (tid < kLanes) {
             M = sm[0];
-            for (uint32_t i = 1; i < 16; ++i) M = fmaxf(M, sm[i]);
+#pragma unroll
+            for (uint32_t i = 1; i < kGroups; ++i) M = fmaxf(M, sm[i]);
             L = 0.0f;
             o = pf4{0.0f, 0.0f, 0.0f, 0.0f};
-            for (uint32_t i = 0; i < 16; ++i) {
+#pragma unroll
+            for (uint32_t i = 0; i < kGroups; ++i) {
                 const float e = share(sm[i], M);
                 L += e * sl[i];
                 o += e * red[i][tid];
@@ -636,6 +658,7 @@ GH_KERNEL __launch_bounds__(256) void gh_paged_join(GhPagedAttnArgs a) {
         }
         return;
     }
+    const GH_GLOBAL float2* ml = gh_gp<float2>(a.part_ml) + part;
     for (uint32_t h = wave; h < G; h += 4) {
         float M = -__builtin_inff(), L = 0.0f;
         for (uint32_t s = lane; s < ns; s += 64) {
@@ -652,9 +675,11 @@ GH_KERNEL __launch_bounds__(256) void gh_paged_join(GhPagedAttnArgs a) {
         }
     }
     __syncthreads();
-    add_scores(a, row, kvh, sm, sl, 1024 * ((blockIdx.x - a.q_heads) % a.blocks) + 4 * tid, 1024 * a.blocks,
-               gh_gp<uint32_t>(a.p.lengths)[row]);
+    add_scores(a, row, kvh, sm, sl, pos, 1024 * a.blocks, len, raw);
 }
+}  // namespace
+GH_KERNEL __launch_bounds__(256) void gh_paged_join(GhPagedAttnArgs a) { paged_join<1>(a); }
+GH_KERNEL __launch_bounds__(256) void gh_paged_join2(GhPagedAttnArgs a) { paged_join<2>(a); }
 
 // ---- eviction -----------------------------------------------------------------------------------
 // Two launches. gh_paged_select, grid (kv heads, rows, layers), 512 threads: the budget - recent largest

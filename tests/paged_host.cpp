@@ -55,6 +55,6 @@ void host_reset(gh_backend* b, uint64_t limit) { launches.clear(), scratch_bytes
 uint64_t host_scratch(void) { return scratch_bytes; }
 uint32_t host_launches(void) { return (uint32_t)launches.size(); }
 const void* host_launch(uint32_t i) { return &launches[i]; }
-// kernel ids: write, the first attention, join, select, move
-void host_kernels(uint32_t* k) { k[0] = K_PAGED_WRITE, k[1] = K_PAGED_ATTN, k[2] = K_PAGED_JOIN, k[3] = K_PAGED_SELECT, k[4] = K_PAGED_MOVE; }
+// kernel ids: write, the first attention, join, select, move, join in halves
+void host_kernels(uint32_t* k) { k[0] = K_PAGED_WRITE, k[1] = K_PAGED_ATTN, k[2] = K_PAGED_JOIN, k[3] = K_PAGED_SELECT, k[4] = K_PAGED_MOVE, k[5] = K_PAGED_JOIN2; }
 }

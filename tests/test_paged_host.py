@@ -52,9 +52,9 @@ class Host:
         self.lib, self.b = lib, lib.host_backend(cus)
         self.enc = lib.host_encoder(self.b)
         self.at = 1 << 40
-        ids = (C.c_uint32 * 5)()
+        ids = (C.c_uint32 * 6)()
         lib.host_kernels(ids)
-        self.ids = dict(zip(("write", "attn", "join", "select", "move"), ids))
+        self.ids = dict(zip(("write", "attn", "join", "select", "move", "join2"), ids))
 
     def buf(self, nbytes, off=0):
         b = F.GhBuf(self.at + off, nbytes, 0, F.BUF_ALLOC, 0, 0)
@@ -232,8 +232,9 @@ def test_attention_plans_stay_within_their_scratch(host, seed):
         assert a.p.lengths - kv.lengths.addr == row * 4
         if scored:
             assert a.p.score - kv.score.addr == row * heads * width * page * 4
-        if g.kernel == host.ids["join"]:
-            assert row + a.rows == at and (g.gx, g.gy, g.gz) == (heads * group + heads * a.blocks, a.rows, 2)
+        if g.kernel in (host.ids["join"], host.ids["join2"]):
+            assert row + a.rows == at
+            assert (g.gx, g.gy, g.gz) == (heads * group + heads * a.blocks, a.rows, 1 + (g.kernel == host.ids["join2"]))
         else:
             assert row == at
             at += a.rows
