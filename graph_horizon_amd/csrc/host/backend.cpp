@@ -5,7 +5,6 @@
 #include <hip/hip_runtime_api.h>
 
 #include <algorithm>
-#include <chrono>
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
@@ -855,7 +854,7 @@ int gh_create(const gh_config* cfg, gh_backend** out) {
     if (!rc) rc = ensure_workspace(b, 0);
     if (!rc) rc = hip_check(b, hipHostMalloc((void**)&b->result, kResultBytes, hipHostMallocDefault), "hipHostMalloc");
     if (!rc) rc = hip_check(b, hipHostMalloc((void**)&b->paged_fault, 64, hipHostMallocDefault), "hipHostMalloc");
-    if (!rc) b->paged_fault[0] = b->paged_fault[1] = 0;
+    if (!rc) *b->paged_fault = 0;
     if (!rc) rc = noalloc_init(b);
     if (!rc) {
         b->xcds = probe_xcds(b);
@@ -1021,33 +1020,11 @@ int gh_begin(gh_backend* b, gh_encoder** enc) {
     return GH_OK;
 }
 
-// Waits for the stream by a word in pinned host memory that a last launch writes: 2.7 us sooner than
-// hipStreamSynchronize wakes up (8.5 / 11.2 us for a launch and the wait), which counts for the few
-// microseconds of a token's append or attention. What takes longer than kSpin, or fails, is left to
-// hipStreamSynchronize.
-static int wait_by_word(gh_backend* b) {
-    constexpr auto kSpin = std::chrono::milliseconds(2);
-    volatile uint32_t* word = b->paged_fault + 1;
-    const uint32_t next = *word + 1;
-    GhEltArgs e{(uint64_t)word, 0, 0, 1, next};
-    if (launch(b, K_FILL_U32, 1, 1, 1, 64, &e) == GH_OK) {
-        const auto end = std::chrono::steady_clock::now() + kSpin;
-        do {
-            for (int i = 0; i < 64; ++i) {
-                if (*word == next) return GH_OK;
-                __builtin_ia32_pause();
-            }
-        } while (std::chrono::steady_clock::now() < end);
-    }
-    return hip_check(b, hipStreamSynchronize(b->stream), "submit");
-}
-
 int gh_submit(gh_backend* b, gh_encoder* enc) {
     int rc = check_enc(b, enc);
     if (rc) return rc;
     b->enc_open = false;
-    rc = b->paged_used ? wait_by_word(b) : hip_check(b, hipStreamSynchronize(b->stream), "submit");
-    b->paged_used = false;
+    rc = hip_check(b, hipStreamSynchronize(b->stream), "submit");
     if (const uint32_t what = *b->paged_fault) {
         *b->paged_fault = 0;
         if (enc->latched == GH_OK)

@@ -176,7 +176,6 @@ struct gh_backend {
     uint32_t* result = nullptr;  // pinned host memory that the read-back kernels write
     // pinned host word in which the paged kernels leave what they found wrong (GH_PAGED_*), 0: nothing
     volatile uint32_t* paged_fault = nullptr;
-    bool paged_used = false;  // the open encoder holds a paged operator
     size_t ws_bytes = 0;
     void* counters = nullptr;  // attention merge counters, zero between launches
     size_t counter_slots = 0;

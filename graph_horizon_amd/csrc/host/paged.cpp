@@ -91,7 +91,6 @@ int entry(gh_backend* b, gh_encoder* enc, F body) {
     } catch (...) {
         rc = GH_E_INVALID;
     }
-    if (!rc) b->paged_used = true;
     return latch(enc, rc);
 }
 
