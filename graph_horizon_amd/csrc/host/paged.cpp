@@ -105,7 +105,7 @@ int write(gh_backend* b, const gh_kv_paged* kv, const gh_buf* k, const gh_buf* v
     a.v = v->addr;
     a.tokens = tokens;
     a.groups = ceil_div((uint64_t)(a.q_heads + 2 * kv->kv.kv_heads) * 16, 256);
-    if (n * a.groups > 0x7FFFFFFFull) return fail(b, GH_E_RANGE, std::string(what) + ": too many vectors");
+    if (n * a.groups > 0xFFFFFFull) return fail(b, GH_E_RANGE, std::string(what) + ": too many vectors");
     return launch(b, K_PAGED_WRITE, (uint32_t)(n * a.groups), 1, 1, 256, &a);
 }
 
@@ -203,6 +203,7 @@ int evict(gh_backend* b, const gh_kv_paged* dst, const gh_kv_paged* src, const g
     if (!src->score.addr || !dst->score.addr) return fail(b, GH_E_INVALID, "kv_evict_paged: no scores kept");
     if (budget == 0 || recent > budget) return fail(b, GH_E_INVALID, "kv_evict_paged: recent > budget, or budget 0");
     if (budget > capacity(dst)) return fail(b, GH_E_RANGE, "kv_evict_paged: budget beyond dst's table");
+    if (budget > (1u << 27)) return fail(b, GH_E_UNSUPPORTED, "kv_evict_paged: budget beyond 2^27");
     if (s.block_count > 0xFFFFu) return fail(b, GH_E_UNSUPPORTED, "kv_evict_paged: more than 65535 layers");
     const bool same = dst->score.addr == src->score.addr;
     if (same ? dst->table_width != src->table_width : overlap(dst->score, src->score))

@@ -1,9 +1,11 @@
 """The operators over paged caches (gh_*_paged): append with RoPE, decode attention with and without the
 accumulation of weights, eviction, and a run of all of them, against 64-bit definitions (tests/paged.py)."""
+import threading
+
 import numpy as np
 import pytest
 
-from graph_horizon_amd import GhError, GhKvPaged, HipBackend, Yarn
+from graph_horizon_amd import GhError, GhKvPaged, HipBackend, HipModel, Yarn, synth
 from graph_horizon_amd import _ffi as F
 from paged import D, Paged, attend, check_attention, keep, pages_of
 
@@ -399,7 +401,101 @@ def test_bad_device_data_is_an_error_of_its_row(hip, rng):
     dst.free()
 
 
+def test_longer_rows_than_the_call_says(hip, rng):
+    """A row past max_len is an error of that row; the others and what lies behind the last row are as ever."""
+    p = Paged(hip, rng, [40, 300, 33], 16, 2, scored=True)
+    q = rng.standard_normal((3, 8, D)).astype(np.float16)
+    qb, ob = hip.from_host(q), hip.from_host(np.full((4, 8, D), 7, np.float16))
+    before = p.read("score")
+    with pytest.raises(GhError) as e:
+        hip.attention_decode_paged(ob, qb, p.handle(), 8, 299, 0)
+    assert e.value.code == -5
+    out, after = hip.download(ob, np.float16, 4 * 8 * D).reshape(4, 8, D), p.read("score")
+    for r in (0, 2):
+        s = p.cells(r, int(p.lengths[r]))
+        want, _, bound, _ = attend(q[r, 4:], p.k[0, s, 1], p.v[0, s, 1])
+        assert np.all(np.abs(out[r, 4:] - want) <= bound)
+    assert np.all(out[3] == 7) and np.array_equal(after[0, 1], before[0, 1])
+    for b in (qb, ob):
+        hip.free_buffer(b)
+    p.free()
+
+
+def test_what_lies_behind_the_last_row_stays(hip, rng):
+    """Buffers with room for one more row: no operator writes there."""
+    p, heads, group = Paged(hip, rng, [30, 0, 65], 16, 2, scored=True), 2, 4
+    q = rng.standard_normal((4, heads * group, D)).astype(np.float16)
+    k = rng.standard_normal((3, heads, D)).astype(np.float16)
+    qb, kb, pb = hip.from_host(q), hip.from_host(k), hip.from_host(np.array([3, 4, 5], np.uint32))
+    mark = np.full((4, heads * group, D), 7, np.float16)
+    ob, rb = hip.from_host(mark), hip.from_host(mark)
+    hip.rope_kv_write_paged(p.handle(), rb, qb, kb, kb, heads * group, pb, 1, 5, YARN, 0)
+    hip.attention_decode_paged(ob, rb, p.handle(), heads * group, 0, 0)
+    for b in (ob, rb):
+        assert np.all(hip.download(b, np.float16, mark.size).reshape(mark.shape)[3] == 7)
+    dst = Paged(hip, rng, [20, 0, 20], 16, 2, scored=True)
+    kept = hip.from_host(np.full((4, 2, 20), 99, np.uint32))
+    lengths = hip.from_host(np.full(4, 99, np.uint32))
+    h = dst.handle()
+    h.lengths = lengths
+    hip.kv_evict_paged(h, p.handle(), kept, 20, 5)
+    got = hip.download(kept, np.uint32, 160).reshape(4, 2, 20)
+    assert np.all(got[[1, 3]] == 99) and not np.any(got[[0, 2]] == 99)
+    assert list(hip.download(lengths, np.uint32, 4)) == [20, 99, 20, 99]
+    for b in (qb, kb, pb, ob, rb, kept, lengths):
+        hip.free_buffer(b)
+    p.free()
+    dst.free()
+
+
 # ---- together ----
+
+def test_two_backends_at_once(rng):
+    """Two backends (a stream and scratch each) in two threads over one pool."""
+    with HipBackend(0) as a, HipBackend(0) as b:
+        p = Paged(a, rng, [5000, 0, 77, 3000], 16, 4)
+        q = [rng.standard_normal((4, 16, D)).astype(np.float16) for _ in range(2)]
+        got = [[], []]
+
+        def work(i, hip):
+            qb, ob = hip.from_host(q[i]), hip.alloc_buffer(q[i].nbytes)
+            for _ in range(20):
+                hip.attention_decode_paged(ob, qb, p.handle(), 16, 0, 0)
+                got[i].append(hip.download(ob, np.float16, q[i].size).reshape(q[i].shape))
+            hip.free_buffer(qb)
+            hip.free_buffer(ob)
+
+        threads = [threading.Thread(target=work, args=(i, hip)) for i, hip in enumerate((a, b))]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        for i in range(2):
+            assert len(got[i]) == 20
+            check_attention(p, 0, q[i], got[i][0])
+            assert all(np.array_equal(x.view(np.uint16), got[i][0].view(np.uint16)) for x in got[i])
+        p.free()
+
+
+def test_recorded_decode_graphs_survive_the_scratch_of_paged_attention(rng):
+    """Paged attention that moves the backend's workspace between two runs of a model's replayed decode."""
+    shape = synth.SHAPES["tiny"]
+    with HipBackend(0) as hip:
+        m = HipModel(hip, synth.model_config(shape, 64, 16))
+        for layer, tid, fmt, data in synth.model_tensors(shape, 1):
+            m.load_tensor(layer, tid, fmt, data)
+        m.prefill(np.arange(8), 0)
+        first = m.decode_greedy(3, 8, 12)
+        before = hip.scratch_info()[0]
+        p = Paged(hip, rng, [9000] * 6, 64, 2, scored=True)
+        old = p.read("score")
+        q, out = run_attention(hip, p, 16, rng)
+        check_attention(p, 0, q, out, old, p.read("score"))
+        assert hip.scratch_info()[0] > before
+        assert np.array_equal(m.decode_greedy(3, 8, 12), first)
+        p.free()
+        m.close()
+
 
 def test_serving_run(hip, rng):
     """Prompts go into pages, then steps of append and attention over two layers in one encoder each, an

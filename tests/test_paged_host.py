@@ -179,6 +179,8 @@ def test_attention_refusals(host):
                          ((shorter(o), q, kv, 8, 0, 0), RANGE), ((o, shift_buf(q, 4), kv, 8, 0, 0), RANGE),
                          ((None, q, kv, 8, 0, 0), RANGE)):
         assert host.call(name, *args)[0] == status, args
+    wide = host.kv(heads=9000, slots=16, layers=1, rows=1)
+    assert host.call(name, q, q, wide, 72000, 0, 0)[0] == UNSUPPORTED
     assert host.call(name, o, q, kv, 8, 0, 0, limit=1000)[0] == OOM
 
 
