@@ -89,7 +89,7 @@ const KernelName kKernels[] = {
     {K_PAGED_ATTN, "gh_paged_attn"}, {K_PAGED_ATTN_S, "gh_paged_attn_s"},
     {K_PAGED_SPLIT, "gh_paged_split"}, {K_PAGED_SPLIT_S, "gh_paged_split_s"},
     {K_PAGED_JOIN, "gh_paged_join"}, {K_PAGED_JOIN2, "gh_paged_join2"},
-    {K_PAGED_SELECT, "gh_paged_select"}, {K_PAGED_MOVE, "gh_paged_move"},
+    {K_PAGED_SELECT, "gh_paged_select"}, {K_PAGED_MOVE, "gh_paged_move"}, {K_PAGED_MOVE_S, "gh_paged_move_s"},
 };
 
 const char* kModules[] = {"gh_quant", "gh_gemv", "gh_glue", "gh_attention", "gh_gemm", "gh_gemm_few", "gh_paged"};

@@ -140,6 +140,7 @@ enum GhKernel : int {
     K_PAGED_JOIN2,  // two workgroups per query head
     K_PAGED_SELECT,
     K_PAGED_MOVE,
+    K_PAGED_MOVE_S,  // reads past the caches
     K_COUNT
 };
 

@@ -19,6 +19,7 @@ bool fits(const gh_buf* buf, uint64_t bytes, uint64_t align) {
 bool overlap(const gh_buf& a, const gh_buf& b) { return a.addr < b.addr + b.bytes && b.addr < a.addr + a.bytes; }
 
 constexpr uint32_t kPagedRows = 512;  // rows that one attention launch lays out
+constexpr uint64_t kStreamBytes = 128ull << 20;  // half the last-level cache
 constexpr uint32_t kSpanTiles = 32;   // tiles of a gh_paged_split workgroup at most (its waves hold 64 each)
 
 uint64_t capacity(const gh_kv_paged* kv) { return (uint64_t)kv->table_width * kv->page_size; }
@@ -156,7 +157,7 @@ int attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv_pag
     }
     // From half the last-level cache on, the next call will not find this one's K and V there, and reads past
     // it are faster (64 rows of 8192 368 / 346 us, 1 of 32768 36.0 / 34.0; 16 of up to 2500, 83 MB: 31.2 / 37.7).
-    a.stream = 128ull << 20;
+    a.stream = kStreamBytes;
     // scratch of a row: its partials, and with scores each query head's
     const uint64_t acc = (uint64_t)q_heads * 512, ml = acc / 64, raw = scored ? (uint64_t)q_heads * a.raw_len * 4 : 0;
     // rows in groups that the kernel lays out at once and whose scratch fits 512 MiB
@@ -227,7 +228,8 @@ int evict(gh_backend* b, const gh_kv_paged* dst, const gh_kv_paged* src, const g
     a.act = (uint64_t)ws;
     a.kept = kept ? kept->addr : (uint64_t)ws + (uint64_t)src->rows * 4;
     rc = launch(b, K_PAGED_SELECT, s.kv_heads, src->rows, s.block_count, 512, &a);
-    if (!rc) rc = launch(b, K_PAGED_MOVE, ceil_div(budget, 16), src->rows, s.block_count, 256, &a);
+    const bool stream = list * budget * 512 >= kStreamBytes;
+    if (!rc) rc = launch(b, stream ? K_PAGED_MOVE_S : K_PAGED_MOVE, ceil_div(budget, 16), src->rows, s.block_count, 256, &a);
     return rc;
 }
 

@@ -836,7 +836,9 @@ GH_KERNEL __launch_bounds__(512) void gh_paged_select(GhPagedEvictArgs a) {
     else select_kept<false>(a, n, from, to, kept);
 }
 
-GH_KERNEL __launch_bounds__(256) void gh_paged_move(GhPagedEvictArgs a) {
+namespace {
+template <bool STREAM>
+__device__ __forceinline__ void paged_move(const GhPagedEvictArgs& a) {
     const uint32_t row = blockIdx.y, layer = blockIdx.z, tid = threadIdx.x;
     if (!gh_gp<uint32_t>(a.act)[row]) return;
     if (blockIdx.x == 0 && layer == 0 && tid == 0) gh_gpw<uint32_t>(a.dst.lengths)[row] = a.budget;
@@ -851,11 +853,16 @@ GH_KERNEL __launch_bounds__(256) void gh_paged_move(GhPagedEvictArgs a) {
         if (s == kBad || d == kBad) continue;
         const uint64_t in = layer * a.src_layer + ((uint64_t)s * heads + h) * 256 + part;
         const uint64_t to = layer * a.dst_layer + ((uint64_t)d * heads + h) * 256 + part;
-        // stored past the caches: a second pass over what is moved is far off (34 layers of 2048 slots 131.9 ->
-        // 124.6 us with the selection; loads too: 122.5, but 17.5 -> 22.5 where the source is still in cache)
+        // stored past the caches, as what is moved is not wanted again soon, and where much is moved (the host's
+        // rule) read past them too: 34 layers of 2048 slots 131.9, 124.6 and 122.5 us with the selection; 2 layers
+        // of 4 rows of 560, whose source is still in cache, 18.1, 17.5 and 22.5
         typedef uint32_t u4v __attribute__((ext_vector_type(4)));
-        const u4v k = *gh_gp<u4v>(a.src.kc + in), v = *gh_gp<u4v>(a.src.vc + in);
+        const GH_GLOBAL u4v *kp = gh_gp<u4v>(a.src.kc + in), *vp = gh_gp<u4v>(a.src.vc + in);
+        const u4v k = STREAM ? __builtin_nontemporal_load(kp) : *kp, v = STREAM ? __builtin_nontemporal_load(vp) : *vp;
         __builtin_nontemporal_store(k, gh_gpw<u4v>(a.dst.kc + to));
         __builtin_nontemporal_store(v, gh_gpw<u4v>(a.dst.vc + to));
     }
 }
+}  // namespace
+GH_KERNEL __launch_bounds__(256) void gh_paged_move(GhPagedEvictArgs a) { paged_move<false>(a); }
+GH_KERNEL __launch_bounds__(256) void gh_paged_move_s(GhPagedEvictArgs a) { paged_move<true>(a); }

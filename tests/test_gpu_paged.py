@@ -50,6 +50,16 @@ def test_attention(hip, rng, name, page, heads, group, scored):
     p.free()
 
 
+@pytest.mark.parametrize("scored", [False, True])
+def test_attention_past_the_cache(hip, rng, scored):
+    """128 MiB of K and V, from which they are read with another cache policy."""
+    p = Paged(hip, rng, [20000, 13000, 17], 64, 8, scored=scored)
+    before = p.read("score") if scored else None
+    q, out = run_attention(hip, p, 32, rng)
+    check_attention(p, 0, q, out, before, p.read("score") if scored else None)
+    p.free()
+
+
 @pytest.mark.parametrize("max_len", [300, 320, 1000, 4096])
 @pytest.mark.parametrize("group", [2, 4])
 def test_attention_launch_longer_than_rows(hip, rng, max_len, group):
@@ -307,6 +317,7 @@ def evict_case(hip, rng, lengths, page, heads, layers, budget, recent, score=Non
     ([2], 16, 1, 1, 1, 0), ([2], 16, 1, 1, 1, 1), ([17, 16, 0, 40], 16, 2, 2, 16, 3), ([600, 601, 64], 32, 8, 3, 560, 64),
     ([5000, 4097, 2049], 64, 2, 2, 2048, 256), ([300], 128, 3, 1, 299, 0), ([300], 16, 3, 1, 200, 200),
     ([20001], 256, 1, 1, 7001, 1), ([100, 50], 16, 5, 2, 200, 10),
+    ([8300], 64, 8, 4, 8200, 100),  # 128 MiB are moved
 ])
 @pytest.mark.parametrize("alias", [False, True])
 def test_evict(hip, rng, lengths, page, heads, layers, budget, recent, alias):
