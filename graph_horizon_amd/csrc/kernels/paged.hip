@@ -132,6 +132,12 @@ __device__ __forceinline__ float share(float m, float M) {
     return m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - M);
 }
 
+// two outputs as FP16: sums times 1 / Σ weights (one division, where a quotient each takes ten instructions; two
+// FP32 roundings before the one to FP16)
+__device__ __forceinline__ uint32_t out2(float x, float y, float inv) {
+    return (uint32_t)gh_f2h(x * inv) | (uint32_t)gh_f2h(y * inv) << 16;
+}
+
 // element t of the 16-byte slices of four positions, twice (the hi and the lo slots)
 __device__ __forceinline__ ph8 v_column(const uint4 (&v)[4], int t) {
     auto word = [&](int i) __attribute__((always_inline)) {
@@ -373,12 +379,12 @@ __device__ __forceinline__ void paged_chunk(const GhPagedAttnArgs& a, const Rows
         const float L = lanes4_sum(x.l);
         if (n >= G) return;
         if (!SCORED && begin + since == sh.first[row] && begin + i == sh.first[row + 1]) {
+            const float inv = 1.0f / L;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 uint32_t w[4];
 #pragma unroll
-                for (int t = 0; t < 4; ++t)
-                    w[t] = (uint32_t)gh_f2h(x.acc[2 * t][j] / L) | (uint32_t)gh_f2h(x.acc[2 * t + 1][j] / L) << 16;
+                for (int t = 0; t < 4; ++t) w[t] = out2(x.acc[2 * t][j], x.acc[2 * t + 1][j], inv);
                 *gh_gpw<uint4>(a.out + ((uint64_t)row * a.q_heads + kvh * G + n) * 256 + 64 * g + 16 * j) =
                     make_uint4(w[0], w[1], w[2], w[3]);
             }
@@ -544,7 +550,7 @@ __device__ __forceinline__ void paged_split(const GhPagedAttnArgs& a) {
             v.x += e * y.x;
             v.y += e * y.y;
         }
-        if (whole) gh_gpw<uint32_t>(out)[i] = (uint32_t)gh_f2h(v.x / L) | (uint32_t)gh_f2h(v.y / L) << 16;
+        if (whole) gh_gpw<uint32_t>(out)[i] = out2(v.x, v.y, 1.0f / L);
         else gh_gpw<float2>(a.part_acc)[part * 64 + i] = v;
         if (d == 0) {
             sM[h] = M;
@@ -652,9 +658,9 @@ __device__ __forceinline__ void paged_join(const GhPagedAttnArgs& a) {
                 L += e * sl[i];
                 o += e * red[i][tid];
             }
+            const float inv = 1.0f / L;
             gh_gpw<uint2>(a.out)[((uint64_t)row * a.q_heads + blockIdx.x) * 32 + d4] =
-                make_uint2((uint32_t)gh_f2h(o.x / L) | (uint32_t)gh_f2h(o.y / L) << 16,
-                           (uint32_t)gh_f2h(o.z / L) | (uint32_t)gh_f2h(o.w / L) << 16);
+                make_uint2(out2(o.x, o.y, inv), out2(o.z, o.w, inv));
         }
         return;
     }
