@@ -160,18 +160,22 @@ int attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv_pag
     a.stream = kStreamBytes;
     // scratch of a row: its partials, and with scores each query head's
     const uint64_t acc = (uint64_t)q_heads * 512, ml = acc / 64, raw = scored ? (uint64_t)q_heads * a.raw_len * 4 : 0;
-    // rows in groups that the kernel lays out at once and whose scratch fits 512 MiB
-    const uint64_t per = (acc + ml) * (split ? a.chunks : 1) + raw;
+    // rows in groups that the kernel lays out at once and whose scratch fits 512 MiB, or what memory there is
+    const uint64_t per = (acc + ml) * (split ? a.chunks : 1) + raw, layout = (kPagedRows + 4) * 4;
     const uint64_t room = std::min<uint64_t>((512ull << 20) / per, (1u << 30) / tiles1);  // tiles count in 32 bits
-    const uint32_t step = (uint32_t)std::min<uint64_t>(std::min(kv->rows, kPagedRows), std::max<uint64_t>(1, room));
-    const uint64_t parts = split ? (uint64_t)a.chunks * step : a.chunks + step, layout = (kPagedRows + 4) * 4;
+    uint32_t step = (uint32_t)std::min<uint64_t>(std::min(kv->rows, kPagedRows), std::max<uint64_t>(1, room));
+    auto parts = [&] { return split ? (uint64_t)a.chunks * step : (uint64_t)a.chunks + step; };
     char* ws = nullptr;
-    int rc = workspace_at(b, layout + (acc + ml) * parts + raw * step, &ws);
+    int rc = GH_OK;
+    while ((rc = workspace_at(b, layout + (acc + ml) * parts() + raw * step, &ws)) == GH_E_OOM && step > 1) {
+        step = (step + 1) / 2;
+        b->err.clear();
+    }
     if (rc) return rc;
     a.layout = split ? 0 : (uint64_t)ws;
     a.part_acc = (uint64_t)ws + layout;
-    a.raw = scored ? a.part_acc + acc * parts : 0;
-    a.part_ml = a.part_acc + acc * parts + raw * step;
+    a.raw = scored ? a.part_acc + acc * parts() : 0;
+    a.part_ml = a.part_acc + acc * parts() + raw * step;
     const GhPages p0 = a.p;
     for (uint32_t r = 0; r < kv->rows; r += step) {
         a.rows = std::min(step, kv->rows - r);

@@ -215,6 +215,20 @@ def test_attention_without_scratch(rng):
         p.free()
 
 
+@pytest.mark.parametrize("scored,lengths,limit", [(False, [400, 90, 0, 511, 33, 500, 17, 1], 4 << 20),
+                                                  (True, [3000, 100, 2000, 1, 700], 20 << 20)])
+def test_attention_with_scratch_for_some_rows(rng, scored, lengths, limit):
+    """Rows take turns in what scratch there is (all of it: 4.3 and 25 MB)."""
+    with HipBackend(0) as hip:
+        p = Paged(hip, rng, lengths, 16, 8, scored=scored)
+        for n in (limit, 0):
+            hip.set_scratch_limit(n)
+            before = p.read("score") if scored else None
+            q, out = run_attention(hip, p, 128, rng)
+            check_attention(p, 0, q, out, before, p.read("score") if scored else None)
+        p.free()
+
+
 # ---- append ----
 
 @pytest.mark.parametrize("scored", [False, True])

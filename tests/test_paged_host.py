@@ -182,6 +182,15 @@ def test_attention_refusals(host):
     wide = host.kv(heads=9000, slots=16, layers=1, rows=1)
     assert host.call(name, q, q, wide, 72000, 0, 0)[0] == UNSUPPORTED
     assert host.call(name, o, q, kv, 8, 0, 0, limit=1000)[0] == OOM
+    # with room for some of the rows, as many launches as it takes
+    many = host.kv(rows=40, width=64, slots=1024, scored=True)
+    q = host.buf(40 * 8 * 256)
+    rc, whole = host.call(name, q, q, many, 8, 0, 0)
+    rc2, parts = host.call(name, q, q, many, 8, 0, 0, limit=host.lib.host_scratch() // 3)
+    assert rc == rc2 == 0 and len(whole) == 2 and len(parts) > 4
+    args = [AttnArgs.from_buffer_copy(bytes(g.args)) for g in parts if g.kernel not in (host.ids["join"], host.ids["join2"])]
+    assert sum(a.rows for a in args) == 40
+    assert [(a.q - q.addr) // 2048 for a in args] == [sum(b.rows for b in args[:i]) for i in range(len(args))]
 
 
 def test_evict_refusals(host):
