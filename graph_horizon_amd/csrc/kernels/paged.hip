@@ -19,6 +19,20 @@ __device__ __forceinline__ uint32_t row_length(const GhPages& p, uint32_t row, u
     return 0;
 }
 
+// Inclusive sum over the wave in DPP steps: within rows of 16 lanes, then the rows' totals onward.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t scan_step(uint32_t v) {
+    return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, true);
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v = scan_step<0x111, 0xF>(v);     // row_shr:1
+    v = scan_step<0x112, 0xF>(v);     // row_shr:2
+    v = scan_step<0x114, 0xF>(v);     // row_shr:4
+    v = scan_step<0x118, 0xF>(v);     // row_shr:8
+    v = scan_step<0x142, 0xA>(v);     // row_bcast:15 into rows 1 and 3
+    return scan_step<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
+}
+
 // Slot of a row's position, kBad where the table's page is beyond the pool.
 __device__ __forceinline__ uint32_t slot_of(const GhPages& p, uint32_t row, uint32_t pos) {
     const uint32_t page = gh_gp<uint32_t>(p.table)[(uint64_t)row * p.width + (pos >> p.shift)];
@@ -289,8 +303,9 @@ struct RowsLds {
     uint32_t sums[4];
 };
 
-// Fills sh from the rows' lengths (longer ones than max_len count 0); 256 threads.
-__device__ __forceinline__ void lay_out_rows(const GhPagedAttnArgs& a, RowsLds& sh, bool report) {
+// Fills sh from the rows' lengths (longer ones than max_len count 0); 256 threads. Up to 64 rows: lane r also gets
+// the first tile behind row r.
+__device__ __forceinline__ uint32_t lay_out_rows(const GhPagedAttnArgs& a, RowsLds& sh, bool report) {
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
     if (a.rows <= 64) {  // each wave by itself, the same values
         uint32_t n = lane < a.rows ? gh_gp<uint32_t>(a.p.lengths)[lane] : 0u;
@@ -298,15 +313,11 @@ __device__ __forceinline__ void lay_out_rows(const GhPagedAttnArgs& a, RowsLds& 
             if (report) fault(a.p, GH_PAGED_LENGTH);
             n = 0;
         }
-        uint32_t upto = (n + 15) >> 4;
-        for (uint32_t o = 1; o < a.rows; o <<= 1) {
-            const uint32_t x = __shfl_up(upto, o, 64);
-            if (lane >= o) upto += x;
-        }
+        const uint32_t upto = wave_scan((n + 15) >> 4);
         sh.len[lane] = n;
         if (lane == 0) sh.first[0] = 0;
         sh.first[lane + 1] = upto;
-        return;
+        return upto;
     }
     uint32_t n[2], t[2];
 #pragma unroll
@@ -319,12 +330,7 @@ __device__ __forceinline__ void lay_out_rows(const GhPagedAttnArgs& a, RowsLds& 
         }
         t[i] = (n[i] + 15) >> 4;
     }
-    uint32_t upto = t[0] + t[1];
-#pragma unroll
-    for (uint32_t o = 1; o < 64; o <<= 1) {
-        const uint32_t x = __shfl_up(upto, o, 64);
-        if (lane >= o) upto += x;
-    }
+    uint32_t upto = wave_scan(t[0] + t[1]);
     if (lane == 63) sh.sums[wave] = upto;
     sh.len[2 * tid] = n[0];
     sh.len[2 * tid + 1] = n[1];
@@ -334,14 +340,15 @@ __device__ __forceinline__ void lay_out_rows(const GhPagedAttnArgs& a, RowsLds& 
     sh.first[2 * tid + 1] = upto - t[1];
     sh.first[2 * tid + 2] = upto;
     __syncthreads();
+    return 0;
 }
 
 // One chunk of the rows' tiles for one kv head by one wave.
 constexpr int kStream = 2;  // cache policy of reads that will not be wanted again soon (nt)
 
 template <bool SCORED, int CACHE>
-__device__ __forceinline__ void paged_chunk(const GhPagedAttnArgs& a, const RowsLds& sh, uint32_t total, uint32_t per,
-                                            uint32_t chunk, uint32_t kvh) {
+__device__ __forceinline__ void paged_chunk(const GhPagedAttnArgs& a, const RowsLds& sh, uint32_t behind, uint32_t total,
+                                            uint32_t per, uint32_t chunk, uint32_t kvh) {
     const uint32_t lane = threadIdx.x & 63u, n = lane & 15u, g = lane >> 4, G = a.group;
     const uint32_t begin = chunk * per, tiles = min(per, total - begin), row_bytes = a.p.kv_heads * 256;
 
@@ -350,13 +357,18 @@ __device__ __forceinline__ void paged_chunk(const GhPagedAttnArgs& a, const Rows
     auto look_up = [&](uint32_t from) __attribute__((always_inline)) {
         const uint32_t t = begin + from + lane;
         t_slot = t_pos = t_row = 0;
+        uint32_t lo = 0;  // the row with first[lo] <= t < first[lo + 1]
+        if (a.rows <= 64) lo = (uint32_t)__popcll(__ballot(behind <= begin + from));  // of the first tile
         if (from + lane >= tiles) return;
-        uint32_t lo = 0, hi = a.rows;  // first[lo] <= t < first[hi]
-        while (hi - lo > 1) {
-            const uint32_t mid = (lo + hi) >> 1;
-            if (sh.first[mid] <= t) lo = mid;
-            else hi = mid;
+        if (a.rows > 64) {
+            uint32_t hi = a.rows;
+            while (hi - lo > 1) {
+                const uint32_t mid = (lo + hi) >> 1;
+                if (sh.first[mid] <= t) lo = mid;
+                else hi = mid;
+            }
         }
+        while (sh.first[lo + 1] <= t) ++lo;
         t_pos = (t - sh.first[lo]) * 16;
         const uint32_t page = gh_gp<uint32_t>(a.p.table)[(uint64_t)lo * a.p.width + (t_pos >> a.p.shift)];
         const bool bad = page >= a.p.pages;
@@ -372,7 +384,7 @@ __device__ __forceinline__ void paged_chunk(const GhPagedAttnArgs& a, const Rows
 
     ph8 qf[4];
     Sums x;
-    uint32_t row = 0xFFFFu, since = 0;  // the row at hand and the tile it began with
+    uint32_t row, since;  // the row at hand and the tile it began with
     uint64_t raw = 0;
     // the row's sums up to tile i: its output if they are whole, else a partial
     auto flush = [&](uint32_t i) __attribute__((always_inline)) {
@@ -400,6 +412,15 @@ __device__ __forceinline__ void paged_chunk(const GhPagedAttnArgs& a, const Rows
         if (g == 0) gh_gpw<float2>(a.part_ml)[part] = make_float2(x.m, L);
     };
 
+    auto start = [&](uint32_t info, uint32_t i) __attribute__((always_inline)) {
+        row = info & 0xFFFFu;
+        since = i;
+        x.clear();
+        load_q(a, row, kvh, qf);
+        if (SCORED) raw = a.raw + (((uint64_t)row * a.p.kv_heads + kvh) * G + n) * a.raw_len * 4;
+    };
+    start(__builtin_amdgcn_readlane(t_row, 0), 0);
+
     // K of the next tile is asked for as soon as this one's products are made, V behind its last use
     Tile r;
     Where w = where(0);
@@ -409,12 +430,8 @@ __device__ __forceinline__ void paged_chunk(const GhPagedAttnArgs& a, const Rows
         const uint32_t info = __builtin_amdgcn_readlane(t_row, i & 63u);
         const uint32_t pos = SCORED ? __builtin_amdgcn_readlane(t_pos, i & 63u) : 0u;
         if ((info & 0xFFFFu) != row) {
-            if (i) flush(i);
-            row = info & 0xFFFFu;
-            since = i;
-            x.clear();
-            load_q(a, row, kvh, qf);
-            if (SCORED) raw = a.raw + (((uint64_t)row * a.p.kv_heads + kvh) * G + n) * a.raw_len * 4;
+            flush(i);
+            start(info, i);
         }
         pf4 st = tile_products(r, qf);
         if ((i & 63u) == 63) look_up(i + 1);
@@ -438,7 +455,7 @@ __device__ __forceinline__ void paged_attn(const GhPagedAttnArgs& a) {
     __shared__ RowsLds sh;
     const uint32_t unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t chunk = unit / a.p.kv_heads, kvh = unit % a.p.kv_heads;
-    lay_out_rows(a, sh, blockIdx.x == 0);
+    const uint32_t behind = lay_out_rows(a, sh, blockIdx.x == 0);
     const uint32_t total = sh.first[a.rows];
     const uint32_t half = (2 * total + a.chunks - 1) / a.chunks;
     const uint32_t per = max(a.least, half <= a.solo ? half : (total + a.chunks - 1) / a.chunks);
@@ -451,8 +468,8 @@ __device__ __forceinline__ void paged_attn(const GhPagedAttnArgs& a) {
             for (uint32_t i = threadIdx.x; i < a.q_heads * 64; i += 256)
                 gh_gpw<uint32_t>(a.out)[(uint64_t)r * a.q_heads * 64 + i] = 0u;
     if (chunk >= a.chunks || chunk * per >= total) return;
-    if ((uint64_t)total * a.p.kv_heads * 8192 >= a.stream) paged_chunk<SCORED, kStream>(a, sh, total, per, chunk, kvh);
-    else paged_chunk<SCORED, 0>(a, sh, total, per, chunk, kvh);
+    if ((uint64_t)total * a.p.kv_heads * 8192 >= a.stream) paged_chunk<SCORED, kStream>(a, sh, behind, total, per, chunk, kvh);
+    else paged_chunk<SCORED, 0>(a, sh, behind, total, per, chunk, kvh);
 }
 }  // namespace
 
@@ -700,20 +717,6 @@ GH_KERNEL __launch_bounds__(256) void gh_paged_join2(GhPagedAttnArgs a) { paged_
 namespace {
 // f32 total order as unsigned order
 __device__ __forceinline__ uint32_t order_key(uint32_t bits) { return bits ^ ((uint32_t)((int32_t)bits >> 31) | 0x80000000u); }
-
-// Inclusive sum over the wave in DPP steps: within rows of 16 lanes, then the rows' totals onward.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t scan_step(uint32_t v) {
-    return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, true);
-}
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
-    v = scan_step<0x111, 0xF>(v);     // row_shr:1
-    v = scan_step<0x112, 0xF>(v);     // row_shr:2
-    v = scan_step<0x114, 0xF>(v);     // row_shr:4
-    v = scan_step<0x118, 0xF>(v);     // row_shr:8
-    v = scan_step<0x142, 0xA>(v);     // row_bcast:15 into rows 1 and 3
-    return scan_step<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
-}
 
 constexpr uint32_t kHeld = 4;  // steps of 2048 scores that a workgroup keeps in registers
 
