@@ -57,7 +57,9 @@ class HipBackend:
         if rc != F.GH_OK:
             raise GhError(rc, "gh_create", "(no gfx950 device, or code objects missing)")
         self.h = h
-        self.enc = None
+        self.enc = None  # the open encoder's handle
+        self._slot = C.c_void_p()
+        self._slot_ref = C.byref(self._slot)
 
     def close(self):
         if self.h:
@@ -116,10 +118,9 @@ class HipBackend:
 
     # ---- encoder ----
     def begin(self):
-        e = C.c_void_p()
-        self._ok(self.lib.gh_begin(self.h, C.byref(e)), "begin")
-        self.enc = e
-        return e
+        self._ok(self.lib.gh_begin(self.h, self._slot_ref), "begin")
+        self.enc = self._slot
+        return self.enc
 
     def submit(self):
         e, self.enc = self.enc, None
@@ -132,12 +133,14 @@ class HipBackend:
         own = self.enc is None
         if own:
             self.begin()
-        rc = getattr(self.lib, name)(self.h, self.enc, *args)
+        lib, h = self.lib, self.h
+        rc = getattr(lib, name)(h, self._slot, *args)
         if own:
-            e, self.enc = self.enc, None
-            rs = self.lib.gh_submit(self.h, e)
+            self.enc = None
+            rs = lib.gh_submit(h, self._slot)
             rc = rc if rc != F.GH_OK else rs
-        self._ok(rc, name)
+        if rc != F.GH_OK:
+            self._ok(rc, name)
 
     # ---- numeric ops (contract.rs order) ----
     def dequant_rows(self, out, w, row0, rows):
@@ -183,26 +186,24 @@ class HipBackend:
         self._run("gh_attention_prefill", C.byref(out), C.byref(q), C.byref(kv), q_heads, base,
                   n, layer)
 
-    # ---- a batch of sequences over paged caches (GhKvPaged) ----
+    # ---- a batch of sequences over paged caches (GhKvPaged); structures are passed by reference ----
     def kv_write_paged(self, kv: GhKvPaged, k, v, tokens, layer):
         """Append `tokens` K/V vectors per row at the end of its positions."""
-        self._run("gh_kv_write_paged", C.byref(kv), C.byref(k), C.byref(v), tokens, layer)
+        self._run("gh_kv_write_paged", kv, k, v, tokens, layer)
 
     def rope_kv_write_paged(self, kv: GhKvPaged, q_out, q, k, v, q_heads, positions, tokens, max_pos,
                             yarn: Yarn, layer):
         """RoPE of q (into q_out) and k at the rows' own positions, and the append, in one launch."""
-        self._run("gh_rope_kv_write_paged", C.byref(kv), C.byref(q_out), C.byref(q), C.byref(k), C.byref(v),
-                  q_heads, C.byref(positions), tokens, max_pos, C.byref(yarn.c()), layer)
+        self._run("gh_rope_kv_write_paged", kv, q_out, q, k, v, q_heads, positions, tokens, max_pos, yarn.c(), layer)
 
     def attention_decode_paged(self, out, q, kv: GhKvPaged, q_heads, max_len, layer):
         """One token per row over its cached positions; adds the attention weights to kv.score if kept."""
-        self._run("gh_attention_decode_paged", C.byref(out), C.byref(q), C.byref(kv), q_heads, max_len, layer)
+        self._run("gh_attention_decode_paged", out, q, kv, q_heads, max_len, layer)
 
     def kv_evict_paged(self, dst: GhKvPaged, src: GhKvPaged, kept, budget, recent):
         """Rows longer than `budget` keep their last `recent` and best-scored positions, in dst's pages;
         kept: a buffer for the kept positions, or None."""
-        self._run("gh_kv_evict_paged", C.byref(dst), C.byref(src), None if kept is None else C.byref(kept),
-                  budget, recent)
+        self._run("gh_kv_evict_paged", dst, src, kept, budget, recent)
 
     # ---- read-back ----
     def read_logits(self, logits, vocab) -> np.ndarray:
