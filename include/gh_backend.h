@@ -215,13 +215,15 @@ int gh_attention_decode_noalloc(gh_backend* b, gh_encoder* enc, const gh_buf* ou
 /* Append: `tokens` new K and V vectors per row, FP16 [rows][tokens][kv_heads][128], to the positions
  * lengths[r] - tokens .. lengths[r] - 1 of `layer` (the lengths already count them); their scores, where
  * kept, become 0. Vectors before a row's first position (lengths[r] < tokens) are skipped. The bytes of
- * gh_kv_write. Rows must not share the pages that they append to. */
+ * gh_kv_write. Rows must not share the pages that they append to, and k and v must not lie in slots that the
+ * call writes. */
 int gh_kv_write_paged(gh_backend* b, gh_encoder* enc, const gh_kv_paged* kv, const gh_buf* k,
                       const gh_buf* v, uint32_t tokens, uint32_t layer);
 /* RoPE and append in one launch: token t of row r is rotated for position positions[r] + t (u32 [rows] on
  * the device; after an eviction a row stands further on than its length says), queries FP16
  * [rows][tokens][q_heads][128] from q to q_out (may be the same buffer) with the query's post-scale, keys on
- * their way into the cache. The values of gh_rope_yarn and gh_kv_write. max_pos: the largest of the positions
+ * their way into the cache; of skipped vectors (gh_kv_write_paged) the queries are skipped too. The values of
+ * gh_rope_yarn and gh_kv_write. max_pos: the largest of the positions
  * positions[r] + t of this call, at most 262143 (it sizes the rotation table). */
 int gh_rope_kv_write_paged(gh_backend* b, gh_encoder* enc, const gh_kv_paged* kv, const gh_buf* q_out,
                            const gh_buf* q, const gh_buf* k, const gh_buf* v, uint32_t q_heads,

@@ -200,6 +200,30 @@ def test_attention_infinities_and_nan_stay_where_they_are_seen(hip, rng):
     p.free()
 
 
+@pytest.mark.parametrize("lengths", [[200, 90], [7000, 3000]])  # both divisions of the work
+def test_attention_a_query_that_is_not_finite_is_its_own(hip, rng, lengths):
+    """A NaN and an infinity in two heads' queries: those heads are NaN, the others of the same kv head as ever,
+    and scores are NaN where such a weight was added."""
+    p = Paged(hip, rng, lengths, 16, 8, scored=True)
+    before = p.read("score")
+    q = rng.standard_normal((2, 32, D)).astype(np.float16)
+    q[0, 5, 3], q[1, 30, 100] = np.nan, np.inf
+    q, out = run_attention(hip, p, 32, rng, q=q)
+    after = p.read("score")
+    for r, odd in ((0, 5), (1, 30)):
+        s = p.cells(r, lengths[r])
+        for h in range(8):
+            for i in range(4 * h, 4 * h + 4):
+                if i == odd:
+                    assert np.isnan(out[r, i]).all()
+                    continue
+                want, _, bound, _ = attend(q[r, i:i + 1], p.k[0, s, h], p.v[0, s, h])
+                assert np.all(np.abs(out[r, i:i + 1] - want) <= bound), (r, i)
+            assert np.isnan(after[0, r, h, :lengths[r]]).all() == (odd // 4 == h)
+            assert np.array_equal(after[0, r, h, lengths[r]:], before[0, r, h, lengths[r]:])
+    p.free()
+
+
 def test_attention_without_scratch(rng):
     """Scratch that cannot be had is an error, and the next call works."""
     with HipBackend(0) as hip:
