@@ -18,6 +18,11 @@ bool fits(const gh_buf* buf, uint64_t bytes, uint64_t align) {
 
 bool overlap(const gh_buf& a, const gh_buf& b) { return a.addr < b.addr + b.bytes && b.addr < a.addr + a.bytes; }
 
+// the bytes at a and b overlap
+bool meet(const gh_buf* a, uint64_t a_bytes, const gh_buf* b, uint64_t b_bytes) {
+    return a->addr < b->addr + b_bytes && b->addr < a->addr + a_bytes;
+}
+
 constexpr uint32_t kPagedRows = 512;  // rows that one attention launch lays out
 constexpr uint64_t kStreamBytes = 128ull << 20;  // half the last-level cache
 constexpr uint32_t kSpanTiles = 32;   // tiles of a gh_paged_split workgroup at most (its waves hold 64 each)
@@ -120,6 +125,7 @@ int attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv_pag
     const uint64_t bytes = (uint64_t)kv->rows * q_heads * 256;
     if (!fits(q, bytes, 16) || !fits(out, bytes, 16))
         return fail(b, GH_E_RANGE, "attention_decode_paged: buffer too small or not on 16 bytes");
+    if (out->addr != q->addr && meet(out, bytes, q, bytes)) return fail(b, GH_E_INVALID, "attention_decode_paged: out overlaps q");
     if (max_len > capacity(kv)) return fail(b, GH_E_RANGE, "attention_decode_paged: max_len beyond the table");
     if (max_len == 0) max_len = (uint32_t)capacity(kv);
 
@@ -263,8 +269,11 @@ int gh_rope_kv_write_paged(gh_backend* b, gh_encoder* enc, const gh_kv_paged* kv
         const uint64_t bytes = (uint64_t)kv->rows * tokens * q_heads * 256;
         if (!fits(q, bytes, 16) || !fits(q_out, bytes, 16) || !fits(positions, (uint64_t)kv->rows * 4, 4))
             return fail(b, GH_E_RANGE, "rope_kv_write_paged: buffer too small or not on 16 bytes");
-        const gh_buf in{q->addr, bytes, 0, 0, 0, 0}, to{q_out->addr, bytes, 0, 0, 0, 0};
-        if (q->addr != q_out->addr && overlap(in, to)) return fail(b, GH_E_INVALID, "rope_kv_write_paged: q_out overlaps q");
+        if (q->addr != q_out->addr && meet(q, bytes, q_out, bytes))
+            return fail(b, GH_E_INVALID, "rope_kv_write_paged: q_out overlaps q");
+        const uint64_t heads = bytes / q_heads * kv->kv.kv_heads;
+        if ((k && meet(q_out, bytes, k, heads)) || (v && meet(q_out, bytes, v, heads)))
+            return fail(b, GH_E_INVALID, "rope_kv_write_paged: q_out overlaps k or v");
         rc = ensure_rope(b, b->rope, yarn, max_pos + 1);
         if (rc) return rc;
         GhPagedWriteArgs a{};

@@ -90,6 +90,20 @@ def test_attention_repeats_bit_for_bit(hip, rng):
     p.free()
 
 
+@pytest.mark.parametrize("scored", [False, True])
+@pytest.mark.parametrize("lengths,width", [([0, 300, 17], 20), ([5000, 0, 40, 700], 313), ([3000, 2500, 9, 0] * 5, 188)])
+def test_attention_into_its_queries(hip, rng, lengths, width, scored):
+    """out is q's own buffer, in spans of one and more and in chunks: the bits of the call with two buffers."""
+    p = Paged(hip, rng, lengths, 16, 4, width=width, scored=scored)
+    q, want = run_attention(hip, p, 16, rng)
+    buf = hip.from_host(q)
+    hip.attention_decode_paged(buf, buf, p.handle(), 16, 0, 0)
+    got = hip.download(buf, np.float16, q.size).reshape(q.shape)
+    assert np.array_equal(got.view(np.uint16), want.view(np.uint16))
+    hip.free_buffer(buf)
+    p.free()
+
+
 def test_attention_equals_contiguous_decode(hip, rng):
     """Pages in order are the contiguous cache: both operators within twice the bound of each."""
     n, heads, group = 777, 8, 4

@@ -193,6 +193,25 @@ def test_attention_refusals(host):
     assert [(a.q - q.addr) // 2048 for a in args] == [sum(b.rows for b in args[:i]) for i in range(len(args))]
 
 
+def test_outputs_are_an_input_itself_or_apart(host):
+    kv, part = host.kv(), 3 * 8 * 256
+    q, k, v, pos = host.buf(3 * part), host.buf(part), host.buf(part), host.buf(12)
+    yarn = F.GhYarn(128, 16384, 1e6, 16.0, 32.0, 1.0, 1.0, 0.1)
+
+    def at(b, off):
+        return F.GhBuf(b.addr + off, part, 0, F.BUF_ALLOC, 0, 0)
+
+    # views of one buffer: q itself, next to it, and half a vector on
+    for off, status in ((0, 0), (part, 0), (2 * part, 0), (part - 16, INVALID), (128, INVALID)):
+        assert host.call("gh_attention_decode_paged", at(q, off), q, kv, 8, 0, 0)[0] == status, off
+        assert host.call("gh_attention_decode_paged", q, at(q, off), kv, 8, 0, 0)[0] == status, off
+        assert host.call("gh_rope_kv_write_paged", kv, at(q, off), q, k, v, 8, pos, 1, 9, yarn, 0)[0] == status, off
+    kv_bytes = 3 * 2 * 256
+    for off, status in ((0, INVALID), (kv_bytes - 16, INVALID), (kv_bytes, 0)):
+        assert host.call("gh_rope_kv_write_paged", kv, at(k, off), q, k, v, 8, pos, 1, 9, yarn, 0)[0] == status, off
+        assert host.call("gh_rope_kv_write_paged", kv, at(v, off), q, k, v, 8, pos, 1, 9, yarn, 0)[0] == status, off
+
+
 def test_evict_refusals(host):
     name = "gh_kv_evict_paged"
     src, dst = host.kv(scored=True), host.kv(scored=True, width=3)
