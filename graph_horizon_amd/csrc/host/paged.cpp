@@ -23,6 +23,12 @@ bool meet(const gh_buf* a, uint64_t a_bytes, const gh_buf* b, uint64_t b_bytes) 
     return a->addr < b->addr + b_bytes && b->addr < a->addr + a_bytes;
 }
 
+// The bytes of a buffer that a call uses.
+struct Span {
+    uint64_t at = 0, bytes = 0;
+};
+bool meet(const Span& a, const Span& b) { return a.bytes && b.bytes && a.at < b.at + b.bytes && b.at < a.at + a.bytes; }
+
 constexpr uint32_t kPagedRows = 512;  // rows that one attention launch lays out
 constexpr uint64_t kStreamBytes = 128ull << 20;  // half the last-level cache
 constexpr uint32_t kSpanTiles = 32;   // tiles of a gh_paged_split workgroup at most (its waves hold 64 each)
@@ -54,6 +60,24 @@ int check_paged(gh_backend* b, const gh_kv_paged* p, uint32_t layer, const char*
         return no(GH_E_RANGE, "scores too small or not on 16 bytes");
     return GH_OK;
 }
+
+// What a checked handle uses of its buffers. Operators write all but the table.
+enum { CACHE_K, CACHE_V, SCORE, LENGTHS, TABLE, PARTS };
+struct Parts {
+    Span part[PARTS];
+    explicit Parts(const gh_kv_paged* p) {
+        const gh_kv& kv = p->kv;
+        part[CACHE_K].bytes = part[CACHE_V].bytes = (uint64_t)kv.block_count * kv.context * kv.kv_heads * 256;
+        part[CACHE_K].at = kv.k.addr;
+        part[CACHE_V].at = kv.v.addr;
+        if (p->score.addr) part[SCORE] = {p->score.addr, (uint64_t)kv.block_count * p->rows * kv.kv_heads * capacity(p) * 4};
+        part[LENGTHS] = {p->lengths.addr, (uint64_t)p->rows * 4};
+        part[TABLE] = {p->table.addr, (uint64_t)p->rows * p->table_width * 4};
+    }
+    bool met(const Span& x) const {
+        return std::any_of(part, part + PARTS, [&](const Span& y) { return meet(x, y); });
+    }
+};
 
 GhPages pages(gh_backend* b, const gh_kv_paged* p, uint32_t layer) {
     const gh_kv& kv = p->kv;
@@ -224,6 +248,17 @@ int evict(gh_backend* b, const gh_kv_paged* dst, const gh_kv_paged* src, const g
     const uint64_t list = (uint64_t)s.block_count * src->rows * s.kv_heads;
     if (list > (1ull << 40)) return fail(b, GH_E_RANGE, "kv_evict_paged: too many rows");
     if (kept && !fits(kept, list * budget * 4, 4)) return fail(b, GH_E_RANGE, "kv_evict_paged: kept too small");
+    // Workgroups read while others write, and the kept positions are indexes of src's table when they are read again:
+    // what is written lies in nothing that is read but its own counterpart.
+    const Parts from(src), to(dst);
+    if (kept && (from.met({kept->addr, list * budget * 4}) || to.met({kept->addr, list * budget * 4})))
+        return fail(b, GH_E_INVALID, "kv_evict_paged: kept overlaps a cache, table, lengths or scores");
+    for (int w = 0; w < TABLE; ++w)
+        for (int r = 0; r < PARTS; ++r)
+            if (w != r && meet(to.part[w], from.part[r]))
+                return fail(b, GH_E_INVALID, "kv_evict_paged: a buffer of dst overlaps another one of src");
+    if (to.part[TABLE].at == from.part[TABLE].at && to.part[CACHE_K].at == from.part[CACHE_K].at)
+        return fail(b, GH_E_INVALID, "kv_evict_paged: dst has src's pages");
     GhPagedEvictArgs a{};
     a.src = pages(b, src, 0);
     a.dst = pages(b, dst, 0);

@@ -243,7 +243,8 @@ int gh_attention_decode_paged(gh_backend* b, gh_encoder* enc, const gh_buf* out,
  * they are: nothing of theirs is written. src's pages are only read, so other rows may share them; dst's
  * pages of the evicted rows must be no page that src's rows use, and none of them twice. dst has src's rows,
  * page_size, block_count and heads, and the scores; its lengths and, with the same table_width, its scores may
- * be src's own buffers. */
+ * be src's own buffers, and its caches src's or parts of them; otherwise no buffer of dst that is written lies in one of
+ * src, and kept lies in none of either. */
 int gh_kv_evict_paged(gh_backend* b, gh_encoder* enc, const gh_kv_paged* dst, const gh_kv_paged* src,
                       const gh_buf* kept, uint32_t budget, uint32_t recent);
 

@@ -288,3 +288,43 @@ def test_attention_plans_stay_within_their_scratch(host, seed):
         assert regions[0][0] >= SCRATCH and regions[-1][0] + regions[-1][1] <= SCRATCH + size
         assert all(x + nx <= y for (x, nx), (y, _) in zip(regions, regions[1:]))
     assert at == rows
+
+
+def at_end(b, size):
+    """A buffer of `size` bytes that begins with the last 16 bytes of b."""
+    return F.GhBuf(b.addr + (b.bytes - 16) // 16 * 16, size, 0, F.BUF_ALLOC, 0, 0)
+
+
+def with_(kv, **bufs):
+    kv = F.GhKvPaged.from_buffer_copy(kv)
+    for name, b in bufs.items():
+        setattr(kv.kv if name in ("k", "v") else kv, name, b)
+    return kv
+
+
+def test_what_an_eviction_writes_lies_apart_from_what_it_reads(host):
+    """The kept list is read again as positions while scores, lengths and vectors are written: it meets none of the
+    handles' buffers; dst's scores, lengths and vectors meet nothing of src's but their own counterparts."""
+    name = "gh_kv_evict_paged"
+    src, dst = host.kv(scored=True), host.kv(scored=True, width=3)
+    kept_bytes = 2 * 3 * 2 * 16 * 4
+    for kv in (src, dst):
+        for b in (kv.kv.k, kv.kv.v, kv.table, kv.lengths, kv.score):
+            for kept in (F.GhBuf(b.addr, kept_bytes, 0, F.BUF_ALLOC, 0, 0), at_end(b, kept_bytes),
+                         F.GhBuf(b.addr - kept_bytes + 4, kept_bytes, 0, F.BUF_ALLOC, 0, 0)):
+                assert host.call(name, dst, src, kept, 16, 1)[0] == INVALID
+        for b in (kv.table, kv.lengths, kv.score):
+            behind = F.GhBuf(b.addr + b.bytes, kept_bytes, 0, F.BUF_ALLOC, 0, 0)
+            assert host.call(name, dst, src, behind, 16, 1)[0] == 0
+    for written in ("score", "lengths", "k", "v"):
+        size = getattr(dst.kv if written in "kv" else dst, written).bytes
+        for read in ("k", "v", "table", "lengths", "score"):
+            if read == written:
+                continue
+            b = getattr(src.kv if read in "kv" else src, read)
+            assert host.call(name, with_(dst, **{written: at_end(b, size)}), src, None, 16, 1)[0] == INVALID, (written, read)
+    same = with_(src, table=host.buf(src.table.bytes))  # in place: scores, lengths and pool are src's own
+    assert host.call(name, same, src, None, 16, 1)[0] == 0
+    assert host.call(name, with_(same, lengths=host.buf(12)), src, None, 16, 1)[0] == 0
+    assert host.call(name, src, src, None, 16, 1)[0] == INVALID  # the same pages
+
