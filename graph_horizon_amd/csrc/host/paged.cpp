@@ -16,8 +16,6 @@ bool fits(const gh_buf* buf, uint64_t bytes, uint64_t align) {
     return buf && buf->addr && buf->bytes >= bytes && buf->addr % align == 0;
 }
 
-bool overlap(const gh_buf& a, const gh_buf& b) { return a.addr < b.addr + b.bytes && b.addr < a.addr + a.bytes; }
-
 // the bytes at a and b overlap
 bool meet(const gh_buf* a, uint64_t a_bytes, const gh_buf* b, uint64_t b_bytes) {
     return a->addr < b->addr + b_bytes && b->addr < a->addr + a_bytes;
@@ -240,17 +238,17 @@ int evict(gh_backend* b, const gh_kv_paged* dst, const gh_kv_paged* src, const g
     if (budget > capacity(dst)) return fail(b, GH_E_RANGE, "kv_evict_paged: budget beyond dst's table");
     if (budget > (1u << 27)) return fail(b, GH_E_UNSUPPORTED, "kv_evict_paged: budget beyond 2^27");
     if (s.block_count > 0xFFFFu) return fail(b, GH_E_UNSUPPORTED, "kv_evict_paged: more than 65535 layers");
-    const bool same = dst->score.addr == src->score.addr;
-    if (same ? dst->table_width != src->table_width : overlap(dst->score, src->score))
-        return fail(b, GH_E_INVALID, "kv_evict_paged: scores overlap");
-    if (dst->lengths.addr != src->lengths.addr && overlap(dst->lengths, src->lengths))
-        return fail(b, GH_E_INVALID, "kv_evict_paged: lengths overlap");
     const uint64_t list = (uint64_t)s.block_count * src->rows * s.kv_heads;
     if (list > (1ull << 40)) return fail(b, GH_E_RANGE, "kv_evict_paged: too many rows");
     if (kept && !fits(kept, list * budget * 4, 4)) return fail(b, GH_E_RANGE, "kv_evict_paged: kept too small");
     // Workgroups read while others write, and the kept positions are indexes of src's table when they are read again:
     // what is written lies in nothing that is read but its own counterpart.
     const Parts from(src), to(dst);
+    const bool same = dst->score.addr == src->score.addr;
+    if (same ? dst->table_width != src->table_width : meet(to.part[SCORE], from.part[SCORE]))
+        return fail(b, GH_E_INVALID, "kv_evict_paged: scores overlap");
+    if (dst->lengths.addr != src->lengths.addr && meet(to.part[LENGTHS], from.part[LENGTHS]))
+        return fail(b, GH_E_INVALID, "kv_evict_paged: lengths overlap");
     if (kept && (from.met({kept->addr, list * budget * 4}) || to.met({kept->addr, list * budget * 4})))
         return fail(b, GH_E_INVALID, "kv_evict_paged: kept overlaps a cache, table, lengths or scores");
     for (int w = 0; w < TABLE; ++w)

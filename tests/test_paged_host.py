@@ -328,3 +328,14 @@ def test_what_an_eviction_writes_lies_apart_from_what_it_reads(host):
     assert host.call(name, with_(same, lengths=host.buf(12)), src, None, 16, 1)[0] == 0
     assert host.call(name, src, src, None, 16, 1)[0] == INVALID  # the same pages
 
+
+def test_eviction_buffers_may_be_parts_of_longer_ones(host):
+    """Only the bytes that a call uses count, not what its buffers hold behind them."""
+    name = "gh_kv_evict_paged"
+    src, dst = host.kv(scored=True), host.kv(scored=True, width=3)
+    for field in ("score", "lengths"):
+        n, m = getattr(src, field).bytes, getattr(dst, field).bytes
+        whole = host.buf(n + m)
+        lo = with_(src, **{field: whole})
+        hi = with_(dst, **{field: F.GhBuf(whole.addr + n, m, 0, F.BUF_ALLOC, 0, 0)})
+        assert host.call(name, hi, lo, None, 40, 1)[0] == 0, field
