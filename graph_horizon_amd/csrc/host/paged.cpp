@@ -33,6 +33,24 @@ constexpr uint32_t kSpanTiles = 32;   // tiles of a gh_paged_split workgroup at 
 
 uint64_t capacity(const gh_kv_paged* kv) { return (uint64_t)kv->table_width * kv->page_size; }
 
+// What a handle uses of its buffers. Operators write all but the table.
+enum { CACHE_K, CACHE_V, SCORE, LENGTHS, TABLE, PARTS };
+struct Parts {
+    Span part[PARTS];
+    explicit Parts(const gh_kv_paged* p) {
+        const gh_kv& kv = p->kv;
+        part[CACHE_K].bytes = part[CACHE_V].bytes = (uint64_t)kv.block_count * kv.context * kv.kv_heads * 256;
+        part[CACHE_K].at = kv.k.addr;
+        part[CACHE_V].at = kv.v.addr;
+        if (p->score.addr) part[SCORE] = {p->score.addr, (uint64_t)kv.block_count * p->rows * kv.kv_heads * capacity(p) * 4};
+        part[LENGTHS] = {p->lengths.addr, (uint64_t)p->rows * 4};
+        part[TABLE] = {p->table.addr, (uint64_t)p->rows * p->table_width * 4};
+    }
+    bool met(const Span& x) const {
+        return std::any_of(part, part + PARTS, [&](const Span& y) { return meet(x, y); });
+    }
+};
+
 // Everything about the handle that the host can see. `layer`: the one the call uses.
 int check_paged(gh_backend* b, const gh_kv_paged* p, uint32_t layer, const char* what) {
     auto no = [&](int code, const char* why) { return fail(b, code, std::string(what) + ": " + why); };
@@ -56,26 +74,13 @@ int check_paged(gh_backend* b, const gh_kv_paged* p, uint32_t layer, const char*
         return no(GH_E_RANGE, "table or lengths too small");
     if (p->score.addr && !fits(&p->score, (uint64_t)score, 16))
         return no(GH_E_RANGE, "scores too small or not on 16 bytes");
+    // the workgroups of a launch read lengths and pages each for itself, while others write
+    const Parts own(p);
+    for (int i = 0; i < PARTS; ++i)
+        for (int j = 0; j < i; ++j)
+            if (meet(own.part[i], own.part[j])) return no(GH_E_INVALID, "the handle's buffers overlap");
     return GH_OK;
 }
-
-// What a checked handle uses of its buffers. Operators write all but the table.
-enum { CACHE_K, CACHE_V, SCORE, LENGTHS, TABLE, PARTS };
-struct Parts {
-    Span part[PARTS];
-    explicit Parts(const gh_kv_paged* p) {
-        const gh_kv& kv = p->kv;
-        part[CACHE_K].bytes = part[CACHE_V].bytes = (uint64_t)kv.block_count * kv.context * kv.kv_heads * 256;
-        part[CACHE_K].at = kv.k.addr;
-        part[CACHE_V].at = kv.v.addr;
-        if (p->score.addr) part[SCORE] = {p->score.addr, (uint64_t)kv.block_count * p->rows * kv.kv_heads * capacity(p) * 4};
-        part[LENGTHS] = {p->lengths.addr, (uint64_t)p->rows * 4};
-        part[TABLE] = {p->table.addr, (uint64_t)p->rows * p->table_width * 4};
-    }
-    bool met(const Span& x) const {
-        return std::any_of(part, part + PARTS, [&](const Span& y) { return meet(x, y); });
-    }
-};
 
 GhPages pages(gh_backend* b, const gh_kv_paged* p, uint32_t layer) {
     const gh_kv& kv = p->kv;

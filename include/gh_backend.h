@@ -97,8 +97,8 @@ typedef struct gh_kv {
  * slots p·page_size .. + page_size of every layer. Sequence r is row r of the batch: its position j
  * lives at slot j mod page_size of page table[r][j / page_size]. Rows may share pages (a common
  * prompt) as long as nothing is written to them. Table and lengths live on the device and are the
- * caller's to fill (gh_upload); places of the table past a row's length are never read for an
- * address. A row of length 0 is free: nothing is read, written or scored for it.
+ * caller's to fill (gh_upload); the five buffers lie apart. Places of the table past a row's length are never read for
+ * an address. A row of length 0 is free: nothing is read, written or scored for it.
  * Kernels check what the host cannot: a length beyond table_width·page_size (or the call's max_len),
  * a page number beyond the pool or a position beyond max_pos touches no memory, and the next
  * gh_submit returns GH_E_RANGE; that row's results are unspecified then, other rows' are not touched. */

@@ -339,3 +339,29 @@ def test_eviction_buffers_may_be_parts_of_longer_ones(host):
         lo = with_(src, **{field: whole})
         hi = with_(dst, **{field: F.GhBuf(whole.addr + n, m, 0, F.BUF_ALLOC, 0, 0)})
         assert host.call(name, hi, lo, None, 40, 1)[0] == 0, field
+
+
+def test_a_handles_buffers_lie_apart(host):
+    big, yarn = host.buf(1 << 30), F.GhYarn(128, 16384, 1e6, 16.0, 32.0, 1.0, 1.0, 0.1)
+    good = host.kv(scored=True)
+    names = ("k", "v", "table", "lengths", "score")
+    for one in names:
+        for other in names:
+            if one == other:
+                continue
+            kv = host.kv(scored=True)
+            b, size = (getattr(kv.kv if n in "kv" else kv, n) for n in (one, other))
+            kv = with_(kv, **{other: at_end(b, size.bytes)})
+            for name, args in (("gh_kv_write_paged", (kv, big, big, 1, 0)),
+                               ("gh_rope_kv_write_paged", (kv, big, host.buf(1 << 20), big, big, 8, big, 1, 100, yarn, 0)),
+                               ("gh_attention_decode_paged", (big, big, kv, 8, 0, 0)),
+                               ("gh_kv_evict_paged", (good, kv, None, 8, 1)), ("gh_kv_evict_paged", (kv, good, None, 8, 1))):
+                assert host.call(name, *args)[0] == INVALID, (one, other, name)
+    # one allocation, cut up
+    kv = host.kv(scored=True)
+    whole, at = host.buf(1 << 23), 0
+    for n in names:
+        size = getattr(kv.kv if n in "kv" else kv, n).bytes
+        kv = with_(kv, **{n: F.GhBuf(whole.addr + at, whole.bytes - at, 0, F.BUF_ALLOC, 0, 0)})
+        at += (size + 15) // 16 * 16
+    assert host.call("gh_attention_decode_paged", big, big, kv, 8, 0, 0)[0] == 0
