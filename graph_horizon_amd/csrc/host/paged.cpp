@@ -133,6 +133,9 @@ int write(gh_backend* b, const gh_kv_paged* kv, const gh_buf* k, const gh_buf* v
     if (tokens == 0 || n > 0x7FFFFFFFull) return fail(b, GH_E_INVALID, std::string(what) + ": tokens");
     if (!fits(k, bytes, 16) || !fits(v, bytes, 16))
         return fail(b, GH_E_RANGE, std::string(what) + ": vectors too small or not on 16 bytes");
+    const Span score = Parts(kv).part[SCORE];
+    if (meet(score, {k->addr, bytes}) || meet(score, {v->addr, bytes}))
+        return fail(b, GH_E_INVALID, std::string(what) + ": k or v overlaps the scores");
     a.p = pages(b, kv, layer);
     a.k = k->addr;
     a.v = v->addr;
@@ -153,6 +156,9 @@ int attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv_pag
     if (!fits(q, bytes, 16) || !fits(out, bytes, 16))
         return fail(b, GH_E_RANGE, "attention_decode_paged: buffer too small or not on 16 bytes");
     if (out->addr != q->addr && meet(out, bytes, q, bytes)) return fail(b, GH_E_INVALID, "attention_decode_paged: out overlaps q");
+    const Parts own(kv);
+    if (own.met({out->addr, bytes}) || meet(own.part[SCORE], {q->addr, bytes}))
+        return fail(b, GH_E_INVALID, "attention_decode_paged: out overlaps a buffer of the handle, or q its scores");
     if (max_len > capacity(kv)) return fail(b, GH_E_RANGE, "attention_decode_paged: max_len beyond the table");
     if (max_len == 0) max_len = (uint32_t)capacity(kv);
 
@@ -312,6 +318,12 @@ int gh_rope_kv_write_paged(gh_backend* b, gh_encoder* enc, const gh_kv_paged* kv
         const uint64_t heads = bytes / q_heads * kv->kv.kv_heads;
         if ((k && meet(q_out, bytes, k, heads)) || (v && meet(q_out, bytes, v, heads)))
             return fail(b, GH_E_INVALID, "rope_kv_write_paged: q_out overlaps k or v");
+        const Parts own(kv);
+        const Span turned{q_out->addr, bytes}, at{positions->addr, (uint64_t)kv->rows * 4};
+        if (own.met(turned) || meet(turned, at) || meet(own.part[SCORE], {q->addr, bytes}))
+            return fail(b, GH_E_INVALID, "rope_kv_write_paged: q_out overlaps a buffer of the handle or positions, or q its scores");
+        if (meet(at, own.part[CACHE_K]) || meet(at, own.part[CACHE_V]) || meet(at, own.part[SCORE]))
+            return fail(b, GH_E_INVALID, "rope_kv_write_paged: positions overlap the caches or the scores");
         rc = ensure_rope(b, b->rope, yarn, max_pos + 1);
         if (rc) return rc;
         GhPagedWriteArgs a{};

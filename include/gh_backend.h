@@ -215,23 +215,23 @@ int gh_attention_decode_noalloc(gh_backend* b, gh_encoder* enc, const gh_buf* ou
 /* Append: `tokens` new K and V vectors per row, FP16 [rows][tokens][kv_heads][128], to the positions
  * lengths[r] - tokens .. lengths[r] - 1 of `layer` (the lengths already count them); their scores, where
  * kept, become 0. Vectors before a row's first position (lengths[r] < tokens) are skipped. The bytes of
- * gh_kv_write. Rows must not share the pages that they append to, and k and v must not lie in slots that the
- * call writes. */
+ * gh_kv_write. Rows must not share the pages that they append to; k and v must not lie in slots that the
+ * call writes, nor in the scores. */
 int gh_kv_write_paged(gh_backend* b, gh_encoder* enc, const gh_kv_paged* kv, const gh_buf* k,
                       const gh_buf* v, uint32_t tokens, uint32_t layer);
 /* RoPE and append in one launch: token t of row r is rotated for position positions[r] + t (u32 [rows] on
  * the device; after an eviction a row stands further on than its length says), queries FP16
- * [rows][tokens][q_heads][128] from q to q_out (q itself, or no part of q, k or v) with the query's
- * post-scale, keys on their way into the cache; of skipped vectors (gh_kv_write_paged) the queries are
- * skipped too. The values of gh_rope_yarn and gh_kv_write. max_pos: the largest of the positions
+ * [rows][tokens][q_heads][128] from q to q_out (q itself, or no part of q, k or v; no part of kv's buffers
+ * or of positions) with the query's post-scale, keys on their way into the cache; of skipped vectors
+ * (gh_kv_write_paged) the queries are skipped too. The values of gh_rope_yarn and gh_kv_write. max_pos: the largest of the positions
  * positions[r] + t of this call, at most 262143 (it sizes the rotation table). */
 int gh_rope_kv_write_paged(gh_backend* b, gh_encoder* enc, const gh_kv_paged* kv, const gh_buf* q_out,
                            const gh_buf* q, const gh_buf* k, const gh_buf* v, uint32_t q_heads,
                            const gh_buf* positions, uint32_t tokens, uint32_t max_pos, const gh_yarn* yarn,
                            uint32_t layer);
 /* Attention of one new token per row over its lengths[r] positions: q, out FP16 [rows][q_heads][128] (out is
- * q itself or no part of it), 1 to 16 query heads per kv head. Free rows get zeros. max_len: no row is longer
- * (0: table_width·page_size); it sizes the launch. Where scores are kept, each position's attention weight,
+ * q itself or no part of it, and no part of kv's buffers), 1 to 16 query heads per kv head. Free rows get
+ * zeros. max_len: no row is longer (0: table_width·page_size); it sizes the launch. Where scores are kept, each position's attention weight,
  * summed over the query heads of a kv head, is added to its score. */
 int gh_attention_decode_paged(gh_backend* b, gh_encoder* enc, const gh_buf* out, const gh_buf* q,
                               const gh_kv_paged* kv, uint32_t q_heads, uint32_t max_len, uint32_t layer);

@@ -365,3 +365,36 @@ def test_a_handles_buffers_lie_apart(host):
         kv = with_(kv, **{n: F.GhBuf(whole.addr + at, whole.bytes - at, 0, F.BUF_ALLOC, 0, 0)})
         at += (size + 15) // 16 * 16
     assert host.call("gh_attention_decode_paged", big, big, kv, 8, 0, 0)[0] == 0
+
+
+def test_outputs_lie_apart_from_the_handle(host):
+    """Attention's out and the append's q_out meet no buffer of the handle, nor positions; no input lies in the scores that
+    the call writes, and positions in nothing that it writes."""
+    kv = host.kv(scored=True)
+    yarn = F.GhYarn(128, 16384, 1e6, 16.0, 32.0, 1.0, 1.0, 0.1)
+    n = 3 * 8 * 256
+    q, o, k, v, pos = host.buf(n), host.buf(n), host.buf(3 * 2 * 256), host.buf(3 * 2 * 256), host.buf(12)
+
+    def rope(o=o, q=q, k=k, v=v, pos=pos):
+        return host.call("gh_rope_kv_write_paged", kv, o, q, k, v, 8, pos, 1, 9, yarn, 0)[0]
+
+    def attend(o=o, q=q):
+        return host.call("gh_attention_decode_paged", o, q, kv, 8, 0, 0)[0]
+
+    assert rope() == attend() == 0
+    for b in (kv.kv.k, kv.kv.v, kv.table, kv.lengths, kv.score):
+        for off in (-(n - 16), 0, (b.bytes - 1) // 16 * 16):
+            bad = F.GhBuf(b.addr + off, n, 0, F.BUF_ALLOC, 0, 0)
+            assert rope(o=bad) == attend(o=bad) == INVALID
+            assert rope(o=bad, q=bad) == attend(o=bad, q=bad) == INVALID  # in place
+    s = kv.score
+    for off in (0, (s.bytes - 1) // 16 * 16):
+        bad = F.GhBuf(s.addr + off, n, 0, F.BUF_ALLOC, 0, 0)
+        assert rope(q=bad) == rope(k=bad) == rope(v=bad) == rope(pos=bad) == attend(q=bad) == INVALID
+        assert host.call("gh_kv_write_paged", kv, bad, v, 1, 0)[0] == host.call("gh_kv_write_paged", kv, k, bad, 1, 0)[0] == INVALID
+    for b in (kv.kv.k, kv.kv.v, o):
+        assert rope(pos=F.GhBuf(b.addr + b.bytes - 4, 12, 0, F.BUF_ALLOC, 0, 0)) == INVALID
+    assert rope(pos=kv.lengths) == 0
+    # vectors may come from slots of the pool that the call does not write
+    part = F.GhBuf(kv.kv.k.addr, n, 0, F.BUF_ALLOC, 0, 0)
+    assert rope(q=part) == rope(k=part) == rope(v=part) == attend(q=part) == 0
