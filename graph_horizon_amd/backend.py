@@ -134,7 +134,12 @@ class HipBackend:
         if own:
             self.begin()
         lib, h = self.lib, self.h
-        rc = getattr(lib, name)(h, self._slot, *args)
+        try:
+            rc = getattr(lib, name)(h, self._slot, *args)
+        except BaseException:  # an argument of a wrong type: nothing was recorded
+            if own:
+                self.submit()
+            raise
         if own:
             self.enc = None
             rs = lib.gh_submit(h, self._slot)
