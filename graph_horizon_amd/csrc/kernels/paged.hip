@@ -108,7 +108,8 @@ GH_KERNEL __launch_bounds__(256) void gh_paged_write(GhPagedWriteArgs a) {
 //                   twice: a lane's weights split into FP16 hi + lo (truncated, so both are positive), so
 //                   that P·V keeps 22 bits of each weight. Output row m stands for value dim 8 m + t.
 // Weights are 2^(s - m + 15), m the running maximum: hi + lo then reach 2^-39 of the largest weight. Both
-// parts are at least 2^-24, so that an infinite V gives an infinity and not infinity times 0.
+// parts are at least 2^-24, so that an infinite V gives an infinity and not infinity times 0, but those of a score
+// of -inf are 0: an infinite V gives NaN there, and a row of nothing else 0 / 0.
 // K and V are read through buffer resources whose range ends at the row's last position: what a page holds
 // past it reads as zero, without a memory access, and has weight 0. The next tile's K is asked for as soon as
 // this one's products are made, its V behind the last use of this one's: one set of registers, 126 to 158
@@ -162,15 +163,16 @@ __device__ __forceinline__ ph8 v_column(const uint4 (&v)[4], int t) {
     return __builtin_bit_cast(ph8, make_uint4(d0, d1, d0, d1));
 }
 
-// two weights' FP16 hi parts in *hi, lo parts in *lo
-__device__ __forceinline__ void weight_parts(float p0, float p1, uint32_t* hi, uint32_t* lo) {
+// two weights' FP16 hi parts in *hi, lo parts in *lo; s0, s1: their scores
+__device__ __forceinline__ void weight_parts(float p0, float p1, float s0, float s1, uint32_t* hi, uint32_t* lo) {
     typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-    const pu2 one = {1, 1};
+    const float none = -__builtin_inff();
+    const pu2 least = {(uint16_t)(s0 != none), (uint16_t)(s1 != none)};
     const uint32_t h = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(p0, p1));
     const h2 hv = __builtin_bit_cast(h2, h);
     const uint32_t l = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(p0 - (float)hv.x, p1 - (float)hv.y));
-    *hi = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(pu2, h), one));
-    *lo = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(pu2, l), one));
+    *hi = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(pu2, h), least));
+    *lo = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(pu2, l), least));
 }
 
 // A tile's addresses: K and V of one head from the slot of the tile's first position, `count` positions long
@@ -249,8 +251,8 @@ __device__ __forceinline__ void tile_add(Sums& x, pf4 st, const Tile& r) {
     for (int j = 0; j < 4; ++j) p[j] = __builtin_amdgcn_exp2f(st[j] + up);
     x.l = x.l * f + ((p[0] + p[1]) + (p[2] + p[3]));
     uint32_t h0, h1, l0, l1;
-    weight_parts(p[0], p[1], &h0, &l0);
-    weight_parts(p[2], p[3], &h1, &l1);
+    weight_parts(p[0], p[1], st[0], st[1], &h0, &l0);
+    weight_parts(p[2], p[3], st[2], st[3], &h1, &l1);
     const ph8 pv = __builtin_bit_cast(ph8, make_uint4(h0, h1, l0, l1));
 #pragma unroll
     for (int t = 0; t < 8; ++t) {

@@ -232,7 +232,9 @@ int gh_rope_kv_write_paged(gh_backend* b, gh_encoder* enc, const gh_kv_paged* kv
 /* Attention of one new token per row over its lengths[r] positions: q, out FP16 [rows][q_heads][128] (out is
  * q itself or no part of it, and no part of kv's buffers), 1 to 16 query heads per kv head. Free rows get
  * zeros. max_len: no row is longer (0: table_width·page_size); it sizes the launch. Where scores are kept, each position's attention weight,
- * summed over the query heads of a kv head, is added to its score. */
+ * summed over the query heads of a kv head, is added to its score. In the products with V a weight is held to
+ * 2^-38 of the row's largest and is at least that, unless its score is -inf: n positions add up to n·2^-38 of their
+ * mean V, and an infinite V shows whatever its finite score. A row whose scores are all -inf gives NaN. */
 int gh_attention_decode_paged(gh_backend* b, gh_encoder* enc, const gh_buf* out, const gh_buf* q,
                               const gh_kv_paged* kv, uint32_t q_heads, uint32_t max_len, uint32_t layer);
 /* Eviction by accumulated attention weight: of every row longer than `budget`, for each layer and kv head by

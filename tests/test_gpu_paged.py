@@ -704,3 +704,33 @@ def test_prefill_into_a_run_of_pages(hip, rng):
         assert np.all(np.abs(out[h * group:(h + 1) * group] - want) <= bound)
     for b in (kc, vc, kb, vb, qb, ob, table, lengths, k1, v1, q1):
         hip.free_buffer(b)
+
+
+@pytest.mark.parametrize("lengths", [[200, 90, 20], [7000, 20, 3000, 40]])  # both divisions of the work
+def test_attention_of_scores_of_minus_infinity(hip, rng, lengths):
+    """Such a position has weight 0: times an infinite V that is NaN, in its dim alone, and a row of nothing else is
+    0 / 0, whether one wave or many have it."""
+    p = Paged(hip, rng, lengths, 16, 8)
+    cells = [p.cells(r, n) for r, n in enumerate(lengths)]
+    p.k[0, cells[0][[7, 60]], 0, 0] = np.inf  # head 0 of row 0: two positions
+    p.v[0, cells[0][7], 0, 5] = np.inf
+    p.v[0, cells[0][60], 0, 6] = -np.inf
+    p.v[0, cells[0][8], 0, 7] = np.inf  # a weight like any other
+    for r in range(len(lengths)):  # head 1 of all rows: every position
+        p.k[0, cells[r], 1, 0] = np.inf
+    p.upload()
+    q = np.abs(rng.standard_normal((len(lengths), 32, D))).astype(np.float16)
+    q[:, :, 0] = -1
+    q, out = run_attention(hip, p, 32, rng, q=q)
+    assert np.isnan(out[0, :4, 5]).all() and np.isnan(out[0, :4, 6]).all() and np.all(out[0, :4, 7] == np.inf)
+    seen = np.delete(cells[0], [7, 60])
+    v = p.v[0, seen, 0].copy()
+    v[7, 7] = 0
+    want, _, bound, _ = attend(q[0, :4], p.k[0, seen, 0], v)
+    dims = np.r_[:5, 8:D]
+    assert np.all(np.abs(out[0, :4] - want)[:, dims] <= bound[:, dims])
+    assert np.isnan(out[:, 4:8]).all()
+    for r in range(len(lengths)):
+        want, _, bound, _ = attend(q[r, 8:12], p.k[0, cells[r], 2], p.v[0, cells[r], 2])
+        assert np.all(np.abs(out[r, 8:12] - want) <= bound)
+    p.free()
