@@ -95,8 +95,6 @@ const KernelName kKernels[] = {
 const char* kModules[] = {"gh_quant", "gh_gemv", "gh_glue", "gh_attention", "gh_gemm", "gh_gemm_few", "gh_paged"};
 
 constexpr uint32_t kArgmaxBlocks = 256;
-// argmax scratch at the front of the workspace: f32[256] values, u32[256] indices
-constexpr size_t kArgmaxBytes = 256 * 4 * 2;
 constexpr size_t kResultBytes = 2 * 128 * 4;  // read_argmax's index, or read_topk's 128 indices and values
 
 std::string library_dir() {

@@ -217,7 +217,11 @@ int noalloc_init(gh_backend* b);
 int hip_check(gh_backend* b, hipError_t e, const char* what);
 int launch(gh_backend* b, GhKernel k, uint32_t gx, uint32_t gy, uint32_t gz, uint32_t bx,
            const void* args, uint32_t shmem = 0);
+// argmax scratch at the front of the workspace: f32[256] values, u32[256] indices
+constexpr size_t kArgmaxBytes = 256 * 4 * 2;
 int ensure_workspace(gh_backend* b, size_t bytes);
+// What the workspace holds behind it at present.
+inline size_t workspace_room(const gh_backend* b) { return b->ws_bytes > kArgmaxBytes ? b->ws_bytes - kArgmaxBytes : 0; }
 // `bytes` of the workspace for one call's launches, 16-byte aligned, behind the argmax scratch.
 int workspace_at(gh_backend* b, size_t bytes, char** at);
 // Workgroups of `block` threads and `shmem` bytes of LDS resident on the whole device at once.

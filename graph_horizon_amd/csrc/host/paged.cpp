@@ -127,6 +127,17 @@ int entry(gh_backend* b, gh_encoder* enc, F body) {
     return latch(enc, rc);
 }
 
+// `bytes` of the workspace. It grows by half (at most 64 MiB) more than asked where there is memory for that: sizes
+// that follow the longest row rise every 16 tokens, and a growth waits for the stream and moves what recorded graphs hold.
+int scratch(gh_backend* b, uint64_t bytes, char** at) {
+    if (bytes > workspace_room(b)) {
+        const int rc = workspace_at(b, bytes + std::min<uint64_t>(bytes / 2, 64ull << 20), at);
+        if (rc != GH_E_OOM) return rc;
+        b->err.clear();
+    }
+    return workspace_at(b, bytes, at);
+}
+
 int write(gh_backend* b, const gh_kv_paged* kv, const gh_buf* k, const gh_buf* v, uint32_t tokens, uint32_t layer,
           GhPagedWriteArgs a, const char* what) {
     const uint64_t n = (uint64_t)kv->rows * tokens, bytes = n * kv->kv.kv_heads * 256;
@@ -206,7 +217,7 @@ int attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv_pag
     auto parts = [&] { return split ? (uint64_t)a.chunks * step : (uint64_t)a.chunks + step; };
     char* ws = nullptr;
     int rc = GH_OK;
-    while ((rc = workspace_at(b, layout + (acc + ml) * parts() + raw * step, &ws)) == GH_E_OOM && step > 1) {
+    while ((rc = scratch(b, layout + (acc + ml) * parts() + raw * step, &ws)) == GH_E_OOM && step > 1) {
         step = (step + 1) / 2;
         b->err.clear();
     }
@@ -277,7 +288,7 @@ int evict(gh_backend* b, const gh_kv_paged* dst, const gh_kv_paged* src, const g
     a.budget = budget;
     a.recent = recent;
     char* ws = nullptr;
-    int rc = workspace_at(b, (uint64_t)src->rows * 4 + (kept ? 0 : list * budget * 4), &ws);
+    int rc = scratch(b, (uint64_t)src->rows * 4 + (kept ? 0 : list * budget * 4), &ws);
     if (rc) return rc;
     a.act = (uint64_t)ws;
     a.kept = kept ? kept->addr : (uint64_t)ws + (uint64_t)src->rows * 4;

@@ -12,6 +12,8 @@ struct Launch {
 std::vector<Launch> launches;
 uint64_t scratch_bytes = 0, scratch_limit = 0;
 constexpr uint64_t kScratchAt = 1ull << 50;
+bool keeps_scratch = false;         // as the backend does: only a request beyond what there is asks for memory
+std::vector<uint64_t> asked;        // those requests, refused ones too
 size_t args_size(GhKernel k) {
     return k == K_PAGED_WRITE ? sizeof(GhPagedWriteArgs) : k >= K_PAGED_SELECT ? sizeof(GhPagedEvictArgs) : sizeof(GhPagedAttnArgs);
 }
@@ -31,6 +33,14 @@ int launch(gh_backend*, GhKernel k, uint32_t gx, uint32_t gy, uint32_t gz, uint3
     return GH_OK;
 }
 int workspace_at(gh_backend* b, size_t bytes, char** at) {
+    if (keeps_scratch) {
+        *at = (char*)kScratchAt;
+        if (bytes <= workspace_room(b)) return GH_OK;
+        asked.push_back(bytes);
+        if (scratch_limit && bytes > scratch_limit) return fail(b, GH_E_OOM, "scratch");
+        b->ws_bytes = bytes + kArgmaxBytes;
+        return GH_OK;
+    }
     if (scratch_limit && bytes > scratch_limit) return fail(b, GH_E_OOM, "scratch");
     scratch_bytes = bytes;
     *at = (char*)kScratchAt;
@@ -52,6 +62,10 @@ const char* host_error(gh_backend* b) { return b->err.c_str(); }
 int host_latched(gh_backend* b) { return b->enc.latched; }
 uint32_t host_rope_positions(gh_backend* b) { return b->rope.positions; }
 void host_reset(gh_backend* b, uint64_t limit) { launches.clear(), scratch_bytes = 0, scratch_limit = limit, b->enc.latched = 0, b->rope.positions = 0; }
+// from here on the scratch of one call is there for the next; returns how many requests there were so far
+uint32_t host_keep_scratch(void) { return keeps_scratch = true, (uint32_t)asked.size(); }
+void host_drop_scratch(gh_backend* b) { keeps_scratch = false, asked.clear(), b->ws_bytes = 0; }
+uint64_t host_asked(uint32_t i) { return asked[i]; }
 uint64_t host_scratch(void) { return scratch_bytes; }
 uint32_t host_launches(void) { return (uint32_t)launches.size(); }
 const void* host_launch(uint32_t i) { return &launches[i]; }

@@ -398,3 +398,43 @@ def test_outputs_lie_apart_from_the_handle(host):
     # vectors may come from slots of the pool that the call does not write
     part = F.GhBuf(kv.kv.k.addr, n, 0, F.BUF_ALLOC, 0, 0)
     assert rope(q=part) == rope(k=part) == rope(v=part) == attend(q=part) == 0
+
+
+@pytest.fixture
+def scratch(host):
+    """A host whose scratch stays from call to call: requests() are the sizes that it had to ask for."""
+    lib = host.lib
+    lib.host_drop_scratch.argtypes = [C.c_void_p]
+    lib.host_asked.restype = C.c_uint64
+    lib.host_keep_scratch()
+    host.requests = lambda: [lib.host_asked(i) for i in range(lib.host_keep_scratch())]
+    yield host
+    lib.host_drop_scratch(host.b)
+
+
+@pytest.mark.parametrize("scored", [False, True])
+def test_a_growing_length_seldom_asks_for_scratch(scratch, scored):
+    """A decode loop that passes its longest length: scratch grows with room to spare, by half."""
+    kv = scratch.kv(layers=1, slots=64, heads=8, page=64, width=64, rows=16, scored=scored)
+    q = scratch.buf(16 * 64 * 256)
+    for length in range(500, 4000):
+        assert scratch.call("gh_attention_decode_paged", q, q, kv, 64, length, 0)[0] == 0
+    assert len(scratch.requests()) <= 6  # 1.5^6 > 8
+    lists = scratch.kv(layers=4, slots=64, heads=8, page=64, width=64, rows=16, scored=True)
+    to = with_(lists, table=scratch.buf(lists.table.bytes))
+    before = len(scratch.requests())
+    for budget in range(2000, 4000, 10):
+        assert scratch.call("gh_kv_evict_paged", to, lists, None, budget, 1)[0] == 0
+    assert len(scratch.requests()) - before <= 3
+
+
+def test_scratch_without_room_to_spare_is_what_the_call_needs(scratch):
+    kv = scratch.kv(layers=1, slots=64, heads=8, page=64, width=64, rows=4, scored=True)
+    q = scratch.buf(4 * 64 * 256)
+    assert scratch.call("gh_attention_decode_paged", q, q, kv, 64, 4000, 0)[0] == 0
+    with_room = scratch.requests()[0]
+    scratch.lib.host_drop_scratch(scratch.b)
+    scratch.lib.host_keep_scratch()
+    rc, got = scratch.call("gh_attention_decode_paged", q, q, kv, 64, 4000, 0, limit=with_room - 1)
+    first, second = scratch.requests()
+    assert rc == 0 and len(got) == 2 and first == with_room and second < with_room <= 3 * second // 2 + 1
