@@ -898,6 +898,7 @@ int gh_free_buffer(gh_backend* b, gh_buf* buf) {
         return fail(b, GH_E_INVALID, "free_buffer: a view never owns its storage");
     int rc = hip_check(b, hipStreamSynchronize(b->stream), "hipStreamSynchronize");
     if (!rc) rc = hip_check(b, hipFree((void*)buf->addr), "hipFree");
+    if (!rc && buf->bytes >= b->ws_short / 8) b->ws_short = 0;  // scratch that could not be had may be there now
     if (buf->kind == GH_BUF_WEIGHT) b->w16.erase(buf->addr);  // its FP16 copy no longer applies
     *buf = gh_buf{};
     return rc;
@@ -1815,6 +1816,7 @@ int gh_stream_probe(gh_backend* b, gh_encoder* enc, const gh_buf* src, uint64_t 
 int gh_set_scratch_limit(gh_backend* b, uint64_t bytes) {
     if (!b) return GH_E_INVALID;
     b->scratch_limit = bytes;
+    b->ws_short = 0;
     return GH_OK;
 }
 

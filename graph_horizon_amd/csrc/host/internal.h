@@ -178,6 +178,10 @@ struct gh_backend {
     // pinned host word in which the paged kernels leave what they found wrong (GH_PAGED_*), 0: nothing
     volatile uint32_t* paged_fault = nullptr;
     size_t ws_bytes = 0;
+    // the least scratch that a paged operator could not have (0: none so far, or much was freed since), and how
+    // many calls did with less without asking
+    uint64_t ws_short = 0;
+    uint32_t ws_did_with_less = 0;
     void* counters = nullptr;  // attention merge counters, zero between launches
     size_t counter_slots = 0;
     size_t scratch_limit = 0;  // gh_set_scratch_limit: larger scratch blocks fail as without memory; 0: none

@@ -130,12 +130,20 @@ int entry(gh_backend* b, gh_encoder* enc, F body) {
 // `bytes` of the workspace. It grows by half (at most 64 MiB) more than asked where there is memory for that: sizes
 // that follow the longest row rise every 16 tokens, and a growth waits for the stream and moves what recorded graphs hold.
 int scratch(gh_backend* b, uint64_t bytes, char** at) {
-    if (bytes > workspace_room(b)) {
-        const int rc = workspace_at(b, bytes + std::min<uint64_t>(bytes / 2, 64ull << 20), at);
+    auto ask = [&](uint64_t n) {
+        const bool grows = n > workspace_room(b);
+        const int rc = workspace_at(b, n, at);
+        if (rc == GH_E_OOM) b->ws_short = b->ws_short ? std::min(b->ws_short, n) : n;
+        else if (!rc && grows && n >= b->ws_short) b->ws_short = 0;
+        return rc;
+    };
+    const uint64_t more = bytes + std::min<uint64_t>(bytes / 2, 64ull << 20);
+    if (bytes > workspace_room(b) && (!b->ws_short || more < b->ws_short)) {
+        const int rc = ask(more);
         if (rc != GH_E_OOM) return rc;
         b->err.clear();
     }
-    return workspace_at(b, bytes, at);
+    return ask(bytes);
 }
 
 int write(gh_backend* b, const gh_kv_paged* kv, const gh_buf* k, const gh_buf* v, uint32_t tokens, uint32_t layer,
@@ -215,13 +223,24 @@ int attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv_pag
     const uint64_t room = std::min<uint64_t>((512ull << 20) / per, (1u << 30) / tiles1);  // tiles count in 32 bits
     uint32_t step = (uint32_t)std::min<uint64_t>(std::min(kv->rows, kPagedRows), std::max<uint64_t>(1, room));
     auto parts = [&] { return split ? (uint64_t)a.chunks * step : (uint64_t)a.chunks + step; };
+    auto need = [&] { return layout + (acc + ml) * parts() + raw * step; };
+    // Where memory was short (ws_short), the scratch that there is holds half or more of what could be had then, and rows take
+    // turns in it: a refusal costs two allocations, two frees and a wait. Every 256th such call asks for all again, as others
+    // may have freed memory. Where it holds not one row, as many are tried as were not refused.
+    if (b->ws_short && need() > workspace_room(b)) {
+        const uint64_t fixed = layout + (split ? 0 : (acc + ml) * a.chunks);
+        auto rows_in = [&](uint64_t bytes) { return bytes > fixed ? (uint32_t)std::min<uint64_t>((bytes - fixed) / per, step) : 0; };
+        const uint32_t now = rows_in(workspace_room(b)), untried = rows_in(b->ws_short - 1);
+        if (++b->ws_did_with_less % 256 == 0) b->ws_short = 0;
+        else if (now || untried) step = now ? now : untried;
+    }
     char* ws = nullptr;
     int rc = GH_OK;
-    while ((rc = scratch(b, layout + (acc + ml) * parts() + raw * step, &ws)) == GH_E_OOM && step > 1) {
+    while ((rc = scratch(b, need(), &ws)) == GH_E_OOM && step > 1) {
         step = (step + 1) / 2;
         b->err.clear();
     }
-    if (rc) return rc;
+    if (rc) return b->ws_short = 0, rc;
     a.layout = split ? 0 : (uint64_t)ws;
     a.part_acc = (uint64_t)ws + layout;
     a.raw = scored ? a.part_acc + acc * parts() : 0;
@@ -289,7 +308,7 @@ int evict(gh_backend* b, const gh_kv_paged* dst, const gh_kv_paged* src, const g
     a.recent = recent;
     char* ws = nullptr;
     int rc = scratch(b, (uint64_t)src->rows * 4 + (kept ? 0 : list * budget * 4), &ws);
-    if (rc) return rc;
+    if (rc) return b->ws_short = 0, rc;
     a.act = (uint64_t)ws;
     a.kept = kept ? kept->addr : (uint64_t)ws + (uint64_t)src->rows * 4;
     rc = launch(b, K_PAGED_SELECT, s.kv_heads, src->rows, s.block_count, 512, &a);

@@ -734,3 +734,41 @@ def test_attention_of_scores_of_minus_infinity(hip, rng, lengths):
         want, _, bound, _ = attend(q[r, 8:12], p.k[0, cells[r], 2], p.v[0, cells[r], 2])
         assert np.all(np.abs(out[r, 8:12] - want) <= bound)
     p.free()
+
+
+def test_attention_without_memory_does_not_ask_each_time(rng):
+    """Calls after the first keep the scratch that it found; with memory again the rows go together."""
+    with HipBackend(0) as hip:
+        p = Paged(hip, rng, [3000, 100, 2000, 1, 700], 16, 8, scored=True)
+        hip.set_scratch_limit(20 << 20)  # all rows: 25 MB
+        q = None
+        for call in range(4):
+            before = p.read("score")
+            q, out = run_attention(hip, p, 128, rng, q=q)
+            check_attention(p, 0, q, out, before, p.read("score"))
+            info = hip.scratch_info()
+            assert call == 0 or info == last
+            last = info
+        hip.set_scratch_limit(0)
+        before = p.read("score")
+        q, out = run_attention(hip, p, 128, rng, q=q)
+        check_attention(p, 0, q, out, before, p.read("score"))
+        assert hip.scratch_info()[0] > last[0]
+        p.free()
+
+
+def test_attention_of_growing_rows_seldom_moves_its_scratch(rng):
+    """The call's longest row from 600 to 3000 in steps of 16: five times half as much again."""
+    with HipBackend(0) as hip:
+        p = Paged(hip, rng, [3000] * 8, 16, 8, scored=True)
+        qb = hip.from_host(rng.standard_normal((8, 128, D)).astype(np.float16))
+        ob, lengths = hip.alloc_buffer(qb.bytes), p.bufs["lengths"]
+        sizes = []
+        for n in range(600, 3001, 16):
+            hip.upload(lengths, np.full(8, n, np.uint32))
+            hip.attention_decode_paged(ob, qb, p.handle(), 128, n, 0)
+            sizes.append(hip.scratch_info()[0])
+        assert len(set(sizes)) <= 6
+        hip.free_buffer(qb)
+        hip.free_buffer(ob)
+        p.free()

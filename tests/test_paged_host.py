@@ -438,3 +438,54 @@ def test_scratch_without_room_to_spare_is_what_the_call_needs(scratch):
     rc, got = scratch.call("gh_attention_decode_paged", q, q, kv, 64, 4000, 0, limit=with_room - 1)
     first, second = scratch.requests()
     assert rc == 0 and len(got) == 2 and first == with_room and second < with_room <= 3 * second // 2 + 1
+
+
+def rows_of(host, got):
+    """Rows of each attention launch."""
+    return [AttnArgs.from_buffer_copy(bytes(g.args)).rows for g in got if g.kernel not in (host.ids["join"], host.ids["join2"])]
+
+
+@pytest.mark.parametrize("scored,heads", [(True, 8), (False, 8), (False, 64)])
+def test_scratch_that_could_not_be_had_is_not_asked_for_again(scratch, scored, heads):
+    """With memory for some of the rows only the first call looks for how many; later ones take turns in what there
+    is, also where a row's share grows, and now and then one looks again."""
+    rows = 64
+    kv = scratch.kv(layers=1, slots=64, heads=heads, page=64, width=64, rows=rows, scored=scored)
+    q = scratch.buf(rows * 8 * heads * 256)
+
+    def call(max_len, limit):
+        return scratch.call("gh_attention_decode_paged", q, q, kv, 8 * heads, max_len, 0, limit=limit)
+
+    rc, got = call(500, 0)
+    need = scratch.requests()[0] * 2 // 3  # without the room to spare
+    scratch.lib.host_drop_scratch(scratch.b)
+    scratch.lib.host_keep_scratch()
+    limit = need // 3
+    rc, got = call(500, limit)
+    taken = rows_of(scratch, got)
+    assert rc == 0 and sum(taken) == rows and len(taken) > 2
+    found = len(scratch.requests())
+    assert found > 2
+    for length in [500] * 40 + list(range(500, 512)):
+        rc, got = call(length, limit)
+        assert rc == 0 and sum(rows_of(scratch, got)) == rows and len(rows_of(scratch, got)) <= len(taken)
+    assert len(scratch.requests()) == found
+    calls = 0
+    while len(rows_of(scratch, call(500, 0)[1])) > 1:
+        calls += 1
+        assert calls < 300
+    assert len(scratch.requests()) == found + 1
+
+
+def test_scratch_for_longer_rows_under_a_limit(scratch):
+    kv = scratch.kv(layers=1, slots=64, heads=8, page=64, width=64, rows=16, scored=True)
+    q = scratch.buf(16 * 64 * 256)
+    limit = 12 << 20  # the chunks take 8.1 MiB of it
+    for length in range(600, 2600, 10):
+        rc, got = scratch.call("gh_attention_decode_paged", q, q, kv, 64, length, 0, limit=limit)
+        assert rc == 0 and sum(rows_of(scratch, got)) == 16
+    assert len(scratch.requests()) <= 8
+    # a row that fits nowhere is an error each time, and shorter ones go on
+    for _ in range(3):
+        assert scratch.call("gh_attention_decode_paged", q, q, kv, 64, 4096, 0, limit=1 << 20)[0] in (0, OOM)
+        assert scratch.call("gh_attention_decode_paged", q, q, kv, 64, 2600, 0, limit=limit)[0] == 0
