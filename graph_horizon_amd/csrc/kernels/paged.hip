@@ -319,6 +319,10 @@ __device__ __forceinline__ uint32_t lay_out_rows(const GhPagedAttnArgs& a, RowsL
         sh.len[lane] = n;
         if (lane == 0) sh.first[0] = 0;
         sh.first[lane + 1] = upto;
+        // The wave reads what its other lanes wrote, and the other waves write the same values over it: nothing waits for
+        // them, and the fence keeps the wave's own writes before its reads.
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
         return upto;
     }
     uint32_t n[2], t[2];
