@@ -772,3 +772,252 @@ def test_attention_of_growing_rows_seldom_moves_its_scratch(rng):
         hip.free_buffer(qb)
         hip.free_buffer(ob)
         p.free()
+
+
+# ---- batches of many rows, chunks of many tiles ----
+
+def many_lengths(rng, rows, most):
+    """Rows up to `most`, some free, one of them at the front, the last one whole."""
+    lengths = [int(n) for n in rng.integers(1, most + 1, rows)]
+    for r in rng.choice(rows, rows // 10, replace=False):
+        lengths[r] = 0
+    lengths[0], lengths[-1] = 0, most
+    return lengths
+
+
+@pytest.mark.parametrize("scored", [False, True])
+@pytest.mark.parametrize("rows,heads,most,width", [
+    (64, 4, 700, 64), (65, 4, 700, 64),   # chunks, up to 64 rows and past them
+    (130, 2, 300, 64), (300, 2, 150, 64), (512, 1, 100, 40), (600, 1, 120, 40),  # chunks, 600 in two groups
+    (100, 1, 300, 19),                    # spans, five a row
+    (600, 2, 90, 6),                      # spans, one a row, two groups of rows
+])
+def test_attention_of_many_rows(hip, rng, rows, heads, most, width, scored):
+    p = Paged(hip, rng, many_lengths(rng, rows, most), 16, heads, width=width, scored=scored)
+    before = p.read("score") if scored else None
+    q, out = run_attention(hip, p, 4 * heads, rng)
+    check_attention(p, 0, q, out, before, p.read("score") if scored else None)
+    p.free()
+
+
+@pytest.mark.parametrize("scored", [False, True])
+def test_attention_of_many_tiles_a_wave(hip, rng, scored):
+    """64 kv heads: 32 chunks of 79 tiles, more than a wave looks up at once, with rows that begin at tiles 65, 66 and 69 of
+    a chunk. Rows go over the same pages again and again."""
+    heads, lengths = 64, [20000, 5, 1300, 19003]
+    p = Paged(hip, rng, [256] * 4, 16, heads, width=1250, scored=scored)
+    used = p.table[:, :16].ravel()
+    p.table = rng.choice(used, (4, 1250)).astype(np.uint32)
+    p.lengths = np.array(lengths, np.uint32)
+    hip.upload(p.bufs["table"], p.table)
+    hip.upload(p.bufs["lengths"], p.lengths)
+    before = p.read("score") if scored else None
+    q, out = run_attention(hip, p, 2 * heads, rng)
+    after = p.read("score") if scored else None
+    for r, n in enumerate(lengths):
+        s = p.cells(r, n)
+        for h in (0, 3, 31, 62, 63):
+            want, w, bound, wb = attend(q[r, 2 * h:2 * h + 2], p.k[0, s, h], p.v[0, s, h])
+            assert np.all(np.abs(out[r, 2 * h:2 * h + 2] - want) <= bound), (r, h)
+            if scored:
+                total = before[0, r, h, :n].astype(np.float64) + w.sum(0)
+                assert np.all(np.abs(after[0, r, h, :n] - total) <= wb.sum(0) + 3 * 2.0 ** -24 * total), (r, h)
+                assert np.array_equal(after[0, r, h, n:], before[0, r, h, n:])
+    p.free()
+
+
+# ---- what the host cannot check, in every division of the work ----
+
+@pytest.mark.parametrize("bad", ["length", "max_len", "page", "last_page"])
+@pytest.mark.parametrize("rows,heads,most,width", [
+    (24, 8, 700, 100), (80, 2, 700, 64),  # chunks
+    (3, 2, 300, 19), (100, 1, 300, 19),   # spans
+])
+def test_attention_of_bad_rows_leaves_the_others_alone(hip, rng, rows, heads, most, width, bad):
+    """GH_E_RANGE at the submit; other rows' outputs and scores are as ever, and so are all scores past the rows. The
+    next call works."""
+    p = Paged(hip, rng, many_lengths(rng, rows, most), 16, heads, width=width, scored=True)
+    odd = rows // 2
+    if p.lengths[odd] < 40:  # of the length before it
+        p.lengths[odd], p.table[odd] = p.lengths[-1], p.table[-1]
+    good_lengths, good_table = p.lengths.copy(), p.table.copy()
+    n = int(good_lengths[odd])
+    max_len = 0
+    if bad == "length":
+        p.lengths[odd] = 16 * width + 1
+    elif bad == "max_len":
+        max_len = most
+        p.lengths[odd] = most + 1
+        if most + 1 <= 16 * width:
+            p.table[odd] = p.table[-1, 0]
+    else:
+        p.table[odd, 1 if bad == "page" else (n - 1) // 16] = p.slots // 16 if bad == "page" else 0xFFFFFFFF
+    p.upload()
+    before = p.read("score")
+    q = rng.standard_normal((rows, 4 * heads, D)).astype(np.float16)
+    qb, ob = hip.from_host(q), hip.from_host(np.full((rows + 1, 4 * heads, D), 7, np.float16))
+    with pytest.raises(GhError) as e:
+        hip.attention_decode_paged(ob, qb, p.handle(), 4 * heads, max_len, 0)
+    assert e.value.code == -5
+    out, after = hip.download(ob, np.float16, (rows + 1) * 4 * heads * D).reshape(rows + 1, 4 * heads, D), p.read("score")
+    assert np.all(out[rows] == 7)
+    others = np.arange(rows) != odd
+    p.lengths = np.where(others, good_lengths, 0)
+    out[odd] = 0
+    after[:, odd] = before[:, odd]
+    check_attention(p, 0, q, out[:rows], before, after)
+    p.lengths, p.table = good_lengths, good_table
+    p.upload()
+    hip.attention_decode_paged(ob, qb, p.handle(), 4 * heads, max_len, 0)
+    got = hip.download(ob, np.float16, rows * 4 * heads * D).reshape(rows, 4 * heads, D)
+    check_attention(p, 0, q, got)
+    for b in (qb, ob):
+        hip.free_buffer(b)
+    p.free()
+
+
+@pytest.mark.parametrize("bad", ["length", "page"])
+@pytest.mark.parametrize("tokens", [1, 5])
+def test_writes_of_bad_rows_leave_everything_else_alone(hip, rng, bad, tokens):
+    """The whole pool and the scores: rows 0 and 2 have their vectors, nothing else changed."""
+    p = Paged(hip, rng, [100, 96, 300], 16, 2, layers=2, scored=True)
+    good = p.lengths.copy()
+    at = [p.cells(r, int(good[r]))[-tokens:] for r in range(3)]
+    if bad == "length":
+        p.lengths[1] = 16 * p.width + 1
+    else:
+        p.table[1, 5] = p.slots // 16  # the page of all its new positions
+    p.upload()
+    k, v = (rng.standard_normal((3, tokens, 2, D)).astype(np.float16) for _ in range(2))
+    kb, vb = hip.from_host(k), hip.from_host(v)
+    with pytest.raises(GhError) as e:
+        hip.kv_write_paged(p.handle(), kb, vb, tokens, 1)
+    assert e.value.code == -5
+    for r in (0, 2):
+        p.k[1, at[r]], p.v[1, at[r]] = k[r], v[r]
+        p.score[1, r, :, int(good[r]) - tokens:int(good[r])] = 0
+    for name in ("k", "v", "score", "table", "lengths"):
+        assert np.array_equal(p.read(name).view(np.uint8), getattr(p, name).view(np.uint8)), name
+    hip.free_buffer(kb)
+    hip.free_buffer(vb)
+    p.free()
+
+
+@pytest.mark.parametrize("tokens", [1, 5])
+@pytest.mark.parametrize("over", [1, 3])
+def test_positions_past_max_pos_touch_no_memory(hip, rng, tokens, over):
+    """Of a row whose last `over` tokens lie past max_pos those are skipped, in the queries, the pool and the scores."""
+    heads, group, max_pos = 2, 4, 500
+    lengths, q_heads = [100, 96, 300], heads * group
+    p = Paged(hip, rng, lengths, 16, heads, scored=True)
+    positions = np.array([7, max_pos - tokens + 1 + over, 450], np.uint32)
+    q = rng.standard_normal((3, tokens, q_heads, D)).astype(np.float16)
+    k, v = (rng.standard_normal((3, tokens, heads, D)).astype(np.float16) for _ in range(2))
+    qb, kb, vb, pb, ob = (hip.from_host(x) for x in (q, k, v, positions, np.full_like(q, 7)))
+    with pytest.raises(GhError) as e:
+        hip.rope_kv_write_paged(p.handle(), ob, qb, kb, vb, q_heads, pb, tokens, max_pos, YARN, 0)
+    assert e.value.code == -5
+    got = hip.download(ob, np.float16, q.size).reshape(q.shape)
+    skipped = np.zeros((3, tokens), bool)
+    skipped[1, max(0, tokens - over):] = True
+    for r in range(3):
+        for t in range(tokens):
+            at = p.cells(r, lengths[r])[lengths[r] - tokens + t]
+            if skipped[r, t]:
+                assert np.all(got[r, t] == 7)
+                continue
+            for name, x, role in (("q", q[r, t], F.ROPE_QUERY), ("k", k[r, t], F.ROPE_KEY)):
+                b = hip.from_host(x)
+                hip.rope_yarn(b, len(x), D, int(positions[r]) + t, YARN, role)
+                y = hip.download(b, np.float16, x.size).reshape(x.shape)
+                hip.free_buffer(b)
+                if name == "q":
+                    assert np.array_equal(got[r, t].view(np.uint16), y.view(np.uint16))
+                else:
+                    p.k[0, at] = y
+            p.v[0, at] = v[r, t]
+            p.score[0, r, :, lengths[r] - tokens + t] = 0
+    for name in ("k", "v", "score"):
+        assert np.array_equal(p.read(name).view(np.uint8), getattr(p, name).view(np.uint8)), name
+    for b in (qb, kb, vb, pb, ob):
+        hip.free_buffer(b)
+    p.free()
+
+
+def test_rope_write_at_far_positions_has_the_bits_of_the_single_operations(hip, rng):
+    """Past the original context, where queries have a temperature, and up to the last position of the table."""
+    positions = np.array([16383, 16384, 100001, 262142], np.uint32)
+    p = Paged(hip, rng, [20, 30, 2, 33], 16, 2)
+    q = rng.standard_normal((4, 2, 8, D)).astype(np.float16)
+    k, v = (rng.standard_normal((4, 2, 2, D)).astype(np.float16) for _ in range(2))
+    qb, kb, vb, pb, ob = (hip.from_host(x) for x in (q, k, v, positions, q))
+    hip.rope_kv_write_paged(p.handle(), ob, qb, kb, vb, 8, pb, 2, 262143, YARN, 0)
+    got, pool = hip.download(ob, np.float16, q.size).reshape(q.shape), p.read("k")
+    for r in range(4):
+        for t in range(2):
+            at = p.cells(r, int(p.lengths[r]))[int(p.lengths[r]) - 2 + t]
+            for x, y, role in ((q[r, t], got[r, t], F.ROPE_QUERY), (k[r, t], pool[0, at], F.ROPE_KEY)):
+                b = hip.from_host(x)
+                hip.rope_yarn(b, len(x), D, int(positions[r]) + t, YARN, role)
+                assert np.array_equal(hip.download(b, np.float16, x.size).view(np.uint16), y.ravel().view(np.uint16))
+                hip.free_buffer(b)
+    for b in (qb, kb, vb, pb, ob):
+        hip.free_buffer(b)
+    p.free()
+
+
+@pytest.mark.parametrize("bad", ["length", "page", "dst_page"])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_eviction_of_bad_rows_leaves_the_others_alone(hip, rng, bad, in_place):
+    """Row 1 has a length or a page that does not fit: rows 0 and 2 move as ever, row 3 stays, no page of another row is
+    written, and of a row whose length is bad nothing is."""
+    lengths, budget, recent, heads = [100, 90, 300, 40], 50, 10, 2
+    src = Paged(hip, rng, lengths, 16, heads, 2, scored=True)
+    dst = Paged(hip, rng, [budget] * 3 + [0], 16, heads, 2, scored=True, width=src.width if in_place else None, garbage=np.float16(3))
+    dst.k[:], dst.v[:], dst.score[:] = 3, 4, -1
+    dst.lengths = np.arange(90, 94, dtype=np.uint32)
+    mine = dst.cells(1, 64)
+    if bad == "length":
+        src.lengths[1] = 16 * src.width + 1
+    elif bad == "page":
+        src.table[1, :6] = src.slots // 16
+    else:
+        dst.table[1, :4] = dst.slots // 16
+    src.upload()
+    dst.upload()
+    if in_place:
+        dst.score, dst.lengths = src.score.copy(), src.lengths.copy()
+        for name in ("score", "lengths"):
+            hip.free_buffer(dst.bufs[name])
+            dst.bufs[name] = src.bufs[name]
+    kept = hip.from_host(np.full((2, 4, heads, budget), 99999, np.uint32))
+    with pytest.raises(GhError) as e:
+        hip.kv_evict_paged(dst.handle(), src.handle(), kept, budget, recent)
+    assert e.value.code == -5
+    got = hip.download(kept, np.uint32, 8 * heads * budget).reshape(2, 4, heads, budget)
+    want_kept = np.full_like(got, 99999)
+    for r in (0, 2):
+        dst.lengths[r] = budget
+        old, new = src.cells(r, lengths[r]), dst.cells(r, budget)
+        for layer in range(2):
+            for h in range(heads):
+                best = keep(src.score[layer, r, h, :lengths[r]], budget, recent)
+                want_kept[layer, r, h] = best
+                dst.score[layer, r, h, :budget] = src.score[layer, r, h, best]
+                dst.k[layer, new, h], dst.v[layer, new, h] = src.k[layer, old[best], h], src.v[layer, old[best], h]
+    now = {name: dst.read(name) for name in ("k", "v", "score", "lengths")}
+    if bad != "length":  # its results are unspecified, within its own pages, scores, list and length
+        got[:, 1] = want_kept[:, 1]
+        now["score"][:, 1] = dst.score[:, 1]
+        now["lengths"][1] = dst.lengths[1]
+        now["k"][:, mine], now["v"][:, mine] = dst.k[:, mine], dst.v[:, mine]
+    assert np.array_equal(got, want_kept)
+    for name, x in now.items():
+        assert np.array_equal(x.view(np.uint8), getattr(dst, name).view(np.uint8)), name
+    for name in ("k", "v", "table") + (() if in_place else ("lengths", "score")):
+        assert np.array_equal(src.read(name).view(np.uint8), getattr(src, name).view(np.uint8)), "source " + name
+    hip.free_buffer(kept)
+    if in_place:
+        dst.bufs.pop("score"), dst.bufs.pop("lengths")
+    src.free()
+    dst.free()
