@@ -72,3 +72,33 @@ const void* host_launch(uint32_t i) { return &launches[i]; }
 // kernel ids: write, the first attention, join, select, move, join in halves
 void host_kernels(uint32_t* k) { k[0] = K_PAGED_WRITE, k[1] = K_PAGED_ATTN, k[2] = K_PAGED_JOIN, k[3] = K_PAGED_SELECT, k[4] = K_PAGED_MOVE, k[5] = K_PAGED_JOIN2; }
 }
+
+// sizes and offsets of what the tests read through their own declarations
+#include <cstddef>
+extern "C" {
+struct HostField {
+    const char* name;
+    uint32_t offset, size;
+};
+#define FIELD(type, name) {#name, (uint32_t)offsetof(type, name), (uint32_t)sizeof(((type*)nullptr)->name)}
+const HostField* host_pages_fields(void) {
+    static const HostField f[] = {FIELD(GhPages, kc), FIELD(GhPages, vc), FIELD(GhPages, table), FIELD(GhPages, lengths),
+                                  FIELD(GhPages, score), FIELD(GhPages, fault), FIELD(GhPages, width), FIELD(GhPages, shift),
+                                  FIELD(GhPages, pages), FIELD(GhPages, kv_heads), {nullptr, sizeof(GhPages), 0}};
+    return f;
+}
+const HostField* host_attn_fields(void) {
+    static const HostField f[] = {FIELD(GhPagedAttnArgs, p), FIELD(GhPagedAttnArgs, q), FIELD(GhPagedAttnArgs, out),
+                                  FIELD(GhPagedAttnArgs, part_acc), FIELD(GhPagedAttnArgs, part_ml), FIELD(GhPagedAttnArgs, raw),
+                                  FIELD(GhPagedAttnArgs, stream), FIELD(GhPagedAttnArgs, layout), FIELD(GhPagedAttnArgs, q_heads),
+                                  FIELD(GhPagedAttnArgs, group), FIELD(GhPagedAttnArgs, rows), FIELD(GhPagedAttnArgs, max_len),
+                                  FIELD(GhPagedAttnArgs, chunks), FIELD(GhPagedAttnArgs, least), FIELD(GhPagedAttnArgs, solo),
+                                  FIELD(GhPagedAttnArgs, raw_len), FIELD(GhPagedAttnArgs, scale), FIELD(GhPagedAttnArgs, blocks),
+                                  {nullptr, sizeof(GhPagedAttnArgs), 0}};
+    return f;
+}
+static_assert(K_PAGED_ATTN_S == K_PAGED_ATTN + 1 && K_PAGED_SPLIT == K_PAGED_ATTN + 2 && K_PAGED_SPLIT_S == K_PAGED_ATTN + 3,
+              "the tests tell the attention kernels apart by their distance from the first");
+static_assert(K_PAGED_WRITE < K_PAGED_SELECT && K_PAGED_JOIN2 < K_PAGED_SELECT && K_PAGED_MOVE_S + 1 == K_COUNT,
+              "args_size takes every kernel from the selection on for one of the eviction");
+}

@@ -489,3 +489,21 @@ def test_scratch_for_longer_rows_under_a_limit(scratch):
     for _ in range(3):
         assert scratch.call("gh_attention_decode_paged", q, q, kv, 64, 4096, 0, limit=1 << 20)[0] in (0, OOM)
         assert scratch.call("gh_attention_decode_paged", q, q, kv, 64, 2600, 0, limit=limit)[0] == 0
+
+
+class Field(C.Structure):
+    _fields_ = [("name", C.c_char_p), ("offset", C.c_uint32), ("size", C.c_uint32)]
+
+
+@pytest.mark.parametrize("which,mine", [("host_pages_fields", Pages), ("host_attn_fields", AttnArgs)])
+def test_argument_structures_are_the_kernels(lib, which, mine):
+    """Pages and AttnArgs above have the fields, offsets and sizes of the ones in gh_kargs.h."""
+    call = getattr(lib, which)
+    call.restype = C.POINTER(Field)
+    fields, i = call(), 0
+    while fields[i].name:
+        name, kind = mine._fields_[i]
+        assert fields[i].name.decode() == name
+        assert (fields[i].offset, fields[i].size) == (getattr(mine, name).offset, C.sizeof(kind)), name
+        i += 1
+    assert i == len(mine._fields_) and fields[i].offset == C.sizeof(mine)
