@@ -193,9 +193,9 @@ int attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv_pag
     // Tiles of 16 positions and kv heads (8 KiB of K and V) that the rows can hold. Rows of one span, or few
     // tiles in all: each row by itself in fixed spans (gh_paged_split), which start sooner (no row needs the
     // others' lengths) and need no join where a row has one span; else all rows together in equal chunks
-    // (gh_paged_attn), which balances ragged rows. us, spans / chunks: 1 row of 500 8.3 / 10.4, 3 of 3000 13.9 /
-    // 15.3, 256 of up to 300 40.8 / 54, 12 of up to 1000 15.1 / 15.0, 64 of up to 600 29.3 / 25.3, 8 of up to 8192
-    // 46.3 / 34.2, 32 of up to 4000 70.8 / 54.2.
+    // (gh_paged_attn), which balances ragged rows. us back to back, spans / chunks: 1 row of 500 9.4 / 11.9, 3 of
+    // 3000 14.0 / 15.4, 256 of up to 300 40.4 / 48.0, 12 of up to 1000 15.2 / 14.4, 64 of up to 600 28.5 / 22.9, 8 of
+    // up to 8192 45.9 / 33.4, 32 of up to 4000 69.3 / 52.0.
     const uint32_t tiles1 = ceil_div(max_len, 16);
     const uint64_t most = (uint64_t)kv->rows * hk * tiles1;
     const bool split = tiles1 <= kSpanTiles || most < 6144;
@@ -206,15 +206,15 @@ int attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv_pag
         a.chunks = ceil_div(tiles1, a.least);
     } else {
         // eight waves per CU, all of them at once: with more, the rows' streams disturb each other (64 rows of
-        // 8192 with 4 / 6 / 8 / 10 / 12 waves per CU: 394 / 377 / 326 / 381 / 344 us). Half of them where that
+        // 8192 with 4 / 6 / 8 / 10 / 12 waves per CU: 389 / 376 / 324 / 378 / 342 us). Half of them where that
         // gives a wave at most 12 tiles: a second workgroup on some CUs would only make those the last
-        // (16 rows of up to 2500: 31.8 / 26.9 us).
+        // (16 rows of up to 2500: 29.2 / 26.5 us).
         a.least = 4;
         a.chunks = std::max(1u, 8 * b->cus / hk);
         a.solo = 12;
     }
     // From half the last-level cache on, the next call will not find this one's K and V there, and reads past
-    // it are faster (64 rows of 8192 368 / 346 us, 1 of 32768 36.0 / 34.0; 16 of up to 2500, 83 MB: 31.2 / 37.7).
+    // it are faster (64 rows of 8192 362 / 324 us, 1 of 32768 33.8 / 31.6; 16 of up to 2500, 83 MB: 26.2 / 32.3).
     a.stream = kStreamBytes;
     // scratch of a row: its partials, and with scores each query head's
     const uint64_t acc = (uint64_t)q_heads * 512, ml = acc / 64, raw = scored ? (uint64_t)q_heads * a.raw_len * 4 : 0;

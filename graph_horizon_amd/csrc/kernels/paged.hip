@@ -48,7 +48,7 @@ __device__ __forceinline__ uint32_t slot_of(const GhPages& p, uint32_t row, uint
 // Thread = 8 values (16 bytes) of one head of one token: the token's query heads, then its key and value
 // heads; a.groups workgroups per token. Rotation as in gh_rope: adjacent pairs turned by the (position, pair)
 // table's (cos, sin) in FP32, queries times the post-scale, one rounding. Bound by launch latency at decode
-// sizes (256 tokens of 32 + 8 heads 3.9 us) and by memory at prompt sizes (2000 tokens of 8 heads, 16 MB, 4.6 us);
+// sizes (256 tokens of 32 + 8 heads 4.1 us traced) and by memory at prompt sizes (2000 tokens of 8 heads, 16 MB, 4.9 us);
 // the vector, the row's length and its position are asked for at once.
 namespace {
 __device__ __forceinline__ uint32_t turn(uint32_t v, float2 c, float scale) {
@@ -112,9 +112,9 @@ GH_KERNEL __launch_bounds__(256) void gh_paged_write(GhPagedWriteArgs a) {
 // of -inf are 0: an infinite V gives NaN there, and a row of nothing else 0 / 0.
 // K and V are read through buffer resources whose range ends at the row's last position: what a page holds
 // past it reads as zero, without a memory access, and has weight 0. The next tile's K is asked for as soon as
-// this one's products are made, its V behind the last use of this one's: one set of registers, 126 to 158
-// VGPRs. (A second and third set of registers, with 146 and 178 VGPRs, measured no different: 64 rows of 8192
-// 365 / 363 us, at 366 with one.)
+// this one's products are made, its V behind the last use of this one's: one set of registers, 125 to 154
+// VGPRs. (Two sets: 64 rows of 8192 330 / 333 us with the wait for the call, with half the waves per CU 394 / 403.)
+// Other times of attention here are of calls back to back, both launches.
 // Two divisions of the work over waves, paged_attn and paged_split (the host's rule says when), then
 // gh_paged_join where a row is in several parts.
 namespace {
@@ -454,7 +454,7 @@ __device__ __forceinline__ void paged_chunk(const GhPagedAttnArgs& a, const Rows
 
 // All rows' tiles in equal chunks. Grid: a wave per (chunk, kv head), heads first, 256 threads. A workgroup's
 // four waves read four heads of the same positions, 1 KiB in a row per position (four chunks of one head
-// instead: 64 rows of 8192 346 -> 396 us). The number of tiles is known on the device alone: every workgroup
+// instead: 64 rows of 8192 324 -> 376 us, 32 up to 4000 52.7 -> 57.4). The number of tiles is known on the device alone: every workgroup
 // adds up the rows' lengths, workgroup 0 leaves the result for the join.
 template <bool SCORED>
 __device__ __forceinline__ void paged_attn(const GhPagedAttnArgs& a) {
@@ -595,7 +595,8 @@ GH_KERNEL __launch_bounds__(256) void gh_paged_split_s(GhPagedAttnArgs a) { page
 // x < q_heads: 128 / HALVES dims of the output of one query head: M = max m_s, out = Σ 2^(m_s - M) acc_s /
 // Σ 2^(m_s - M) l_s; 8·HALVES groups of threads take every so many-th partial, four dims per thread, each with a
 // running maximum, and add up in group order. Bound by its chain of loads; two halves where few rows have many
-// partials each (1 row of 32768, 256 partials: 7.6 us with one, 5.9 with two), one where many rows have few.
+// partials each (1 row of 32768, 256 partials: attention and join 33.2 us with one, 31.7 with two), one where many rows have
+// few (32 up to 4000 52.7 with one, 53.3 with two).
 // Else: the scores of a kv head, every blocks-th 1024 positions (add_scores).
 namespace {
 template <uint32_t HALVES>
@@ -715,11 +716,11 @@ GH_KERNEL __launch_bounds__(256) void gh_paged_join2(GhPagedAttnArgs a) { paged_
 // scores of the older positions by a radix select over the scores' order as 32-bit keys (11, 11 and 10 bits
 // per pass, counted in LDS, until a whole bin stays), then one pass in ascending order that writes the kept
 // positions and moves their scores; equal keys are taken from the front. Bound by its barriers and LDS atomics:
-// 272 lists of 4096 in 10.2 us (16.5 with the scores read in every pass and shuffles through LDS). In place:
+// 272 lists of 4096 in 9.8 us (16.5 with the scores read in every pass and shuffles through LDS). In place:
 // a step's scores are read before a barrier and written after it, at or before where they came from.
 // gh_paged_move, grid (16-slot blocks of the budget, rows, layers), 256 threads: 16 lanes per 256-byte vector,
 // consecutive groups of lanes the heads of one slot, so that writes are contiguous; bound by memory, 570 MB
-// in and out at 5.0 TB/s.
+// in and out at 5.1 TB/s.
 namespace {
 // f32 total order as unsigned order
 __device__ __forceinline__ uint32_t order_key(uint32_t bits) { return bits ^ ((uint32_t)((int32_t)bits >> 31) | 0x80000000u); }

@@ -223,7 +223,7 @@ int gh_kv_write_paged(gh_backend* b, gh_encoder* enc, const gh_kv_paged* kv, con
  * the device; after an eviction a row stands further on than its length says), queries FP16
  * [rows][tokens][q_heads][128] from q to q_out (q itself, or no part of q, k or v; no part of kv's buffers
  * or of positions) with the query's post-scale, keys on their way into the cache; of skipped vectors
- * (gh_kv_write_paged) the queries are skipped too. The values of gh_rope_yarn and gh_kv_write. max_pos: the largest of the positions
+ * (gh_kv_write_paged) the queries are skipped too. The values of gh_rope_yarn (angles in FP32, as the keys of a prefill have them) and gh_kv_write. max_pos: the largest of the positions
  * positions[r] + t of this call, at most 262143 (it sizes the rotation table). */
 int gh_rope_kv_write_paged(gh_backend* b, gh_encoder* enc, const gh_kv_paged* kv, const gh_buf* q_out,
                            const gh_buf* q, const gh_buf* k, const gh_buf* v, uint32_t q_heads,
@@ -234,7 +234,9 @@ int gh_rope_kv_write_paged(gh_backend* b, gh_encoder* enc, const gh_kv_paged* kv
  * zeros. max_len: no row is longer (0: table_width·page_size); it sizes the launch. Where scores are kept, each position's attention weight,
  * summed over the query heads of a kv head, is added to its score. In the products with V a weight is held to
  * 2^-38 of the row's largest and is at least that, unless its score is -inf: n positions add up to n·2^-38 of their
- * mean V, and an infinite V shows whatever its finite score. A row whose scores are all -inf gives NaN. */
+ * mean V, and an infinite V leaves an infinity or NaN whatever its score. A row whose scores are all -inf gives
+ * NaN. max_len also sizes the call's scratch: with scores 4 bytes per query head and position of every row, in groups of
+ * rows that take at most 512 MiB. */
 int gh_attention_decode_paged(gh_backend* b, gh_encoder* enc, const gh_buf* out, const gh_buf* q,
                               const gh_kv_paged* kv, uint32_t q_heads, uint32_t max_len, uint32_t layer);
 /* Eviction by accumulated attention weight: of every row longer than `budget`, for each layer and kv head by
