@@ -26,7 +26,7 @@ STATUS = {
 FMT_F32, FMT_F16, FMT_Q4_K, FMT_Q6_K = 0, 1, 12, 14
 BUF_ALLOC, BUF_VIEW, BUF_WEIGHT = 1, 2, 3
 ROPE_QUERY, ROPE_KEY = 0, 1
-KV_F16 = 0
+KV_F16, KV_INT8, KV_Q4 = 0, 1, 2
 NO_LAYER = 0xFFFFFFFF
 (T_ATTN_NORM, T_ATTN_Q, T_ATTN_K, T_ATTN_V, T_ATTN_OUTPUT, T_FFN_NORM, T_FFN_GATE, T_FFN_UP,
  T_FFN_DOWN) = range(9)
@@ -63,6 +63,10 @@ class GhKvPaged(C.Structure):
 class GhSampling(C.Structure):
     _fields_ = [("temperature", C.c_float), ("top_p", C.c_float), ("top_k", C.c_uint32),
                 ("min_p", C.c_float), ("repeat_penalty", C.c_float), ("seed", C.c_uint64)]
+
+
+class GhSampleParams(C.Structure):
+    _fields_ = [("temperature", C.c_float), ("top_p", C.c_float), ("top_k", C.c_uint32), ("min_p", C.c_float)]
 
 
 SAMPLE_GREEDY, SAMPLE_TOPK, SAMPLE_FALLBACK = 0, 1, 2
@@ -116,6 +120,7 @@ SIGNATURES = {
     "gh_rmsnorm_x": (I32, [P, P, BUFP, BUFP, BUFP, U32, F32, U32]),
     "gh_rope_yarn": (I32, [P, P, BUFP, U32, U32, U32, C.POINTER(GhYarn), U32]),
     "gh_rope_yarn_batched": (I32, [P, P, BUFP, BUFP, U32, U32, U32, U32, U32, C.POINTER(GhYarn)]),
+    "gh_norm_rope_batched": (I32, [P, P, BUFP, BUFP, U32, U32, U32, U32, U32, BUFP, BUFP, F32, C.POINTER(GhYarn)]),
     "gh_silu_mul": (I32, [P, P, BUFP, BUFP, BUFP, U32]),
     "gh_residual_add": (I32, [P, P, BUFP, BUFP, U32]),
     "gh_attention_decode": (I32, [P, P, BUFP, BUFP, C.POINTER(GhKv), U32, U32, U32]),
@@ -124,8 +129,12 @@ SIGNATURES = {
     "gh_kv_write_paged": (I32, [P, P, C.POINTER(GhKvPaged), BUFP, BUFP, U32, U32]),
     "gh_rope_kv_write_paged": (I32, [P, P, C.POINTER(GhKvPaged), BUFP, BUFP, BUFP, BUFP, U32, BUFP, U32,
                                      U32, C.POINTER(GhYarn), U32]),
+    "gh_norm_rope_kv_write_paged": (I32, [P, P, C.POINTER(GhKvPaged), BUFP, BUFP, BUFP, BUFP, U32, BUFP, BUFP, F32,
+                                          BUFP, U32, U32, C.POINTER(GhYarn), U32]),
+    "gh_kv_read_paged": (I32, [P, P, BUFP, BUFP, C.POINTER(GhKvPaged), U32, U32]),
     "gh_attention_decode_paged": (I32, [P, P, BUFP, BUFP, C.POINTER(GhKvPaged), U32, U32, U32]),
     "gh_kv_evict_paged": (I32, [P, P, C.POINTER(GhKvPaged), C.POINTER(GhKvPaged), BUFP, U32, U32]),
+    "gh_sample_rows": (I32, [P, P, BUFP, BUFP, BUFP, U32, U32, U32, BUFP, BUFP]),
     "gh_read_logits": (I32, [P, BUFP, U64, P]),
     "gh_read_argmax": (I32, [P, BUFP, U64, C.POINTER(U32)]),
     "gh_read_topk": (I32, [P, BUFP, U64, U64, P, P, C.POINTER(U64)]),

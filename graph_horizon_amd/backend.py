@@ -177,6 +177,10 @@ class HipBackend:
         self._run("gh_rope_yarn_batched", C.byref(q), C.byref(k), q_heads, kv_heads, head_dim,
                   base, rows, C.byref(yarn.c()))
 
+    def norm_rope_batched(self, q, k, q_heads, kv_heads, head_dim, base, rows, q_norm, k_norm, eps, yarn: Yarn):
+        """Norms of the heads of q and k and RoPE at base.., in place."""
+        self._run("gh_norm_rope_batched", q, k, q_heads, kv_heads, head_dim, base, rows, q_norm, k_norm, eps, yarn.c())
+
     def silu_mul(self, out, gate, up, n):
         self._run("gh_silu_mul", C.byref(out), C.byref(gate), C.byref(up), n)
 
@@ -201,6 +205,16 @@ class HipBackend:
         """RoPE of q (into q_out) and k at the rows' own positions, and the append, in one launch."""
         self._run("gh_rope_kv_write_paged", kv, q_out, q, k, v, q_heads, positions, tokens, max_pos, yarn.c(), layer)
 
+    def norm_rope_kv_write_paged(self, kv: GhKvPaged, q_out, q, k, v, q_heads, q_norm, k_norm, eps, positions, tokens,
+                                 max_pos, yarn: Yarn, layer):
+        """rope_kv_write_paged with norms of the heads of q and k before the rotation."""
+        self._run("gh_norm_rope_kv_write_paged", kv, q_out, q, k, v, q_heads, q_norm, k_norm, eps, positions, tokens,
+                  max_pos, yarn.c(), layer)
+
+    def kv_read_paged(self, k, v, kv: GhKvPaged, tokens, layer):
+        """The last `tokens` positions of each row as FP16 vectors."""
+        self._run("gh_kv_read_paged", k, v, kv, tokens, layer)
+
     def attention_decode_paged(self, out, q, kv: GhKvPaged, q_heads, max_len, layer):
         """One token per row over its cached positions; adds the attention weights to kv.score if kept."""
         self._run("gh_attention_decode_paged", out, q, kv, q_heads, max_len, layer)
@@ -209,6 +223,12 @@ class HipBackend:
         """Rows longer than `budget` keep their last `recent` and best-scored positions, in dst's pages;
         kept: a buffer for the kept positions, or None."""
         self._run("gh_kv_evict_paged", dst, src, kept, budget, recent)
+
+    # ---- sampling of a batch ----
+    def sample_rows(self, tokens, probs, logits, rows, vocab, stride, params, uniform):
+        """Each row's next token by its GhSampleParams and its random number, all on the device; probs: a buffer for
+        the tokens' shares of the kept sum, or None."""
+        self._run("gh_sample_rows", tokens, probs, logits, rows, vocab, stride, params, uniform)
 
     # ---- read-back ----
     def read_logits(self, logits, vocab) -> np.ndarray:

@@ -85,6 +85,13 @@ const KernelName kKernels[] = {
     {K_GEMM_FEW_MIXED_T32, "gh_gemm_few_mixed_t32"},
     {K_GEMM_FEW_Q4K_T48, "gh_gemm_few_q4k_t48"}, {K_GEMM_FEW_Q6K_T48, "gh_gemm_few_q6k_t48"},
     {K_GEMM_FEW_MIXED_T48, "gh_gemm_few_mixed_t48"},
+    {K_NORM_ROPE, "gh_norm_rope"},
+    {K_SAMPLE_MAX, "gh_sample_max"}, {K_SAMPLE_BINS, "gh_sample_bins"},
+    {K_SAMPLE_COLLECT, "gh_sample_collect"}, {K_SAMPLE_PICK, "gh_sample_pick"},
+    {K_PAGED_READ, "gh_paged_read"}, {K_PAGED_NORM_WRITE, "gh_paged_norm_write"},
+    {K_PAGED4_WRITE, "gh_paged4_write"}, {K_PAGED4_NORM_WRITE, "gh_paged4_norm_write"}, {K_PAGED4_READ, "gh_paged4_read"},
+    {K_PAGED4_ATTN, "gh_paged4_attn"}, {K_PAGED4_ATTN_S, "gh_paged4_attn_s"},
+    {K_PAGED4_SPLIT, "gh_paged4_split"}, {K_PAGED4_SPLIT_S, "gh_paged4_split_s"}, {K_PAGED4_MOVE, "gh_paged4_move"},
     {K_PAGED_WRITE, "gh_paged_write"},
     {K_PAGED_ATTN, "gh_paged_attn"}, {K_PAGED_ATTN_S, "gh_paged_attn_s"},
     {K_PAGED_SPLIT, "gh_paged_split"}, {K_PAGED_SPLIT_S, "gh_paged_split_s"},
@@ -92,7 +99,7 @@ const KernelName kKernels[] = {
     {K_PAGED_SELECT, "gh_paged_select"}, {K_PAGED_MOVE, "gh_paged_move"}, {K_PAGED_MOVE_S, "gh_paged_move_s"},
 };
 
-const char* kModules[] = {"gh_quant", "gh_gemv", "gh_glue", "gh_attention", "gh_gemm", "gh_gemm_few", "gh_paged"};
+const char* kModules[] = {"gh_quant", "gh_gemv", "gh_glue", "gh_attention", "gh_gemm", "gh_gemm_few", "gh_paged", "gh_paged4", "gh_sample"};
 
 constexpr uint32_t kArgmaxBlocks = 256;
 constexpr size_t kResultBytes = 2 * 128 * 4;  // read_argmax's index, or read_topk's 128 indices and values

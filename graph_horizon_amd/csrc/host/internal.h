@@ -3,8 +3,10 @@
 #define GH_HOST_INTERNAL_H
 #include <hip/hip_runtime_api.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <cstring>
+#include <new>
 #include <string>
 #include <unordered_map>
 #include <vector>
@@ -131,6 +133,22 @@ enum GhKernel : int {
     K_GEMM5_Q4K,
     K_GEMM5_Q6K,
     K_GEMM5_MIXED,
+    K_NORM_ROPE,
+    K_SAMPLE_MAX,
+    K_SAMPLE_BINS,
+    K_SAMPLE_COLLECT,
+    K_SAMPLE_PICK,
+    K_PAGED_READ,
+    K_PAGED_NORM_WRITE,
+    // 4-bit pools
+    K_PAGED4_WRITE,
+    K_PAGED4_NORM_WRITE,
+    K_PAGED4_READ,
+    K_PAGED4_ATTN,
+    K_PAGED4_ATTN_S,
+    K_PAGED4_SPLIT,
+    K_PAGED4_SPLIT_S,
+    K_PAGED4_MOVE,
     K_PAGED_WRITE,
     K_PAGED_ATTN,
     K_PAGED_ATTN_S,  // keeps the scores for gh_paged_join
@@ -214,6 +232,35 @@ int fail(gh_backend* b, int code, const std::string& msg);
 int check_enc(gh_backend* b, gh_encoder* enc);
 // records an op's status in the encoder (reported again by gh_submit)
 int latch(gh_encoder* enc, int rc);
+
+// Calls that allocate scratch or a rotation table do it on the backend's device, whatever the thread's is.
+struct OnDevice {
+    int before = 0;
+    bool moved = false;
+    explicit OnDevice(const gh_backend* b) {
+        moved = hipGetDevice(&before) == hipSuccess && before != b->device && hipSetDevice(b->device) == hipSuccess;
+    }
+    ~OnDevice() {
+        if (moved) (void)hipSetDevice(before);
+    }
+};
+
+// An entry point's body: the encoder checked, errors latched, no exception let out.
+template <class F>
+int entry(gh_backend* b, gh_encoder* enc, F body) {
+    int rc = check_enc(b, enc);
+    if (rc) return rc;
+    try {
+        OnDevice on(b);
+        rc = body();
+    } catch (const std::bad_alloc&) {
+        rc = GH_E_OOM;
+    } catch (...) {
+        rc = GH_E_INVALID;
+    }
+    return latch(enc, rc);
+}
+
 int check_attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv* kv,
                     uint32_t q_heads, uint32_t last_pos, uint32_t rows, uint32_t layer);
 // Resolves this device's address of the no-allocation scratch array (at gh_create).
@@ -228,6 +275,24 @@ int ensure_workspace(gh_backend* b, size_t bytes);
 inline size_t workspace_room(const gh_backend* b) { return b->ws_bytes > kArgmaxBytes ? b->ws_bytes - kArgmaxBytes : 0; }
 // `bytes` of the workspace for one call's launches, 16-byte aligned, behind the argmax scratch.
 int workspace_at(gh_backend* b, size_t bytes, char** at);
+// `bytes` of the workspace. It grows by half (at most 64 MiB) more than asked where there is memory for that: sizes
+// that follow the longest row rise every 16 tokens, and a growth waits for the stream and moves what recorded graphs hold.
+inline int growing_scratch(gh_backend* b, uint64_t bytes, char** at) {
+    auto ask = [&](uint64_t n) {
+        const bool grows = n > workspace_room(b);
+        const int rc = workspace_at(b, n, at);
+        if (rc == GH_E_OOM) b->ws_short = b->ws_short ? std::min(b->ws_short, n) : n;
+        else if (!rc && grows && n >= b->ws_short) b->ws_short = 0;
+        return rc;
+    };
+    const uint64_t more = bytes + std::min<uint64_t>(bytes / 2, 64ull << 20);
+    if (bytes > workspace_room(b) && (!b->ws_short || more < b->ws_short)) {
+        const int rc = ask(more);
+        if (rc != GH_E_OOM) return rc;
+        b->err.clear();
+    }
+    return ask(bytes);
+}
 // Workgroups of `block` threads and `shmem` bytes of LDS resident on the whole device at once.
 uint32_t resident_wgs(gh_backend* b, GhKernel k, uint32_t block, uint32_t shmem);
 // Builds (or rebuilds, for other parameters or more positions) table t for `positions`

@@ -1,8 +1,7 @@
 // Operators over paged KV caches (gh_kv_paged): checks, launch plans and scratch. The kernels are in
-// kernels/paged.hip.
+// kernels/paged.hip and, for 4-bit pools, norms and the read-back, kernels/paged4.hip.
 #include <algorithm>
 #include <cmath>
-#include <new>
 
 #include "internal.h"
 
@@ -31,6 +30,10 @@ constexpr uint32_t kPagedRows = 512;  // rows that one attention launch lays out
 constexpr uint64_t kStreamBytes = 128ull << 20;  // half the last-level cache
 constexpr uint32_t kSpanTiles = 32;   // tiles of a gh_paged_split workgroup at most (its waves hold 64 each)
 
+bool four_bits(const gh_kv& kv) { return kv.scheme == GH_KV_Q4; }
+uint32_t vector_bytes(const gh_kv& kv) { return four_bits(kv) ? 80 : 256; }
+// bytes of a layer of K or V
+uint64_t layer_bytes(const gh_kv& kv) { return (uint64_t)kv.context * kv.kv_heads * vector_bytes(kv); }
 uint64_t capacity(const gh_kv_paged* kv) { return (uint64_t)kv->table_width * kv->page_size; }
 
 // What a handle uses of its buffers. Operators write all but the table.
@@ -39,7 +42,7 @@ struct Parts {
     Span part[PARTS];
     explicit Parts(const gh_kv_paged* p) {
         const gh_kv& kv = p->kv;
-        part[CACHE_K].bytes = part[CACHE_V].bytes = (uint64_t)kv.block_count * kv.context * kv.kv_heads * 256;
+        part[CACHE_K].bytes = part[CACHE_V].bytes = kv.block_count * layer_bytes(kv);
         part[CACHE_K].at = kv.k.addr;
         part[CACHE_V].at = kv.v.addr;
         if (p->score.addr) part[SCORE] = {p->score.addr, (uint64_t)kv.block_count * p->rows * kv.kv_heads * capacity(p) * 4};
@@ -56,7 +59,7 @@ int check_paged(gh_backend* b, const gh_kv_paged* p, uint32_t layer, const char*
     auto no = [&](int code, const char* why) { return fail(b, code, std::string(what) + ": " + why); };
     if (!p) return no(GH_E_INVALID, "null");
     const gh_kv& kv = p->kv;
-    if (kv.scheme != GH_KV_F16) return no(GH_E_UNSUPPORTED, "only the f16 KV scheme");
+    if (kv.scheme != GH_KV_F16 && kv.scheme != GH_KV_Q4) return no(GH_E_UNSUPPORTED, "only the f16 and q4 KV schemes");
     if (kv.head_dim != 128 || kv.value_dim != 128) return no(GH_E_UNSUPPORTED, "head_dim 128 only");
     if (kv.kv_heads == 0 || kv.kv_heads > 0xFFFFu) return no(GH_E_INVALID, "kv_heads");
     if (p->page_size < 16 || p->page_size > 32768 || (p->page_size & (p->page_size - 1)))
@@ -65,7 +68,7 @@ int check_paged(gh_backend* b, const gh_kv_paged* p, uint32_t layer, const char*
     if (p->rows == 0 || p->rows > 0xFFFFu) return no(GH_E_INVALID, "1 to 65535 rows");
     if (p->table_width == 0 || capacity(p) > 0x7FFFFFFFull) return no(GH_E_INVALID, "table_width");
     if (layer >= kv.block_count) return no(GH_E_RANGE, "layer beyond the pool");
-    const unsigned __int128 cache = (unsigned __int128)kv.block_count * kv.context * kv.kv_heads * 256;
+    const unsigned __int128 cache = (unsigned __int128)kv.block_count * kv.context * kv.kv_heads * vector_bytes(kv);
     const unsigned __int128 score = (unsigned __int128)kv.block_count * p->rows * kv.kv_heads * capacity(p) * 4;
     if ((cache | score) >> 63) return no(GH_E_RANGE, "cache too small");
     if (!fits(&kv.k, (uint64_t)cache, 16) || !fits(&kv.v, (uint64_t)cache, 16))
@@ -84,7 +87,7 @@ int check_paged(gh_backend* b, const gh_kv_paged* p, uint32_t layer, const char*
 
 GhPages pages(gh_backend* b, const gh_kv_paged* p, uint32_t layer) {
     const gh_kv& kv = p->kv;
-    const uint64_t at = (uint64_t)layer * kv.context * kv.kv_heads * 256;
+    const uint64_t at = layer * layer_bytes(kv);
     GhPages g{};
     g.kc = kv.k.addr + at;
     g.vc = kv.v.addr + at;
@@ -99,55 +102,9 @@ GhPages pages(gh_backend* b, const gh_kv_paged* p, uint32_t layer) {
     return g;
 }
 
-// The calls allocate scratch and a rotation table: on the backend's device, whatever the thread's is.
-struct OnDevice {
-    int before = 0;
-    bool moved = false;
-    explicit OnDevice(const gh_backend* b) {
-        moved = hipGetDevice(&before) == hipSuccess && before != b->device && hipSetDevice(b->device) == hipSuccess;
-    }
-    ~OnDevice() {
-        if (moved) (void)hipSetDevice(before);
-    }
-};
-
-// An entry point's body: the encoder checked, errors latched, no exception let out.
-template <class F>
-int entry(gh_backend* b, gh_encoder* enc, F body) {
-    int rc = check_enc(b, enc);
-    if (rc) return rc;
-    try {
-        OnDevice on(b);
-        rc = body();
-    } catch (const std::bad_alloc&) {
-        rc = GH_E_OOM;
-    } catch (...) {
-        rc = GH_E_INVALID;
-    }
-    return latch(enc, rc);
-}
-
-// `bytes` of the workspace. It grows by half (at most 64 MiB) more than asked where there is memory for that: sizes
-// that follow the longest row rise every 16 tokens, and a growth waits for the stream and moves what recorded graphs hold.
-int scratch(gh_backend* b, uint64_t bytes, char** at) {
-    auto ask = [&](uint64_t n) {
-        const bool grows = n > workspace_room(b);
-        const int rc = workspace_at(b, n, at);
-        if (rc == GH_E_OOM) b->ws_short = b->ws_short ? std::min(b->ws_short, n) : n;
-        else if (!rc && grows && n >= b->ws_short) b->ws_short = 0;
-        return rc;
-    };
-    const uint64_t more = bytes + std::min<uint64_t>(bytes / 2, 64ull << 20);
-    if (bytes > workspace_room(b) && (!b->ws_short || more < b->ws_short)) {
-        const int rc = ask(more);
-        if (rc != GH_E_OOM) return rc;
-        b->err.clear();
-    }
-    return ask(bytes);
-}
-
 int write(gh_backend* b, const gh_kv_paged* kv, const gh_buf* k, const gh_buf* v, uint32_t tokens, uint32_t layer,
           GhPagedWriteArgs a, const char* what) {
+    const GhKernel kernel = four_bits(kv->kv) ? a.q_norm ? K_PAGED4_NORM_WRITE : K_PAGED4_WRITE : a.q_norm ? K_PAGED_NORM_WRITE : K_PAGED_WRITE;
     const uint64_t n = (uint64_t)kv->rows * tokens, bytes = n * kv->kv.kv_heads * 256;
     if (tokens == 0 || n > 0x7FFFFFFFull) return fail(b, GH_E_INVALID, std::string(what) + ": tokens");
     if (!fits(k, bytes, 16) || !fits(v, bytes, 16))
@@ -161,7 +118,80 @@ int write(gh_backend* b, const gh_kv_paged* kv, const gh_buf* k, const gh_buf* v
     a.tokens = tokens;
     a.groups = ceil_div((uint64_t)(a.q_heads + 2 * kv->kv.kv_heads) * 16, 256);
     if (n * a.groups > 0xFFFFFFull) return fail(b, GH_E_RANGE, std::string(what) + ": too many vectors");
-    return launch(b, K_PAGED_WRITE, (uint32_t)(n * a.groups), 1, 1, 256, &a);
+    return launch(b, kernel, (uint32_t)(n * a.groups), 1, 1, 256, &a);
+}
+
+// RoPE of q and k and the append; `a` holds the norms, if any.
+int rope_write(gh_backend* b, const gh_kv_paged* kv, const gh_buf* q_out, const gh_buf* q, const gh_buf* k, const gh_buf* v,
+               uint32_t q_heads, const gh_buf* positions, uint32_t tokens, uint32_t max_pos, const gh_yarn* yarn, uint32_t layer,
+               GhPagedWriteArgs a, const char* what) {
+    auto no = [&](int code, const char* why) { return fail(b, code, std::string(what) + ": " + why); };
+    int rc = check_paged(b, kv, layer, what);
+    if (rc) return rc;
+    if (!yarn_valid(yarn) || yarn->rope_dim > 128) return no(GH_E_INVALID, "invalid YaRN parameters");
+    if (max_pos >= kMaxRopePositions) return no(GH_E_RANGE, "position beyond the table limit");
+    if (q_heads == 0 || q_heads > 0xFFFFFu) return no(GH_E_INVALID, "q_heads");
+    const uint64_t bytes = (uint64_t)kv->rows * tokens * q_heads * 256;
+    if (!fits(q, bytes, 16) || !fits(q_out, bytes, 16) || !fits(positions, (uint64_t)kv->rows * 4, 4))
+        return no(GH_E_RANGE, "buffer too small or not on 16 bytes");
+    if (q->addr != q_out->addr && meet(q, bytes, q_out, bytes))
+        return no(GH_E_INVALID, "q_out overlaps q");
+    const uint64_t heads = bytes / q_heads * kv->kv.kv_heads;
+    if ((k && meet(q_out, bytes, k, heads)) || (v && meet(q_out, bytes, v, heads)))
+        return no(GH_E_INVALID, "q_out overlaps k or v");
+    const Parts own(kv);
+    const Span turned{q_out->addr, bytes}, at{positions->addr, (uint64_t)kv->rows * 4};
+    if (own.met(turned) || meet(turned, at) || meet(own.part[SCORE], {q->addr, bytes}))
+        return no(GH_E_INVALID, "q_out overlaps a buffer of the handle or positions, or q its scores");
+    if (meet(at, own.part[CACHE_K]) || meet(at, own.part[CACHE_V]) || meet(at, own.part[SCORE]))
+        return no(GH_E_INVALID, "positions overlap the caches or the scores");
+    rc = ensure_rope(b, b->rope, yarn, max_pos + 1);
+    if (rc) return rc;
+    a.q = q->addr;
+    a.q_out = q_out->addr;
+    a.q_heads = q_heads;
+    a.positions = positions->addr;
+    a.table = (uint64_t)b->rope.table;
+    a.post = (uint64_t)b->rope.post;
+    a.pairs = yarn->rope_dim / 2;
+    a.max_pos = max_pos;
+    return write(b, kv, k, v, tokens, layer, a, what);
+}
+
+// The norm weights, which the launch reads while it writes q_out and the pool.
+int check_norms(gh_backend* b, const gh_kv_paged* kv, const gh_buf* q_out, const gh_buf* q_norm, const gh_buf* k_norm, float eps,
+                uint64_t row_bytes, const char* what) {
+    auto no = [&](int code, const char* why) { return fail(b, code, std::string(what) + ": " + why); };
+    const int rc = check_paged(b, kv, 0, what);
+    if (rc) return rc;
+    if (!(eps >= 0.0f) || std::isinf(eps)) return no(GH_E_INVALID, "eps");
+    if (!fits(q_norm, 256, 16) || !fits(k_norm, 256, 16)) return no(GH_E_RANGE, "norm weights too small or not on 16 bytes");
+    const Parts own(kv);
+    for (const gh_buf* w : {q_norm, k_norm}) {
+        const Span span{w->addr, 256};
+        if ((q_out && meet(span, {q_out->addr, kv->rows * row_bytes})) || meet(span, own.part[CACHE_K]) ||
+            meet(span, own.part[CACHE_V]) || meet(span, own.part[SCORE]))
+            return no(GH_E_INVALID, "norm weights overlap q_out, the caches or the scores");
+    }
+    return GH_OK;
+}
+
+int read(gh_backend* b, const gh_buf* k, const gh_buf* v, const gh_kv_paged* kv, uint32_t tokens, uint32_t layer) {
+    auto no = [&](int code, const char* why) { return fail(b, code, std::string("kv_read_paged: ") + why); };
+    const uint64_t n = (uint64_t)kv->rows * tokens, bytes = n * kv->kv.kv_heads * 256;
+    if (tokens == 0 || n > 0x7FFFFFFFull) return no(GH_E_INVALID, "tokens");
+    if (!fits(k, bytes, 16) || !fits(v, bytes, 16)) return no(GH_E_RANGE, "vectors too small or not on 16 bytes");
+    const Parts own(kv);
+    const Span ks{k->addr, bytes}, vs{v->addr, bytes};
+    if (meet(ks, vs) || own.met(ks) || own.met(vs)) return no(GH_E_INVALID, "k and v overlap, or a buffer of the handle");
+    GhPagedReadArgs a{};
+    a.p = pages(b, kv, layer);
+    a.k = k->addr;
+    a.v = v->addr;
+    a.tokens = tokens;
+    a.groups = ceil_div((uint64_t)kv->kv.kv_heads * 32, 256);
+    if (n * a.groups > 0xFFFFFFull) return no(GH_E_RANGE, "too many vectors");
+    return launch(b, four_bits(kv->kv) ? K_PAGED4_READ : K_PAGED_READ, (uint32_t)(n * a.groups), 1, 1, 256, &a);
 }
 
 int attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv_paged* kv, uint32_t q_heads,
@@ -188,7 +218,9 @@ int attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv_pag
     a.max_len = max_len;
     a.scale = 1.4426950408889634f / std::sqrt(128.0f);
     const bool scored = kv->score.addr != 0;
-    a.raw_len = (max_len + 15) / 16 * 16;
+    const bool q4 = four_bits(kv->kv);
+    const uint32_t tile = q4 ? 32 : 16;  // positions
+    a.raw_len = (max_len + tile - 1) / tile * tile;
     a.blocks = scored ? std::min(ceil_div(max_len, 1024), 64u) : 0;
     // Tiles of 16 positions and kv heads (8 KiB of K and V) that the rows can hold. Rows of one span, or few
     // tiles in all: each row by itself in fixed spans (gh_paged_split), which start sooner (no row needs the
@@ -196,10 +228,19 @@ int attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv_pag
     // (gh_paged_attn), which balances ragged rows. us back to back, spans / chunks: 1 row of 500 9.4 / 11.9, 3 of
     // 3000 14.0 / 15.4, 256 of up to 300 40.4 / 48.0, 12 of up to 1000 15.2 / 14.4, 64 of up to 600 28.5 / 22.9, 8 of
     // up to 8192 45.9 / 33.4, 32 of up to 4000 69.3 / 52.0.
-    const uint32_t tiles1 = ceil_div(max_len, 16);
+    const uint32_t tiles1 = ceil_div(max_len, tile);
     const uint64_t most = (uint64_t)kv->rows * hk * tiles1;
     const bool split = tiles1 <= kSpanTiles || most < 6144;
-    if (split) {
+    if (q4) {
+        if (split) {
+            a.least = 2 * std::min(std::max(ceil_div(most, 8ull * b->cus) * 4, 4u), kSpanTiles);
+            a.chunks = ceil_div(max_len, 16 * a.least);
+        } else {
+            a.least = 2;
+            a.chunks = std::max(1u, 16 * b->cus / hk);
+            a.solo = 6;
+        }
+    } else if (split) {
         // about two workgroups per CU, each wave at most 8 tiles (1 row of 9000, in spans of 4 / 12 / 32 / 64 tiles:
         // 16.5 / 14.3 / 16.7 / 23.8 us)
         a.least = std::min(std::max(ceil_div(most, 8ull * b->cus) * 4, 4u), kSpanTiles);
@@ -236,7 +277,7 @@ int attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv_pag
     }
     char* ws = nullptr;
     int rc = GH_OK;
-    while ((rc = scratch(b, need(), &ws)) == GH_E_OOM && step > 1) {
+    while ((rc = growing_scratch(b, need(), &ws)) == GH_E_OOM && step > 1) {
         step = (step + 1) / 2;
         b->err.clear();
     }
@@ -254,11 +295,11 @@ int attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv_pag
         a.q = q->addr + (uint64_t)r * q_heads * 256;
         a.out = out->addr + (uint64_t)r * q_heads * 256;
         if (split) {
-            rc = launch(b, scored ? K_PAGED_SPLIT_S : K_PAGED_SPLIT, hk, a.chunks, a.rows, 256, &a, 4 * group * 134 * 4);
+            rc = launch(b, q4 ? scored ? K_PAGED4_SPLIT_S : K_PAGED4_SPLIT : scored ? K_PAGED_SPLIT_S : K_PAGED_SPLIT, hk, a.chunks, a.rows, 256, &a, 4 * group * 134 * 4);
         } else {
             // no more chunks than the rows' tiles can fill
             const uint64_t chunks = std::min<uint64_t>(a.chunks, ceil_div((uint64_t)a.rows * tiles1, a.least));
-            rc = launch(b, scored ? K_PAGED_ATTN_S : K_PAGED_ATTN, ceil_div(hk * chunks, 4), 1, 1, 256, &a);
+            rc = launch(b, q4 ? scored ? K_PAGED4_ATTN_S : K_PAGED4_ATTN : scored ? K_PAGED_ATTN_S : K_PAGED_ATTN, ceil_div(hk * chunks, 4), 1, 1, 256, &a);
         }
         // the halves of the heads apart where a row may have more partials than one round of the join takes (64)
         const uint32_t halves = a.chunks > 64 * a.rows ? 2 : 1;
@@ -272,8 +313,8 @@ int attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv_pag
 int evict(gh_backend* b, const gh_kv_paged* dst, const gh_kv_paged* src, const gh_buf* kept, uint32_t budget,
           uint32_t recent) {
     const gh_kv &s = src->kv, &d = dst->kv;
-    if (d.block_count != s.block_count || d.kv_heads != s.kv_heads || dst->page_size != src->page_size || dst->rows != src->rows)
-        return fail(b, GH_E_INVALID, "kv_evict_paged: dst and src differ in rows, page_size, block_count or heads");
+    if (d.block_count != s.block_count || d.kv_heads != s.kv_heads || d.scheme != s.scheme || dst->page_size != src->page_size || dst->rows != src->rows)
+        return fail(b, GH_E_INVALID, "kv_evict_paged: dst and src differ in rows, page_size, block_count, heads or scheme");
     if (!src->score.addr || !dst->score.addr) return fail(b, GH_E_INVALID, "kv_evict_paged: no scores kept");
     if (budget == 0 || recent > budget) return fail(b, GH_E_INVALID, "kv_evict_paged: recent > budget, or budget 0");
     if (budget > capacity(dst)) return fail(b, GH_E_RANGE, "kv_evict_paged: budget beyond dst's table");
@@ -301,19 +342,19 @@ int evict(gh_backend* b, const gh_kv_paged* dst, const gh_kv_paged* src, const g
     GhPagedEvictArgs a{};
     a.src = pages(b, src, 0);
     a.dst = pages(b, dst, 0);
-    a.src_layer = (uint64_t)s.context * s.kv_heads * 256;
-    a.dst_layer = (uint64_t)d.context * d.kv_heads * 256;
+    a.src_layer = layer_bytes(s);
+    a.dst_layer = layer_bytes(d);
     a.rows = src->rows;
     a.budget = budget;
     a.recent = recent;
     char* ws = nullptr;
-    int rc = scratch(b, (uint64_t)src->rows * 4 + (kept ? 0 : list * budget * 4), &ws);
+    int rc = growing_scratch(b, (uint64_t)src->rows * 4 + (kept ? 0 : list * budget * 4), &ws);
     if (rc) return b->ws_short = 0, rc;
     a.act = (uint64_t)ws;
     a.kept = kept ? kept->addr : (uint64_t)ws + (uint64_t)src->rows * 4;
     rc = launch(b, K_PAGED_SELECT, s.kv_heads, src->rows, s.block_count, 512, &a);
     const bool stream = list * budget * 512 >= kStreamBytes;
-    if (!rc) rc = launch(b, stream ? K_PAGED_MOVE_S : K_PAGED_MOVE, ceil_div(budget, 16), src->rows, s.block_count, 256, &a);
+    if (!rc) rc = launch(b, four_bits(s) ? K_PAGED4_MOVE : stream ? K_PAGED_MOVE_S : K_PAGED_MOVE, ceil_div(budget, 16), src->rows, s.block_count, 256, &a);
     return rc;
 }
 
@@ -334,38 +375,32 @@ int gh_rope_kv_write_paged(gh_backend* b, gh_encoder* enc, const gh_kv_paged* kv
                            const gh_buf* positions, uint32_t tokens, uint32_t max_pos, const gh_yarn* yarn,
                            uint32_t layer) {
     return entry(b, enc, [&] {
-        const char* what = "rope_kv_write_paged";
-        int rc = check_paged(b, kv, layer, what);
-        if (rc) return rc;
-        if (!yarn_valid(yarn) || yarn->rope_dim > 128) return fail(b, GH_E_INVALID, "rope_kv_write_paged: invalid YaRN parameters");
-        if (max_pos >= kMaxRopePositions) return fail(b, GH_E_RANGE, "rope_kv_write_paged: position beyond the table limit");
-        if (q_heads == 0 || q_heads > 0xFFFFFu) return fail(b, GH_E_INVALID, "rope_kv_write_paged: q_heads");
-        const uint64_t bytes = (uint64_t)kv->rows * tokens * q_heads * 256;
-        if (!fits(q, bytes, 16) || !fits(q_out, bytes, 16) || !fits(positions, (uint64_t)kv->rows * 4, 4))
-            return fail(b, GH_E_RANGE, "rope_kv_write_paged: buffer too small or not on 16 bytes");
-        if (q->addr != q_out->addr && meet(q, bytes, q_out, bytes))
-            return fail(b, GH_E_INVALID, "rope_kv_write_paged: q_out overlaps q");
-        const uint64_t heads = bytes / q_heads * kv->kv.kv_heads;
-        if ((k && meet(q_out, bytes, k, heads)) || (v && meet(q_out, bytes, v, heads)))
-            return fail(b, GH_E_INVALID, "rope_kv_write_paged: q_out overlaps k or v");
-        const Parts own(kv);
-        const Span turned{q_out->addr, bytes}, at{positions->addr, (uint64_t)kv->rows * 4};
-        if (own.met(turned) || meet(turned, at) || meet(own.part[SCORE], {q->addr, bytes}))
-            return fail(b, GH_E_INVALID, "rope_kv_write_paged: q_out overlaps a buffer of the handle or positions, or q its scores");
-        if (meet(at, own.part[CACHE_K]) || meet(at, own.part[CACHE_V]) || meet(at, own.part[SCORE]))
-            return fail(b, GH_E_INVALID, "rope_kv_write_paged: positions overlap the caches or the scores");
-        rc = ensure_rope(b, b->rope, yarn, max_pos + 1);
-        if (rc) return rc;
+        return rope_write(b, kv, q_out, q, k, v, q_heads, positions, tokens, max_pos, yarn, layer, GhPagedWriteArgs{},
+                          "rope_kv_write_paged");
+    });
+}
+
+int gh_norm_rope_kv_write_paged(gh_backend* b, gh_encoder* enc, const gh_kv_paged* kv, const gh_buf* q_out,
+                                const gh_buf* q, const gh_buf* k, const gh_buf* v, uint32_t q_heads,
+                                const gh_buf* q_norm, const gh_buf* k_norm, float eps, const gh_buf* positions,
+                                uint32_t tokens, uint32_t max_pos, const gh_yarn* yarn, uint32_t layer) {
+    return entry(b, enc, [&] {
+        const char* what = "norm_rope_kv_write_paged";
         GhPagedWriteArgs a{};
-        a.q = q->addr;
-        a.q_out = q_out->addr;
-        a.q_heads = q_heads;
-        a.positions = positions->addr;
-        a.table = (uint64_t)b->rope.table;
-        a.post = (uint64_t)b->rope.post;
-        a.pairs = yarn->rope_dim / 2;
-        a.max_pos = max_pos;
-        return write(b, kv, k, v, tokens, layer, a, what);
+        const int rc = check_norms(b, kv, q_out, q_norm, k_norm, eps, (uint64_t)tokens * q_heads * 256, what);
+        if (rc) return rc;
+        a.q_norm = q_norm->addr;
+        a.k_norm = k_norm->addr;
+        a.eps = eps;
+        return rope_write(b, kv, q_out, q, k, v, q_heads, positions, tokens, max_pos, yarn, layer, a, what);
+    });
+}
+
+int gh_kv_read_paged(gh_backend* b, gh_encoder* enc, const gh_buf* k, const gh_buf* v, const gh_kv_paged* kv,
+                     uint32_t tokens, uint32_t layer) {
+    return entry(b, enc, [&] {
+        const int rc = check_paged(b, kv, layer, "kv_read_paged");
+        return rc ? rc : read(b, k, v, kv, tokens, layer);
     });
 }
 

@@ -168,6 +168,26 @@ struct GhRopeArgs {
     uint32_t groups;  // workgroups per row
 };
 
+// Norms and RoPE of `rows` rows of query and key heads at positions base .., in place.
+struct GhNormRopeArgs {
+    uint64_t q;       // f16 [rows][heads][head_dim], with post-scale
+    uint64_t k;       // f16 [rows][kheads][head_dim]
+    uint64_t q_norm;  // f16 [head_dim]
+    uint64_t k_norm;
+    uint64_t table;   // float2 [positions][pairs]
+    uint64_t post;    // float [positions]
+    uint32_t heads;
+    uint32_t kheads;
+    uint32_t head_dim;  // a multiple of 8, at most 8 lanes
+    uint32_t pairs;
+    uint32_t base;
+    uint32_t rows;
+    uint32_t lanes;   // of a head: 1, 2, 4, .. 64
+    uint32_t groups;  // workgroups per row
+    float eps;
+    uint32_t pad;
+};
+
 struct GhEltArgs {
     uint64_t out;
     uint64_t a;
@@ -249,7 +269,31 @@ struct GhArgmaxArgs {
     uint32_t blocks;
 };
 
-// ---- paged caches (kernels/paged.hip) ----
+// Sampling of rows of logits (kernels/sample.hip). Scratch of a row: the chunks' maxima, (largest of all as order and
+// index, largest finite one's order) u64 x 2 [64]; bins u64 sums, u32 counts [GH_SAMPLE_BINS], u32 length of the list; list.
+#define GH_SAMPLE_BINS 1024u
+#define GH_SAMPLE_LIST 8192u
+#define GH_SAMPLE_BIN_BYTES (GH_SAMPLE_BINS * 12u + 16u)
+#define GH_SAMPLE_ROW_BYTES (64u * 16u + GH_SAMPLE_BIN_BYTES + GH_SAMPLE_LIST * 8u)
+struct GhSampleArgs {
+    uint64_t logits;   // f32 [rows][stride]
+    uint64_t params;   // gh_sample_params [rows]
+    uint64_t uniform;  // f32 [rows]
+    uint64_t tokens;   // u32 [rows]
+    uint64_t probs;    // f32 [rows], 0: not wanted
+    uint64_t part;
+    uint64_t bins;
+    uint64_t list;     // u64 [rows][GH_SAMPLE_LIST]
+    double scale;      // of weights in fixed point: a power of two, vocab times which is at most 2^62
+    uint32_t vocab;
+    uint32_t stride;
+    uint32_t chunks;   // of a row, at most 64
+    uint32_t per;      // logits of a chunk, a multiple of 4
+    uint32_t wide;     // rows start on 16 bytes
+    uint32_t pad;
+};
+
+// ---- paged caches (kernels/paged.hip, kernels/paged4.hip) ----
 // What a kernel found that the host cannot check, left in pinned host memory for gh_submit.
 #define GH_PAGED_LENGTH 1u    // a row longer than its table, or than the call's max_len
 #define GH_PAGED_PAGE 2u      // a page number beyond the pool
@@ -257,7 +301,7 @@ struct GhArgmaxArgs {
 
 // The rows' view of one layer of a page pool.
 struct GhPages {
-    uint64_t kc;       // f16 [slots][kv_heads][128] of the layer (all layers: of layer 0)
+    uint64_t kc;       // [slots][kv_heads] vectors of the layer (all layers: of layer 0), f16 [128] or 80 bytes
     uint64_t vc;
     uint64_t table;    // u32 [rows][width]
     uint64_t lengths;  // u32 [rows]
@@ -283,9 +327,21 @@ struct GhPagedWriteArgs {
     uint32_t tokens;
     uint32_t max_pos;
     uint32_t groups;   // workgroups per token
+    float eps;
+    uint64_t q_norm;   // f16 [128] weights of the queries' norm, and of the keys' (gh_paged*_norm_write)
+    uint64_t k_norm;
 };
 
-// Decode attention, in tiles of 16 positions. Partials (what one row has in one workgroup's or wave's share):
+// The last `tokens` positions of each row as f16 [rows][tokens][kv_heads][128].
+struct GhPagedReadArgs {
+    GhPages p;
+    uint64_t k;
+    uint64_t v;
+    uint32_t tokens;
+    uint32_t groups;   // workgroups per token
+};
+
+// Decode attention, in tiles of 16 positions (4-bit: 32, but `least` of the spans counts 16 there too). Partials (what one row has in one workgroup's or wave's share):
 // acc f32 [kv_heads][group][128] and (m, l) float2 [kv_heads][group].
 // gh_paged_attn: all rows' tiles, one row after the other, are cut into chunks of `per` tiles, the larger of
 // `least` and an equal share of `chunks` (of chunks / 2 where that is at most `solo`); the part of row r in chunk c
@@ -307,7 +363,7 @@ struct GhPagedAttnArgs {
     uint32_t chunks;
     uint32_t least;
     uint32_t solo;
-    uint32_t raw_len;  // max_len rounded up to 16
+    uint32_t raw_len;  // max_len rounded up to whole tiles
     float scale;       // log2(e) / sqrt(128)
     uint32_t blocks;   // gh_paged_join: workgroups per kv head that add scores
 };

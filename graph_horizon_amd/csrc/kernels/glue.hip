@@ -1,5 +1,5 @@
 // Decode/prefill glue: RMSNorm, YaRN RoPE, SiLU·up, residual add, KV append, argmax.
-#include "gh_common.h"
+#include "gh_head.h"
 
 // rmsnorm_x (backend/cpu/kernels/elementwise/normalization.rs:12-40): one 256-thread
 // workgroup per row, Σx² in gh_rms_inverse_256's order (thread t: the 16-value items t, t + 256, ...),
@@ -85,6 +85,31 @@ GH_KERNEL __launch_bounds__(256) void gh_rope(GhRopeArgs a) {
         const float2 c = *gh_gp<float2>(cs);
         *gh_gpw<uint32_t>(p) = rope_pair(*gh_gp<uint32_t>(p), c.x, c.y, scale);
     }
+}
+
+// Norms of query and key heads and their rotation in one pass, FP16 in place: x / sqrt(mean x² + eps) · w over each
+// head, then as gh_rope. A head is a.lanes lanes of 8 values (a power of two; those past head_dim hold zeros), the
+// sum of squares a few lane exchanges, and nothing is rounded between the two. Bound by memory.
+GH_KERNEL __launch_bounds__(256) void gh_norm_rope(GhNormRopeArgs a) {
+    const uint32_t row = blockIdx.x / a.groups, item = (blockIdx.x % a.groups) * 256 + threadIdx.x;
+    uint32_t head = item / a.lanes;
+    const uint32_t part = item & (a.lanes - 1);
+    if (head >= a.heads + a.kheads) return;  // whole heads
+    const bool key = head >= a.heads, there = 8 * part < a.head_dim;
+    if (key) head -= a.heads;
+    const uint64_t p = (key ? a.k : a.q) + (((uint64_t)row * (key ? a.kheads : a.heads) + head) * a.head_dim + 8 * part) * 2;
+    uint4 raw = make_uint4(0u, 0u, 0u, 0u), weight = raw;
+    if (there) {
+        raw = *gh_gp<uint4>(p);
+        weight = *gh_gp<uint4>((key ? a.k_norm : a.q_norm) + 16 * part);
+    }
+    const uint32_t pos = a.base + row;
+    const float scale = key ? 1.0f : gh_gp<float>(a.post)[pos];
+    float x[8];
+    gh_unpack8(raw, x);
+    gh_head_norm(x, weight, a.head_dim, a.eps, a.lanes);
+    if (4 * part < a.pairs) gh_turn4(x, gh_gp<float2>(a.table) + (uint64_t)pos * a.pairs, 4 * part, a.pairs, scale);
+    if (there) *gh_gpw<uint4>(p) = gh_pack8(x);
 }
 
 // The elementwise kernels below take 8 consecutive values per thread: 16-byte accesses where a.pad

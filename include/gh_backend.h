@@ -77,7 +77,12 @@ typedef struct gh_yarn {
 } gh_yarn;
 
 enum gh_rope_role { GH_ROPE_QUERY = 0, GH_ROPE_KEY = 1 }; /* backend/rope.rs:23-27 */
-enum gh_kv_scheme { GH_KV_F16 = 0, GH_KV_INT8 = 1 };      /* kv_cache/scheme.rs */
+/* F16 and INT8: kv_cache/scheme.rs. Q4 has no counterpart in the reference: a vector of 128 values takes 80 bytes, 64 of
+ * codes (dims 2 i and 2 i + 1 in the low and high half of byte i), then for each 32 dims a step d and a minimum m in FP16. Code c
+ * stands for f16(m + d c). Of 32 values, m is the least in FP16, d a fifteenth of their range cut off to FP16, and the
+ * code (x - m) / d as the nearest whole number, ties to even, 0 to 15 (0 where d is 0); 32 values with an infinity or a
+ * NaN among them stand for NaN. */
+enum gh_kv_scheme { GH_KV_F16 = 0, GH_KV_INT8 = 1, GH_KV_Q4 = 2 };
 
 /* Request KV handle (kv_cache/mod.rs:29-38). Caches are [layer][context][kv_heads][dim]. */
 typedef struct gh_kv {
@@ -103,7 +108,7 @@ typedef struct gh_kv {
  * a page number beyond the pool or a position beyond max_pos touches no memory, and the next
  * gh_submit returns GH_E_RANGE; that row's results are unspecified then, other rows' are not touched. */
 typedef struct gh_kv_paged {
-    gh_kv kv;            /* f16 scheme, head_dim = value_dim = 128; k, v on 16 bytes */
+    gh_kv kv;            /* f16 or q4 scheme, head_dim = value_dim = 128; k, v on 16 bytes */
     gh_buf table;        /* u32 [rows][table_width] page numbers */
     gh_buf lengths;      /* u32 [rows] cached positions of each row */
     gh_buf score;        /* FP32 [block_count][rows][kv_heads][table_width·page_size] accumulated attention
@@ -185,6 +190,13 @@ int gh_rope_yarn(gh_backend* b, gh_encoder* enc, const gh_buf* x, uint32_t heads
 int gh_rope_yarn_batched(gh_backend* b, gh_encoder* enc, const gh_buf* q, const gh_buf* k,
                          uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t base,
                          uint32_t rows, const gh_yarn* yarn);
+/* rope_yarn_batched with norms in the same pass (no counterpart in the reference): each head of q and k, FP16 in place,
+ * is divided by sqrt(its mean square + eps) and multiplied by its norm's weight (FP16 [head_dim]), then rotated (dims past
+ * rope_dim are not, nor scaled), with one rounding. head_dim: a multiple of 8 up to 512; buffers on 16 bytes and apart. */
+int gh_norm_rope_batched(gh_backend* b, gh_encoder* enc, const gh_buf* q, const gh_buf* k,
+                         uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t base,
+                         uint32_t rows, const gh_buf* q_norm, const gh_buf* k_norm, float eps,
+                         const gh_yarn* yarn);
 /* silu_mul, contract.rs:252-259: out = f16(f16(silu(gate)) * up) */
 int gh_silu_mul(gh_backend* b, gh_encoder* enc, const gh_buf* out, const gh_buf* gate,
                 const gh_buf* up, uint32_t n);
@@ -215,7 +227,7 @@ int gh_attention_decode_noalloc(gh_backend* b, gh_encoder* enc, const gh_buf* ou
 /* Append: `tokens` new K and V vectors per row, FP16 [rows][tokens][kv_heads][128], to the positions
  * lengths[r] - tokens .. lengths[r] - 1 of `layer` (the lengths already count them); their scores, where
  * kept, become 0. Vectors before a row's first position (lengths[r] < tokens) are skipped. The bytes of
- * gh_kv_write. Rows must not share the pages that they append to; k and v must not lie in slots that the
+ * gh_kv_write, or the vectors' codes in a q4 pool. Rows must not share the pages that they append to; k and v must not lie in slots that the
  * call writes, nor in the scores. */
 int gh_kv_write_paged(gh_backend* b, gh_encoder* enc, const gh_kv_paged* kv, const gh_buf* k,
                       const gh_buf* v, uint32_t tokens, uint32_t layer);
@@ -229,13 +241,25 @@ int gh_rope_kv_write_paged(gh_backend* b, gh_encoder* enc, const gh_kv_paged* kv
                            const gh_buf* q, const gh_buf* k, const gh_buf* v, uint32_t q_heads,
                            const gh_buf* positions, uint32_t tokens, uint32_t max_pos, const gh_yarn* yarn,
                            uint32_t layer);
+/* gh_rope_kv_write_paged with norms in the same pass: each head of q and k is divided by sqrt(its mean square + eps)
+ * and multiplied by its norm's weight (FP16 [128], on 16 bytes, no part of what the call writes) before the rotation. A query
+ * is rounded once, and so is a key, to FP16 or to its code. */
+int gh_norm_rope_kv_write_paged(gh_backend* b, gh_encoder* enc, const gh_kv_paged* kv, const gh_buf* q_out,
+                                const gh_buf* q, const gh_buf* k, const gh_buf* v, uint32_t q_heads,
+                                const gh_buf* q_norm, const gh_buf* k_norm, float eps, const gh_buf* positions,
+                                uint32_t tokens, uint32_t max_pos, const gh_yarn* yarn, uint32_t layer);
+/* The way back of gh_kv_write_paged: what the positions lengths[r] - tokens .. lengths[r] - 1 of `layer` hold, as FP16
+ * [rows][tokens][kv_heads][128] in k and v (apart, and no part of kv's buffers). Vectors before a row's first position are
+ * left as they are. With it a prefix in pages, in 4 bits too, becomes the contiguous cache that a prefill attends to. */
+int gh_kv_read_paged(gh_backend* b, gh_encoder* enc, const gh_buf* k, const gh_buf* v, const gh_kv_paged* kv,
+                     uint32_t tokens, uint32_t layer);
 /* Attention of one new token per row over its lengths[r] positions: q, out FP16 [rows][q_heads][128] (out is
  * q itself or no part of it, and no part of kv's buffers), 1 to 16 query heads per kv head. Free rows get
  * zeros. max_len: no row is longer (0: table_width·page_size); it sizes the launch. Where scores are kept, each position's attention weight,
  * summed over the query heads of a kv head, is added to its score. In the products with V a weight is held to
  * 2^-38 of the row's largest and is at least that, unless its score is -inf: n positions add up to n·2^-38 of their
  * mean V, and an infinite V leaves an infinity or NaN whatever its score. A row whose scores are all -inf gives
- * NaN. max_len also sizes the call's scratch: with scores 4 bytes per query head and position of every row, in groups of
+ * NaN. In a q4 pool weights are held to 2^-11 of themselves and 2^-39 of the row's largest. max_len also sizes the call's scratch: with scores 4 bytes per query head and position of every row, in groups of
  * rows that take at most 512 MiB. */
 int gh_attention_decode_paged(gh_backend* b, gh_encoder* enc, const gh_buf* out, const gh_buf* q,
                               const gh_kv_paged* kv, uint32_t q_heads, uint32_t max_len, uint32_t layer);
@@ -246,11 +270,30 @@ int gh_attention_decode_paged(gh_backend* b, gh_encoder* enc, const gh_buf* out,
  * (u32 [block_count][rows][kv_heads][budget], or NULL) receives their former positions. Shorter rows stay as
  * they are: nothing of theirs is written. src's pages are only read, so other rows may share them; dst's
  * pages of the evicted rows must be no page that src's rows use, and none of them twice. dst has src's rows,
- * page_size, block_count and heads, and the scores; its lengths and, with the same table_width, its scores may
+ * page_size, scheme, block_count and heads, and the scores; its lengths and, with the same table_width, its scores may
  * be src's own buffers, and its caches src's or parts of them; otherwise no buffer of dst that is written lies in one of
  * src, and kept lies in none of either. */
 int gh_kv_evict_paged(gh_backend* b, gh_encoder* enc, const gh_kv_paged* dst, const gh_kv_paged* src,
                       const gh_buf* kept, uint32_t budget, uint32_t recent);
+
+/* ---- sampling of a batch (no counterpart in the reference, which samples one row on the host) ---- */
+typedef struct gh_sample_params { /* one row's; the fields of gh_sampling */
+    float temperature; /* <= 0 or NaN: greedy argmax */
+    float top_p;       /* 1: off */
+    uint32_t top_k;    /* 0: off */
+    float min_p;       /* 0: off */
+} gh_sample_params;
+/* The next token of each row of logits, FP32 [rows][stride] of which the first vocab count, with settings and a
+ * uniform random number in [0, 1) per row, all on the device (params on 16 bytes): the token that gh_sample draws, with
+ * weights, sums and comparisons in 64 bits where gh_sample has FP32. Tokens with a finite logit, ranked by (logit descending
+ * by f32 total order, index ascending), have weights exp((logit - largest) / temperature). Kept are the first top_k; of these
+ * the fewest whose sum reaches top_p of theirs; of these the ones of at least min_p of the largest (always one). The draw
+ * is the first at which the running sum passes uniform (below 0 or NaN: 0; from 1 on: the last number below it) times
+ * the kept sum. A greedy row, and one without a finite logit, takes gh_read_argmax's token. tokens: u32 [rows]; probs: FP32
+ * [rows] or NULL, the drawn token's share of the kept sum (1 for a greedy row). Both lie apart from the inputs and from each
+ * other. vocab: at most 2^24. Scratch: 79 KB per row, for at most 128 MiB of rows at a time. */
+int gh_sample_rows(gh_backend* b, gh_encoder* enc, const gh_buf* tokens, const gh_buf* probs, const gh_buf* logits,
+                   uint32_t rows, uint32_t vocab, uint32_t stride, const gh_buf* params, const gh_buf* uniform);
 
 /* ---- read-back, contract.rs:300-318 (synchronous) ---- */
 int gh_read_logits(gh_backend* b, const gh_buf* logits, uint64_t vocab, float* dst);
