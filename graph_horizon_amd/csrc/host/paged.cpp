@@ -231,13 +231,17 @@ int attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv_pag
     const uint32_t tiles1 = ceil_div(max_len, tile);
     const uint64_t most = (uint64_t)kv->rows * hk * tiles1;
     const bool split = tiles1 <= kSpanTiles || most < 6144;
+    GhPaged4AttnArgs t{};
     if (q4) {
         if (split) {
             a.least = 2 * std::min(std::max(ceil_div(most, 8ull * b->cus) * 4, 4u), kSpanTiles);
             a.chunks = ceil_div(max_len, 16 * a.least);
         } else {
             a.least = 2;
-            a.chunks = std::max(1u, 16 * b->cus / hk);
+            t.heads = std::min(hk, 4u);
+            t.groups = ceil_div(hk, t.heads);
+            t.teams = 4 / t.heads;
+            a.chunks = std::max(1u, 3 * b->cus / t.groups) * t.teams;
             a.solo = 6;
         }
     } else if (split) {
@@ -299,7 +303,9 @@ int attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv_pag
         } else {
             // no more chunks than the rows' tiles can fill
             const uint64_t chunks = std::min<uint64_t>(a.chunks, ceil_div((uint64_t)a.rows * tiles1, a.least));
-            rc = launch(b, q4 ? scored ? K_PAGED4_ATTN_S : K_PAGED4_ATTN : scored ? K_PAGED_ATTN_S : K_PAGED_ATTN, ceil_div(hk * chunks, 4), 1, 1, 256, &a);
+            t.a = a;
+            if (q4) rc = launch(b, scored ? K_PAGED4_ATTN_S : K_PAGED4_ATTN, ceil_div(chunks, 8 * t.teams) * 8 * t.groups, 1, 1, 256, &t);
+            else rc = launch(b, scored ? K_PAGED_ATTN_S : K_PAGED_ATTN, ceil_div(hk * chunks, 4), 1, 1, 256, &a);
         }
         // the halves of the heads apart where a row may have more partials than one round of the join takes (64)
         const uint32_t halves = a.chunks > 64 * a.rows ? 2 : 1;

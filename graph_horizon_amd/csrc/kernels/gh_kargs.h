@@ -368,6 +368,17 @@ struct GhPagedAttnArgs {
     uint32_t blocks;   // gh_paged_join: workgroups per kv head that add scores
 };
 
+// gh_paged4_attn: workgroups of 4 waves, `teams` teams of `heads` each, which have a chunk and a wave per kv head; the kv heads
+// are in `groups` groups of so many. Workgroups i and i + 8, .. i + 8 (groups - 1) have the groups of the same chunks, so that they
+// run on one XCD and share the lines in which two groups' heads meet.
+struct GhPaged4AttnArgs {
+    GhPagedAttnArgs a;
+    uint32_t heads;
+    uint32_t teams;
+    uint32_t groups;
+    uint32_t pad;
+};
+
 // Eviction. Strides of a layer: slots of the pools, rows for the scores.
 struct GhPagedEvictArgs {
     GhPages src;

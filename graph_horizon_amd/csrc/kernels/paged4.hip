@@ -2,36 +2,38 @@
 // decode attention, eviction. The append with norms and the read-back are here for FP16 pools too.
 //
 // A vector of 128 values takes 80 bytes: 64 of codes, dims 2 i and 2 i + 1 in the low and high nibble of byte i, then
-// per 32 dims a step d and a minimum m in FP16 (d in the low half of a dword). Code c stands for f16(m + d c), one
-// rounding. What the device cannot trust (lengths, pages, positions) is checked as in paged.hip.
+// per 32 dims a step d and a minimum m in FP16 (d in the low half of a dword). Code c stands for m + d c.
+// What the device cannot trust (lengths, pages, positions) is checked as in paged.hip.
 #include "gh_head.h"
 #include "gh_paged.h"
 
 namespace {
 constexpr uint32_t kVector = 80;  // bytes
 typedef _Float16 ph2 __attribute__((ext_vector_type(2)));
+typedef _Float16 ph4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ uint32_t as_u(ph2 v) { return __builtin_bit_cast(uint32_t, v); }
 __device__ __forceinline__ ph2 as_h(uint32_t v) { return __builtin_bit_cast(ph2, v); }
 
 // The codes in the low nibbles of both halves of w, and in the second nibbles, as FP16: a nibble in the low bits of
-// 1024's mantissa is 1024 + c, in the next ones 1024 + 16 c, and both ways back are exact.
-__device__ __forceinline__ ph2 codes_low(uint32_t w) {
-    return as_h((w & 0x000F000Fu) | 0x64006400u) - ph2{(_Float16)1024.0f, (_Float16)1024.0f};
+// 1024's mantissa is 1024 + c, in the next ones 1024 + 16 c, and both ways back are exact. The constants are held in registers
+// (opaque to the compiler), so that mask and exponent are one v_and_or_b32.
+struct Masks {
+    uint32_t low, high, up;
+    __device__ __forceinline__ Masks() : low(0x000F000Fu), high(0x00F000F0u), up(0x64006400u) {
+        asm("" : "+s"(low));
+        asm("" : "+s"(high));
+        asm("" : "+v"(up));
+    }
+};
+__device__ __forceinline__ ph2 codes_low(uint32_t w, const Masks& c) {
+    return as_h((w & c.low) | c.up) - ph2{(_Float16)1024.0f, (_Float16)1024.0f};
 }
-__device__ __forceinline__ ph2 codes_high(uint32_t w) {
-    const ph2 x = as_h((w & 0x00F000F0u) | 0x64006400u);
-    return __builtin_elementwise_fma(x, ph2{(_Float16)0.0625f, (_Float16)0.0625f}, ph2{(_Float16)-64.0f, (_Float16)-64.0f});
+__device__ __forceinline__ ph2 codes_high(uint32_t w, const Masks& c) {
+    return __builtin_elementwise_fma(as_h((w & c.high) | c.up), ph2{(_Float16)0.0625f, (_Float16)0.0625f}, ph2{(_Float16)-64.0f, (_Float16)-64.0f});
 }
 // The low halves of two dwords, and the high ones.
 __device__ __forceinline__ uint32_t lows(uint32_t x0, uint32_t x1) { return __builtin_amdgcn_perm(x1, x0, 0x05040100u); }
 __device__ __forceinline__ uint32_t highs(uint32_t x0, uint32_t x1) { return __builtin_amdgcn_perm(x1, x0, 0x07060302u); }
-// Eight codes as values, in the order (0, 4), (1, 5), (2, 6), (3, 7); dm: step and minimum.
-__device__ __forceinline__ uint4 eight(uint32_t w, uint32_t dm) {
-    const ph2 d = as_h(lows(dm, dm)), m = as_h(highs(dm, dm));
-    const uint32_t w8 = w >> 8;
-    return make_uint4(as_u(__builtin_elementwise_fma(codes_low(w), d, m)), as_u(__builtin_elementwise_fma(codes_high(w), d, m)),
-                      as_u(__builtin_elementwise_fma(codes_low(w8), d, m)), as_u(__builtin_elementwise_fma(codes_high(w8), d, m)));
-}
 }  // namespace
 
 // ---- append ----------------------------------------------------------------------------------
@@ -149,8 +151,13 @@ __device__ __forceinline__ void paged_read(const GhPagedReadArgs& a) {
     if constexpr (Q4) {
         const uint64_t from = cache + vector * kVector;
         const uint32_t w = *gh_gp<uint32_t>(from + 4 * part), dm = *gh_gp<uint32_t>(from + 64 + (part & ~3u));
-        const uint4 y = eight(w, dm);  // (0, 4), (1, 5), (2, 6), (3, 7)
-        x = make_uint4(lows(y.x, y.y), lows(y.z, y.w), highs(y.x, y.y), highs(y.z, y.w));
+        const ph2 d = as_h(lows(dm, dm)), m = as_h(highs(dm, dm));
+        const Masks c;
+        uint32_t y[4];  // codes 0 and 4, 1 and 5, 2 and 6, 3 and 7
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            y[i] = as_u(__builtin_elementwise_fma(i & 1 ? codes_high(w >> (8 * (i >> 1)), c) : codes_low(w >> (8 * (i >> 1)), c), d, m));
+        x = make_uint4(lows(y[0], y[1]), lows(y[2], y[3]), highs(y[0], y[1]), highs(y[2], y[3]));
     } else {
         x = *gh_gp<uint4>(cache + vector * 256 + 16 * part);
     }
@@ -162,79 +169,141 @@ GH_KERNEL __launch_bounds__(256) void gh_paged_read(GhPagedReadArgs a) { paged_r
 
 // ---- decode attention ---------------------------------------------------------------------------
 // The plan of paged.hip: a wave takes the G <= 16 query heads of one kv head over tiles, here of 32 positions in two
-// halves of 16, each within one page and so at one address. Per half:
-//   S^T = K·Q^T     4 x v_mfma_f32_16x16x32_f16: a lane's 32 k-slots are the 32 dims 32 (l / 16) .. + 32 of position
-//                   l % 16, which is 16 bytes of codes in one load with one step and one minimum (the query's fragments
-//                   are in the order in which the codes come out of their dwords);
-// and per tile
-//   O^T += V^T·P^T  per 8-dim tile t one v_mfma_f32_16x16x32_f16 over the 32 positions: a lane has dims 8 (l % 16) ..
-//                   + 8, a dword of codes, of 4 (l / 16) + i of both halves. Bytes of two positions are gathered
-//                   in one dword before they become values, so that steps and minima apply to pairs of positions.
-// Values are f16(m + d c), as a read-back gives them. Weights are 2^(s - m + 15) in FP16, nearest: 2^-11 of each and
-// 2^-39 of the largest; next to the output's own 2^-11 this is half an FP16 cache's MFMAs and none of its splitting (a V
-// here is finite or NaN, so a weight of 0 hides nothing). A maximum that stays leaves the sums unscaled.
+// halves of 16, each within one page and so at one address. Vectors of 80 bytes fill no lines, but those of adjacent heads lie
+// in a row: the four waves of a workgroup take up to four heads of the same positions and bring their bytes to LDS together, five
+// 16-byte loads a lane, asked for a tile ahead. (64 rows of 8192, 671 MB: fragments loaded straight from memory, 20 loads of 64 to 1024
+// bytes, 282 us; each wave its own head through LDS 204; so 131, of which the loads alone take 114 and all but them 104.)
+// Per half, S^T = K·Q^T with the codes as they are: a nibble in the low bits of an FP16 number is c 2^-24, in the next ones
+// c 2^-20, and the matrix cores take subnormals, so that a mask is all it needs. v_mfma_f32_16x16x32_f16 s (0..3) covers dims
+// 32 s .. + 32, one step and minimum a position: lane l has dims 32 s + 8 (l / 16) .. + 8 of position l % 16, which
+// four row swaps make of the 16 bytes in a row that it reads. The sums are those of exact products in FP32; steps come to
+// the lanes that need them by a product with a unit vector, and the minima's part is one product with the sums of the query over
+// its groups, in FP16 hi + lo. So no key is rounded, for less than the conversion of its codes to FP16 takes.
+// O^T += V^T·P^T per tile: per 8-dim tile t products over the 32 positions: a lane has dims 8 (l % 16) .. + 8, a dword of
+// codes, of positions 4 (l / 16) + i of both halves. Bytes of two positions are gathered in one dword before they
+// become f16(m + d c), so that steps and minima apply to pairs of positions. Weights are 2^(s - m + 15), FP16 hi + lo
+// each in a product of its own: 22 bits, and 2^-39 of the largest weight. V here is finite or NaN, so a weight of 0 hides
+// nothing. A maximum that stays leaves the sums unscaled.
 namespace {
 struct Tile4 {
-    uint4 k[2];                // position l % 16 of each half, dims 32 (l / 16) .. + 32
-    uint32_t kd[2];
-    uint32_t v[8], vd[8];      // [4 half + i]: position 4 (l / 16) + i, dims 8 (l % 16) .. + 8
+    uint4 x[5];  // 16-byte pieces l of each half's K and of each half's V, then the 64 H + l % 16 H-th of the (l / 16 H)-th
 };
+constexpr uint32_t kHalfBytes = 16 * kVector, kTileBytes = 4 * kHalfBytes;
+constexpr uint32_t kStageBytes = kTileBytes + kVector;  // of a head, so that a team's pieces meet no bank twice
 
-// K and V of one head from the slot of a half's first position, `count` positions long (0: nothing is read).
-struct Half {
-    __amdgpu_buffer_rsrc_t k, v;
-};
-__device__ __forceinline__ Half half_at(const GhPages& p, uint32_t slot, uint32_t count, uint32_t kvh) {
-    const uint32_t row_bytes = p.kv_heads * kVector;
-    const uint64_t at = (uint64_t)slot * row_bytes + kvh * kVector;
-    const int range = count ? (int)((count - 1) * row_bytes + kVector) : 0;
-    return {__builtin_amdgcn_make_buffer_rsrc((void*)(p.kc + at), 0, range, kBufWord3),
-            __builtin_amdgcn_make_buffer_rsrc((void*)(p.vc + at), 0, range, kBufWord3)};
-}
+// A tile's slots of its first and 17th position and their number of positions (0: nothing is read).
 struct Where {
-    Half half[2];
+    uint32_t slot0, slot1, count;
 };
-__device__ __forceinline__ Where tile_at(const GhPages& p, uint32_t slot0, uint32_t slot1, uint32_t count, uint32_t kvh) {
-    return {{half_at(p, slot0, min(count, 16u), kvh), half_at(p, slot1, max(count, 16u) - 16u, kvh)}};
-}
-template <int CACHE>
-__device__ __forceinline__ void load_k(const Where& w, uint32_t row_bytes, Tile4& r) {
-    const uint32_t lane = threadIdx.x & 63u, n = lane & 15u, g = lane >> 4;
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        r.k[u] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(w.half[u].k, n * row_bytes + 16 * g, 0, CACHE));
-        r.kd[u] = __builtin_amdgcn_raw_buffer_load_b32(w.half[u].k, n * row_bytes + 64 + 4 * g, 0, CACHE);
+// A team of H waves takes H heads of the same tiles, and its 64 H lanes their bytes: 16 positions of H heads are 80 H pieces
+// of 16 bytes, in a row if these are all heads. What a lane keeps of its pieces (first: the team's first head, l: the lane
+// in the team):
+struct Pieces {
+    uint64_t base, k, v;    // of the fifth piece, and of K and V of the team's heads
+    uint32_t at, row, off;  // of the first four; the fifth's position, and where it is in its row
+    uint32_t row_bytes, range;
+    uint32_t to, to5;       // places in LDS
+    // There are `have` of the H heads (fewer in the last group): the places of others are read from these.
+    __device__ __forceinline__ Pieces(const GhPages& p, uint32_t first, uint32_t heads, uint32_t l, uint32_t have) {
+        const uint32_t per = 5 * heads;  // pieces of a position
+        row_bytes = p.kv_heads * kVector;
+        range = have * kVector;
+        k = p.kc + first * kVector;
+        v = p.vc + first * kVector;
+        const uint32_t q = l / per, r = l % per;
+        at = q * row_bytes + r % (5 * have) * 16;
+        to = r / 5 * kStageBytes + q * kVector + r % 5 * 16;
+        const uint32_t block = l / (16 * heads), piece = 64 * heads + l % (16 * heads), r5 = piece % per;
+        row = piece / per;
+        off = r5 % (5 * have) * 16;
+        to5 = r5 / 5 * kStageBytes + block * kHalfBytes + row * kVector + r5 % 5 * 16;
+        base = (block < 2 ? k : v) + off;
+        second = block & 1;
     }
-}
+    bool second;            // the fifth is of the second half
+};
 template <int CACHE>
-__device__ __forceinline__ void load_v(const Where& w, uint32_t row_bytes, Tile4& r) {
-    const uint32_t lane = threadIdx.x & 63u, n = lane & 15u, g = lane >> 4;
+__device__ __forceinline__ void load_tile(const Where w, const Pieces& p, Tile4& r) {
+    if (w.count == 0) return;
+    const uint32_t c0 = min(w.count, 16u), c1 = w.count - c0, s0 = w.slot0, s1 = w.slot1;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        r.v[i] = __builtin_amdgcn_raw_buffer_load_b32(w.half[i >> 2].v, (4 * g + (i & 3)) * row_bytes + 4 * n, 0, CACHE);
-        r.vd[i] = __builtin_amdgcn_raw_buffer_load_b32(w.half[i >> 2].v, (4 * g + (i & 3)) * row_bytes + 64 + (n & ~3u), 0, CACHE);
+    for (int i = 0; i < 4; ++i) {
+        const uint64_t at = (i < 2 ? p.k : p.v) + (uint64_t)(i & 1 ? s1 : s0) * p.row_bytes;
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+            (void*)at, 0, (i & 1 ? c1 : c0) ? (int)(((i & 1 ? c1 : c0) - 1) * p.row_bytes + p.range) : 0, kBufWord3);
+        r.x[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, p.at, 0, CACHE));
     }
+    // past the half's positions: the last one again, which has another's weight, and hides nothing that is not seen there
+    uint32_t row = p.row;
+    if (w.count < 32) row = min(row, max(p.second ? c1 : c0, 1u) - 1);
+    typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+    const GH_GLOBAL u4v* from = gh_gp<u4v>(p.base + (uint64_t)((p.second ? s1 : s0) + row) * p.row_bytes);
+    r.x[4] = __builtin_bit_cast(uint4, CACHE ? __builtin_nontemporal_load(from) : *from);
+}
+// The lane's pieces into the team's part of LDS.
+__device__ __forceinline__ void store_tile(const Tile4& r, const Pieces& p, char* lds) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *(uint4*)(lds + i * kHalfBytes + p.to) = r.x[i];
+    *(uint4*)(lds + p.to5) = r.x[4];
+}
+// A wave's own stores and reads of LDS stay in order.
+__device__ __forceinline__ void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
-// B fragments of the G queries of a kv head: head n = l % 16 (zero past G), dims 32 (l / 16) + 8 s .. + 8 in the
-// order of eight().
-__device__ __forceinline__ void load_q4(const GhPagedAttnArgs& a, uint32_t row, uint32_t kvh, ph8 (&qf)[4]) {
+// B fragments of the G queries of a kv head: head n = l % 16 (zero past G). x: dims 32 s + 8 (l / 16) .. + 8 in the order
+// (0, 4), (1, 5), (2, 6), (3, 7), those that meet codes of 2^-20 times 2^-4. sums: 2^-9 of the sum over the dims of group l / 16,
+// hi and lo, in the places of the minima. step: 2^15 in the place of the step of group s.
+struct Query {
+    ph8 x[4];
+    ph4 sums, step[4];
+};
+__device__ __forceinline__ void load_q4(const GhPagedAttnArgs& a, uint32_t row, uint32_t kvh, Query& q) {
     const uint32_t lane = threadIdx.x & 63u, n = lane & 15u, g = lane >> 4, G = a.group;
-    const GH_GLOBAL uint4* qp = gh_gp<uint4>(a.q + (((uint64_t)row * a.q_heads + kvh * G + min(n, G - 1)) * 128 + 32 * g) * 2);
+    const GH_GLOBAL uint4* qp = gh_gp<uint4>(a.q + (((uint64_t)row * a.q_heads + kvh * G + min(n, G - 1)) * 128 + 8 * g) * 2);
+    const ph2 down = {(_Float16)0.0625f, (_Float16)0.0625f};
+    float mine = 0.0f;
+#pragma unroll
+    for (uint32_t s = 0; s < 4; ++s) {
+        uint4 x = qp[4 * s];
+        if (n >= G) x = make_uint4(0u, 0u, 0u, 0u);
+        float v[8];
+        gh_unpack8(x, v);
+        const float sum = lanes4_sum(((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7])));
+        if (s == g) mine = sum;
+        q.x[s] = __builtin_bit_cast(ph8, make_uint4(lows(x.x, x.z), as_u(as_h(highs(x.x, x.z)) * down),
+                                                    lows(x.y, x.w), as_u(as_h(highs(x.y, x.w)) * down)));
+        const uint32_t one = s == g ? 0x7800u : 0u;
+        q.step[s] = __builtin_bit_cast(ph4, make_uint2(one, 0u));
+    }
+    mine *= 0x1p-9f;
+    const uint32_t hi = gh_f2h(mine), lo = gh_f2h(mine - gh_h2f(hi));
+    q.sums = __builtin_bit_cast(ph4, make_uint2(hi << 16, lo << 16));
+}
+
+// Products of a half, times 2^-9, from its K in LDS.
+__device__ __forceinline__ pf4 half_products(const char* lds, const Query& q) {
+    const uint32_t lane = threadIdx.x & 63u, n = lane & 15u, g = lane >> 4;
+    const uint4 k = *(const uint4*)(lds + n * kVector + 16 * g);
+    const uint32_t dm = *(const uint32_t*)(lds + n * kVector + 64 + 4 * g);
+    // lane g has dwords 4 g + j; it takes 4 s + g: row j and lane group g change places
+    const auto a = __builtin_amdgcn_permlane32_swap(k.x, k.z, false, false), b = __builtin_amdgcn_permlane32_swap(k.y, k.w, false, false);
+    const auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false), d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+    const uint32_t w[4] = {c[0], c[1], d[0], d[1]};
+    const ph4 dms = __builtin_bit_cast(ph4, make_uint2(dm, dm));
+    const pf4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    pf4 sum = __builtin_amdgcn_mfma_f32_16x16x16f16(dms, q.sums, zero, 0, 0, 0);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-        const uint4 x = qp[s];
-        const uint4 y = make_uint4(lows(x.x, x.z), highs(x.x, x.z), lows(x.y, x.w), highs(x.y, x.w));
-        qf[s] = __builtin_bit_cast(ph8, n < G ? y : make_uint4(0u, 0u, 0u, 0u));
-    }
-}
-
-__device__ __forceinline__ pf4 half_products(const uint4& k, uint32_t dm, const ph8 (&qf)[4]) {
-    const uint32_t w[4] = {k.x, k.y, k.z, k.w};
-    pf4 st = {0.0f, 0.0f, 0.0f, 0.0f};
+        const uint32_t w8 = w[s] >> 8;
+        const ph8 codes = __builtin_bit_cast(ph8, make_uint4(w[s] & 0x000F000Fu, w[s] & 0x00F000F0u, w8 & 0x000F000Fu, w8 & 0x00F000F0u));
+        const pf4 st = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, q.x[s], zero, 0, 0, 0);
+        const pf4 step = __builtin_amdgcn_mfma_f32_16x16x16f16(dms, q.step[s], zero, 0, 0, 0);
 #pragma unroll
-    for (int s = 0; s < 4; ++s) st = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ph8, eight(w[s], dm)), qf[s], st, 0, 0, 0);
-    return st;
+        for (int i = 0; i < 4; ++i) sum[i] = __builtin_fmaf(step[i], st[i], sum[i]);
+    }
+    return sum;
 }
 // -inf past the tile's positions
 __device__ __forceinline__ void hide(pf4 (&st)[2], uint32_t count) {
@@ -244,10 +313,41 @@ __device__ __forceinline__ void hide(pf4 (&st)[2], uint32_t count) {
     for (int i = 0; i < 8; ++i)
         if (16 * (i >> 2) + 4 * g + (i & 3) >= count) st[i >> 2][i & 3] = -__builtin_inff();
 }
+// The largest of two and of three, without the instructions by which fmaxf quiets its inputs first. (Ordinary vector results
+// go in: none of a matrix instruction, which would need waits of their own.)
+__device__ __forceinline__ float larger(float x, float y) {
+    float r;
+    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(x), "v"(y));
+    return r;
+}
+__device__ __forceinline__ float largest(float x, float y, float z) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+    return r;
+}
+__device__ __forceinline__ float lanes4_larger(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = larger(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return larger(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+// A lane's V of a tile: dwords and steps with minima [4 half + i] of position 4 (l / 16) + i, dims 8 (l % 16) .. + 8.
+struct Values {
+    uint32_t v[8], dm[8];
+};
+__device__ __forceinline__ void load_v(const char* lds, Values& y) {
+    const uint32_t lane = threadIdx.x & 63u, n = lane & 15u, g = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const char* at = lds + (i >> 2) * kHalfBytes + (4 * g + (i & 3)) * kVector;
+        y.v[i] = *(const uint32_t*)(at + 4 * n);
+        y.dm[i] = *(const uint32_t*)(at + 64 + (n & ~3u));
+    }
+}
 // st: products, which times `scale` are scores in base 2
-__device__ __forceinline__ void tile_add(Sums& x, const pf4 (&st)[2], float scale, const Tile4& r) {
-    float top = fmaxf(fmaxf(fmaxf(st[0][0], st[0][1]), fmaxf(st[0][2], st[0][3])), fmaxf(fmaxf(st[1][0], st[1][1]), fmaxf(st[1][2], st[1][3])));
-    const float mx = fmaxf(x.m, lanes4_max(top) * scale);
+__device__ __forceinline__ void tile_add(Sums& x, const pf4 (&st)[2], float scale, const Masks& c, const Values& y) {
+    const float top = largest(largest(st[0][0], st[0][1], st[0][2]), largest(st[0][3], st[1][0], st[1][1]), larger(st[1][2], st[1][3]));
+    const float mx = larger(x.m, lanes4_larger(top) * scale);
     if (__builtin_amdgcn_ballot_w64(mx != x.m)) {
         const float f = share(x.m, mx);
         x.m = mx;
@@ -258,31 +358,40 @@ __device__ __forceinline__ void tile_add(Sums& x, const pf4 (&st)[2], float scal
     // nothing but -inf so far: every weight 0
     const float up = mx == -__builtin_inff() ? 0.0f : kUp - mx;
     float p[8];
-    uint32_t ph[4];
+    uint32_t hi[4], lo[4];
 #pragma unroll
     for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i >> 2][i & 3], scale, up));
     x.l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) ph[i] = as_u(ph2{(_Float16)p[2 * i], (_Float16)p[2 * i + 1]});
-    const ph8 pv = __builtin_bit_cast(ph8, make_uint4(ph[0], ph[1], ph[2], ph[3]));
+    for (int i = 0; i < 4; ++i) {
+        const ph2 h = __builtin_bit_cast(ph2, __builtin_amdgcn_cvt_pkrtz(p[2 * i], p[2 * i + 1]));
+        hi[i] = as_u(h);
+        lo[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)h.x, -1.0f, p[2 * i]), __builtin_fmaf((float)h.y, -1.0f, p[2 * i + 1])));
+    }
+    const ph8 p0 = __builtin_bit_cast(ph8, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+    const ph8 p1 = __builtin_bit_cast(ph8, make_uint4(lo[0], lo[1], lo[2], lo[3]));
     ph2 d[4], m[4];  // of two positions
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        d[i] = as_h(lows(r.vd[2 * i], r.vd[2 * i + 1]));
-        m[i] = as_h(highs(r.vd[2 * i], r.vd[2 * i + 1]));
+        d[i] = as_h(lows(y.dm[2 * i], y.dm[2 * i + 1]));
+        m[i] = as_h(highs(y.dm[2 * i], y.dm[2 * i + 1]));
     }
 #pragma unroll
     for (uint32_t b = 0; b < 4; ++b) {
-        uint32_t lo[4], hi[4];
+        uint32_t v0[4], v1[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             // byte b of both positions, in the low bytes of the halves
-            const uint32_t w = __builtin_amdgcn_perm(r.v[2 * i + 1], r.v[2 * i], 0x0C000C00u | (4 + b) << 16 | b);
-            lo[i] = as_u(__builtin_elementwise_fma(codes_low(w), d[i], m[i]));
-            hi[i] = as_u(__builtin_elementwise_fma(codes_high(w), d[i], m[i]));
+            const uint32_t w = __builtin_amdgcn_perm(y.v[2 * i + 1], y.v[2 * i], 0x0C000C00u | (4 + b) << 16 | b);
+            v0[i] = as_u(__builtin_elementwise_fma(codes_low(w, c), d[i], m[i]));
+            v1[i] = as_u(__builtin_elementwise_fma(codes_high(w, c), d[i], m[i]));
         }
-        x.acc[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ph8, make_uint4(lo[0], lo[1], lo[2], lo[3])), pv, x.acc[2 * b], 0, 0, 0);
-        x.acc[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ph8, make_uint4(hi[0], hi[1], hi[2], hi[3])), pv, x.acc[2 * b + 1], 0, 0, 0);
+        const ph8 a0 = __builtin_bit_cast(ph8, make_uint4(v0[0], v0[1], v0[2], v0[3]));
+        const ph8 a1 = __builtin_bit_cast(ph8, make_uint4(v1[0], v1[1], v1[2], v1[3]));
+        x.acc[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, p0, x.acc[2 * b], 0, 0, 0);
+        x.acc[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, p0, x.acc[2 * b + 1], 0, 0, 0);
+        x.acc[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, p1, x.acc[2 * b], 0, 0, 0);
+        x.acc[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, p1, x.acc[2 * b + 1], 0, 0, 0);
     }
 }
 // The scores of the lane's head at positions `pos` and on of a row, past its length too (raw_len is whole tiles).
@@ -308,12 +417,17 @@ __device__ __forceinline__ bool tile_slots(const GhPages& p, uint32_t row, uint3
     return good;
 }
 
-// One chunk of the rows' tiles for one kv head by one wave.
+// One chunk of the rows' tiles for a team's heads. All teams of the workgroup go through `rounds` tiles, where their chunks
+// have fewer with nothing in the last. lds: the team's, mine0: the wave's, in the first of two buffers; kvh: the wave's head,
+// if `there` is one.
 template <bool SCORED, int CACHE>
 __device__ __forceinline__ void paged4_chunk(const GhPagedAttnArgs& a, const RowsLds& sh, uint32_t behind, uint32_t total,
-                                             uint32_t per, uint32_t chunk, uint32_t kvh) {
+                                             uint32_t per, uint32_t chunk, uint32_t rounds, uint32_t kvh, bool there, bool idle, const Pieces& pieces,
+                                             char* lds, const char* mine0) {
     const uint32_t lane = threadIdx.x & 63u, n = lane & 15u, G = a.group;
-    const uint32_t begin = chunk * per, tiles = min(per, total - begin), row_bytes = a.p.kv_heads * kVector;
+    const uint32_t begin = min(chunk * per, total), tiles = idle ? 0u : min(per, total - begin);
+    const Masks masks;
+    const float scale = a.scale * 512.0f;
 
     // lane i: slots, first position, and row | positions << 16 of tile i of the current 64
     uint32_t t_slot0 = 0, t_slot1 = 0, t_pos = 0, t_row = 0;
@@ -339,10 +453,10 @@ __device__ __forceinline__ void paged4_chunk(const GhPagedAttnArgs& a, const Row
     look_up(0);
     auto where = [&](uint32_t i) __attribute__((always_inline)) {
         const uint32_t count = i < tiles ? __builtin_amdgcn_readlane(t_row, i & 63u) >> 16 : 0u;
-        return tile_at(a.p, __builtin_amdgcn_readlane(t_slot0, i & 63u), __builtin_amdgcn_readlane(t_slot1, i & 63u), count, kvh);
+        return Where{(uint32_t)__builtin_amdgcn_readlane(t_slot0, i & 63u), (uint32_t)__builtin_amdgcn_readlane(t_slot1, i & 63u), count};
     };
 
-    ph8 qf[4];
+    Query q;
     Sums x;
     uint32_t row, since;  // the row at hand and the tile it began with
     uint64_t raw = 0;
@@ -357,41 +471,47 @@ __device__ __forceinline__ void paged4_chunk(const GhPagedAttnArgs& a, const Row
         row = info & 0xFFFFu;
         since = i;
         x.clear();
-        load_q4(a, row, kvh, qf);
+        load_q4(a, row, kvh, q);
         if (SCORED) raw = a.raw + (((uint64_t)row * a.p.kv_heads + kvh) * G + n) * a.raw_len * 4;
     };
-    start(__builtin_amdgcn_readlane(t_row, 0), 0);
+    if (there && tiles) start(__builtin_amdgcn_readlane(t_row, 0), 0);
 
-    // K of the next tile is asked for as soon as this one's products are made, V behind its last use
     Tile4 r;
-    Where w = where(0);
-    load_k<CACHE>(w, row_bytes, r);
-    load_v<CACHE>(w, row_bytes, r);
-    for (uint32_t i = 0; i < tiles; ++i) {
+    load_tile<CACHE>(where(0), pieces, r);
+    for (uint32_t i = 0; i < rounds; ++i) {
         const uint32_t info = __builtin_amdgcn_readlane(t_row, i & 63u);
         const uint32_t pos = SCORED ? __builtin_amdgcn_readlane(t_pos, i & 63u) : 0u;
+        char* buf = lds + (i & 1) * (4 * kStageBytes);
+        const char* mine = mine0 + (i & 1) * (4 * kStageBytes);
+        // two buffers in turn: behind the barrier all have read the tile before
+        if (!idle) store_tile(r, pieces, buf);
+        gh_lds_barrier();
+        if ((i & 63u) == 63) look_up(i + 1);
+        load_tile<CACHE>(where(i + 1), pieces, r);
+        if (!there || i >= tiles) continue;
         if ((info & 0xFFFFu) != row) {
             flush(i);
             start(info, i);
         }
-        pf4 st[2] = {half_products(r.k[0], r.kd[0], qf), half_products(r.k[1], r.kd[1], qf)};
-        if ((i & 63u) == 63) look_up(i + 1);
-        w = where(i + 1);
-        load_k<CACHE>(w, row_bytes, r);
+        pf4 st[2] = {half_products(mine, q), half_products(mine + kHalfBytes, q)};
         hide(st, info >> 16);
-        if (SCORED && n < G) keep_scores(raw, pos, st, a.scale);
-        tile_add(x, st, a.scale, r);
-        load_v<CACHE>(w, row_bytes, r);
+        if (SCORED && n < G) keep_scores(raw, pos, st, scale);
+        Values y;
+        load_v(mine + 2 * kHalfBytes, y);
+        tile_add(x, st, scale, masks, y);
     }
-    flush(tiles);
+    if (there && tiles) flush(tiles);
 }
 
-// All rows' tiles in equal chunks, as gh_paged_attn.
+// All rows' tiles in equal chunks, as gh_paged_attn, with a team per chunk.
 template <bool SCORED>
-__device__ __forceinline__ void paged4_attn(const GhPagedAttnArgs& a) {
+__device__ __forceinline__ void paged4_attn(const GhPaged4AttnArgs& t) {
     __shared__ RowsLds sh;
-    const uint32_t unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t chunk = unit / a.p.kv_heads, kvh = unit % a.p.kv_heads;
+    __shared__ __align__(16) char stage[8 * kStageBytes];
+    const GhPagedAttnArgs& a = t.a;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), team = wave / t.heads, member = wave % t.heads;
+    const uint32_t set = blockIdx.x / (8 * t.groups) * 8 + blockIdx.x % 8, first = set * t.teams, chunk = first + team;
+    const uint32_t head = blockIdx.x / 8 % t.groups * t.heads, kvh = head + member;
     const uint32_t behind = lay_out_rows<5>(a, sh, blockIdx.x == 0);
     const uint32_t total = sh.first[a.rows];
     const uint32_t half = (2 * total + a.chunks - 1) / a.chunks;
@@ -404,15 +524,23 @@ __device__ __forceinline__ void paged4_attn(const GhPagedAttnArgs& a) {
         if (sh.len[r] == 0)
             for (uint32_t i = threadIdx.x; i < a.q_heads * 64; i += 256)
                 gh_gpw<uint32_t>(a.out)[(uint64_t)r * a.q_heads * 64 + i] = 0u;
-    if (chunk >= a.chunks || chunk * per >= total) return;
-    if ((uint64_t)total * a.p.kv_heads * (64 * kVector) >= a.stream) paged4_chunk<SCORED, kStream>(a, sh, behind, total, per, chunk, kvh);
-    else paged4_chunk<SCORED, 0>(a, sh, behind, total, per, chunk, kvh);
+    if (first * per >= total) return;  // the whole workgroup
+    const uint32_t rounds = min(per, total - first * per), heads = min(t.heads, a.p.kv_heads - head);
+    const bool idle = team >= t.teams, there = !idle && member < heads;  // three heads leave a wave without a team
+    const Pieces pieces(a.p, head, t.heads, threadIdx.x - team * t.heads * 64, heads);
+    char* lds = stage + team * t.heads * kStageBytes;
+    const char* mine = lds + member * kStageBytes;
+    if ((uint64_t)total * a.p.kv_heads * (64 * kVector) >= a.stream)
+        paged4_chunk<SCORED, kStream>(a, sh, behind, total, per, chunk, rounds, kvh, there, idle, pieces, lds, mine);
+    else
+        paged4_chunk<SCORED, 0>(a, sh, behind, total, per, chunk, rounds, kvh, there, idle, pieces, lds, mine);
 }
 
 // Each row in spans, as gh_paged_split: of a.least / 2 tiles, of which wave w takes w, w + 4, ...
 template <bool SCORED>
 __device__ __forceinline__ void paged4_split(const GhPagedAttnArgs& a) {
     extern __shared__ __align__(16) float dyn[];  // per wave and head: 132 floats of acc, then m and l
+    __shared__ __align__(16) char stage[4][kTileBytes];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, n = lane & 15u, G = a.group;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t kvh = blockIdx.x, split = blockIdx.y, row = blockIdx.z;
@@ -426,42 +554,47 @@ __device__ __forceinline__ void paged4_split(const GhPagedAttnArgs& a) {
         return;
     }
     if (begin >= len) return;
-    ph8 qf[4];
-    load_q4(a, row, kvh, qf);
+    Query q;
+    load_q4(a, row, kvh, q);
+    const float scale = a.scale * 512.0f;
     const uint32_t end = min(len, begin + span);
     uint32_t t_slot0 = 0, t_slot1 = 0, t_count = 0;
     if (mine < end) {
         const uint32_t count = min(end - mine, 32u);
         if (tile_slots(a.p, row, mine, count, &t_slot0, &t_slot1)) t_count = count;
     }
-    const uint32_t tiles = first < end ? (end - first + 127) / 128 : 0u, row_bytes = a.p.kv_heads * kVector;
+    const uint32_t tiles = first < end ? (end - first + 127) / 128 : 0u;
+    const Pieces pieces(a.p, kvh, 1, lane, 1);
+    const Masks masks;
     auto where = [&](uint32_t i) __attribute__((always_inline)) {
         const uint32_t count = i < tiles ? __builtin_amdgcn_readlane(t_count, i & 63u) : 0u;
-        return tile_at(a.p, __builtin_amdgcn_readlane(t_slot0, i & 63u), __builtin_amdgcn_readlane(t_slot1, i & 63u), count, kvh);
+        return Where{(uint32_t)__builtin_amdgcn_readlane(t_slot0, i & 63u), (uint32_t)__builtin_amdgcn_readlane(t_slot1, i & 63u), count};
     };
     const uint64_t raw = a.raw + (((uint64_t)row * a.p.kv_heads + kvh) * G + n) * a.raw_len * 4;
     Sums x;
     x.clear();
     if (tiles) {
+        char* lds = stage[wave];
         Tile4 r;
-        Where w = where(0);
-        load_k<0>(w, row_bytes, r);
-        load_v<0>(w, row_bytes, r);
+        load_tile<0>(where(0), pieces, r);
         for (uint32_t i = 0; i < tiles; ++i) {
-            pf4 st[2] = {half_products(r.k[0], r.kd[0], qf), half_products(r.k[1], r.kd[1], qf)};
-            w = where(i + 1);
-            load_k<0>(w, row_bytes, r);
+            wave_order();
+            store_tile(r, pieces, lds);
+            wave_order();
+            load_tile<0>(where(i + 1), pieces, r);
+            pf4 st[2] = {half_products(lds, q), half_products(lds + kHalfBytes, q)};
             hide(st, __builtin_amdgcn_readlane(t_count, i & 63u));
-            if (SCORED && n < G) keep_scores(raw, first + 128 * i, st, a.scale);
-            tile_add(x, st, a.scale, r);
-            load_v<0>(w, row_bytes, r);
+            if (SCORED && n < G) keep_scores(raw, first + 128 * i, st, scale);
+            Values y;
+            load_v(lds + 2 * kHalfBytes, y);
+            tile_add(x, st, scale, masks, y);
         }
     }
     split_finish<SCORED>(a, x, dyn, row, kvh, split, span, len);
 }
 }  // namespace
-GH_KERNEL __launch_bounds__(256, 4) void gh_paged4_attn(GhPagedAttnArgs a) { paged4_attn<false>(a); }
-GH_KERNEL __launch_bounds__(256, 4) void gh_paged4_attn_s(GhPagedAttnArgs a) { paged4_attn<true>(a); }
+GH_KERNEL __launch_bounds__(256, 3) void gh_paged4_attn(GhPaged4AttnArgs a) { paged4_attn<false>(a); }
+GH_KERNEL __launch_bounds__(256, 3) void gh_paged4_attn_s(GhPaged4AttnArgs a) { paged4_attn<true>(a); }
 GH_KERNEL __launch_bounds__(256) void gh_paged4_split(GhPagedAttnArgs a) { paged4_split<false>(a); }
 GH_KERNEL __launch_bounds__(256) void gh_paged4_split_s(GhPagedAttnArgs a) { paged4_split<true>(a); }
 

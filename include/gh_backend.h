@@ -79,7 +79,7 @@ typedef struct gh_yarn {
 enum gh_rope_role { GH_ROPE_QUERY = 0, GH_ROPE_KEY = 1 }; /* backend/rope.rs:23-27 */
 /* F16 and INT8: kv_cache/scheme.rs. Q4 has no counterpart in the reference: a vector of 128 values takes 80 bytes, 64 of
  * codes (dims 2 i and 2 i + 1 in the low and high half of byte i), then for each 32 dims a step d and a minimum m in FP16. Code c
- * stands for f16(m + d c). Of 32 values, m is the least in FP16, d a fifteenth of their range cut off to FP16, and the
+ * stands for m + d c. Of 32 values, m is the least in FP16, d a fifteenth of their range cut off to FP16, and the
  * code (x - m) / d as the nearest whole number, ties to even, 0 to 15 (0 where d is 0); 32 values with an infinity or a
  * NaN among them stand for NaN. */
 enum gh_kv_scheme { GH_KV_F16 = 0, GH_KV_INT8 = 1, GH_KV_Q4 = 2 };
@@ -248,7 +248,7 @@ int gh_norm_rope_kv_write_paged(gh_backend* b, gh_encoder* enc, const gh_kv_page
                                 const gh_buf* q, const gh_buf* k, const gh_buf* v, uint32_t q_heads,
                                 const gh_buf* q_norm, const gh_buf* k_norm, float eps, const gh_buf* positions,
                                 uint32_t tokens, uint32_t max_pos, const gh_yarn* yarn, uint32_t layer);
-/* The way back of gh_kv_write_paged: what the positions lengths[r] - tokens .. lengths[r] - 1 of `layer` hold, as FP16
+/* The way back of gh_kv_write_paged: what the positions lengths[r] - tokens .. lengths[r] - 1 of `layer` hold, in FP16
  * [rows][tokens][kv_heads][128] in k and v (apart, and no part of kv's buffers). Vectors before a row's first position are
  * left as they are. With it a prefix in pages, in 4 bits too, becomes the contiguous cache that a prefill attends to. */
 int gh_kv_read_paged(gh_backend* b, gh_encoder* enc, const gh_buf* k, const gh_buf* v, const gh_kv_paged* kv,
@@ -259,7 +259,7 @@ int gh_kv_read_paged(gh_backend* b, gh_encoder* enc, const gh_buf* k, const gh_b
  * summed over the query heads of a kv head, is added to its score. In the products with V a weight is held to
  * 2^-38 of the row's largest and is at least that, unless its score is -inf: n positions add up to n·2^-38 of their
  * mean V, and an infinite V leaves an infinity or NaN whatever its score. A row whose scores are all -inf gives
- * NaN. In a q4 pool weights are held to 2^-11 of themselves and 2^-39 of the row's largest. max_len also sizes the call's scratch: with scores 4 bytes per query head and position of every row, in groups of
+ * NaN. In a q4 pool values are rounded to FP16 for these products, and keys are not. max_len also sizes the call's scratch: with scores 4 bytes per query head and position of every row, in groups of
  * rows that take at most 512 MiB. */
 int gh_attention_decode_paged(gh_backend* b, gh_encoder* enc, const gh_buf* out, const gh_buf* q,
                               const gh_kv_paged* kv, uint32_t q_heads, uint32_t max_len, uint32_t layer);

@@ -3,7 +3,7 @@ import numpy as np
 
 from graph_horizon_amd import GhKvPaged
 from graph_horizon_amd import _ffi as F
-from paged import D, Paged
+from paged import D, Paged, attend
 
 VECTOR = 80
 
@@ -33,14 +33,63 @@ def parts(b):
     return c, dm[..., 0::2], dm[..., 1::2]
 
 
-def unpack(b):
-    """The FP16 values that vectors of bytes stand for."""
+def values(b):
+    """What vectors of bytes stand for, in 64 bits."""
     c, d, m = parts(b)
-    return (m[..., None] + d[..., None] * c).astype(np.float16).reshape(*b.shape[:-1], D)
+    return (m[..., None] + d[..., None] * c).reshape(*b.shape[:-1], D)
+
+
+def unpack(b):
+    """The same in FP16, as a read-back gives it."""
+    return values(b).astype(np.float16)
+
+
+def attend4(q, kb, vb):
+    """paged.attend over vectors of bytes: (out, weights, error bounds of both). The bounds count, besides those of
+    paged.attend: keys are sums of d·c and m, of which each product and sum is rounded in FP32 by itself (a half step of
+    their sizes' sum for each of 32 dims, and eight more for the groups' sums); the query's sum over a group is held to 2^-22
+    and to 2^-16 (an FP16 subnormal times 2^9); half of its dims to 2^-21 (a subnormal times 2^4); a value is rounded to FP16."""
+    half = 2.0 ** -24
+    k, v = values(kb), values(vb)
+    out, w, bound, wb = attend(q, k, v)
+    q = np.abs(q.astype(np.float64))
+    c, d, m = parts(kb)
+    dc, m = (d[..., None] * c).reshape(k.shape), np.repeat(np.abs(m), 32, -1)
+    ds = (40 * half * (q @ (dc + m).T) + 2.0 ** -22 * (q @ m.T) + 2.0 ** -16 * m.sum(1) / 32 + 2.0 ** -21 * dc.sum(1)) / np.sqrt(D)
+    ds = ds.max(1, keepdims=True)
+    a = np.abs(v)
+    return out, w, bound + 4 * ds * (w @ a) + 2.0 ** -11 * (w @ a), wb + 4 * ds * w
+
+
+def check_attention4(p, layer, q, out, before=None, after=None):
+    """paged.check_attention over the pool's bytes."""
+    g = q.shape[1] // p.heads
+    for r, n in enumerate(p.lengths):
+        n = int(n)
+        if n == 0:
+            assert not out[r].view(np.uint16).any(), "a free row's output"
+        s = p.cells(r, n)
+        for h in range(p.heads):
+            hs = slice(h * g, h * g + g)
+            if n:
+                want, w, ob, wb = attend4(q[r, hs], p.kb[layer, s, h], p.vb[layer, s, h])
+                err = np.abs(out[r, hs].astype(np.float64) - want)
+                assert np.all(err <= ob), (r, h, float((err / ob).max()))
+            if before is not None:
+                old, new = before[layer, r, h], after[layer, r, h]
+                if n:
+                    total = old[:n].astype(np.float64) + w.sum(0)
+                    bound = wb.sum(0) + (g + 1) * 2.0 ** -24 * np.abs(total)
+                    err = np.abs(new[:n] - total)
+                    assert np.all(err <= bound), (r, h, float((err / bound).max()))
+                assert np.array_equal(new[n:].view(np.uint32), old[n:].view(np.uint32)), "scores past the row"
+    if before is not None:
+        others = [i for i in range(p.layers) if i != layer]
+        assert np.array_equal(before[others], after[others]), "other layers' scores"
 
 
 class Paged4(Paged):
-    """k, v are the FP16 values that the pool's bytes kb, vb stand for."""
+    """A pool of which kb, vb are the bytes, and k, v the FP16 values that a read-back gives."""
 
     def upload(self):
         if "k" not in self.bufs:

@@ -3,29 +3,14 @@ the read-back), against 64-bit definitions over the values that the pool's bytes
 import numpy as np
 import pytest
 
-import paged
-from graph_horizon_amd import GhError, GhSampleParams, Yarn
+from graph_horizon_amd import GhError, Yarn
 from graph_horizon_amd import _ffi as F
 from paged import D, Paged, keep, pages_of
-from paged4 import VECTOR, Paged4, pack, parts, unpack
+from paged4 import VECTOR, Paged4, check_attention4, pack, parts, unpack
 
 pytestmark = pytest.mark.gpu
 YARN = Yarn(128, 16384, 1e6, 16.0, 32.0, 1.0, 1.0, 0.1)
 HALF = 2.0 ** -24  # FP32's half step
-attend_fp16 = paged.attend
-
-
-def attend(q, k, v):
-    """paged.attend with weights in one FP16 part: off by half a step of it, and what is below 2^-24 / 2 of the
-    scaled weights (2^-40 of the largest) can vanish."""
-    out, w, bound, wb = attend_fp16(q, k, v)
-    v = np.abs(v.astype(np.float64))
-    return out, w, bound + 2.0 ** -11 * (w @ v) + 2.0 ** -39 * w.max(1, keepdims=True) * v.sum(0), wb
-
-
-@pytest.fixture(autouse=True)
-def bounds(monkeypatch):
-    monkeypatch.setattr(paged, "attend", attend)
 
 
 def run_attention(hip, p, q_heads, rng, layer=0, max_len=0, q=None):
@@ -59,7 +44,7 @@ def test_attention(hip, rng, name, page, heads, group, scored):
     p = Paged4(hip, rng, LENGTHS[name], page, heads, layers=2, scored=scored)
     before = None if not scored else p.read("score")
     q, out = run_attention(hip, p, heads * group, rng, layer=1)
-    paged.check_attention(p, 1, q, out, before, p.read("score") if scored else None)
+    check_attention4(p, 1, q, out, before, p.read("score") if scored else None)
     assert np.array_equal(p.read("k"), p.kb) and np.array_equal(p.read("v"), p.vb)
     for name in ("table", "lengths"):
         assert np.array_equal(p.read(name), getattr(p, name)), name
@@ -76,7 +61,18 @@ def test_attention_in_chunks(hip, rng, lengths, page, heads, width, scored):
     p = Paged4(hip, rng, lengths, page, heads, width=width, scored=scored)
     before = p.read("score") if scored else None
     q, out = run_attention(hip, p, 2 * heads, rng)
-    paged.check_attention(p, 0, q, out, before, p.read("score") if scored else None)
+    check_attention4(p, 0, q, out, before, p.read("score") if scored else None)
+    p.free()
+
+
+@pytest.mark.parametrize("heads,group", [(1, 4), (2, 3), (3, 2), (4, 1), (5, 2), (9, 1), (12, 4)])
+def test_attention_in_chunks_of_any_number_of_heads(hip, rng, heads, group):
+    """Teams of one to four waves, with and without waves over; a pool whose rows of all heads end off 128 bytes."""
+    lengths = [int(n) for n in rng.integers(0, 400, 30)] + [2000, 0, 33]
+    p = Paged4(hip, rng, lengths, 16, heads, width=8 * 1024 // 16, scored=heads % 2 == 1)
+    before = p.read("score") if p.score is not None else None
+    q, out = run_attention(hip, p, heads * group, rng)
+    check_attention4(p, 0, q, out, before, None if before is None else p.read("score"))
     p.free()
 
 
@@ -84,7 +80,7 @@ def test_attention_past_the_cache(hip, rng):
     """128 MiB of vectors, from which they are read with another cache policy."""
     p = Paged4(hip, rng, [60000, 45000, 17], 64, 8, width=1000)
     q, out = run_attention(hip, p, 32, rng)
-    paged.check_attention(p, 0, q, out)
+    check_attention4(p, 0, q, out)
     p.free()
 
 
@@ -94,7 +90,7 @@ def test_attention_launch_longer_than_rows(hip, rng, max_len, group):
     p = Paged4(hip, rng, [300, 0, 17], 16, 4, width=256, scored=True)
     before = p.read("score")
     q, out = run_attention(hip, p, 4 * group, rng, max_len=max_len)
-    paged.check_attention(p, 0, q, out, before, p.read("score"))
+    check_attention4(p, 0, q, out, before, p.read("score"))
     p.free()
 
 
@@ -104,7 +100,7 @@ def test_attention_row_groups(hip, rng):
     p = Paged4(hip, rng, lengths, 16, 1, scored=True)
     before = p.read("score")
     q, out = run_attention(hip, p, 2, rng)
-    paged.check_attention(p, 0, q, out, before, p.read("score"))
+    check_attention4(p, 0, q, out, before, p.read("score"))
     p.free()
 
 
@@ -127,7 +123,7 @@ def test_attention_shared_and_repeated_pages(hip, rng):
     p.table[2, :4] = p.table[2, [0, 1, 0, 1]]
     p.upload()
     q, out = run_attention(hip, p, 8, rng)
-    paged.check_attention(p, 0, q, out)
+    check_attention4(p, 0, q, out)
     p.free()
 
 
@@ -154,7 +150,7 @@ def test_attention_pool_past_4_gib(hip, rng, heads):
     h.table = tb
     qb, ob = hip.from_host(q), hip.alloc_buffer(q.nbytes)
     hip.attention_decode_paged(ob, qb, h, 4 * heads, 0, 0)
-    paged.check_attention(small, 0, q, hip.download(ob, np.float16, q.size).reshape(q.shape))
+    check_attention4(small, 0, q, hip.download(ob, np.float16, q.size).reshape(q.shape))
     # and what the read-back finds there
     n = 130 * 2 * heads * D
     kb, vb = hip.alloc_buffer(2 * n), hip.alloc_buffer(2 * n)
@@ -183,7 +179,7 @@ def test_attention_peaked_and_flat_weights(hip, rng):
     p.kb, p.vb = pack(k), pack(v)
     p.upload()
     q, out = run_attention(hip, p, 1, rng, q=q)
-    paged.check_attention(p, 0, q, out)
+    check_attention4(p, 0, q, out)
     assert 0.2 < out[1, 0, 1] < 0.7  # 30000 * 2^-26 * 1000
     p.free()
 
@@ -215,7 +211,7 @@ def test_attention_largest_values(hip, rng):
     p.upload()
     assert np.isfinite(unpack(p.vb)[0, at]).all()
     q, out = run_attention(hip, p, 4, rng)
-    paged.check_attention(p, 0, q, out)
+    check_attention4(p, 0, q, out)
     p.free()
 
 
@@ -243,7 +239,7 @@ def test_attention_reports_what_does_not_fit(hip, rng, what, rows):
     out = hip.download(ob, np.float16, q.size).reshape(q.shape)
     p.lengths[0] = 0
     out[0] = 0
-    paged.check_attention(p, 0, q, out)
+    check_attention4(p, 0, q, out)
     for b in (qb, ob):
         hip.free_buffer(b)
     p.free()
