@@ -86,7 +86,7 @@ int gh_sample_rows(gh_backend* b, gh_encoder* enc, const gh_buf* tokens, const g
         a.stride = stride;
         a.wide = logits->addr % 16 == 0 && stride % 4 == 0;
         a.scale = 1.0;
-        while (a.scale * 2 * vocab <= 0x1p62) a.scale *= 2;
+        for (a.shift = 0; a.shift < 51 && a.scale * 2 * vocab <= 0x1p62; ++a.shift) a.scale *= 2;
         uint32_t step = std::min<uint32_t>(rows, kSampleScratch / GH_SAMPLE_ROW_BYTES);
         char* ws = nullptr;
         int rc = GH_OK;

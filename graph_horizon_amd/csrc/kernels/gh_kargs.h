@@ -284,13 +284,13 @@ struct GhSampleArgs {
     uint64_t part;
     uint64_t bins;
     uint64_t list;     // u64 [rows][GH_SAMPLE_LIST]
-    double scale;      // of weights in fixed point: a power of two, vocab times which is at most 2^62
+    double scale;      // of weights in fixed point: 2^shift, at most 2^51, and vocab times it at most 2^62
     uint32_t vocab;
     uint32_t stride;
     uint32_t chunks;   // of a row, at most 64
     uint32_t per;      // logits of a chunk, a multiple of 4
     uint32_t wide;     // rows start on 16 bytes
-    uint32_t pad;
+    int32_t shift;
 };
 
 // ---- paged caches (kernels/paged.hip, kernels/paged4.hip) ----

@@ -1,5 +1,6 @@
 // Decode/prefill glue: RMSNorm, YaRN RoPE, SiLU·up, residual add, KV append, argmax.
 #include "gh_head.h"
+#include "gh_wave64.h"
 
 // rmsnorm_x (backend/cpu/kernels/elementwise/normalization.rs:12-40): one 256-thread
 // workgroup per row, Σx² in gh_rms_inverse_256's order (thread t: the 16-value items t, t + 256, ...),
@@ -289,35 +290,6 @@ __device__ __forceinline__ uint64_t topk_key(uint32_t bits, uint32_t idx) {
     return ((uint64_t)~ord << 32) | idx;
 }
 
-// The smaller (keep_min) or larger of x and lane ^ stride's x: DPP moves within 16 lanes (xor 4 as
-// xor 7 then xor 3), row swaps beyond, which leave the lane's own and its partner's value in the two
-// registers (through ds_bpermute: partial 13.5 us, final 13.9 at k = 40).
-template <int CTRL>
-__device__ __forceinline__ uint64_t topk_dpp(uint64_t x) {
-    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, 0xF, 0xF, false);
-    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(x >> 32), CTRL, 0xF, 0xF, false);
-    return ((uint64_t)hi << 32) | lo;
-}
-__device__ __forceinline__ uint64_t topk_exchange(uint64_t x, uint32_t stride, bool keep_min) {
-    uint64_t y;
-    if (stride >= 16) {
-        const uint32_t l = (uint32_t)x, h = (uint32_t)(x >> 32);
-        const auto a = stride == 16 ? __builtin_amdgcn_permlane16_swap(l, l, false, false)
-                                    : __builtin_amdgcn_permlane32_swap(l, l, false, false);
-        const auto b = stride == 16 ? __builtin_amdgcn_permlane16_swap(h, h, false, false)
-                                    : __builtin_amdgcn_permlane32_swap(h, h, false, false);
-        x = ((uint64_t)b[0] << 32) | a[0];
-        y = ((uint64_t)b[1] << 32) | a[1];
-    } else if (stride == 8) {
-        y = topk_dpp<0x128>(x);  // row_ror:8
-    } else if (stride == 4) {
-        y = topk_dpp<0x1B>(topk_dpp<0x141>(x));  // row_half_mirror, quad_perm [3,2,1,0]
-    } else {
-        y = stride == 2 ? topk_dpp<0x4E>(x) : topk_dpp<0xB1>(x);  // quad_perm [2,3,0,1], [1,0,3,2]
-    }
-    return ((x > y) == keep_min) ? y : x;
-}
-
 template <int V>
 struct TopkList {
     uint64_t r[V];
@@ -336,7 +308,7 @@ __device__ __forceinline__ void topk_merge(TopkList<V>& l, bool up) {
 #pragma unroll
     for (uint32_t s = 32; s > 0; s >>= 1)
 #pragma unroll
-        for (int v = 0; v < V; ++v) l.r[v] = topk_exchange(l.r[v], s, ((lane & s) == 0) == up);
+        for (int v = 0; v < V; ++v) l.r[v] = gh_exchange64(l.r[v], s, ((lane & s) == 0) == up);
 }
 
 // The smallest 64 V of an ascending and a descending list, sorted.
@@ -361,7 +333,7 @@ __device__ __forceinline__ TopkList<V> topk_of_512(uint64_t (&x)[8]) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const bool up = ((lane & size) == 0) == ((i & 1) == 0);
-                x[i] = topk_exchange(x[i], s, ((lane & s) == 0) == up);
+                x[i] = gh_exchange64(x[i], s, ((lane & s) == 0) == up);
             }
     TopkList<V> l[4];
 #pragma unroll

@@ -4,7 +4,7 @@
 // Tokens rank by (logit descending by f32 total order, index ascending), those with a finite logit. Token i has weight
 // w = exp((l - M) / T), M the row's largest logit. Every filter keeps a prefix of the ranking, and the draw
 // is the first rank whose running sum of weights passes u times the kept sum, so all a row needs are four searches in the
-// running counts and sums. Sums are of whole numbers, w in fixed point: the same in any order, and off by 2^-45 at a
+// running counts and sums. Sums are of whole numbers, w in fixed point: the same in any order, and off by 2^-46 at a
 // vocabulary of 2^17, so that what lies next to a border of the kept or drawn range falls where 64 bits put it.
 //
 // Four launches; a row's logits are read three times, from memory once:
@@ -13,18 +13,23 @@
 //                     that a bin holds at most 3 % of any smooth distribution whatever its spread;
 //   gh_sample_collect the tokens of the bins in which a search can end: the running sums up to the bins are known, and
 //                     bound the top-k sum, then the kept sum, then the draw's target;
-//   gh_sample_pick    sorts these tokens and searches them. More than fit are searched in the row itself.
+//   gh_sample_pick    searches these tokens, or, where they are more than the list takes, the row itself.
 // What the device cannot trust is only the settings: any bits give a token of the row.
-#include "gh_common.h"
+#include "gh_wave64.h"
 
 namespace {
 constexpr uint32_t kBins = GH_SAMPLE_BINS, kList = GH_SAMPLE_LIST;
 constexpr uint32_t kNone = 0xFFFFFFFFu;
+constexpr uint32_t kLoads = 8;  // 16-byte loads that a thread has in flight
+constexpr uint32_t kBlock = 256 * 4 * kLoads;
 
 // f32 total order as unsigned order, and back
 __device__ __forceinline__ uint32_t order_key(uint32_t bits) { return bits ^ ((uint32_t)((int32_t)bits >> 31) | 0x80000000u); }
 __device__ __forceinline__ float order_value(uint32_t key) { return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xFFFFFFFFu)); }
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
+// Ascending in rank order.
+__device__ __forceinline__ uint64_t rank_key(float l, uint32_t i) { return (uint64_t)~order_key(__float_as_uint(l)) << 32 | i; }
+__device__ __forceinline__ float value_of(uint64_t key) { return order_value(~(uint32_t)(key >> 32)); }
 
 // The bin of distance d >= 0.
 __device__ __forceinline__ uint32_t bin_of(float d) {
@@ -38,66 +43,91 @@ struct Row {
     uint32_t top_k;
     double u, inv;      // the draw's number, 1 / T
     float top;          // M
-    uint32_t best;      // index of the largest of all logits, infinite ones too (what a greedy row takes)
+    uint32_t best;      // a greedy row's token: the index of the largest of all logits, infinite ones too
     bool greedy;        // T <= 0, or no finite logit
 };
-__device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const uint64_t y = __shfl_xor((unsigned long long)v, o, 64);
-        v = v > y ? v : y;
-    }
-    return v;
-}
 __device__ __forceinline__ Row row_of(const GhSampleArgs& a, uint32_t row) {
     const uint32_t lane = threadIdx.x & 63u;
     const uint4 p = gh_gp<uint4>(a.params)[row];
-    const uint64_t part = a.part + (uint64_t)row * 64 * 16;
-    uint64_t any = 0, fin = 0;
-    if (lane < a.chunks) {
-        const ulonglong2 x = gh_gp<ulonglong2>(part)[lane];
-        any = x.x;
-        fin = x.y;
-    }
-    any = wave_max64(any);
-    fin = wave_max64(fin);
+    const float u = gh_gp<float>(a.uniform)[row];
+    ulonglong2 x = make_ulonglong2(0, 0);
+    if (lane < a.chunks) x = gh_gp<ulonglong2>(a.part + (uint64_t)row * 64 * 16)[lane];
+    const uint32_t fin = (uint32_t)gh_max64(x.y);
     Row r;
     r.temperature = __uint_as_float(p.x);
     r.top_p = __uint_as_float(p.y);
     r.top_k = p.z;
     r.min_p = __uint_as_float(p.w);
-    const float u = gh_gp<float>(a.uniform)[row];
     r.u = u > 0.0f ? fminf(u, 0.99999994f) : 0.0f;
     r.inv = 1.0 / (double)r.temperature;
-    r.top = order_value((uint32_t)fin);
-    r.best = any ? ~(uint32_t)any : 0u;
+    r.top = order_value(fin);
     r.greedy = !(r.temperature > 0.0f) || fin == 0;
+    r.best = 0;
+    if (r.greedy) {
+        const uint64_t any = gh_max64(x.x);
+        r.best = any ? ~(uint32_t)any : 0u;
+    }
     return r;
 }
-__device__ __forceinline__ double weight(const Row& r, float l) { return exp(((double)l - (double)r.top) * r.inv); }
-__device__ __forceinline__ uint64_t fixed(const GhSampleArgs& a, double w) { return (uint64_t)__double2ull_rn(w * a.scale); }
 
-// Calls body(logit, index) for the chunk's tokens, in no order.
-template <class F>
-__device__ __forceinline__ void each_logit(const GhSampleArgs& a, uint32_t row, uint32_t first, uint32_t end, uint32_t threads, F body) {
+// exp(x) of x <= 0 as 2^(n / 64) e^r, n the nearest whole number to 64 x / ln 2 and |r| <= ln 2 / 128: powers of two by
+// 64ths from a table (Tang's method), e^r by its series to r^5 / 5!, whose rest is below 2^-57.
+__device__ __forceinline__ void fill_exp(double* table) {
+    if (threadIdx.x < 64) table[threadIdx.x] = exp2((double)threadIdx.x * 0x1p-6);
+}
+__device__ __forceinline__ double exp_scaled(const double* table, double x, int up) {
+    x = x > -200.0 ? x : -200.0;  // (and what is not a number: none here)
+    const double shift = 0x1.8p52;
+    const double z = __builtin_fma(x, 0x1.71547652b82fep+6, shift), n = z - shift;
+    const int whole = (int)(uint32_t)__builtin_bit_cast(uint64_t, z);
+    // ln 2 / 64 in two parts, the first short enough for exact products with n
+    double r = __builtin_fma(n, -0x1.62e42fefap-7, x);
+    r = __builtin_fma(n, -0x1.cf79abc9e3b3ap-46, r);
+    double p = __builtin_fma(r, 1.0 / 120, 1.0 / 24);
+    p = __builtin_fma(r, p, 1.0 / 6);
+    p = __builtin_fma(r, p, 0.5);
+    p = __builtin_fma(r * r, p, r);
+    const double t = table[whole & 63];
+    return __builtin_ldexp(__builtin_fma(t, p, t), (whole >> 6) + up);
+}
+__device__ __forceinline__ double weight(const Row& r, const double* table, float l) {
+    return exp_scaled(table, ((double)l - (double)r.top) * r.inv, 0);
+}
+// The weight in fixed point, nearest: at most 2^51, so that 2^52 more leaves it in the mantissa.
+__device__ __forceinline__ uint64_t fixed(const GhSampleArgs& a, const Row& r, const double* table, float l) {
+    const double w = exp_scaled(table, ((double)l - (double)r.top) * r.inv, a.shift);
+    return __builtin_bit_cast(uint64_t, w + 0x1p52) & 0xFFFFFFFFFFFFFull;
+}
+
+// LOADS times four logits of a block of a row, the k-th four of a thread 4 THREADS k further on; NaN past `end`.
+template <uint32_t THREADS, uint32_t LOADS>
+__device__ __forceinline__ void load_block(const GhSampleArgs& a, uint32_t row, uint32_t block, uint32_t end, float4 (&v)[LOADS]) {
     const GH_GLOBAL float* l = gh_gp<float>(a.logits) + (uint64_t)row * a.stride;
-    for (uint32_t i = first + 4 * threadIdx.x; i < end; i += 8 * threads) {
-        float v[2][4];
 #pragma unroll
-        for (uint32_t k = 0; k < 2; ++k) {
-            const uint32_t at = i + 4 * threads * k;
-            if (a.wide && at + 4 <= end) {
-                const float4 x = *(const GH_GLOBAL float4*)(l + at);
-                v[k][0] = x.x, v[k][1] = x.y, v[k][2] = x.z, v[k][3] = x.w;
-            } else {
-#pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) v[k][j] = at + j < end ? l[at + j] : __uint_as_float(0x7FC00000u);
-            }
+    for (uint32_t k = 0; k < LOADS; ++k) {
+        const uint32_t at = block + 4 * (threadIdx.x + THREADS * k);
+        const float none = __uint_as_float(0x7FC00000u);
+        v[k] = make_float4(none, none, none, none);
+        if (a.wide && at + 4 <= end) {
+            v[k] = *(const GH_GLOBAL float4*)(l + at);
+        } else if (at < end) {
+            v[k].x = l[at];
+            if (at + 1 < end) v[k].y = l[at + 1];
+            if (at + 2 < end) v[k].z = l[at + 2];
+            if (at + 3 < end) v[k].w = l[at + 3];
         }
+    }
+}
+// body(logit, index) for each of a block's tokens.
+template <uint32_t THREADS, uint32_t LOADS, class F>
+__device__ __forceinline__ void each_of(const float4 (&v)[LOADS], uint32_t block, F body) {
 #pragma unroll
-        for (uint32_t k = 0; k < 2; ++k)
-#pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) body(v[k][j], i + 4 * threads * k + j);
+    for (uint32_t k = 0; k < LOADS; ++k) {
+        const uint32_t at = block + 4 * (threadIdx.x + THREADS * k);
+        body(v[k].x, at);
+        body(v[k].y, at + 1);
+        body(v[k].z, at + 2);
+        body(v[k].w, at + 3);
     }
 }
 }  // namespace
@@ -108,16 +138,28 @@ GH_KERNEL __launch_bounds__(256) void gh_sample_max(GhSampleArgs a) {
     const uint32_t tid = threadIdx.x, row = blockIdx.y, first = blockIdx.x * a.per, end = min(a.vocab, first + a.per);
     GH_GLOBAL uint32_t* bins = gh_gpw<uint32_t>(a.bins + (uint64_t)row * GH_SAMPLE_BIN_BYTES);
     for (uint32_t i = blockIdx.x * 256 + tid; i < GH_SAMPLE_BIN_BYTES / 4; i += gridDim.x * 256) bins[i] = 0u;
-    uint64_t any = 0;
     uint32_t fin = 0;
-    each_logit(a, row, first, end, 256, [&](float l, uint32_t i) __attribute__((always_inline)) {
-        if (finite(l)) fin = max(fin, order_key(__float_as_uint(l)));
-        // -0 and 0 are equal here; a NaN is never the largest
-        const uint64_t key = (uint64_t)order_key(__float_as_uint(l + 0.0f)) << 32 | (uint32_t)~i;
-        if (l > -__builtin_inff()) any = any > key ? any : key;
-    });
-    any = wave_max64(any);
-    const uint64_t top = wave_max64(fin);
+    float4 v[kLoads];
+    for (uint32_t block = first; block < end; block += kBlock) {
+        load_block<256>(a, row, block, end, v);
+        each_of<256>(v, block, [&](float l, uint32_t) __attribute__((always_inline)) {
+            if (finite(l)) fin = max(fin, order_key(__float_as_uint(l)));
+        });
+    }
+    // the index of the largest, infinite ones too, for rows that are or turn out greedy
+    uint64_t any = 0;
+    if (!(gh_gp<float4>(a.params)[row].x > 0.0f) || __syncthreads_or(fin) == 0) {
+        for (uint32_t block = first; block < end; block += kBlock) {
+            load_block<256>(a, row, block, end, v);
+            each_of<256>(v, block, [&](float l, uint32_t i) __attribute__((always_inline)) {
+                // -0 and 0 are equal here; a NaN is never the largest
+                const uint64_t key = (uint64_t)order_key(__float_as_uint(l + 0.0f)) << 32 | (uint32_t)~i;
+                if (l > -__builtin_inff()) any = any > key ? any : key;
+            });
+        }
+    }
+    any = gh_max64(any);
+    const uint64_t top = gh_max64(fin);
     if ((tid & 63u) == 0) {
         red[tid >> 6][0] = any;
         red[tid >> 6][1] = top;
@@ -137,26 +179,35 @@ GH_KERNEL __launch_bounds__(256) void gh_sample_max(GhSampleArgs a) {
 GH_KERNEL __launch_bounds__(256) void gh_sample_bins(GhSampleArgs a) {
     __shared__ unsigned long long sum[kBins];
     __shared__ uint32_t count[kBins];
+    __shared__ double table[64];
     const uint32_t tid = threadIdx.x, row = blockIdx.y, first = blockIdx.x * a.per, end = min(a.vocab, first + a.per);
+    float4 v[kLoads];
+    load_block<256>(a, row, first, end, v);
     for (uint32_t i = tid; i < kBins; i += 256) {
         sum[i] = 0;
         count[i] = 0;
     }
+    fill_exp(table);
     const Row r = row_of(a, row);
     if (r.greedy) return;
     __syncthreads();
-    each_logit(a, row, first, end, 256, [&](float l, uint32_t) __attribute__((always_inline)) {
-        if (!finite(l)) return;
-        const uint32_t b = bin_of(r.top - l);
-        atomicAdd(&count[b], 1u);
-        const uint64_t w = fixed(a, weight(r, l));
-        if (w) atomicAdd(&sum[b], (unsigned long long)w);
-    });
+    for (uint32_t block = first;;) {
+        each_of<256>(v, block, [&](float l, uint32_t) __attribute__((always_inline)) {
+            if (!finite(l)) return;
+            const uint32_t b = bin_of(r.top - l);
+            atomicAdd(&count[b], 1u);
+            const uint64_t w = fixed(a, r, table, l);
+            if (w) atomicAdd(&sum[b], (unsigned long long)w);
+        });
+        block += kBlock;
+        if (block >= end) break;
+        load_block<256>(a, row, block, end, v);
+    }
     __syncthreads();
     const uint64_t bins = a.bins + (uint64_t)row * GH_SAMPLE_BIN_BYTES;
     for (uint32_t i = tid; i < kBins; i += 256) {
         if (!count[i]) continue;
-        atomicAdd((unsigned long long*)bins + i, sum[i]);
+        if (sum[i]) atomicAdd((unsigned long long*)bins + i, sum[i]);
         atomicAdd((uint32_t*)(bins + kBins * 8) + i, count[i]);
     }
 }
@@ -168,7 +219,6 @@ struct Plan {
     uint32_t keep;          // min(top_k, tokens)
     uint32_t k;             // bin of the last of them
     bool partly;            // not all of that bin's
-    uint64_t all;           // sum over all tokens
     uint32_t p0, p1;        // top-p's, first and last (kNone: off)
     uint32_t m0, m1;        // min-p's
     uint32_t d0, d1;        // the draw's
@@ -182,309 +232,404 @@ struct PlanLds {
     uint64_t sum[kBins];
     uint32_t count[kBins];
     uint64_t wave_sum[16];
-    uint32_t wave_count[16];
-    uint32_t found[5], listed;
+    uint32_t wave_count[16], wave_listed[16];
+    uint32_t found[5];
 };
 __device__ __forceinline__ uint64_t before(const PlanLds& s, uint32_t b) { return b ? s.sum[b - 1] : 0; }
 __device__ __forceinline__ uint32_t count_before(const PlanLds& s, uint32_t b) { return b ? s.count[b - 1] : 0; }
 
-__device__ __forceinline__ uint64_t wave_scan64(uint64_t v) {
-    const uint32_t lane = threadIdx.x & 63u;
-#pragma unroll
-    for (uint32_t o = 1; o < 64; o <<= 1) {
-        const uint64_t y = __shfl_up((unsigned long long)v, o, 64);
-        if (lane >= o) v += y;
-    }
-    return v;
-}
-
-// The first bin whose running value satisfies `is`, at most `last`; THREADS threads, each kBins / THREADS bins.
-template <uint32_t THREADS, class F>
-__device__ __forceinline__ void first_bin(uint32_t* found, F is) {
-    constexpr uint32_t kEach = kBins / THREADS;
-#pragma unroll
-    for (uint32_t j = 0; j < kEach; ++j) {
-        const uint32_t b = threadIdx.x * kEach + j;
-        if (is(b)) {
-            atomicMin(found, b);
-            break;
-        }
-    }
-}
-
 // All threads get the same plan. u64 sums are compared as doubles, as the searches compare them.
 template <uint32_t THREADS>
 __device__ __forceinline__ Plan plan_of(const GhSampleArgs& a, const Row& r, uint32_t row, PlanLds& s) {
-    constexpr uint32_t kEach = kBins / THREADS;
+    constexpr uint32_t kEach = kBins / THREADS, kWaves = THREADS / 64;  // bins of a thread, in a row
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
     const uint64_t bins = a.bins + (uint64_t)row * GH_SAMPLE_BIN_BYTES;
-    uint64_t w[kEach], ws = 0;
-    uint32_t c[kEach], cs = 0;
+    uint64_t w[kEach];
+    uint32_t c[kEach];
 #pragma unroll
     for (uint32_t j = 0; j < kEach; ++j) {
         w[j] = gh_gp<uint64_t>(bins)[tid * kEach + j];
         c[j] = gh_gp<uint32_t>(bins + kBins * 8)[tid * kEach + j];
-        ws += w[j];
-        cs += c[j];
     }
-    const uint64_t wu = wave_scan64(ws);
-    const uint32_t cu = (uint32_t)wave_scan64(cs);
+    uint32_t own[kEach];  // the bins' counts
+#pragma unroll
+    for (uint32_t j = 0; j < kEach; ++j) own[j] = c[j];
+#pragma unroll
+    for (uint32_t j = 1; j < kEach; ++j) {
+        w[j] += w[j - 1];
+        c[j] += c[j - 1];
+    }
+    const uint64_t wu = gh_scan64(w[kEach - 1]), cu = gh_scan64(c[kEach - 1]);
     if (lane == 63) {
         s.wave_sum[wave] = wu;
-        s.wave_count[wave] = cu;
+        s.wave_count[wave] = (uint32_t)cu;
     }
     if (tid < 5) s.found[tid] = kBins - 1;
-    if (tid == 0) s.listed = 0;
     __syncthreads();
-    uint64_t wat = wu - ws;
-    uint32_t cat = cu - cs;
-    for (uint32_t i = 0; i < wave; ++i) {
-        wat += s.wave_sum[i];
-        cat += s.wave_count[i];
+    uint64_t w0 = wu - w[kEach - 1];          // before the thread's bins
+    uint32_t c0 = (uint32_t)cu - c[kEach - 1];
+    Plan p;
+    p.tokens = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kWaves; ++i) {
+        w0 += i < wave ? s.wave_sum[i] : 0;
+        c0 += i < wave ? s.wave_count[i] : 0;
+        p.tokens += s.wave_count[i];
     }
 #pragma unroll
     for (uint32_t j = 0; j < kEach; ++j) {
-        s.sum[tid * kEach + j] = wat += w[j];
-        s.count[tid * kEach + j] = cat += c[j];
+        s.sum[tid * kEach + j] = w[j] += w0;
+        s.count[tid * kEach + j] = c[j] += c0;
     }
-    __syncthreads();
-    Plan p;
-    p.tokens = s.count[kBins - 1];
-    p.all = s.sum[kBins - 1];
+    // The first bin up to which the running values satisfy `is`, which stays true once it is: one thread has it.
+    auto first_bin = [&](uint32_t slot, auto is) __attribute__((always_inline)) {
+        if (!is(c[kEach - 1], w[kEach - 1]) || (tid && is(c0, w0))) return;
+        uint32_t j = 0;
+#pragma unroll
+        for (uint32_t i = 0; i + 1 < kEach; ++i) j += j == i && !is(c[i], w[i]);
+        s.found[slot] = tid * kEach + j;
+    };
     p.keep = r.top_k && r.top_k < p.tokens ? r.top_k : p.tokens;
-    first_bin<THREADS>(&s.found[0], [&](uint32_t b) { return s.count[b] >= p.keep; });
+    first_bin(0, [&](uint32_t c, uint64_t) { return c >= p.keep; });
     __syncthreads();
     p.k = s.found[0];
     p.partly = s.count[p.k] > p.keep;
     // the sum of the first top_k lies between lo and hi
-    uint64_t lo = p.partly ? before(s, p.k) : s.sum[p.k], hi = s.sum[p.k];
-    uint32_t c0 = p.k, c1 = p.k;  // the last kept token's bins
+    double lo = (double)(p.partly ? before(s, p.k) : s.sum[p.k]), hi = (double)s.sum[p.k];
+    uint32_t l0 = p.k, l1 = p.k;  // the last kept token's bins
     p.p0 = p.p1 = p.m0 = p.m1 = kNone;
-    const bool nucleus = r.top_p < 1.0f;
-    if (nucleus) {
-        first_bin<THREADS>(&s.found[1], [&](uint32_t b) { return (double)s.sum[b] >= r.top_p * (double)lo; });
-        first_bin<THREADS>(&s.found[2], [&](uint32_t b) { return (double)s.sum[b] >= r.top_p * (double)hi; });
-    }
-    __syncthreads();
-    if (nucleus) {
-        c0 = p.p0 = min(s.found[1], p.k);
-        c1 = p.p1 = min(s.found[2], p.k);
+    if (r.top_p < 1.0f) {
+        const double want0 = r.top_p * lo, want1 = r.top_p * hi;
+        first_bin(1, [&](uint32_t, uint64_t w) { return (double)w >= want0; });
+        first_bin(2, [&](uint32_t, uint64_t w) { return (double)w >= want1; });
+        __syncthreads();
+        l0 = p.p0 = min(s.found[1], p.k);
+        l1 = p.p1 = min(s.found[2], p.k);
     }
     if (r.min_p > 0.0f) {
         // w >= min_p up to a distance of -T ln min_p; d is rounded to FP32
         const double d = -log((double)r.min_p) * (double)r.temperature;
         p.m0 = d > 0.0 ? bin_of((float)(d * (1.0 - 1e-6))) : 0u;
         p.m1 = d > 0.0 ? bin_of((float)(d * (1.0 + 1e-6))) : 0u;
-        c0 = min(c0, p.m0);
-        c1 = min(c1, p.m1);
+        l0 = min(l0, p.m0);
+        l1 = min(l1, p.m1);
     }
     // the kept sum lies between lo and hi
-    if (c0 != p.k || p.partly || nucleus || r.min_p > 0.0f) lo = before(s, c0);
-    hi = s.sum[c1];
-    first_bin<THREADS>(&s.found[3], [&](uint32_t b) { return (double)s.sum[b] > r.u * (double)lo; });
-    first_bin<THREADS>(&s.found[4], [&](uint32_t b) { return (double)s.sum[b] > r.u * (double)hi; });
+    if (p.partly || p.p0 != kNone || p.m0 != kNone) lo = (double)before(s, l0);
+    hi = (double)s.sum[l1];
+    const double want0 = r.u * lo, want1 = r.u * hi;
+    first_bin(3, [&](uint32_t, uint64_t w) { return (double)w > want0; });
+    first_bin(4, [&](uint32_t, uint64_t w) { return (double)w > want1; });
     __syncthreads();
-    p.d0 = min(s.found[3], c1);
-    p.d1 = min(s.found[4], c1);
+    p.d0 = min(s.found[3], l1);
+    p.d1 = min(s.found[4], l1);
     uint32_t listed = 0;
 #pragma unroll
-    for (uint32_t j = 0; j < kEach; ++j) listed += p.has(tid * kEach + j) ? c[j] : 0u;
-    if (listed) atomicAdd(&s.listed, listed);
+    for (uint32_t j = 0; j < kEach; ++j) listed += p.has(tid * kEach + j) ? own[j] : 0u;
+    listed = (uint32_t)gh_scan64(listed);
+    if (lane == 63) s.wave_listed[wave] = listed;
     __syncthreads();
-    p.listed = s.listed;
+    p.listed = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kWaves; ++i) p.listed += s.wave_listed[i];
     return p;
 }
 }  // namespace
 
-// Grid (chunks, rows), 256 threads.
+// Grid (chunks, rows), 256 threads. A block's tokens are counted first, so that it asks for its places in the list once.
 GH_KERNEL __launch_bounds__(256) void gh_sample_collect(GhSampleArgs a) {
     __shared__ PlanLds s;
-    __shared__ uint32_t need[kBins / 32];
-    const uint32_t tid = threadIdx.x, row = blockIdx.y, first = blockIdx.x * a.per, end = min(a.vocab, first + a.per);
+    __shared__ uint32_t need[kBins / 32], places[5];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, row = blockIdx.y, first = blockIdx.x * a.per, end = min(a.vocab, first + a.per);
+    float4 v[kLoads];
+    load_block<256>(a, row, first, end, v);
     const Row r = row_of(a, row);
     if (r.greedy) return;
     const Plan p = plan_of<256>(a, r, row, s);
     if (p.listed > kList) return;
-    if (tid < kBins / 32) {
-        uint32_t bits = 0;
-        for (uint32_t j = 0; j < 32; ++j) bits |= (uint32_t)p.has(32 * tid + j) << j;
-        need[tid] = bits;
+#pragma unroll
+    for (uint32_t j = 0; j < kBins / 256; ++j) {
+        const uint64_t has = __ballot(p.has(256 * j + tid));
+        if (lane < 2) need[8 * j + 2 * wave + lane] = (uint32_t)(has >> (32 * lane));
     }
     __syncthreads();
     const uint64_t list = a.list + (uint64_t)row * kList * 8;
     uint32_t* length = (uint32_t*)(a.bins + (uint64_t)row * GH_SAMPLE_BIN_BYTES + kBins * 12);
-    each_logit(a, row, first, end, 256, [&](float l, uint32_t i) __attribute__((always_inline)) {
-        if (!finite(l)) return;
-        const uint32_t b = bin_of(r.top - l);
-        if (!(need[b >> 5] >> (b & 31u) & 1u)) return;
-        const uint32_t at = atomicAdd(length, 1u);
-        // ascending in rank order
-        if (at < kList) gh_gpw<uint64_t>(list)[at] = (uint64_t)~order_key(__float_as_uint(l)) << 32 | i;
-    });
-}
-
-namespace {
-constexpr uint32_t kPick = 1024;  // threads
-struct PickLds {
-    uint64_t key[kList];  // (~order of the logit) << 32 | index, sorted
-    uint64_t upto[kList]; // running sums
-    uint64_t skip_sum[kBins];   // of a bin: what is before it and not listed
-    uint32_t skip_count[kBins];
-    uint32_t found[8];
-    uint64_t value[8];
-};
-__device__ __forceinline__ float value_of(uint64_t key) { return order_value(~(uint32_t)(key >> 32)); }
-
-// key[0 .. n) sorted, n a power of two.
-__device__ __forceinline__ void sort_keys(uint64_t* key, uint32_t n) {
-    for (uint32_t size = 2; size <= n; size <<= 1)
-        for (uint32_t stride = size >> 1; stride > 0; stride >>= 1) {
-            for (uint32_t t = threadIdx.x; t < n / 2; t += kPick) {
-                const uint32_t i = 2 * t - (t & (stride - 1));
-                const uint64_t x = key[i], y = key[i + stride];
-                if ((x > y) == ((i & size) == 0)) {
-                    key[i] = y;
-                    key[i + stride] = x;
-                }
-            }
+    for (uint32_t block = first;;) {
+        uint32_t mine = 0, bit = 1;  // which of the thread's 32 are wanted
+        each_of<256>(v, block, [&](float l, uint32_t) __attribute__((always_inline)) {
+            const uint32_t b = bin_of(r.top - l);
+            if (finite(l) && (need[b >> 5] >> (b & 31u) & 1u)) mine |= bit;
+            bit <<= 1;
+        });
+        const uint32_t n = __popc(mine), upto = (uint32_t)gh_scan64(n);
+        if (lane == 63) places[wave] = upto;
+        __syncthreads();
+        const uint32_t all = places[0] + places[1] + places[2] + places[3];
+        if (all) {  // of the whole workgroup
+            if (tid == 0) places[4] = atomicAdd(length, all);
             __syncthreads();
+            uint32_t at = places[4] + upto - n;
+            for (uint32_t w = 0; w < wave; ++w) at += places[w];
+            bit = 1;
+            each_of<256>(v, block, [&](float l, uint32_t i) __attribute__((always_inline)) {
+                if (mine & bit) {
+                    if (at < kList) gh_gpw<uint64_t>(list)[at] = rank_key(l, i);
+                    ++at;
+                }
+                bit <<= 1;
+            });
         }
+        block += kBlock;
+        if (block >= end) break;
+        load_block<256>(a, row, block, end, v);
+        __syncthreads();
+    }
 }
-}  // namespace
 
 namespace {
-// Equal logits, and what ranks before them.
-struct Ties {
-    uint32_t key, count, count_before;
-    uint64_t w, before;
-    // how many of them it takes until `is` holds for the sum
+constexpr uint32_t kPick = 1024;  // threads, a bin each
+// A token found by its running values: its key, and the count and sum up to and with it.
+struct Hit {
+    uint64_t key, sum;
+    uint32_t count;
+};
+struct PickLds {
+    uint64_t list[kList];
+    uint64_t few[64];       // the tokens among which a search ends
+    uint64_t sum[kBins];    // of a range of keys, in equal parts
+    uint32_t count[kBins];
+    uint64_t lo[16], hi[16], wave_sum[16];
+    uint32_t wave_count[16];
+    uint32_t found, fill;
+    Hit hit;
+};
+
+// The tokens of the list, or of the row, by key.
+struct Listed {
+    const uint64_t* list;
+    uint32_t n;
     template <class F>
-    __device__ __forceinline__ uint32_t until(F is) const {
-        uint32_t lo = 1, hi = max(count, 1u);
-        while (lo < hi) {
-            const uint32_t mid = (lo + hi) >> 1;
-            if (is(before + mid * w)) hi = mid;
-            else lo = mid + 1;
-        }
-        return lo;
+    __device__ __forceinline__ void each(F body) const {
+        for (uint32_t i = threadIdx.x; i < n; i += kPick) body(list[i]);
     }
 };
-// The first equal logits in rank order up to which the number and the sum of tokens satisfy `is`: eight bits of the logits'
-// order at a time, over the whole row.
-template <class F>
-__device__ __forceinline__ Ties descend(const GhSampleArgs& a, const Row& r, uint32_t row, PlanLds& s, F is) {
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
-    Ties t{0, 0, 0, 0, 0};
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        __syncthreads();
-        if (tid < 256) {
-            s.sum[tid] = 0;
-            s.count[tid] = 0;
+struct Whole {
+    const GhSampleArgs& a;
+    uint32_t row;
+    template <class F>
+    __device__ __forceinline__ void each(F body) const {
+        for (uint32_t block = 0; block < a.vocab; block += 8 * kPick) {
+            float4 v[2];
+            load_block<kPick>(a, row, block, a.vocab, v);
+            each_of<kPick>(v, block, [&](float l, uint32_t i) __attribute__((always_inline)) {
+                if (finite(l)) body(rank_key(l, i));
+            });
         }
-        if (tid == 0) s.found[0] = 255;
+    }
+};
+
+// The first token in rank order up to which count and sum satisfy `is`, which some token's do and stays true once it is. Its bin
+// by the running values of the bins; then, while a range holds more than 64 tokens, the 1024th part of the range of their keys
+// in which it is; then among these, sorted by one wave.
+template <class S, class F>
+__device__ __forceinline__ Hit search(const GhSampleArgs& a, const Row& r, const double* table, const PlanLds& s, PickLds& q, const S& source, F is) {
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+    __syncthreads();
+    if (tid == 0) q.found = kBins - 1;
+    __syncthreads();
+    if (is(s.count[tid], s.sum[tid]) && (tid == 0 || !is(s.count[tid - 1], s.sum[tid - 1]))) q.found = tid;
+    __syncthreads();
+    const uint32_t bin = q.found;
+    uint64_t sum = before(s, bin), lo = 0, hi = ~0ull;
+    uint32_t count = count_before(s, bin), n = s.count[bin] - count;
+    auto inside = [&](uint64_t key) __attribute__((always_inline)) { return key >= lo && key <= hi && bin_of(r.top - value_of(key)) == bin; };
+    while (n > 64) {
+        uint64_t least = ~0ull, most = 0;
+        source.each([&](uint64_t key) __attribute__((always_inline)) {
+            if (!inside(key)) return;
+            least = min(least, key);
+            most = max(most, key);
+        });
+        least = ~gh_max64(~least);
+        most = gh_max64(most);
         __syncthreads();
-        each_logit(a, row, 0, a.vocab, kPick, [&](float l, uint32_t) __attribute__((always_inline)) {
-            const uint32_t key = ~order_key(__float_as_uint(l));
-            if (!finite(l) || (shift < 24 && key >> (shift + 8) != t.key)) return;
-            atomicAdd(&s.count[key >> shift & 255u], 1u);
-            atomicAdd((unsigned long long*)&s.sum[key >> shift & 255u], (unsigned long long)fixed(a, weight(r, l)));
+        if (lane == 0) {
+            q.lo[wave] = least;
+            q.hi[wave] = most;
+        }
+        q.sum[tid] = 0;
+        q.count[tid] = 0;
+        if (tid == 0) q.found = kBins - 1;
+        __syncthreads();
+        for (uint32_t i = 0; i < 16; ++i) {
+            least = min(least, q.lo[i]);
+            most = max(most, q.hi[i]);
+        }
+        lo = least;
+        hi = most;
+        const uint32_t bits = 64 - __clzll((long long)(hi - lo)), shift = bits > 10 ? bits - 10 : 0;
+        source.each([&](uint64_t key) __attribute__((always_inline)) {
+            if (!inside(key)) return;
+            const uint32_t part = (uint32_t)((key - lo) >> shift);
+            atomicAdd(&q.count[part], 1u);
+            atomicAdd((unsigned long long*)&q.sum[part], (unsigned long long)fixed(a, r, table, value_of(key)));
         });
         __syncthreads();
-        uint64_t wu = 0;
-        uint32_t cu = 0;
-        if (tid < 256) {
-            wu = wave_scan64(s.sum[tid]);
-            cu = (uint32_t)wave_scan64(s.count[tid]);
-            if (lane == 63) {
-                s.wave_sum[wave] = wu;
-                s.wave_count[wave] = cu;
-            }
+        const uint64_t w = gh_scan64(q.sum[tid]);
+        const uint32_t c = (uint32_t)gh_scan64(q.count[tid]);
+        if (lane == 63) {
+            q.wave_sum[wave] = w;
+            q.wave_count[wave] = c;
         }
         __syncthreads();
-        if (tid < 256) {
-            for (uint32_t i = 0; i < wave; ++i) {
-                wu += s.wave_sum[i];
-                cu += s.wave_count[i];
-            }
-            s.sum[256 + tid] = wu;
-            s.count[256 + tid] = cu;
-            if (is(t.count_before + cu, t.before + wu)) atomicMin(&s.found[0], tid);
+        uint64_t w0 = sum + w - q.sum[tid];
+        uint32_t c0 = count + c - q.count[tid];
+        for (uint32_t i = 0; i < wave; ++i) {
+            w0 += q.wave_sum[i];
+            c0 += q.wave_count[i];
+        }
+        // one part: the first of those that hold a token and end where `is` is true
+        if (q.count[tid] && is(c0 + q.count[tid], w0 + q.sum[tid]) && !(c0 > count && is(c0, w0))) {
+            q.found = tid;
+            q.hit.sum = w0;
+            q.hit.count = c0;
         }
         __syncthreads();
-        const uint32_t b = s.found[0];
-        t.key = t.key << 8 | b;
-        t.count = s.count[b];
-        t.count_before += s.count[256 + b] - s.count[b];
-        t.before += s.sum[256 + b] - s.sum[b];
+        const uint32_t part = q.found;
+        sum = q.hit.sum;
+        count = q.hit.count;
+        n = q.count[part];
+        lo += (uint64_t)part << shift;
+        hi = min(hi, lo + (((uint64_t)1 << shift) - 1));
+        __syncthreads();
     }
-    t.w = fixed(a, weight(r, order_value(~t.key)));
-    return t;
+    if (tid == 0) q.fill = 0;
+    __syncthreads();
+    source.each([&](uint64_t key) __attribute__((always_inline)) {
+        if (!inside(key)) return;
+        const uint32_t at = atomicAdd(&q.fill, 1u);
+        if (at < 64) q.few[at] = key;
+    });
+    __syncthreads();
+    if (wave == 0) {
+        const uint64_t key = gh_sort64(lane < q.fill ? q.few[lane] : ~0ull);
+        const uint64_t w = sum + gh_scan64(lane < q.fill ? fixed(a, r, table, value_of(key)) : 0);
+        const uint64_t good = __ballot(lane < q.fill && is(count + lane + 1, w));
+        const uint32_t at = good ? (uint32_t)__builtin_ctzll(good) : min(q.fill, 64u) - 1;
+        if (lane == at) q.hit = Hit{key, w, count + lane + 1};
+    }
+    __syncthreads();
+    return q.hit;
 }
 
-// The searches of gh_sample_pick over the whole row. Returns the token, its weight over the kept sum in *prob.
-__device__ __forceinline__ uint32_t pick_from_row(const GhSampleArgs& a, const Row& r, const Plan& p, uint32_t row, PlanLds& s, double* prob) {
+// The row's token; its share of the kept sum in *prob.
+template <class S>
+__device__ __forceinline__ uint32_t pick_by_search(const GhSampleArgs& a, const Row& r, const double* table, const Plan& p, const PlanLds& s,
+                                                   PickLds& q, const S& source, double* prob) {
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
     uint32_t keep = p.keep;
-    uint64_t sum = p.all;
-    if (keep < p.tokens) {
-        const Ties t = descend(a, r, row, s, [&](uint32_t c, uint64_t) { return c >= keep; });
-        sum = t.before + (keep - t.count_before) * t.w;
-    }
-    if (r.top_p < 1.0f) {
+    uint64_t sum = s.sum[p.k];
+    if (p.partly) sum = search(a, r, table, s, q, source, [&](uint32_t c, uint64_t) { return c >= keep; }).sum;
+    if (p.p0 != kNone) {
         const double want = r.top_p * (double)sum;
-        const Ties t = descend(a, r, row, s, [&](uint32_t, uint64_t w) { return (double)w >= want; });
-        const uint32_t j = t.until([&](uint64_t w) { return (double)w >= want; });
-        if (t.count_before + j < keep) {
-            keep = t.count_before + j;
-            sum = t.before + j * t.w;
+        const Hit h = search(a, r, table, s, q, source, [&](uint32_t, uint64_t w) { return (double)w >= want; });
+        if (h.count < keep) {
+            keep = h.count;
+            sum = h.sum;
         }
     }
-    if (r.min_p > 0.0f) {
+    if (p.m0 != kNone) {
+        uint64_t w = 0, c = 0;
+        source.each([&](uint64_t key) __attribute__((always_inline)) {
+            const float l = value_of(key);
+            const uint32_t b = bin_of(r.top - l);
+            if (p.m0 <= b && b <= p.m1 && weight(r, table, l) >= (double)r.min_p) {
+                ++c;
+                w += fixed(a, r, table, l);
+            }
+        });
+        w = gh_scan64(w);
+        c = gh_scan64(c);
         __syncthreads();
-        if (tid == 0) {
-            s.sum[0] = 0;
-            s.count[0] = 0;
+        if (lane == 63) {
+            q.wave_sum[wave] = w;
+            q.wave_count[wave] = (uint32_t)c;
         }
         __syncthreads();
-        uint64_t w = 0;
-        uint32_t c = 0;
-        each_logit(a, row, 0, a.vocab, kPick, [&](float l, uint32_t) __attribute__((always_inline)) {
-            if (!finite(l)) return;
-            const double x = weight(r, l);
-            if (x < (double)r.min_p) return;
-            ++c;
-            w += fixed(a, x);
-        });
-        atomicAdd(&s.count[0], c);
-        atomicAdd((unsigned long long*)&s.sum[0], (unsigned long long)w);
-        __syncthreads();
-        const uint32_t rank = max(s.count[0], 1u);
+        uint64_t to = before(s, p.m0);
+        uint32_t rank = count_before(s, p.m0);
+        for (uint32_t i = 0; i < 16; ++i) {
+            to += q.wave_sum[i];
+            rank += q.wave_count[i];
+        }
+        if (rank == 0) {
+            rank = 1;
+            to = fixed(a, r, table, r.top);
+        }
         if (rank < keep) {
             keep = rank;
-            sum = s.count[0] ? s.sum[0] : fixed(a, 1.0);
+            sum = to;
         }
     }
     const double want = r.u * (double)sum;
-    const Ties t = descend(a, r, row, s, [&](uint32_t, uint64_t w) { return (double)w > want; });
-    const uint32_t j = t.until([&](uint64_t w) { return (double)w > want; });
-    *prob = weight(r, order_value(~t.key)) * a.scale / (double)sum;
-    // the j-th of them by index: each thread counts in a part of the row
-    const GH_GLOBAL uint32_t* l = gh_gp<uint32_t>(a.logits) + (uint64_t)row * a.stride;
-    const uint32_t per = (a.vocab + kPick - 1) / kPick, from = min(tid * per, a.vocab), end = min(from + per, a.vocab);
-    uint32_t mine = 0;
-    for (uint32_t i = from; i < end; ++i) mine += ~order_key(l[i]) == t.key;
-    const uint32_t upto = (uint32_t)wave_scan64(mine);
-    __syncthreads();
-    if (lane == 63) s.wave_count[wave] = upto;
-    if (tid == 0) s.found[0] = r.best;
-    __syncthreads();
-    uint32_t at = upto - mine;
-    for (uint32_t i = 0; i < wave; ++i) at += s.wave_count[i];
-    if (at < j && j <= at + mine)
-        for (uint32_t i = from; i < end; ++i)
-            if (~order_key(l[i]) == t.key && ++at == j) s.found[0] = i;
-    __syncthreads();
-    return s.found[0];
+    const Hit h = search(a, r, table, s, q, source, [&](uint32_t, uint64_t w) { return (double)w > want; });
+    *prob = weight(r, table, value_of(h.key)) * a.scale / (double)sum;
+    return (uint32_t)h.key;
+}
+
+// The same by one wave that has all of the list, at most 64 tokens: lane i the i-th in rank order, with the count and sum of the
+// row's tokens up to it.
+__device__ __forceinline__ uint32_t pick_by_wave(const GhSampleArgs& a, const Row& r, const double* table, const Plan& p, const PlanLds& s,
+                                                 uint64_t key, double* prob) {
+    const uint32_t lane = threadIdx.x & 63u, n = p.listed;
+    key = gh_sort64(key);
+    const bool there = lane < n;
+    const float l = value_of(key);
+    const uint32_t bin = there ? bin_of(r.top - l) : kNone;
+    const uint64_t own = there ? fixed(a, r, table, l) : 0, upto = gh_scan64(own);
+    // the first lane of the token's bin: what is before it in the list is not what is before it in the row
+    const uint32_t left = (uint32_t)__shfl_up((int)bin, 1, 64);
+    const uint64_t heads = __ballot(lane == 0 || bin != left);
+    const uint32_t head = 63 - (uint32_t)__clzll((long long)(heads & (~0ull >> (63 - lane))));
+    const uint64_t skip = __shfl((unsigned long long)(upto - own), (int)head, 64);
+    const uint64_t w = there ? before(s, bin) + upto - skip : 0;
+    const uint32_t c = there ? count_before(s, bin) + lane - head + 1 : 0;
+    auto first = [&](bool is) __attribute__((always_inline)) {
+        const uint64_t good = __ballot(there && is);
+        return good ? (uint32_t)__builtin_ctzll(good) : 64u;
+    };
+    uint32_t keep = p.keep;
+    uint64_t sum = s.sum[p.k];
+    if (p.partly) {
+        const uint32_t i = min(first(c >= keep), n - 1);
+        sum = gh_lane64(w, i);
+    }
+    if (p.p0 != kNone) {
+        const uint32_t i = first((double)w >= r.top_p * (double)sum && bin >= p.p0);
+        const uint32_t ci = (uint32_t)__builtin_amdgcn_readlane(c, i & 63u);
+        if (i < n && ci < keep) {
+            keep = ci;
+            sum = gh_lane64(w, i);
+        }
+    }
+    if (p.m0 != kNone) {
+        const bool in = there && p.m0 <= bin && bin <= p.m1 && weight(r, table, l) >= (double)r.min_p;
+        uint32_t rank = count_before(s, p.m0) + (uint32_t)__popcll(__ballot(in));
+        uint64_t to = before(s, p.m0) + gh_lane64(gh_scan64(in ? own : 0), 63);
+        if (rank == 0) {
+            rank = 1;
+            to = fixed(a, r, table, r.top);
+        }
+        if (rank < keep) {
+            keep = rank;
+            sum = to;
+        }
+    }
+    const uint32_t i = min(first((double)w > r.u * (double)sum && bin >= p.d0), n - 1);
+    const uint64_t hit = gh_lane64(key, i);
+    *prob = weight(r, table, value_of(hit)) * a.scale / (double)sum;
+    return (uint32_t)hit;
 }
 }  // namespace
 
@@ -492,7 +637,8 @@ __device__ __forceinline__ uint32_t pick_from_row(const GhSampleArgs& a, const R
 GH_KERNEL __launch_bounds__(1024) void gh_sample_pick(GhSampleArgs a) {
     __shared__ PlanLds s;
     __shared__ PickLds q;
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, row = blockIdx.x;
+    __shared__ double table[64];
+    const uint32_t tid = threadIdx.x, row = blockIdx.x;
     const Row r = row_of(a, row);
     auto done = [&](uint32_t token, double prob) __attribute__((always_inline)) {
         gh_gpw<uint32_t>(a.tokens)[row] = token;
@@ -502,113 +648,21 @@ GH_KERNEL __launch_bounds__(1024) void gh_sample_pick(GhSampleArgs a) {
         if (tid == 0) done(r.best, 1.0);
         return;
     }
-    const Plan p = plan_of<kPick>(a, r, row, s);
-    if (p.listed > kList) {
-        double prob;
-        const uint32_t token = pick_from_row(a, r, p, row, s, &prob);
-        if (tid == 0) done(token, prob);
-        return;
-    }
-    const uint32_t n = p.listed;
-    uint32_t size = 64;
-    while (size < n) size <<= 1;
+    fill_exp(table);
     const uint64_t list = a.list + (uint64_t)row * kList * 8;
-    for (uint32_t i = tid; i < size; i += kPick) q.key[i] = i < n ? gh_gp<uint64_t>(list)[i] : ~0ull;
-    // of each bin: the sums and counts of the bins before it that are not listed
-    {
-        const uint32_t b = tid;  // kBins == kPick
-        const bool in = p.has(b);
-        const uint64_t w = in ? s.sum[b] - before(s, b) : 0;
-        const uint32_t c = in ? s.count[b] - count_before(s, b) : 0;
-        const uint64_t wu = wave_scan64(w);
-        const uint32_t cu = (uint32_t)wave_scan64(c);
-        __syncthreads();
-        if (lane == 63) {
-            s.wave_sum[wave] = wu;
-            s.wave_count[wave] = cu;
-        }
-        __syncthreads();
-        uint64_t wat = wu - w;
-        uint32_t cat = cu - c;
-        for (uint32_t i = 0; i < wave; ++i) {
-            wat += s.wave_sum[i];
-            cat += s.wave_count[i];
-        }
-        q.skip_sum[b] = before(s, b) - wat;
-        q.skip_count[b] = count_before(s, b) - cat;
-        if (tid < 8) q.found[tid] = kNone;
+    uint64_t key = ~0ull;
+    if (tid < 64) key = gh_gp<uint64_t>(list)[tid];  // on its way while the plan is made
+    const Plan p = plan_of<kPick>(a, r, row, s);
+    double prob;
+    uint32_t token;
+    if (p.listed <= 64) {
+        if (tid >= 64) return;
+        token = pick_by_wave(a, r, table, p, s, tid < p.listed ? key : ~0ull, &prob);
+    } else if (p.listed <= kList) {
+        for (uint32_t i = tid; i < p.listed; i += kPick) q.list[i] = gh_gp<uint64_t>(list)[i];
+        token = pick_by_search(a, r, table, p, s, q, Listed{q.list, p.listed}, &prob);
+    } else {
+        token = pick_by_search(a, r, table, p, s, q, Whole{a, row}, &prob);
     }
-    __syncthreads();
-    sort_keys(q.key, size);
-    // running sums: thread t has kList / kPick tokens in a row
-    constexpr uint32_t kEach = kList / kPick;
-    const uint32_t each = size > kPick ? size / kPick : 1;
-    uint64_t own[kEach], mine = 0;
-#pragma unroll
-    for (uint32_t j = 0; j < kEach; ++j) {
-        const uint32_t i = tid * each + j;
-        own[j] = j < each && i < n ? fixed(a, weight(r, value_of(q.key[i]))) : 0;
-        mine += own[j];
-    }
-    const uint64_t upto = wave_scan64(mine);
-    if (lane == 63) s.wave_sum[wave] = upto;
-    __syncthreads();
-    uint64_t at = upto - mine;
-    for (uint32_t i = 0; i < wave; ++i) at += s.wave_sum[i];
-    // the thread's tokens: running sum of all tokens up to it, and its rank
-#pragma unroll
-    for (uint32_t j = 0; j < kEach; ++j) {
-        const uint32_t i = tid * each + j;
-        if (j < each && i < n) {
-            at += own[j];
-            q.upto[i] = at + q.skip_sum[bin_of(r.top - value_of(q.key[i]))];
-        }
-    }
-    __syncthreads();
-    auto bin_at = [&](uint32_t i) __attribute__((always_inline)) { return bin_of(r.top - value_of(q.key[i])); };
-    auto rank_at = [&](uint32_t i) __attribute__((always_inline)) { return i + q.skip_count[bin_at(i)]; };
-    // the first listed token for which `is`
-    auto first = [&](uint32_t slot, auto is) __attribute__((always_inline)) {
-        for (uint32_t i = tid; i < n; i += kPick)
-            if (is(i)) {
-                atomicMin(&q.found[slot], i);
-                break;
-            }
-        __syncthreads();
-        return q.found[slot];
-    };
-    // how many are kept, and their sum
-    uint32_t keep = p.keep;
-    uint64_t sum = s.sum[p.k];
-    if (p.partly) sum = q.upto[first(0, [&](uint32_t i) { return rank_at(i) + 1 == p.keep; })];
-    if (p.p0 != kNone) {
-        const double want = r.top_p * (double)sum;
-        const uint32_t i = first(1, [&](uint32_t i) { return (double)q.upto[i] >= want && bin_at(i) >= p.p0; });
-        if (i < n && rank_at(i) + 1 < keep) {
-            keep = rank_at(i) + 1;
-            sum = q.upto[i];
-        }
-    }
-    if (p.m0 != kNone) {
-        const uint32_t i = first(2, [&](uint32_t i) {
-            const uint32_t b = bin_at(i);
-            return p.m0 <= b && b <= p.m1 && weight(r, value_of(q.key[i])) < (double)r.min_p;
-        });
-        uint32_t rank = i == kNone ? s.count[p.m1] : rank_at(i);
-        uint64_t to = i == kNone ? s.sum[p.m1] : q.upto[i] - fixed(a, weight(r, value_of(q.key[i])));
-        if (rank == 0) {
-            rank = 1;
-            to = fixed(a, 1.0);
-        }
-        if (rank < keep) {
-            keep = rank;
-            sum = to;
-        }
-    }
-    const double want = r.u * (double)sum;
-    const uint32_t i = min(first(3, [&](uint32_t i) { return (double)q.upto[i] > want && bin_at(i) >= p.d0; }), n - 1);
-    if (tid == 0) {
-        const uint64_t key = q.key[i];
-        done((uint32_t)key, weight(r, value_of(key)) * a.scale / (double)sum);
-    }
+    if (tid == 0) done(token, prob);
 }

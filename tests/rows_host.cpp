@@ -92,7 +92,7 @@ uint32_t host_offset(const char* name) {
 #define FIELD(type, name_) if (!std::strcmp(name, #type "." #name_)) return (uint32_t)offsetof(type, name_);
     FIELD(GhSampleArgs, logits) FIELD(GhSampleArgs, params) FIELD(GhSampleArgs, uniform) FIELD(GhSampleArgs, tokens)
     FIELD(GhSampleArgs, probs) FIELD(GhSampleArgs, part) FIELD(GhSampleArgs, bins) FIELD(GhSampleArgs, list)
-    FIELD(GhSampleArgs, scale) FIELD(GhSampleArgs, chunks) FIELD(GhSampleArgs, per) FIELD(GhSampleArgs, wide)
+    FIELD(GhSampleArgs, scale) FIELD(GhSampleArgs, chunks) FIELD(GhSampleArgs, per) FIELD(GhSampleArgs, wide) FIELD(GhSampleArgs, shift)
     FIELD(GhPagedAttnArgs, q) FIELD(GhPagedAttnArgs, part_acc) FIELD(GhPagedAttnArgs, part_ml) FIELD(GhPagedAttnArgs, raw)
     FIELD(GhPagedAttnArgs, layout) FIELD(GhPagedAttnArgs, rows) FIELD(GhPagedAttnArgs, chunks) FIELD(GhPagedAttnArgs, least)
     FIELD(GhPagedAttnArgs, raw_len) FIELD(GhPagedAttnArgs, max_len) FIELD(GhPagedEvictArgs, src_layer) FIELD(GhPagedEvictArgs, dst_layer)

@@ -288,6 +288,7 @@ def test_sample_plans(host, seed):
         assert spans[0][0] >= SCRATCH and spans[-1][0] + spans[-1][1] <= SCRATCH + host.lib.host_scratch()
         assert all(x + y <= z for (x, y), (z, _) in zip(spans, spans[1:])) and f("bins") % 8 == 0 and f("part") % 16 == 0
         scale = f("scale", C.c_double)
-        assert 2.0 ** 61 < scale * vocab <= 2.0 ** 62
+        assert scale <= 2.0 ** 51 and scale * vocab <= 2.0 ** 62 and (scale == 2.0 ** 51 or 2.0 ** 61 < scale * vocab)
+        assert scale == 2.0 ** f("shift", C.c_int32)
         assert not f("wide", C.c_uint32) or stride % 4 == 0
     assert at == rows
