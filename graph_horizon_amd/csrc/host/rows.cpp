@@ -42,9 +42,9 @@ int gh_norm_rope_batched(gh_backend* b, gh_encoder* enc, const gh_buf* q, const 
         for (const gh_buf* w : {q_norm, k_norm})
             if (meet(q, qb, w, wb) || meet(k, kb, w, wb)) return no(GH_E_INVALID, "q or k overlaps the weights");
         GhNormRopeArgs a{};
-        a.lanes = 1;
-        while (8 * a.lanes < head_dim) a.lanes *= 2;
-        a.groups = ceil_div((uint64_t)(q_heads + kv_heads) * a.lanes, 256);
+        while (8u << a.shift < head_dim) ++a.shift;
+        a.share = 1.0f / (float)head_dim;
+        a.groups = ceil_div((uint64_t)(q_heads + kv_heads) << a.shift, 256);
         if ((uint64_t)rows * a.groups > 0xFFFFFFull) return no(GH_E_RANGE, "too many vectors");
         const int rc = ensure_rope(b, b->rope, yarn, base + rows);
         if (rc || a.groups == 0) return rc;

@@ -39,40 +39,43 @@ __device__ __forceinline__ float gh_group_sum(float v, uint32_t lanes) {
     return v;
 }
 
-// x over the root of the mean square of the head's `dim` values in `lanes` lanes, times the weight.
-__device__ __forceinline__ void gh_head_norm(float (&x)[8], const uint4& weight, uint32_t dim, float eps, uint32_t lanes) {
+// x over the root of the mean square of the head's values in `lanes` lanes, times the weight; share: 1 / their number.
+__device__ __forceinline__ void gh_head_norm(float (&x)[8], const uint4& weight, float share, float eps, uint32_t lanes) {
     float s = 0.0f, w[8];
     gh_unpack8(weight, w);
 #pragma unroll
     for (int i = 0; i < 8; ++i) s += x[i] * x[i];
-    const float inv = 1.0f / __builtin_sqrtf(gh_group_sum(s, lanes) / (float)dim + eps);
+    const float inv = __builtin_amdgcn_rsqf(gh_group_sum(s, lanes) * share + eps);
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * w[i];
 }
 
-// The lane's adjacent pairs first .. first + 3, those below `pairs`, turned by (cos, sin) at cs[first ..] and scaled.
-__device__ __forceinline__ void gh_turn(float (&x)[8], int i, float c, float s, float scale) {
-#pragma clang fp contract(off)
-    const float x0 = x[2 * i], x1 = x[2 * i + 1];
-    x[2 * i] = (x0 * c - x1 * s) * scale;
-    x[2 * i + 1] = (x0 * s + x1 * c) * scale;
-}
-__device__ __forceinline__ void gh_turn4(float (&x)[8], const GH_GLOBAL float2* cs, uint32_t first, uint32_t pairs, float scale) {
-    if ((pairs & 3u) == 0) {  // whole lanes, on 16 bytes
-        const GH_GLOBAL float4* c4 = (const GH_GLOBAL float4*)(cs + first);
+// (cos, sin) of the lane's adjacent pairs first .. first + 3 of one position; those at or past `pairs` are of others. WIDE:
+// `pairs` is a multiple of four, so that these are 32 bytes on 16. (A template, not a branch: the compiler makes one path of the
+// two, with eight loads of a dword, and 2000 rows of 40 heads took 24.7 us.)
+template <bool WIDE>
+__device__ __forceinline__ void gh_load_turns(const GH_GLOBAL float2* cs, uint32_t first, uint32_t pairs, float2 (&c)[4]) {
+    if (WIDE) {
+        const GH_GLOBAL float4* c4 = (const GH_GLOBAL float4*)(cs + min(first, pairs - 4));
         const float4 c0 = c4[0], c1 = c4[1];
-        gh_turn(x, 0, c0.x, c0.y, scale);
-        gh_turn(x, 1, c0.z, c0.w, scale);
-        gh_turn(x, 2, c1.x, c1.y, scale);
-        gh_turn(x, 3, c1.z, c1.w, scale);
-        return;
+        c[0] = make_float2(c0.x, c0.y), c[1] = make_float2(c0.z, c0.w);
+        c[2] = make_float2(c1.x, c1.y), c[3] = make_float2(c1.z, c1.w);
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) c[i] = cs[min(first + i, pairs - 1)];
+    }
+}
+// Those pairs below `pairs` turned and scaled, in gh_rope's operations. all: they are all of the head's.
+__device__ __forceinline__ void gh_turn4(float (&x)[8], const float2 (&c)[4], uint32_t first, uint32_t pairs, float scale, bool all) {
+#pragma clang fp contract(off)
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        y[2 * i] = (x[2 * i] * c[i].x - x[2 * i + 1] * c[i].y) * scale;
+        y[2 * i + 1] = (x[2 * i] * c[i].y + x[2 * i + 1] * c[i].x) * scale;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (first + i < pairs) {
-            const float2 c = cs[first + i];
-            gh_turn(x, i, c.x, c.y, scale);
-        }
+    for (int i = 0; i < 8; ++i) x[i] = all || first + i / 2 < pairs ? y[i] : x[i];
 }
 
 #endif

@@ -178,14 +178,14 @@ struct GhNormRopeArgs {
     uint64_t post;    // float [positions]
     uint32_t heads;
     uint32_t kheads;
-    uint32_t head_dim;  // a multiple of 8, at most 8 lanes
+    uint32_t head_dim;  // a multiple of 8, at most 8 times the lanes
     uint32_t pairs;
     uint32_t base;
     uint32_t rows;
-    uint32_t lanes;   // of a head: 1, 2, 4, .. 64
+    uint32_t shift;   // lanes of a head: 2^shift, up to 64
     uint32_t groups;  // workgroups per row
     float eps;
-    uint32_t pad;
+    float share;      // 1 / head_dim
 };
 
 struct GhEltArgs {

@@ -89,28 +89,36 @@ GH_KERNEL __launch_bounds__(256) void gh_rope(GhRopeArgs a) {
 }
 
 // Norms of query and key heads and their rotation in one pass, FP16 in place: x / sqrt(mean x² + eps) · w over each
-// head, then as gh_rope. A head is a.lanes lanes of 8 values (a power of two; those past head_dim hold zeros), the
-// sum of squares a few lane exchanges, and nothing is rounded between the two. Bound by memory.
-GH_KERNEL __launch_bounds__(256) void gh_norm_rope(GhNormRopeArgs a) {
+// head, then as gh_rope. A head is 2^shift lanes of 8 values (those past head_dim hold zeros), the
+// sum of squares a few lane exchanges, and nothing is rounded between the two. Bound by memory: 2000 rows of 40 heads, 41 MB, 10.5 us (two and
+// four heads per thread, which would share the turns: 12.6 and 11.2).
+template <bool WIDE>
+__device__ __forceinline__ void norm_rope(const GhNormRopeArgs& a) {
     const uint32_t row = blockIdx.x / a.groups, item = (blockIdx.x % a.groups) * 256 + threadIdx.x;
-    uint32_t head = item / a.lanes;
-    const uint32_t part = item & (a.lanes - 1);
+    uint32_t head = item >> a.shift;
+    const uint32_t lanes = 1u << a.shift, part = item & (lanes - 1);
     if (head >= a.heads + a.kheads) return;  // whole heads
     const bool key = head >= a.heads, there = 8 * part < a.head_dim;
     if (key) head -= a.heads;
     const uint64_t p = (key ? a.k : a.q) + (((uint64_t)row * (key ? a.kheads : a.heads) + head) * a.head_dim + 8 * part) * 2;
+    const uint32_t pos = a.base + row;
     uint4 raw = make_uint4(0u, 0u, 0u, 0u), weight = raw;
     if (there) {
         raw = *gh_gp<uint4>(p);
         weight = *gh_gp<uint4>((key ? a.k_norm : a.q_norm) + 16 * part);
     }
-    const uint32_t pos = a.base + row;
-    const float scale = key ? 1.0f : gh_gp<float>(a.post)[pos];
+    float2 c[4];
+    gh_load_turns<WIDE>(gh_gp<float2>(a.table) + (uint64_t)pos * a.pairs, 4 * part, a.pairs, c);
+    const float post = gh_gp<float>(a.post)[pos];
     float x[8];
     gh_unpack8(raw, x);
-    gh_head_norm(x, weight, a.head_dim, a.eps, a.lanes);
-    if (4 * part < a.pairs) gh_turn4(x, gh_gp<float2>(a.table) + (uint64_t)pos * a.pairs, 4 * part, a.pairs, scale);
+    gh_head_norm(x, weight, a.share, a.eps, lanes);
+    gh_turn4(x, c, 4 * part, a.pairs, key ? 1.0f : post, 2 * a.pairs == a.head_dim);
     if (there) *gh_gpw<uint4>(p) = gh_pack8(x);
+}
+GH_KERNEL __launch_bounds__(256) void gh_norm_rope(GhNormRopeArgs a) {
+    if (a.pairs % 4 == 0) norm_rope<true>(a);
+    else norm_rope<false>(a);
 }
 
 // The elementwise kernels below take 8 consecutive values per thread: 16-byte accesses where a.pad

@@ -51,8 +51,8 @@ __device__ __forceinline__ float quad_max(float v) {
 }
 
 // The lane's 8 of 32 values as codes; returns them, step and minimum in *dm. The step is cut off to FP16, so that
-// m + 15 d stays in the values' range. (x - m) / d is a true quotient: FP16 values lie on ties that a product
-// with 1 / d would miss. Values that are not finite make the group NaN.
+// m + 15 d stays in the values' range. (x - m) / d is a true quotient (a product with 1 / d, corrected by what it leaves):
+// FP16 values lie on ties that the product alone would miss. Values that are not finite make the group NaN.
 __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], uint32_t* dm) {
     float lo = x[0], hi = x[0], odd = 0.0f;
 #pragma unroll
@@ -71,17 +71,17 @@ __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], uint32_t* dm) 
         return 0u;
     }
     *dm = d16 | m16 << 16;
-    const float m = gh_h2f(m16), d = gh_h2f(d16);
+    const float m = gh_h2f(m16), d = gh_h2f(d16), r = d > 0.0f ? __builtin_amdgcn_rcpf(d) : 0.0f;
     uint32_t w = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float c = d > 0.0f ? __builtin_rintf((x[i] - m) / d) : 0.0f;
-        w |= (uint32_t)fminf(fmaxf(c, 0.0f), 15.0f) << (4 * i);
+        const float y = x[i] - m, t = y * r, c = __builtin_rintf(__builtin_fmaf(__builtin_fmaf(-t, d, y), r, t));
+        w |= (uint32_t)__builtin_amdgcn_fmed3f(c, 0.0f, 15.0f) << (4 * i);
     }
     return w;
 }
 
-template <bool NORM, bool Q4>
+template <bool NORM, bool Q4, bool WIDE>
 __device__ __forceinline__ void paged_append(const GhPagedWriteArgs& a) {
     const uint32_t token = blockIdx.x / a.groups, row = token / a.tokens, t = token % a.tokens;
     const uint32_t item = (blockIdx.x % a.groups) * 256 + threadIdx.x;
@@ -104,9 +104,14 @@ __device__ __forceinline__ void paged_append(const GhPagedWriteArgs& a) {
     }
     float x[8];
     gh_unpack8(raw, x);
-    if (NORM && !value) gh_head_norm(x, weight, 128, a.eps, 16);
-    if (a.positions && !value && 4 * part < a.pairs)
-        gh_turn4(x, gh_gp<float2>(a.table) + (uint64_t)pos * a.pairs, 4 * part, a.pairs, query ? gh_gp<float>(a.post)[pos] : 1.0f);
+    if (!value) {
+        if (NORM) gh_head_norm(x, weight, 1.0f / 128, a.eps, 16);
+        if (a.positions) {
+            float2 c[4];
+            gh_load_turns<WIDE>(gh_gp<float2>(a.table) + (uint64_t)pos * a.pairs, 4 * part, a.pairs, c);
+            gh_turn4(x, c, 4 * part, a.pairs, query ? gh_gp<float>(a.post)[pos] : 1.0f, a.pairs == 64);
+        }
+    }
     if (query) {
         *gh_gpw<uint4>(a.q_out + in) = gh_pack8(x);
         return;
@@ -127,9 +132,18 @@ __device__ __forceinline__ void paged_append(const GhPagedWriteArgs& a) {
         gh_gpw<float>(a.p.score)[((uint64_t)row * a.p.kv_heads + h) * (a.p.width << a.p.shift) + at] = 0.0f;
 }
 }  // namespace
-GH_KERNEL __launch_bounds__(256) void gh_paged4_write(GhPagedWriteArgs a) { paged_append<false, true>(a); }
-GH_KERNEL __launch_bounds__(256) void gh_paged4_norm_write(GhPagedWriteArgs a) { paged_append<true, true>(a); }
-GH_KERNEL __launch_bounds__(256) void gh_paged_norm_write(GhPagedWriteArgs a) { paged_append<true, false>(a); }
+GH_KERNEL __launch_bounds__(256) void gh_paged4_write(GhPagedWriteArgs a) {
+    if (a.pairs % 4 == 0) paged_append<false, true, true>(a);
+    else paged_append<false, true, false>(a);
+}
+GH_KERNEL __launch_bounds__(256) void gh_paged4_norm_write(GhPagedWriteArgs a) {
+    if (a.pairs % 4 == 0) paged_append<true, true, true>(a);
+    else paged_append<true, true, false>(a);
+}
+GH_KERNEL __launch_bounds__(256) void gh_paged_norm_write(GhPagedWriteArgs a) {
+    if (a.pairs % 4 == 0) paged_append<true, false, true>(a);
+    else paged_append<true, false, false>(a);
+}
 
 // ---- read-back ---------------------------------------------------------------------------------
 // Thread = 8 values of one head of one position, key heads first.
