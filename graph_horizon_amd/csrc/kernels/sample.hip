@@ -430,8 +430,8 @@ struct Whole {
 };
 
 // The first token in rank order up to which count and sum satisfy `is`, which some token's do and stays true once it is. Its bin
-// by the running values of the bins; then, while a range holds more than 64 tokens, the 1024th part of the range of their keys
-// in which it is; then among these, sorted by one wave.
+// by the running values of the bins; then, while there are more than 64 tokens, in which 1024th of them it is, first by the next ten
+// bits of their distance, then by parts of the range of their keys; then among these, sorted by one wave.
 template <class S, class F>
 __device__ __forceinline__ Hit search(const GhSampleArgs& a, const Row& r, const double* table, const PlanLds& s, PickLds& q, const S& source, F is) {
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
@@ -443,35 +443,46 @@ __device__ __forceinline__ Hit search(const GhSampleArgs& a, const Row& r, const
     const uint32_t bin = q.found;
     uint64_t sum = before(s, bin), lo = 0, hi = ~0ull;
     uint32_t count = count_before(s, bin), n = s.count[bin] - count;
-    auto inside = [&](uint64_t key) __attribute__((always_inline)) { return key >= lo && key <= hi && bin_of(r.top - value_of(key)) == bin; };
+    // (the first and the last bin hold distances of any exponent)
+    bool bits = bin && bin < kBins - 1;
+    uint32_t tenth = kNone;  // the distance's ten bits, once known
+    auto ten = [&](uint64_t key) __attribute__((always_inline)) { return __float_as_uint(r.top - value_of(key)) >> 7 & 1023u; };
+    auto inside = [&](uint64_t key) __attribute__((always_inline)) {
+        return key >= lo && key <= hi && bin_of(r.top - value_of(key)) == bin && (tenth == kNone || ten(key) == tenth);
+    };
     while (n > 64) {
-        uint64_t least = ~0ull, most = 0;
-        source.each([&](uint64_t key) __attribute__((always_inline)) {
-            if (!inside(key)) return;
-            least = min(least, key);
-            most = max(most, key);
-        });
-        least = ~gh_max64(~least);
-        most = gh_max64(most);
-        __syncthreads();
-        if (lane == 0) {
-            q.lo[wave] = least;
-            q.hi[wave] = most;
-        }
+        uint32_t shift = 0;
         q.sum[tid] = 0;
         q.count[tid] = 0;
         if (tid == 0) q.found = kBins - 1;
-        __syncthreads();
-        for (uint32_t i = 0; i < 16; ++i) {
-            least = min(least, q.lo[i]);
-            most = max(most, q.hi[i]);
+        if (!bits) {
+            uint64_t least = ~0ull, most = 0;
+            source.each([&](uint64_t key) __attribute__((always_inline)) {
+                if (!inside(key)) return;
+                least = min(least, key);
+                most = max(most, key);
+            });
+            least = ~gh_max64(~least);
+            most = gh_max64(most);
+            if (lane == 0) {
+                q.lo[wave] = least;
+                q.hi[wave] = most;
+            }
+            __syncthreads();
+            for (uint32_t i = 0; i < 16; ++i) {
+                least = min(least, q.lo[i]);
+                most = max(most, q.hi[i]);
+            }
+            lo = least;
+            hi = most;
+            const uint32_t width = 64 - __clzll((long long)(hi - lo));
+            shift = width > 10 ? width - 10 : 0;
+        } else {
+            __syncthreads();
         }
-        lo = least;
-        hi = most;
-        const uint32_t bits = 64 - __clzll((long long)(hi - lo)), shift = bits > 10 ? bits - 10 : 0;
         source.each([&](uint64_t key) __attribute__((always_inline)) {
             if (!inside(key)) return;
-            const uint32_t part = (uint32_t)((key - lo) >> shift);
+            const uint32_t part = bits ? ten(key) : (uint32_t)((key - lo) >> shift);
             atomicAdd(&q.count[part], 1u);
             atomicAdd((unsigned long long*)&q.sum[part], (unsigned long long)fixed(a, r, table, value_of(key)));
         });
@@ -500,8 +511,13 @@ __device__ __forceinline__ Hit search(const GhSampleArgs& a, const Row& r, const
         sum = q.hit.sum;
         count = q.hit.count;
         n = q.count[part];
-        lo += (uint64_t)part << shift;
-        hi = min(hi, lo + (((uint64_t)1 << shift) - 1));
+        if (bits) {
+            tenth = part;
+            bits = false;
+        } else {
+            lo += (uint64_t)part << shift;
+            hi = min(hi, lo + (((uint64_t)1 << shift) - 1));
+        }
         __syncthreads();
     }
     if (tid == 0) q.fill = 0;
