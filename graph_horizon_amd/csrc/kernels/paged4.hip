@@ -52,7 +52,7 @@ __device__ __forceinline__ float quad_max(float v) {
 
 // The lane's 8 of 32 values as codes; returns them, step and minimum in *dm. The step is cut off to FP16, so that
 // m + 15 d stays in the values' range. (x - m) / d is a true quotient (a product with 1 / d, corrected by what it leaves):
-// FP16 values lie on ties that the product alone would miss. Values that are not finite make the group NaN.
+// FP16 values lie on ties that the product alone would miss. Values that FP16 does not hold as finite make the group NaN.
 __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], uint32_t* dm) {
     float lo = x[0], hi = x[0], odd = 0.0f;
 #pragma unroll
@@ -66,7 +66,7 @@ __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], uint32_t* dm) 
     odd = gh_quad_sum(odd);
     const uint32_t m16 = gh_f2h(lo);
     const uint32_t d16 = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz((hi - lo) / 15.0f, 0.0f)) & 0xFFFFu;
-    if (odd != 0.0f) {  // a NaN
+    if (odd != 0.0f || fmaxf(-lo, hi) >= 65520.0f) {  // (odd: a NaN)
         *dm = 0x7E007E00u;
         return 0u;
     }

@@ -307,10 +307,10 @@ __device__ __forceinline__ Plan plan_of(const GhSampleArgs& a, const Row& r, uin
         l1 = p.p1 = min(s.found[2], p.k);
     }
     if (r.min_p > 0.0f) {
-        // w >= min_p up to a distance of -T ln min_p; d is rounded to FP32
-        const double d = -log((double)r.min_p) * (double)r.temperature;
-        p.m0 = d > 0.0 ? bin_of((float)(d * (1.0 - 1e-6))) : 0u;
-        p.m1 = d > 0.0 ? bin_of((float)(d * (1.0 + 1e-6))) : 0u;
+        // w >= min_p up to a distance of -T ln min_p, and a little further, as weights next to 1 round to it; d is rounded to FP32
+        const double d = r.min_p < 1.0f ? -log((double)r.min_p) * (double)r.temperature : 0.0;
+        p.m0 = bin_of((float)(d * (1.0 - 1e-6)));
+        p.m1 = bin_of((float)((d + (double)r.temperature * 0x1p-50) * (1.0 + 1e-6)));
         l0 = min(l0, p.m0);
         l1 = min(l1, p.m1);
     }
