@@ -234,7 +234,11 @@ int attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv_pag
     GhPaged4AttnArgs t{};
     if (q4) {
         if (split) {
-            a.least = 2 * std::min(std::max(ceil_div(most, 8ull * b->cus) * 4, 4u), kSpanTiles);
+            // One span a row up to 512 positions, and up to 1024 where that still gives every other CU a workgroup; else spans as
+            // above. us of a call, so / in spans by the number of tiles alone: 1 row of 200 17.1 / 19.5, 16 of up to 500 20.0 / 21.9, 40 of
+            // up to 500 24.3 / 29.3, 24 of up to 700 22.6 / 26.0, 32 of up to 1000 26.0 / 29.4; 1 of 1000 23.3 / 19.7, 8 of 2000 27.7 / 24.8.
+            const bool one = tiles1 <= kSpanTiles / 2 || (tiles1 <= kSpanTiles && (uint64_t)kv->rows * hk >= b->cus / 2);
+            a.least = 2 * (one ? kSpanTiles : std::min(std::max(ceil_div(most, 8ull * b->cus) * 4, 4u), kSpanTiles));
             a.chunks = ceil_div(max_len, 16 * a.least);
         } else {
             a.least = 2;
