@@ -230,13 +230,16 @@ int attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv_pag
     // up to 8192 45.9 / 33.4, 32 of up to 4000 69.3 / 52.0.
     const uint32_t tiles1 = ceil_div(max_len, tile);
     const uint64_t most = (uint64_t)kv->rows * hk * tiles1;
-    const bool split = tiles1 <= kSpanTiles || most < 6144;
+    // In 4 bits (tiles of 32) spans hold out longer: us of a call, 1 row of 32768 28.9 / 34.5, 4 of 8192 28.5 / 33.7, 16 of up to 2500
+    // 29.0 / 30.9, 12 of up to 4000 35.4 / 32.4, 24 of up to 2500 37.1 / 34.8, 32 of up to 4000 47.7 / 40.2.
+    const bool split = tiles1 <= kSpanTiles || most < (q4 ? 12000u : 6144u);
     GhPaged4AttnArgs t{};
     if (q4) {
         if (split) {
             // One span a row up to 512 positions, and up to 1024 where that still gives every other CU a workgroup; else spans as
-            // above. us of a call, so / in spans by the number of tiles alone: 1 row of 200 17.1 / 19.5, 16 of up to 500 20.0 / 21.9, 40 of
-            // up to 500 24.3 / 29.3, 24 of up to 700 22.6 / 26.0, 32 of up to 1000 26.0 / 29.4; 1 of 1000 23.3 / 19.7, 8 of 2000 27.7 / 24.8.
+            // above. us of a call, so / in spans by the number of tiles alone (before the
+            // launch below): 1 row of 200 17.1 / 19.5, 16 of up to 500 20.0 / 21.9, 40 of up to 500 24.3 / 29.3, 24 of up to 700 22.6 / 26.0, 32 of
+            // up to 1000 26.0 / 29.4; 1 of 1000 23.3 / 19.7, 8 of 2000 27.7 / 24.8.
             const bool one = tiles1 <= kSpanTiles / 2 || (tiles1 <= kSpanTiles && (uint64_t)kv->rows * hk >= b->cus / 2);
             a.least = 2 * (one ? kSpanTiles : std::min(std::max(ceil_div(most, 8ull * b->cus) * 4, 4u), kSpanTiles));
             a.chunks = ceil_div(max_len, 16 * a.least);
@@ -303,7 +306,9 @@ int attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv_pag
         a.q = q->addr + (uint64_t)r * q_heads * 256;
         a.out = out->addr + (uint64_t)r * q_heads * 256;
         if (split) {
-            rc = launch(b, q4 ? scored ? K_PAGED4_SPLIT_S : K_PAGED4_SPLIT : scored ? K_PAGED_SPLIT_S : K_PAGED_SPLIT, hk, a.chunks, a.rows, 256, &a, 4 * group * 134 * 4);
+            const uint32_t lds = 4 * group * 134 * 4;
+            if (q4) rc = launch(b, scored ? K_PAGED4_SPLIT_S : K_PAGED4_SPLIT, 8 * hk, ceil_div((uint64_t)a.chunks * a.rows, 8), 1, 256, &a, lds);
+            else rc = launch(b, scored ? K_PAGED_SPLIT_S : K_PAGED_SPLIT, hk, a.chunks, a.rows, 256, &a, lds);
         } else {
             // no more chunks than the rows' tiles can fill
             const uint64_t chunks = std::min<uint64_t>(a.chunks, ceil_div((uint64_t)a.rows * tiles1, a.least));

@@ -550,14 +550,19 @@ __device__ __forceinline__ void paged4_attn(const GhPaged4AttnArgs& t) {
         paged4_chunk<SCORED, 0>(a, sh, behind, total, per, chunk, rounds, kvh, there, idle, pieces, lds, mine);
 }
 
-// Each row in spans, as gh_paged_split: of a.least / 2 tiles, of which wave w takes w, w + 4, ...
+// Each row in spans, as gh_paged_split: of a.least / 2 tiles, of which wave w takes w, w + 4, ... Grid (8 kv heads, spans / 8): the
+// heads of a span, whose vectors share lines, on one XCD, where workgroups go by their number mod 8, and so from one L2 (us of a call, so /
+// with adjacent heads on adjacent XCDs: 100 rows of up to 1000 36.4 / 45.0, 256 of up to 300 33.2 / 36.9, 1 of 9000 23.3 / 26.0,
+// 1 of 500 19.0 / 19.2).
 template <bool SCORED>
 __device__ __forceinline__ void paged4_split(const GhPagedAttnArgs& a) {
     extern __shared__ __align__(16) float dyn[];  // per wave and head: 132 floats of acc, then m and l
     __shared__ __align__(16) char stage[4][kTileBytes];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, n = lane & 15u, G = a.group;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t kvh = blockIdx.x, split = blockIdx.y, row = blockIdx.z;
+    const uint32_t spot = blockIdx.y * 8 + blockIdx.x % 8, kvh = blockIdx.x / 8;
+    if (spot >= a.chunks * a.rows) return;
+    const uint32_t row = spot / a.chunks, split = spot % a.chunks;
     const uint32_t span = a.least * 16, begin = split * span;  // < max_len
     // the wave's tile i covers positions begin + 128 i + 32 wave .. + 32
     const uint32_t first = begin + 32 * wave, mine = first + 128 * lane;

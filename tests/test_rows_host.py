@@ -177,7 +177,7 @@ def test_attention_plans_stay_within_their_scratch(host, seed):
         if split:
             parts = u("chunks") * u("rows")
             assert u("least") % 8 == 0 and u("least") <= 512 and 16 * u("least") * u("chunks") >= want
-            assert kernel != "split4" or (g.gx, g.gy, g.gz) == (heads, u("chunks"), u("rows"))
+            assert kernel != "split4" or (g.gx == 8 * heads and 8 * g.gy >= parts > 8 * (g.gy - 1) and g.gz == 1)
             assert kernel != "attn4"
         else:
             parts = u("chunks") + u("rows")
