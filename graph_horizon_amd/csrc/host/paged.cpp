@@ -244,12 +244,14 @@ int attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv_pag
             a.least = 2 * (one ? kSpanTiles : std::min(std::max(ceil_div(most, 8ull * b->cus) * 4, 4u), kSpanTiles));
             a.chunks = ceil_div(max_len, 16 * a.least);
         } else {
+            // Teams of up to four waves, a head each, and three workgroups per CU, as many as fit at once (us of a call with two / three /
+            // six of them: 32 rows of up to 4000 41.2 / 40.4 / 40.5; in half as many chunks where those had up to 6 tiles, 8 of up to
+            // 8192 35.1 instead of 33.3)
             a.least = 2;
             t.heads = std::min(hk, 4u);
             t.groups = ceil_div(hk, t.heads);
             t.teams = 4 / t.heads;
             a.chunks = std::max(1u, 3 * b->cus / t.groups) * t.teams;
-            a.solo = 6;
         }
     } else if (split) {
         // about two workgroups per CU, each wave at most 8 tiles (1 row of 9000, in spans of 4 / 12 / 32 / 64 tiles:
@@ -267,6 +269,7 @@ int attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv_pag
     }
     // From half the last-level cache on, the next call will not find this one's K and V there, and reads past
     // it are faster (64 rows of 8192 362 / 324 us, 1 of 32768 33.8 / 31.6; 16 of up to 2500, 83 MB: 26.2 / 32.3).
+    // In 4 bits, of a call: 64 of 8192 155 / 150, 48 of 4000 72.3 / 70.6; 32 of up to 4000, 82 MB: 40.0 / 41.6.
     a.stream = kStreamBytes;
     // scratch of a row: its partials, and with scores each query head's
     const uint64_t acc = (uint64_t)q_heads * 512, ml = acc / 64, raw = scored ? (uint64_t)q_heads * a.raw_len * 4 : 0;

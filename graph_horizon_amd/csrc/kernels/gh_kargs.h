@@ -370,7 +370,7 @@ struct GhPagedAttnArgs {
 
 // gh_paged4_attn: workgroups of 4 waves, `teams` teams of `heads` each, which have a chunk and a wave per kv head; the kv heads
 // are in `groups` groups of so many. Workgroups i and i + 8, .. i + 8 (groups - 1) have the groups of the same chunks, so that they
-// run on one XCD and share the lines in which two groups' heads meet.
+// run on one XCD and share the lines in which two groups' heads meet. Chunks share the tiles out to one each, and have `least` or more.
 struct GhPaged4AttnArgs {
     GhPagedAttnArgs a;
     uint32_t heads;

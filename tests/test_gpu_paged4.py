@@ -56,6 +56,7 @@ def test_attention(hip, rng, name, page, heads, group, scored):
     ([700] * 70 + [0, 3000, 5], 16, 8, 200),   # chunks over more than 64 rows
     ([4000, 0, 3100, 2999, 17, 1024] * 3, 32, 8, 130),  # chunks over few
     ([12345, 5000], 64, 8, 200),
+    ([12345, 5000, 20], 64, 8, 2000),
 ])
 def test_attention_in_chunks(hip, rng, lengths, page, heads, width, scored):
     p = Paged4(hip, rng, lengths, page, heads, width=width, scored=scored)
@@ -69,7 +70,7 @@ def test_attention_in_chunks(hip, rng, lengths, page, heads, width, scored):
 def test_attention_in_chunks_of_any_number_of_heads(hip, rng, heads, group):
     """Teams of one to four waves, with and without waves over; a pool whose rows of all heads end off 128 bytes."""
     lengths = [int(n) for n in rng.integers(0, 400, 30)] + [2000, 0, 33]
-    p = Paged4(hip, rng, lengths, 16, heads, width=8 * 1024 // 16, scored=heads % 2 == 1)
+    p = Paged4(hip, rng, lengths, 16, heads, width=16 * 1024 // 16, scored=heads % 2 == 1)
     before = p.read("score") if p.score is not None else None
     q, out = run_attention(hip, p, heads * group, rng)
     check_attention4(p, 0, q, out, before, None if before is None else p.read("score"))
