@@ -276,14 +276,22 @@ struct Query {
     ph8 x[4];
     ph4 sums, step[4];
 };
-__device__ __forceinline__ void load_q4(const GhPagedAttnArgs& a, uint32_t row, uint32_t kvh, Query& q) {
+struct RawQuery {
+    uint4 x[4];
+};
+__device__ __forceinline__ void ask_q4(const GhPagedAttnArgs& a, uint32_t row, uint32_t kvh, RawQuery& r) {
     const uint32_t lane = threadIdx.x & 63u, n = lane & 15u, g = lane >> 4, G = a.group;
     const GH_GLOBAL uint4* qp = gh_gp<uint4>(a.q + (((uint64_t)row * a.q_heads + kvh * G + min(n, G - 1)) * 128 + 8 * g) * 2);
+#pragma unroll
+    for (uint32_t s = 0; s < 4; ++s) r.x[s] = qp[4 * s];
+}
+__device__ __forceinline__ void make_q4(const GhPagedAttnArgs& a, const RawQuery& r, Query& q) {
+    const uint32_t lane = threadIdx.x & 63u, n = lane & 15u, g = lane >> 4, G = a.group;
     const ph2 down = {(_Float16)0.0625f, (_Float16)0.0625f};
     float mine = 0.0f;
 #pragma unroll
     for (uint32_t s = 0; s < 4; ++s) {
-        uint4 x = qp[4 * s];
+        uint4 x = r.x[s];
         if (n >= G) x = make_uint4(0u, 0u, 0u, 0u);
         float v[8];
         gh_unpack8(x, v);
@@ -487,13 +495,14 @@ __device__ __forceinline__ void paged4_chunk(const GhPagedAttnArgs& a, const Row
         row = info & 0xFFFFu;
         since = i;
         x.clear();
-        load_q4(a, row, kvh, q);
+        RawQuery rq;
+        ask_q4(a, row, kvh, rq);
+        make_q4(a, rq, q);
         if (SCORED) raw = a.raw + (((uint64_t)row * a.p.kv_heads + kvh) * G + n) * a.raw_len * 4;
     };
-    if (there && tiles) start(__builtin_amdgcn_readlane(t_row, 0), 0);
-
     Tile4 r;
     load_tile<CACHE>(where(0), pieces, r);
+    if (there && tiles) start(__builtin_amdgcn_readlane(t_row, 0), 0);
     for (uint32_t i = 0; i < rounds; ++i) {
         const uint32_t info = __builtin_amdgcn_readlane(t_row, i & 63u);
         const uint32_t pos = SCORED ? __builtin_amdgcn_readlane(t_pos, i & 63u) : 0u;
@@ -577,6 +586,8 @@ __device__ __forceinline__ void paged4_split(const GhPagedAttnArgs& a) {
     const uint32_t span = a.least * 16, begin = split * span;  // < max_len
     // the wave's tile i covers positions begin + 128 i + 32 wave .. + 32
     const uint32_t first = begin + 32 * wave, mine = first + 128 * lane;
+    RawQuery rq;
+    ask_q4(a, row, kvh, rq);
     const uint32_t len = row_length(a.p, row, a.max_len, kvh == 0 && split == 0);
     if (len == 0) {
         if (split == 0)
@@ -584,8 +595,6 @@ __device__ __forceinline__ void paged4_split(const GhPagedAttnArgs& a) {
         return;
     }
     if (begin >= len) return;
-    Query q;
-    load_q4(a, row, kvh, q);
     const float scale = a.scale * 512.0f;
     const uint32_t end = min(len, begin + span);
     uint32_t t_slot0 = 0, t_slot1 = 0, t_count = 0;
@@ -607,6 +616,8 @@ __device__ __forceinline__ void paged4_split(const GhPagedAttnArgs& a) {
         char* lds = stage[wave];
         Tile4 r;
         load_tile<0>(where(0), pieces, r);
+        Query q;
+        make_q4(a, rq, q);
         for (uint32_t i = 0; i < tiles; ++i) {
             wave_order();
             store_tile(r, pieces, lds);
