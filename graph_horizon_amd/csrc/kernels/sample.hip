@@ -7,13 +7,16 @@
 // running counts and sums. Sums are of whole numbers, w in fixed point: the same in any order, and off by 2^-46 at a
 // vocabulary of 2^17, so that what lies next to a border of the kept or drawn range falls where 64 bits put it.
 //
-// Four launches; a row's logits are read three times, from memory once:
-//   gh_sample_max     the largest logit of each chunk of a row;
+// Four launches; a row's logits are read three times, from memory once (us of 1 / 8 / 64 rows of 131072):
+//   gh_sample_max     the largest logit of each chunk of a row (3.8 / 4.2 / 10.2; 34 MB of 64 rows);
 //   gh_sample_bins    counts and sums over 1024 bins of the distance d = M - l, 64 per octave from 2^-9 to 2^7, so
-//                     that a bin holds at most 3 % of any smooth distribution whatever its spread;
+//                     that a bin holds at most 3 % of any smooth distribution whatever its spread (5.6 / 6.9 / 13.9: three
+//                     LDS operations a token, two of them atomic; a cheaper exponential, or fewer and larger workgroups, change nothing);
 //   gh_sample_collect the tokens of the bins in which a search can end: the running sums up to the bins are known, and
-//                     bound the top-k sum, then the kept sum, then the draw's target;
-//   gh_sample_pick    searches these tokens, or, where they are more than the list takes, the row itself.
+//                     bound the top-k sum, then the kept sum, then the draw's target (7.5 / 8.5 / 11.6);
+//   gh_sample_pick    searches these tokens, or, where they are more than the list takes, the row itself: one wave where they
+//                     are 64 or fewer, else a workgroup (5.5 / 14.8 / 13.2; from memory without gh_sample_collect, 1 row: 23.3).
+// Chains of dependent loads and barriers bound the launches of few rows.
 // What the device cannot trust is only the settings: any bits give a token of the row.
 #include "gh_wave64.h"
 
