@@ -453,7 +453,8 @@ __device__ __forceinline__ Hit search(const GhSampleArgs& a, const Row& r, const
     auto inside = [&](uint64_t key) __attribute__((always_inline)) {
         return key >= lo && key <= hi && bin_of(r.top - value_of(key)) == bin && (tenth == kNone || ten(key) == tenth);
     };
-    while (n > 64) {
+    // (eight rounds narrow any range of keys to one: a bound for logits that another stream changes meanwhile)
+    for (uint32_t round = 0; n > 64 && round < 8; ++round) {
         uint32_t shift = 0;
         q.sum[tid] = 0;
         q.count[tid] = 0;

@@ -4,7 +4,7 @@ import threading
 import numpy as np
 import pytest
 
-from graph_horizon_amd import GhError, HipBackend, HipModel, Yarn, synth
+from graph_horizon_amd import GhError, GhKvPaged, HipBackend, HipModel, Yarn, synth
 from graph_horizon_amd import _ffi as F
 from paged import D, keep
 from paged4 import Paged4, check_attention4, pack, unpack
@@ -351,6 +351,49 @@ def test_norm_write_beyond_fp16(hip, rng):
     for b in (wb, kb, pb, qb):
         hip.free_buffer(b)
     p.free()
+
+
+@pytest.mark.parametrize("lengths,width", [([40, 300, 77], None), ([5000, 40, 3000, 17], 1200)])  # spans, chunks
+def test_a_query_that_is_not_finite_is_its_own(hip, rng, lengths, width):
+    heads, group = 4, 3
+    p = Paged4(hip, rng, lengths, 16, heads, width=width)
+    q = rng.standard_normal((len(lengths), heads * group, D)).astype(np.float16)
+    plain = run_attention(hip, p, heads * group, rng, q=q)[1]
+    q[0, 1, 5], q[1, 7, 100], q[2, 11, 64] = np.nan, np.inf, -np.inf
+    out = run_attention(hip, p, heads * group, rng, q=q)[1]
+    bad = np.zeros(q.shape[:2], bool)
+    bad[0, 1] = bad[1, 7] = bad[2, 11] = True
+    assert np.array_equal(np.isnan(out).any(-1), bad)
+    assert np.array_equal(out[~bad].view(np.uint16), plain[~bad].view(np.uint16))
+    p.free()
+
+
+def test_append_and_read_back_past_4_gib(hip, rng):
+    """Pages whose byte offsets pass 32 bits (a pool of 4.5 GiB each for K and V); evicted from one to another of these."""
+    page, heads = 64, 8
+    slots = (9 << 29) // (80 * heads) // page * page
+    kc, vc = (hip.alloc_buffer(slots * heads * 80) for _ in range(2))
+    last = slots // page - 1
+    table, other = hip.from_host(np.array([[last, last - 1]], np.uint32)), hip.from_host(np.array([[last - 7, last - 5]], np.uint32))
+    lengths, score = hip.from_host(np.array([100], np.uint32)), hip.from_host(rng.random((1, 1, heads, 2 * page)).astype(np.float32))
+    kv = F.GhKv(kc, vc, F.KV_Q4, 1, slots, heads, D, D)
+    k, v = (rng.standard_normal((1, 100, heads, D)).astype(np.float16) for _ in range(2))
+    kb, vb = hip.from_host(k), hip.from_host(v)
+    rows = [GhKvPaged(kv, t, lengths, score, page, 2, 1) for t in (table, other)]
+    hip.kv_write_paged(rows[0], kb, vb, 100, 0)
+    weight = rng.random((1, 1, heads, 2 * page)).astype(np.float32)
+    hip.upload(score, weight)
+    hip.kv_read_paged(kb, vb, rows[0], 100, 0)
+    for b, x in ((kb, k), (vb, v)):
+        assert np.array_equal(hip.download(b, np.float16, x.size).reshape(x.shape), unpack(pack(x)))
+    hip.kv_evict_paged(rows[1], rows[0], None, 70, 20)
+    hip.kv_read_paged(kb, vb, rows[1], 70, 0)
+    for b, x in ((kb, k), (vb, v)):
+        got = hip.download(b, np.float16, 70 * heads * D).reshape(70, heads, D)
+        for h in range(heads):
+            assert np.array_equal(got[:, h], unpack(pack(x[0, keep(weight[0, 0, h, :100], 70, 20), h])))
+    for b in (kc, vc, table, other, lengths, score, kb, vb):
+        hip.free_buffer(b)
 
 
 # ---- sampling ----
