@@ -114,7 +114,7 @@ int gh_sample_rows(gh_backend* b, gh_encoder* enc, const gh_buf* tokens, const g
             rc = launch(b, K_SAMPLE_MAX, a.chunks, n, 1, 256, &a);
             if (!rc) rc = launch(b, K_SAMPLE_BINS, a.chunks, n, 1, 256, &a);
             if (!rc) rc = launch(b, K_SAMPLE_COLLECT, a.chunks, n, 1, 256, &a);
-            if (!rc) rc = launch(b, K_SAMPLE_PICK, n, 1, 1, 1024, &a);
+            if (!rc) rc = launch(b, K_SAMPLE_PICK, n, 1, 1, GH_SAMPLE_PICK, &a);
             if (rc) return rc;
         }
         return rc;

@@ -15,7 +15,8 @@
 //   gh_sample_collect the tokens of the bins in which a search can end: the running sums up to the bins are known, and
 //                     bound the top-k sum, then the kept sum, then the draw's target (7.5 / 8.5 / 11.6);
 //   gh_sample_pick    searches these tokens, or, where they are more than the list takes, the row itself: one wave where they
-//                     are 64 or fewer, else a workgroup (5.5 / 14.8 / 13.2; from memory without gh_sample_collect, 1 row: 23.3).
+//                     are 64 or fewer, else a workgroup (4.7 / 14.9 / 12.6, with 1024 threads 5.6 / 14.0 / 12.3; from memory without
+//                     gh_sample_collect, 1 row: 23.3).
 // Chains of dependent loads and barriers bound the launches of few rows.
 // What the device cannot trust is only the settings: any bits give a token of the row.
 #include "gh_wave64.h"
@@ -391,7 +392,7 @@ GH_KERNEL __launch_bounds__(256) void gh_sample_collect(GhSampleArgs a) {
 }
 
 namespace {
-constexpr uint32_t kPick = 1024;  // threads, a bin each
+constexpr uint32_t kPick = GH_SAMPLE_PICK, kPickWaves = kPick / 64, kPickBins = kBins / kPick;  // threads, their waves, bins of a thread
 // A token found by its running values: its key, and the count and sum up to and with it.
 struct Hit {
     uint64_t key, sum;
@@ -434,14 +435,20 @@ struct Whole {
 
 // The first token in rank order up to which count and sum satisfy `is`, which some token's do and stays true once it is. Its bin
 // by the running values of the bins; then, while there are more than 64 tokens, in which 1024th of them it is, first by the next ten
-// bits of their distance, then by parts of the range of their keys; then among these, sorted by one wave.
+// bits of their distance, then by parts of the range of their keys; then among these, by one wave.
 template <class S, class F>
 __device__ __forceinline__ Hit search(const GhSampleArgs& a, const Row& r, const double* table, const PlanLds& s, PickLds& q, const S& source, F is) {
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
     __syncthreads();
     if (tid == 0) q.found = kBins - 1;
     __syncthreads();
-    if (is(s.count[tid], s.sum[tid]) && (tid == 0 || !is(s.count[tid - 1], s.sum[tid - 1]))) q.found = tid;
+    const uint32_t mine = tid * kPickBins;  // the thread's bins, or parts of a range
+    if (is(s.count[mine + kPickBins - 1], s.sum[mine + kPickBins - 1]) && (tid == 0 || !is(s.count[mine - 1], s.sum[mine - 1]))) {
+        uint32_t b = mine;
+#pragma unroll
+        for (uint32_t j = 0; j + 1 < kPickBins; ++j) b += b == mine + j && !is(s.count[b], s.sum[b]);
+        q.found = b;
+    }
     __syncthreads();
     const uint32_t bin = q.found;
     uint64_t sum = before(s, bin), lo = 0, hi = ~0ull;
@@ -456,8 +463,11 @@ __device__ __forceinline__ Hit search(const GhSampleArgs& a, const Row& r, const
     // (eight rounds narrow any range of keys to one: a bound for logits that another stream changes meanwhile)
     for (uint32_t round = 0; n > 64 && round < 8; ++round) {
         uint32_t shift = 0;
-        q.sum[tid] = 0;
-        q.count[tid] = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < kPickBins; ++j) {
+            q.sum[tid + kPick * j] = 0;
+            q.count[tid + kPick * j] = 0;
+        }
         if (tid == 0) q.found = kBins - 1;
         if (!bits) {
             uint64_t least = ~0ull, most = 0;
@@ -473,7 +483,7 @@ __device__ __forceinline__ Hit search(const GhSampleArgs& a, const Row& r, const
                 q.hi[wave] = most;
             }
             __syncthreads();
-            for (uint32_t i = 0; i < 16; ++i) {
+            for (uint32_t i = 0; i < kPickWaves; ++i) {
                 least = min(least, q.lo[i]);
                 most = max(most, q.hi[i]);
             }
@@ -491,24 +501,37 @@ __device__ __forceinline__ Hit search(const GhSampleArgs& a, const Row& r, const
             atomicAdd((unsigned long long*)&q.sum[part], (unsigned long long)fixed(a, r, table, value_of(key)));
         });
         __syncthreads();
-        const uint64_t w = gh_scan64(q.sum[tid]);
-        const uint32_t c = (uint32_t)gh_scan64(q.count[tid]);
+        uint64_t ws[kPickBins], wall = 0;
+        uint32_t cs[kPickBins], call = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < kPickBins; ++j) {
+            wall += ws[j] = q.sum[mine + j];
+            call += cs[j] = q.count[mine + j];
+        }
+        const uint64_t w = gh_scan64(wall);
+        const uint32_t c = (uint32_t)gh_scan64(call);
         if (lane == 63) {
             q.wave_sum[wave] = w;
             q.wave_count[wave] = c;
         }
         __syncthreads();
-        uint64_t w0 = sum + w - q.sum[tid];
-        uint32_t c0 = count + c - q.count[tid];
-        for (uint32_t i = 0; i < wave; ++i) {
-            w0 += q.wave_sum[i];
-            c0 += q.wave_count[i];
+        uint64_t w0 = sum + w - wall;
+        uint32_t c0 = count + c - call;
+#pragma unroll
+        for (uint32_t i = 0; i + 1 < kPickWaves; ++i) {
+            w0 += i < wave ? q.wave_sum[i] : 0;
+            c0 += i < wave ? q.wave_count[i] : 0;
         }
         // one part: the first of those that hold a token and end where `is` is true
-        if (q.count[tid] && is(c0 + q.count[tid], w0 + q.sum[tid]) && !(c0 > count && is(c0, w0))) {
-            q.found = tid;
-            q.hit.sum = w0;
-            q.hit.count = c0;
+#pragma unroll
+        for (uint32_t j = 0; j < kPickBins; ++j) {
+            if (cs[j] && is(c0 + cs[j], w0 + ws[j]) && !(c0 > count && is(c0, w0))) {
+                q.found = mine + j;
+                q.hit.sum = w0;
+                q.hit.count = c0;
+            }
+            w0 += ws[j];
+            c0 += cs[j];
         }
         __syncthreads();
         const uint32_t part = q.found;
@@ -533,11 +556,19 @@ __device__ __forceinline__ Hit search(const GhSampleArgs& a, const Row& r, const
     });
     __syncthreads();
     if (wave == 0) {
-        const uint64_t key = gh_sort64(lane < q.fill ? q.few[lane] : ~0ull);
-        const uint64_t w = sum + gh_scan64(lane < q.fill ? fixed(a, r, table, value_of(key)) : 0);
-        const uint64_t good = __ballot(lane < q.fill && is(count + lane + 1, w));
-        const uint32_t at = good ? (uint32_t)__builtin_ctzll(good) : min(q.fill, 64u) - 1;
-        if (lane == at) q.hit = Hit{key, w, count + lane + 1};
+        // each lane's token against all of them, which are few
+        const uint32_t all = min(q.fill, 64u);
+        const uint64_t key = lane < all ? q.few[lane] : ~0ull, w = lane < all ? fixed(a, r, table, value_of(key)) : 0;
+        uint64_t upto = sum;
+        uint32_t rank = count;
+        for (uint32_t i = 0; i < all; ++i) {
+            const bool first = gh_lane64(key, i) <= key;
+            upto += first ? gh_lane64(w, i) : 0;
+            rank += first;
+        }
+        const bool ends = is(rank, upto) && (rank == count + 1 || !is(rank - 1, upto - w));
+        const uint64_t good = __ballot(lane < all && ends), last = __ballot(lane < all && rank == count + all);
+        if (lane == (uint32_t)__builtin_ctzll(good ? good : last | 1ull << 63)) q.hit = Hit{key, upto, rank};
     }
     __syncthreads();
     return q.hit;
@@ -579,7 +610,7 @@ __device__ __forceinline__ uint32_t pick_by_search(const GhSampleArgs& a, const 
         __syncthreads();
         uint64_t to = before(s, p.m0);
         uint32_t rank = count_before(s, p.m0);
-        for (uint32_t i = 0; i < 16; ++i) {
+        for (uint32_t i = 0; i < kPickWaves; ++i) {
             to += q.wave_sum[i];
             rank += q.wave_count[i];
         }
@@ -653,8 +684,8 @@ __device__ __forceinline__ uint32_t pick_by_wave(const GhSampleArgs& a, const Ro
 }
 }  // namespace
 
-// Grid (rows), 1024 threads.
-GH_KERNEL __launch_bounds__(1024) void gh_sample_pick(GhSampleArgs a) {
+// Grid (rows), kPick threads.
+GH_KERNEL __launch_bounds__(kPick) void gh_sample_pick(GhSampleArgs a) {
     __shared__ PlanLds s;
     __shared__ PickLds q;
     __shared__ double table[64];
