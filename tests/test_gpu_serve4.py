@@ -409,6 +409,19 @@ def test_min_p_at_high_temperatures(hip, rng, temperature):
             check(hip, logits, params, [u] * 4)
 
 
+@pytest.mark.parametrize("vocab", [700, 5003, 40001])
+def test_any_settings(hip, rng, vocab):
+    """Rows of all spreads, with ties and masked tokens, each with settings of its own."""
+    rows = 120
+    logits = (10 ** rng.uniform(-3, 2, (rows, 1)) * rng.standard_normal((rows, vocab)) + rng.uniform(-50, 50, (rows, 1))).astype(np.float32)
+    logits[::5] = np.round(logits[::5])
+    logits[1::7, rng.integers(0, vocab, vocab // 2)] = -np.inf
+    params = [(float(10 ** rng.uniform(-2, 1.5)), float(rng.choice([1.0, rng.random(), 0.999, 1e-4])),
+               int(rng.choice([0, rng.integers(1, vocab + 5), rng.integers(1, 60)])), float(rng.choice([0.0, rng.random(), 1e-5])))
+              for _ in range(rows)]
+    check(hip, logits, params, rng.random(rows).astype(np.float32), stride=vocab + 3)
+
+
 def test_largest_vocabulary(hip, rng):
     vocab = 1 << 24
     logits = (2 * rng.standard_normal((2, vocab))).astype(np.float32)
