@@ -273,7 +273,7 @@ struct GhArgmaxArgs {
 // index, largest finite one's order) u64 x 2 [64]; bins u64 sums, u32 counts [GH_SAMPLE_BINS], u32 length of the list; list.
 #define GH_SAMPLE_BINS 1024u
 #define GH_SAMPLE_LIST 8192u
-#define GH_SAMPLE_PICK 512u    // threads of gh_sample_pick
+#define GH_SAMPLE_PICK 1024u   // threads of gh_sample_pick
 #define GH_SAMPLE_BIN_BYTES (GH_SAMPLE_BINS * 12u + 16u)
 #define GH_SAMPLE_ROW_BYTES (64u * 16u + GH_SAMPLE_BIN_BYTES + GH_SAMPLE_LIST * 8u)
 struct GhSampleArgs {

@@ -15,8 +15,8 @@
 //   gh_sample_collect the tokens of the bins in which a search can end: the running sums up to the bins are known, and
 //                     bound the top-k sum, then the kept sum, then the draw's target (7.5 / 8.5 / 11.6);
 //   gh_sample_pick    searches these tokens, or, where they are more than the list takes, the row itself: one wave where they
-//                     are 64 or fewer, else a workgroup (4.7 / 14.9 / 12.6, with 1024 threads 5.6 / 14.0 / 12.3; from memory without
-//                     gh_sample_collect, 1 row: 23.3).
+//                     are 64 or fewer, else a workgroup of 16 waves, half of which look at the bins (4.8 / 12.8 / 10.9; all of
+//                     them 5.6 / 14.0 / 12.3, 8 waves in all 4.7 / 14.9 / 12.6; from memory without gh_sample_collect, 1 row: 23.3).
 // Chains of dependent loads and barriers bound the launches of few rows.
 // What the device cannot trust is only the settings: any bits give a token of the row.
 #include "gh_wave64.h"
@@ -242,52 +242,61 @@ struct PlanLds {
 __device__ __forceinline__ uint64_t before(const PlanLds& s, uint32_t b) { return b ? s.sum[b - 1] : 0; }
 __device__ __forceinline__ uint32_t count_before(const PlanLds& s, uint32_t b) { return b ? s.count[b - 1] : 0; }
 
-// All threads get the same plan. u64 sums are compared as doubles, as the searches compare them.
-template <uint32_t THREADS>
+// All threads of the workgroup get the same plan; the first THREADS look at the bins (of 16 waves, which take 16 cycles for
+// an instruction, half). u64 sums are compared as doubles, as the searches compare them.
+template <uint32_t THREADS, uint32_t ALL>
 __device__ __forceinline__ Plan plan_of(const GhSampleArgs& a, const Row& r, uint32_t row, PlanLds& s) {
     constexpr uint32_t kEach = kBins / THREADS, kWaves = THREADS / 64;  // bins of a thread, in a row
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
     const uint64_t bins = a.bins + (uint64_t)row * GH_SAMPLE_BIN_BYTES;
-    uint64_t w[kEach];
-    uint32_t c[kEach];
+    const bool looks = THREADS == ALL || tid < THREADS;
+    uint64_t w[kEach], wu = 0;
+    uint32_t c[kEach], own[kEach], cu = 0;  // own: the bins' counts
+    if (looks) {
 #pragma unroll
-    for (uint32_t j = 0; j < kEach; ++j) {
-        w[j] = gh_gp<uint64_t>(bins)[tid * kEach + j];
-        c[j] = gh_gp<uint32_t>(bins + kBins * 8)[tid * kEach + j];
-    }
-    uint32_t own[kEach];  // the bins' counts
+        for (uint32_t j = 0; j < kEach; ++j) {
+            w[j] = gh_gp<uint64_t>(bins)[tid * kEach + j];
+            c[j] = gh_gp<uint32_t>(bins + kBins * 8)[tid * kEach + j];
+        }
 #pragma unroll
-    for (uint32_t j = 0; j < kEach; ++j) own[j] = c[j];
+        for (uint32_t j = 0; j < kEach; ++j) own[j] = c[j];
 #pragma unroll
-    for (uint32_t j = 1; j < kEach; ++j) {
-        w[j] += w[j - 1];
-        c[j] += c[j - 1];
+        for (uint32_t j = 1; j < kEach; ++j) {
+            w[j] += w[j - 1];
+            c[j] += c[j - 1];
+        }
+        wu = gh_scan64(w[kEach - 1]);
+        cu = (uint32_t)gh_scan64(c[kEach - 1]);
+        if (lane == 63) {
+            s.wave_sum[wave] = wu;
+            s.wave_count[wave] = cu;
+        }
+        if (tid < 5) s.found[tid] = kBins - 1;
     }
-    const uint64_t wu = gh_scan64(w[kEach - 1]), cu = gh_scan64(c[kEach - 1]);
-    if (lane == 63) {
-        s.wave_sum[wave] = wu;
-        s.wave_count[wave] = (uint32_t)cu;
-    }
-    if (tid < 5) s.found[tid] = kBins - 1;
     __syncthreads();
-    uint64_t w0 = wu - w[kEach - 1];          // before the thread's bins
-    uint32_t c0 = (uint32_t)cu - c[kEach - 1];
     Plan p;
     p.tokens = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < kWaves; ++i) {
-        w0 += i < wave ? s.wave_sum[i] : 0;
-        c0 += i < wave ? s.wave_count[i] : 0;
-        p.tokens += s.wave_count[i];
-    }
+    for (uint32_t i = 0; i < kWaves; ++i) p.tokens += s.wave_count[i];
+    uint64_t w0 = 0;  // before the thread's bins
+    uint32_t c0 = 0;
+    if (looks) {
+        w0 = wu - w[kEach - 1];
+        c0 = cu - c[kEach - 1];
 #pragma unroll
-    for (uint32_t j = 0; j < kEach; ++j) {
-        s.sum[tid * kEach + j] = w[j] += w0;
-        s.count[tid * kEach + j] = c[j] += c0;
+        for (uint32_t i = 0; i < kWaves; ++i) {
+            w0 += i < wave ? s.wave_sum[i] : 0;
+            c0 += i < wave ? s.wave_count[i] : 0;
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kEach; ++j) {
+            s.sum[tid * kEach + j] = w[j] += w0;
+            s.count[tid * kEach + j] = c[j] += c0;
+        }
     }
     // The first bin up to which the running values satisfy `is`, which stays true once it is: one thread has it.
     auto first_bin = [&](uint32_t slot, auto is) __attribute__((always_inline)) {
-        if (!is(c[kEach - 1], w[kEach - 1]) || (tid && is(c0, w0))) return;
+        if (!looks || !is(c[kEach - 1], w[kEach - 1]) || (tid && is(c0, w0))) return;
         uint32_t j = 0;
 #pragma unroll
         for (uint32_t i = 0; i + 1 < kEach; ++i) j += j == i && !is(c[i], w[i]);
@@ -327,11 +336,13 @@ __device__ __forceinline__ Plan plan_of(const GhSampleArgs& a, const Row& r, uin
     __syncthreads();
     p.d0 = min(s.found[3], l1);
     p.d1 = min(s.found[4], l1);
-    uint32_t listed = 0;
+    if (looks) {
+        uint32_t listed = 0;
 #pragma unroll
-    for (uint32_t j = 0; j < kEach; ++j) listed += p.has(tid * kEach + j) ? own[j] : 0u;
-    listed = (uint32_t)gh_scan64(listed);
-    if (lane == 63) s.wave_listed[wave] = listed;
+        for (uint32_t j = 0; j < kEach; ++j) listed += p.has(tid * kEach + j) ? own[j] : 0u;
+        listed = (uint32_t)gh_scan64(listed);
+        if (lane == 63) s.wave_listed[wave] = listed;
+    }
     __syncthreads();
     p.listed = 0;
 #pragma unroll
@@ -349,7 +360,7 @@ GH_KERNEL __launch_bounds__(256) void gh_sample_collect(GhSampleArgs a) {
     load_block<256>(a, row, first, end, v);
     const Row r = row_of(a, row);
     if (r.greedy) return;
-    const Plan p = plan_of<256>(a, r, row, s);
+    const Plan p = plan_of<256, 256>(a, r, row, s);
     if (p.listed > kList) return;
 #pragma unroll
     for (uint32_t j = 0; j < kBins / 256; ++j) {
@@ -392,7 +403,8 @@ GH_KERNEL __launch_bounds__(256) void gh_sample_collect(GhSampleArgs a) {
 }
 
 namespace {
-constexpr uint32_t kPick = GH_SAMPLE_PICK, kPickWaves = kPick / 64, kPickBins = kBins / kPick;  // threads, their waves, bins of a thread
+// Threads, their waves; those that look at bins, their waves, bins of each.
+constexpr uint32_t kPick = GH_SAMPLE_PICK, kPickWaves = kPick / 64, kLook = 512, kLookWaves = kLook / 64, kLookBins = kBins / kLook;
 // A token found by its running values: its key, and the count and sum up to and with it.
 struct Hit {
     uint64_t key, sum;
@@ -442,11 +454,12 @@ __device__ __forceinline__ Hit search(const GhSampleArgs& a, const Row& r, const
     __syncthreads();
     if (tid == 0) q.found = kBins - 1;
     __syncthreads();
-    const uint32_t mine = tid * kPickBins;  // the thread's bins, or parts of a range
-    if (is(s.count[mine + kPickBins - 1], s.sum[mine + kPickBins - 1]) && (tid == 0 || !is(s.count[mine - 1], s.sum[mine - 1]))) {
+    const bool looks = tid < kLook;
+    const uint32_t mine = tid * kLookBins;  // the thread's bins, or parts of a range
+    if (looks && is(s.count[mine + kLookBins - 1], s.sum[mine + kLookBins - 1]) && (tid == 0 || !is(s.count[mine - 1], s.sum[mine - 1]))) {
         uint32_t b = mine;
 #pragma unroll
-        for (uint32_t j = 0; j + 1 < kPickBins; ++j) b += b == mine + j && !is(s.count[b], s.sum[b]);
+        for (uint32_t j = 0; j + 1 < kLookBins; ++j) b += b == mine + j && !is(s.count[b], s.sum[b]);
         q.found = b;
     }
     __syncthreads();
@@ -463,10 +476,9 @@ __device__ __forceinline__ Hit search(const GhSampleArgs& a, const Row& r, const
     // (eight rounds narrow any range of keys to one: a bound for logits that another stream changes meanwhile)
     for (uint32_t round = 0; n > 64 && round < 8; ++round) {
         uint32_t shift = 0;
-#pragma unroll
-        for (uint32_t j = 0; j < kPickBins; ++j) {
-            q.sum[tid + kPick * j] = 0;
-            q.count[tid + kPick * j] = 0;
+        for (uint32_t i = tid; i < kBins; i += kPick) {
+            q.sum[i] = 0;
+            q.count[i] = 0;
         }
         if (tid == 0) q.found = kBins - 1;
         if (!bits) {
@@ -501,37 +513,41 @@ __device__ __forceinline__ Hit search(const GhSampleArgs& a, const Row& r, const
             atomicAdd((unsigned long long*)&q.sum[part], (unsigned long long)fixed(a, r, table, value_of(key)));
         });
         __syncthreads();
-        uint64_t ws[kPickBins], wall = 0;
-        uint32_t cs[kPickBins], call = 0;
+        uint64_t ws[kLookBins], wall = 0, w = 0;
+        uint32_t cs[kLookBins], call = 0, c = 0;
+        if (looks) {
 #pragma unroll
-        for (uint32_t j = 0; j < kPickBins; ++j) {
-            wall += ws[j] = q.sum[mine + j];
-            call += cs[j] = q.count[mine + j];
-        }
-        const uint64_t w = gh_scan64(wall);
-        const uint32_t c = (uint32_t)gh_scan64(call);
-        if (lane == 63) {
-            q.wave_sum[wave] = w;
-            q.wave_count[wave] = c;
+            for (uint32_t j = 0; j < kLookBins; ++j) {
+                wall += ws[j] = q.sum[mine + j];
+                call += cs[j] = q.count[mine + j];
+            }
+            w = gh_scan64(wall);
+            c = (uint32_t)gh_scan64(call);
+            if (lane == 63) {
+                q.wave_sum[wave] = w;
+                q.wave_count[wave] = c;
+            }
         }
         __syncthreads();
-        uint64_t w0 = sum + w - wall;
-        uint32_t c0 = count + c - call;
+        if (looks) {
+            uint64_t w0 = sum + w - wall;
+            uint32_t c0 = count + c - call;
 #pragma unroll
-        for (uint32_t i = 0; i + 1 < kPickWaves; ++i) {
-            w0 += i < wave ? q.wave_sum[i] : 0;
-            c0 += i < wave ? q.wave_count[i] : 0;
-        }
-        // one part: the first of those that hold a token and end where `is` is true
-#pragma unroll
-        for (uint32_t j = 0; j < kPickBins; ++j) {
-            if (cs[j] && is(c0 + cs[j], w0 + ws[j]) && !(c0 > count && is(c0, w0))) {
-                q.found = mine + j;
-                q.hit.sum = w0;
-                q.hit.count = c0;
+            for (uint32_t i = 0; i + 1 < kLookWaves; ++i) {
+                w0 += i < wave ? q.wave_sum[i] : 0;
+                c0 += i < wave ? q.wave_count[i] : 0;
             }
-            w0 += ws[j];
-            c0 += cs[j];
+            // one part: the first of those that hold a token and end where `is` is true
+#pragma unroll
+            for (uint32_t j = 0; j < kLookBins; ++j) {
+                if (cs[j] && is(c0 + cs[j], w0 + ws[j]) && !(c0 > count && is(c0, w0))) {
+                    q.found = mine + j;
+                    q.hit.sum = w0;
+                    q.hit.count = c0;
+                }
+                w0 += ws[j];
+                c0 += cs[j];
+            }
         }
         __syncthreads();
         const uint32_t part = q.found;
@@ -703,7 +719,7 @@ GH_KERNEL __launch_bounds__(kPick) void gh_sample_pick(GhSampleArgs a) {
     const uint64_t list = a.list + (uint64_t)row * kList * 8;
     uint64_t key = ~0ull;
     if (tid < 64) key = gh_gp<uint64_t>(list)[tid];  // on its way while the plan is made
-    const Plan p = plan_of<kPick>(a, r, row, s);
+    const Plan p = plan_of<kLook, kPick>(a, r, row, s);
     double prob;
     uint32_t token;
     if (p.listed <= 64) {
