@@ -57,6 +57,9 @@ def test_attention(hip, rng, name, page, heads, group, scored):
     ([4000, 0, 3100, 2999, 17, 1024] * 3, 32, 8, 130),  # chunks over few
     ([12345, 5000], 64, 8, 200),
     ([12345, 5000, 20], 64, 8, 2000),
+    ([0] * 70, 16, 8, 300),                    # nothing in them
+    ([0] * 20 + [1] + [0] * 30, 16, 8, 300),
+    ([1, 33, 0, 64, 32] * 14, 16, 3, 300),     # as many chunks as tiles allow
 ])
 def test_attention_in_chunks(hip, rng, lengths, page, heads, width, scored):
     p = Paged4(hip, rng, lengths, page, heads, width=width, scored=scored)
