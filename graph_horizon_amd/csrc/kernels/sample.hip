@@ -464,6 +464,7 @@ __device__ __forceinline__ Hit search(const GhSampleArgs& a, const Row& r, const
     }
     __syncthreads();
     const uint32_t bin = q.found;
+    __syncthreads();  // all have read it: the first round below writes it again
     uint64_t sum = before(s, bin), lo = 0, hi = ~0ull;
     uint32_t count = count_before(s, bin), n = s.count[bin] - count;
     // (the first and the last bin hold distances of any exponent)
@@ -579,7 +580,8 @@ __device__ __forceinline__ Hit search(const GhSampleArgs& a, const Row& r, const
         uint32_t rank = count;
         for (uint32_t i = 0; i < all; ++i) {
             const bool first = gh_lane64(key, i) <= key;
-            upto += first ? gh_lane64(w, i) : 0;
+            const uint64_t wi = gh_lane64(w, i);
+            upto += first ? wi : 0;
             rank += first;
         }
         const bool ends = is(rank, upto) && (rank == count + 1 || !is(rank - 1, upto - w));
