@@ -193,7 +193,8 @@ GH_KERNEL __launch_bounds__(256) void gh_paged_read(GhPagedReadArgs a) { paged_r
 // Per half, S^T = K·Q^T with the codes as they are: a nibble in the low bits of an FP16 number is c 2^-24, in the next ones
 // c 2^-20, and the matrix cores take subnormals, so that a mask is all it needs. v_mfma_f32_16x16x32_f16 s (0..3) covers dims
 // 32 s .. + 32, one step and minimum a position: lane l has dims 32 s + 8 (l / 16) .. + 8 of position l % 16, which
-// four row swaps make of the 16 bytes in a row that it reads. The sums are those of exact products in FP32; steps come to
+// four row swaps make of the 16 bytes in a row that it reads. The sums are those of exact products in FP32 (Query says what is held
+// of a query); steps come to
 // the lanes that need them by a product with a unit vector, and the minima's part is one product with the sums of the query over
 // its groups, in FP16 hi + lo. So no key is rounded, for less than the conversion of its codes to FP16 takes.
 // O^T += V^T·P^T per tile: per 8-dim tile t products over the 32 positions: a lane has dims 8 (l % 16) .. + 8, a dword of
@@ -269,12 +270,15 @@ __device__ __forceinline__ void wave_order() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// B fragments of the G queries of a kv head: head n = l % 16 (zero past G). x: dims 32 s + 8 (l / 16) .. + 8 in the order
-// (0, 4), (1, 5), (2, 6), (3, 7), those that meet codes of 2^-20 times 2^-4. sums: 2^-9 of the sum over the dims of group l / 16,
-// hi and lo, in the places of the minima. step: 2^15 in the place of the step of group s.
+// B fragments of the G queries of a kv head: head n = l % 16 (zero past G), times the power of two that brings its largest value
+// to 2^15 or more, so that what follows loses bits of FP16's least steps only far below that. x: dims 32 s + 8 (l / 16) .. + 8 in
+// the order (0, 4), (1, 5), (2, 6), (3, 7), those that meet codes of 2^-20 times 2^-4: exact to 2^-36 of the largest. sums: 2^-9 of
+// the sum over the dims of group l / 16, hi and lo, in the places of the minima: to 2^-22 of it, or 2^-31 of the largest. step: 2^15
+// in the place of the step of group s. scale: what makes products scores in base 2, this power taken out again.
 struct Query {
     ph8 x[4];
     ph4 sums, step[4];
+    float scale;
 };
 struct RawQuery {
     uint4 x[4];
@@ -288,6 +292,21 @@ __device__ __forceinline__ void ask_q4(const GhPagedAttnArgs& a, uint32_t row, u
 __device__ __forceinline__ void make_q4(const GhPagedAttnArgs& a, const RawQuery& r, Query& q) {
     const uint32_t lane = threadIdx.x & 63u, n = lane & 15u, g = lane >> 4, G = a.group;
     const ph2 down = {(_Float16)0.0625f, (_Float16)0.0625f};
+    pu2 top = {0, 0};  // the largest magnitude, as bits
+#pragma unroll
+    for (uint32_t s = 0; s < 4; ++s)
+#pragma unroll
+        for (uint32_t w : {r.x[s].x, r.x[s].y, r.x[s].z, r.x[s].w})
+            top = __builtin_elementwise_max(top, __builtin_bit_cast(pu2, w & 0x7FFF7FFFu));
+    uint32_t largest = top.x > top.y ? top.x : top.y;
+    const auto a16 = __builtin_amdgcn_permlane16_swap(largest, largest, false, false);
+    largest = max(a16[0], a16[1]);
+    const auto a32 = __builtin_amdgcn_permlane32_swap(largest, largest, false, false);
+    largest = max(a32[0], a32[1]);
+    // its exponent, 15 for none: zeros, and infinities and NaN as they are
+    const uint32_t e = largest && largest < 0x7C00u ? __float_as_uint(gh_h2f(largest)) >> 23 : 127u + 15;
+    const float up = __uint_as_float((127u + 127 + 15 - e) << 23);
+    q.scale = a.scale * 512.0f * __uint_as_float((e - 15) << 23);
     float mine = 0.0f;
 #pragma unroll
     for (uint32_t s = 0; s < 4; ++s) {
@@ -295,10 +314,14 @@ __device__ __forceinline__ void make_q4(const GhPagedAttnArgs& a, const RawQuery
         if (n >= G) x = make_uint4(0u, 0u, 0u, 0u);
         float v[8];
         gh_unpack8(x, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= up;
         const float sum = lanes4_sum(((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7])));
         if (s == g) mine = sum;
-        q.x[s] = __builtin_bit_cast(ph8, make_uint4(lows(x.x, x.z), as_u(as_h(highs(x.x, x.z)) * down),
-                                                    lows(x.y, x.w), as_u(as_h(highs(x.y, x.w)) * down)));
+        uint32_t w[4];  // exact
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(v[i], v[i + 4]));
+        q.x[s] = __builtin_bit_cast(ph8, make_uint4(w[0], as_u(as_h(w[1]) * down), w[2], as_u(as_h(w[3]) * down)));
         const uint32_t one = s == g ? 0x7800u : 0u;
         q.step[s] = __builtin_bit_cast(ph4, make_uint2(one, 0u));
     }
@@ -369,7 +392,7 @@ __device__ __forceinline__ void load_v(const char* lds, Values& y) {
         y.dm[i] = *(const uint32_t*)(at + 64 + (n & ~3u));
     }
 }
-// st: products, which times `scale` are scores in base 2
+// st: products, which times the query's `scale` are scores in base 2
 __device__ __forceinline__ void tile_add(Sums& x, const pf4 (&st)[2], float scale, const Masks& c, const Values& y) {
     const float top = largest(largest(st[0][0], st[0][1], st[0][2]), largest(st[0][3], st[1][0], st[1][1]), larger(st[1][2], st[1][3]));
     const float mx = larger(x.m, lanes4_larger(top) * scale);
@@ -451,7 +474,6 @@ __device__ __forceinline__ void paged4_chunk(const GhPagedAttnArgs& a, const Row
                                              char* lds, const char* mine0) {
     const uint32_t lane = threadIdx.x & 63u, n = lane & 15u, G = a.group;
     const Masks masks;
-    const float scale = a.scale * 512.0f;
 
     // lane i: slots, first position, and row | positions << 16 of tile i of the current 64
     uint32_t t_slot0 = 0, t_slot1 = 0, t_pos = 0, t_row = 0;
@@ -520,10 +542,10 @@ __device__ __forceinline__ void paged4_chunk(const GhPagedAttnArgs& a, const Row
         }
         pf4 st[2] = {half_products(mine, q), half_products(mine + kHalfBytes, q)};
         hide(st, info >> 16);
-        if (SCORED && n < G) keep_scores(raw, pos, st, scale);
+        if (SCORED && n < G) keep_scores(raw, pos, st, q.scale);
         Values y;
         load_v(mine + 2 * kHalfBytes, y);
-        tile_add(x, st, scale, masks, y);
+        tile_add(x, st, q.scale, masks, y);
     }
     if (there && tiles) flush(tiles);
 }
@@ -595,7 +617,6 @@ __device__ __forceinline__ void paged4_split(const GhPagedAttnArgs& a) {
         return;
     }
     if (begin >= len) return;
-    const float scale = a.scale * 512.0f;
     const uint32_t end = min(len, begin + span);
     uint32_t t_slot0 = 0, t_slot1 = 0, t_count = 0;
     if (mine < end) {
@@ -625,10 +646,10 @@ __device__ __forceinline__ void paged4_split(const GhPagedAttnArgs& a) {
             load_tile<0>(where(i + 1), pieces, r);
             pf4 st[2] = {half_products(lds, q), half_products(lds + kHalfBytes, q)};
             hide(st, __builtin_amdgcn_readlane(t_count, i & 63u));
-            if (SCORED && n < G) keep_scores(raw, first + 128 * i, st, scale);
+            if (SCORED && n < G) keep_scores(raw, first + 128 * i, st, q.scale);
             Values y;
             load_v(lds + 2 * kHalfBytes, y);
-            tile_add(x, st, scale, masks, y);
+            tile_add(x, st, q.scale, masks, y);
         }
     }
     split_finish<SCORED>(a, x, dyn, row, kvh, split, span, len);

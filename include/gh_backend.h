@@ -259,7 +259,8 @@ int gh_kv_read_paged(gh_backend* b, gh_encoder* enc, const gh_buf* k, const gh_b
  * summed over the query heads of a kv head, is added to its score. In the products with V a weight is held to
  * 2^-38 of the row's largest and is at least that, unless its score is -inf: n positions add up to n·2^-38 of their
  * mean V, and an infinite V leaves an infinity or NaN whatever its score. A row whose scores are all -inf gives
- * NaN. In a q4 pool values are rounded to FP16 for these products, and keys are not. max_len also sizes the call's scratch: with scores 4 bytes per query head and position of every row, in groups of
+ * NaN. In a q4 pool values are rounded to FP16 for these products, and keys are not: a score's sums are FP32, of a query as it is
+ * to 2^-36 of its largest value and its sums over 32 dims to 2^-22 of them or 2^-31 of that value. max_len also sizes the call's scratch: with scores 4 bytes per query head and position of every row, in groups of
  * rows that take at most 512 MiB. */
 int gh_attention_decode_paged(gh_backend* b, gh_encoder* enc, const gh_buf* out, const gh_buf* q,
                               const gh_kv_paged* kv, uint32_t q_heads, uint32_t max_len, uint32_t layer);
