@@ -270,11 +270,12 @@ struct GhArgmaxArgs {
 };
 
 // Sampling of rows of logits (kernels/sample.hip). Scratch of a row: the chunks' maxima, (largest of all as order and
-// index, largest finite one's order) u64 x 2 [64]; bins u64 sums, u32 counts [GH_SAMPLE_BINS], u32 length of the list; list.
+// index, largest finite one's order) u64 x 2 [64]; bins u64, and u64 or without `fine` u32, [GH_SAMPLE_BINS], u32 length of the list
+// in the first of four dwords behind them; list.
 #define GH_SAMPLE_BINS 1024u
-#define GH_SAMPLE_LIST 8192u
+#define GH_SAMPLE_LIST 7680u
 #define GH_SAMPLE_PICK 1024u   // threads of gh_sample_pick
-#define GH_SAMPLE_BIN_BYTES (GH_SAMPLE_BINS * 12u + 16u)
+#define GH_SAMPLE_BIN_BYTES (GH_SAMPLE_BINS * 16u + 16u)
 #define GH_SAMPLE_ROW_BYTES (64u * 16u + GH_SAMPLE_BIN_BYTES + GH_SAMPLE_LIST * 8u)
 struct GhSampleArgs {
     uint64_t logits;   // f32 [rows][stride]
@@ -285,13 +286,16 @@ struct GhSampleArgs {
     uint64_t part;
     uint64_t bins;
     uint64_t list;     // u64 [rows][GH_SAMPLE_LIST]
-    double scale;      // of weights in fixed point: 2^shift, at most 2^51, and vocab times it at most 2^62
+    double scale;      // of weights' whole parts in fixed point: 2^shift, at most 2^51, and vocab times it at most 2^62
     uint32_t vocab;
     uint32_t stride;
     uint32_t chunks;   // of a row, at most 64
     uint32_t per;      // logits of a chunk, a multiple of 4
     uint32_t wide;     // rows start on 16 bytes
     int32_t shift;
+    int32_t fine;         // bits of their further parts, at most 40; 0: there are none
+    uint32_t count_bits;  // below those: a count up to vocab
+    uint32_t bin_bytes;   // from a row's bins to the next one's, at most GH_SAMPLE_BIN_BYTES
 };
 
 // ---- paged caches (kernels/paged.hip, kernels/paged4.hip) ----

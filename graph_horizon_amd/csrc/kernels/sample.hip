@@ -4,8 +4,10 @@
 // Tokens rank by (logit descending by f32 total order, index ascending), those with a finite logit. Token i has weight
 // w = exp((l - M) / T), M the row's largest logit. Every filter keeps a prefix of the ranking, and the draw
 // is the first rank whose running sum of weights passes u times the kept sum, so all a row needs are four searches in the
-// running counts and sums. Sums are of whole numbers, w in fixed point: the same in any order, and off by 2^-46 at a
-// vocabulary of 2^17, so that what lies next to a border of the kept or drawn range falls where 64 bits put it.
+// running counts and sums. Sums are of whole numbers, w in fixed point: the same in any order. One word must leave room for
+// `vocab` weights of 1: at a vocabulary of 2^17 a weight is off by 2^-46 at most, and a sum by 2^-29 of the largest weight. Larger
+// vocabularies, where that grows with their square, take two words (Mass<true>): a sum is off by vocab 2^-54 at most, as in FP64.
+// The second word costs 0.8 us of 22.2 for 1 row of 131072 and 4 of 47.4 for 64, so smaller ones do without.
 //
 // Four launches; a row's logits are read three times, from memory once (us of 1 / 8 / 64 rows of 131072):
 //   gh_sample_max     the largest logit of each chunk of a row (3.8 / 4.2 / 10.2; 34 MB of 64 rows);
@@ -19,6 +21,8 @@
 //                     them 5.6 / 14.0 / 12.3, 8 waves in all 4.7 / 14.9 / 12.6; from memory without gh_sample_collect, 1 row: 23.3).
 // Chains of dependent loads and barriers bound the launches of few rows.
 // What the device cannot trust is only the settings: any bits give a token of the row.
+#include <type_traits>
+
 #include "gh_wave64.h"
 
 namespace {
@@ -97,10 +101,62 @@ __device__ __forceinline__ double exp_scaled(const double* table, double x, int 
 __device__ __forceinline__ double weight(const Row& r, const double* table, float l) {
     return exp_scaled(table, ((double)l - (double)r.top) * r.inv, 0);
 }
-// The weight in fixed point, nearest: at most 2^51, so that 2^52 more leaves it in the mantissa.
-__device__ __forceinline__ uint64_t fixed(const GhSampleArgs& a, const Row& r, const double* table, float l) {
-    const double w = exp_scaled(table, ((double)l - (double)r.top) * r.inv, a.shift);
-    return __builtin_bit_cast(uint64_t, w + 0x1p52) & 0xFFFFFFFFFFFFFull;
+// What tokens weigh together, in fixed point, and their number. Whole parts are 2^-shift of the largest weight. FINE: above the count,
+// in `count_bits` bits, `rest` holds further parts, of 2^-(shift + fine). All of a row's tokens fit both words.
+template <bool FINE>
+struct Mass {
+    uint64_t whole;
+    std::conditional_t<FINE, uint64_t, uint32_t> rest;
+    __device__ __forceinline__ Mass operator+(const Mass& x) const { return Mass{whole + x.whole, rest + x.rest}; }
+    __device__ __forceinline__ Mass operator-(const Mass& x) const { return Mass{whole - x.whole, rest - x.rest}; }
+};
+template <bool FINE>
+__device__ __forceinline__ uint32_t count_of(const GhSampleArgs& a, const Mass<FINE>& m) {
+    return FINE ? (uint32_t)m.rest & ((1u << a.count_bits) - 1) : (uint32_t)m.rest;
+}
+// In whole parts. No smaller for a mass with more tokens.
+template <bool FINE>
+__device__ __forceinline__ double sum_of(const GhSampleArgs& a, const Mass<FINE>& m) {
+    if constexpr (FINE) return (double)m.whole + __builtin_ldexp((double)(m.rest >> a.count_bits), -a.fine);
+    else return (double)m.whole;
+}
+template <bool FINE>
+__device__ __forceinline__ Mass<FINE> scan_mass(const Mass<FINE>& m) {
+    return Mass<FINE>{gh_scan64(m.whole), (decltype(m.rest))gh_scan64(m.rest)};
+}
+template <bool FINE>
+__device__ __forceinline__ Mass<FINE> lane_mass(const Mass<FINE>& m, uint32_t lane) {
+    if constexpr (FINE) return Mass<FINE>{gh_lane64(m.whole, lane), gh_lane64(m.rest, lane)};
+    else return Mass<FINE>{gh_lane64(m.whole, lane), (uint32_t)__builtin_amdgcn_readlane(m.rest, lane)};
+}
+// A token's, its last part nearest. Both words' parts are at most 2^51, so that 2^52 more leaves them in the mantissa. (The
+// largest weight, 1, has no further parts.)
+template <bool FINE>
+__device__ __forceinline__ Mass<FINE> fixed(const GhSampleArgs& a, const Row& r, const double* table, float l) {
+    const double w = exp_scaled(table, ((double)l - (double)r.top) * r.inv, a.shift), whole = FINE ? __builtin_floor(w) : w;
+    const uint64_t bits = 0xFFFFFFFFFFFFFull;
+    Mass<FINE> m{__builtin_bit_cast(uint64_t, whole + 0x1p52) & bits, 1u};
+    if constexpr (FINE) m.rest |= (__builtin_bit_cast(uint64_t, __builtin_ldexp(w - whole, a.fine) + 0x1p52) & bits) << a.count_bits;
+    return m;
+}
+
+// Masses of the bins, or of parts of one: 64 bits each for `rest`, or the first half of them 32.
+template <bool FINE>
+__device__ __forceinline__ Mass<FINE> mass_at(const uint64_t* whole, const uint64_t* rest, uint32_t i) {
+    if constexpr (FINE) return Mass<FINE>{whole[i], rest[i]};
+    else return Mass<FINE>{whole[i], ((const uint32_t*)rest)[i]};
+}
+template <bool FINE>
+__device__ __forceinline__ void put_mass(uint64_t* whole, uint64_t* rest, uint32_t i, const Mass<FINE>& m) {
+    whole[i] = m.whole;
+    if constexpr (FINE) rest[i] = m.rest;
+    else ((uint32_t*)rest)[i] = m.rest;
+}
+template <bool FINE>
+__device__ __forceinline__ void add_mass(uint64_t* whole, uint64_t* rest, uint32_t i, const Mass<FINE>& m) {
+    if constexpr (FINE) atomicAdd((unsigned long long*)rest + i, (unsigned long long)m.rest);
+    else atomicAdd((uint32_t*)rest + i, m.rest);
+    if (m.whole) atomicAdd((unsigned long long*)whole + i, (unsigned long long)m.whole);
 }
 
 // LOADS times four logits of a block of a row, the k-th four of a thread 4 THREADS k further on; NaN past `end`.
@@ -140,8 +196,8 @@ __device__ __forceinline__ void each_of(const float4 (&v)[LOADS], uint32_t block
 GH_KERNEL __launch_bounds__(256) void gh_sample_max(GhSampleArgs a) {
     __shared__ uint64_t red[4][2];
     const uint32_t tid = threadIdx.x, row = blockIdx.y, first = blockIdx.x * a.per, end = min(a.vocab, first + a.per);
-    GH_GLOBAL uint32_t* bins = gh_gpw<uint32_t>(a.bins + (uint64_t)row * GH_SAMPLE_BIN_BYTES);
-    for (uint32_t i = blockIdx.x * 256 + tid; i < GH_SAMPLE_BIN_BYTES / 4; i += gridDim.x * 256) bins[i] = 0u;
+    GH_GLOBAL uint32_t* bins = gh_gpw<uint32_t>(a.bins + (uint64_t)row * a.bin_bytes);
+    for (uint32_t i = blockIdx.x * 256 + tid; i < a.bin_bytes / 4; i += gridDim.x * 256) bins[i] = 0u;
     uint32_t fin = 0;
     float4 v[kLoads];
     for (uint32_t block = first; block < end; block += kBlock) {
@@ -179,18 +235,13 @@ GH_KERNEL __launch_bounds__(256) void gh_sample_max(GhSampleArgs a) {
     }
 }
 
-// Grid (chunks, rows), 256 threads. Bins in LDS, added to the row's by atomics on whole numbers.
-GH_KERNEL __launch_bounds__(256) void gh_sample_bins(GhSampleArgs a) {
-    __shared__ unsigned long long sum[kBins];
-    __shared__ uint32_t count[kBins];
-    __shared__ double table[64];
+namespace {
+template <bool FINE>
+__device__ __forceinline__ void sample_bins(const GhSampleArgs& a, uint64_t* whole, uint64_t* rest, double* table) {
     const uint32_t tid = threadIdx.x, row = blockIdx.y, first = blockIdx.x * a.per, end = min(a.vocab, first + a.per);
     float4 v[kLoads];
     load_block<256>(a, row, first, end, v);
-    for (uint32_t i = tid; i < kBins; i += 256) {
-        sum[i] = 0;
-        count[i] = 0;
-    }
+    for (uint32_t i = tid; i < kBins; i += 256) put_mass(whole, rest, i, Mass<FINE>{0, 0});
     fill_exp(table);
     const Row r = row_of(a, row);
     if (r.greedy) return;
@@ -198,22 +249,27 @@ GH_KERNEL __launch_bounds__(256) void gh_sample_bins(GhSampleArgs a) {
     for (uint32_t block = first;;) {
         each_of<256>(v, block, [&](float l, uint32_t) __attribute__((always_inline)) {
             if (!finite(l)) return;
-            const uint32_t b = bin_of(r.top - l);
-            atomicAdd(&count[b], 1u);
-            const uint64_t w = fixed(a, r, table, l);
-            if (w) atomicAdd(&sum[b], (unsigned long long)w);
+            add_mass(whole, rest, bin_of(r.top - l), fixed<FINE>(a, r, table, l));
         });
         block += kBlock;
         if (block >= end) break;
         load_block<256>(a, row, block, end, v);
     }
     __syncthreads();
-    const uint64_t bins = a.bins + (uint64_t)row * GH_SAMPLE_BIN_BYTES;
+    uint64_t* bins = (uint64_t*)(a.bins + (uint64_t)row * a.bin_bytes);
     for (uint32_t i = tid; i < kBins; i += 256) {
-        if (!count[i]) continue;
-        if (sum[i]) atomicAdd((unsigned long long*)bins + i, sum[i]);
-        atomicAdd((uint32_t*)(bins + kBins * 8) + i, count[i]);
+        const Mass<FINE> m = mass_at<FINE>(whole, rest, i);
+        if (m.rest) add_mass(bins, bins + kBins, i, m);
     }
+}
+}  // namespace
+
+// Grid (chunks, rows), 256 threads. Bins in LDS, added to the row's by atomics on whole numbers.
+GH_KERNEL __launch_bounds__(256) void gh_sample_bins(GhSampleArgs a) {
+    __shared__ uint64_t whole[kBins], rest[kBins];
+    __shared__ double table[64];
+    if (a.fine) sample_bins<true>(a, whole, rest, table);
+    else sample_bins<false>(a, whole, rest, table);
 }
 
 namespace {
@@ -231,90 +287,80 @@ struct Plan {
         return (partly && b == k) || (p0 != kNone && p0 <= b && b <= p1) || (m0 != kNone && m0 <= b && b <= m1) || (d0 <= b && b <= d1);
     }
 };
-// LDS of a plan: inclusive running counts and sums of the bins.
+// LDS of a plan: what the bins hold, running and inclusive.
 struct PlanLds {
-    uint64_t sum[kBins];
-    uint32_t count[kBins];
-    uint64_t wave_sum[16];
-    uint32_t wave_count[16], wave_listed[16];
+    uint64_t whole[kBins], rest[kBins];
+    uint64_t wave_whole[16], wave_rest[16];
+    uint32_t wave_listed[16];
     uint32_t found[5];
 };
-__device__ __forceinline__ uint64_t before(const PlanLds& s, uint32_t b) { return b ? s.sum[b - 1] : 0; }
-__device__ __forceinline__ uint32_t count_before(const PlanLds& s, uint32_t b) { return b ? s.count[b - 1] : 0; }
+template <bool FINE>
+__device__ __forceinline__ Mass<FINE> upto(const PlanLds& s, uint32_t b) { return mass_at<FINE>(s.whole, s.rest, b); }
+template <bool FINE>
+__device__ __forceinline__ Mass<FINE> before(const PlanLds& s, uint32_t b) { return b ? upto<FINE>(s, b - 1) : Mass<FINE>{0, 0}; }
 
 // All threads of the workgroup get the same plan; the first THREADS look at the bins (of 16 waves, which take 16 cycles for
-// an instruction, half). u64 sums are compared as doubles, as the searches compare them.
-template <uint32_t THREADS, uint32_t ALL>
+// an instruction, half). Sums are compared as doubles, as the searches compare them.
+template <bool FINE, uint32_t THREADS, uint32_t ALL>
 __device__ __forceinline__ Plan plan_of(const GhSampleArgs& a, const Row& r, uint32_t row, PlanLds& s) {
     constexpr uint32_t kEach = kBins / THREADS, kWaves = THREADS / 64;  // bins of a thread, in a row
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
-    const uint64_t bins = a.bins + (uint64_t)row * GH_SAMPLE_BIN_BYTES;
+    const GH_GLOBAL uint64_t* bins = gh_gp<uint64_t>(a.bins + (uint64_t)row * a.bin_bytes);
     const bool looks = THREADS == ALL || tid < THREADS;
-    uint64_t w[kEach], wu = 0;
-    uint32_t c[kEach], own[kEach], cu = 0;  // own: the bins' counts
+    Mass<FINE> m[kEach], mu = {0, 0};
+    uint32_t own[kEach];  // the bins' counts
     if (looks) {
 #pragma unroll
         for (uint32_t j = 0; j < kEach; ++j) {
-            w[j] = gh_gp<uint64_t>(bins)[tid * kEach + j];
-            c[j] = gh_gp<uint32_t>(bins + kBins * 8)[tid * kEach + j];
+            m[j].whole = bins[tid * kEach + j];
+            m[j].rest = ((const GH_GLOBAL decltype(mu.rest)*)(bins + kBins))[tid * kEach + j];
         }
 #pragma unroll
-        for (uint32_t j = 0; j < kEach; ++j) own[j] = c[j];
+        for (uint32_t j = 0; j < kEach; ++j) own[j] = count_of(a, m[j]);
 #pragma unroll
-        for (uint32_t j = 1; j < kEach; ++j) {
-            w[j] += w[j - 1];
-            c[j] += c[j - 1];
-        }
-        wu = gh_scan64(w[kEach - 1]);
-        cu = (uint32_t)gh_scan64(c[kEach - 1]);
-        if (lane == 63) {
-            s.wave_sum[wave] = wu;
-            s.wave_count[wave] = cu;
-        }
+        for (uint32_t j = 1; j < kEach; ++j) m[j] = m[j - 1] + m[j];
+        mu = scan_mass(m[kEach - 1]);
+        if (lane == 63) put_mass(s.wave_whole, s.wave_rest, wave, mu);
         if (tid < 5) s.found[tid] = kBins - 1;
     }
     __syncthreads();
     Plan p;
     p.tokens = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < kWaves; ++i) p.tokens += s.wave_count[i];
-    uint64_t w0 = 0;  // before the thread's bins
-    uint32_t c0 = 0;
+    for (uint32_t i = 0; i < kWaves; ++i) p.tokens += count_of(a, mass_at<FINE>(s.wave_whole, s.wave_rest, i));
+    Mass<FINE> m0 = {0, 0};  // before the thread's bins
     if (looks) {
-        w0 = wu - w[kEach - 1];
-        c0 = cu - c[kEach - 1];
+        m0 = mu - m[kEach - 1];
 #pragma unroll
-        for (uint32_t i = 0; i < kWaves; ++i) {
-            w0 += i < wave ? s.wave_sum[i] : 0;
-            c0 += i < wave ? s.wave_count[i] : 0;
-        }
+        for (uint32_t i = 0; i < kWaves; ++i)
+            if (i < wave) m0 = m0 + mass_at<FINE>(s.wave_whole, s.wave_rest, i);
 #pragma unroll
         for (uint32_t j = 0; j < kEach; ++j) {
-            s.sum[tid * kEach + j] = w[j] += w0;
-            s.count[tid * kEach + j] = c[j] += c0;
+            m[j] = m[j] + m0;
+            put_mass(s.whole, s.rest, tid * kEach + j, m[j]);
         }
     }
     // The first bin up to which the running values satisfy `is`, which stays true once it is: one thread has it.
     auto first_bin = [&](uint32_t slot, auto is) __attribute__((always_inline)) {
-        if (!looks || !is(c[kEach - 1], w[kEach - 1]) || (tid && is(c0, w0))) return;
+        if (!looks || !is(m[kEach - 1]) || (tid && is(m0))) return;
         uint32_t j = 0;
 #pragma unroll
-        for (uint32_t i = 0; i + 1 < kEach; ++i) j += j == i && !is(c[i], w[i]);
+        for (uint32_t i = 0; i + 1 < kEach; ++i) j += j == i && !is(m[i]);
         s.found[slot] = tid * kEach + j;
     };
     p.keep = r.top_k && r.top_k < p.tokens ? r.top_k : p.tokens;
-    first_bin(0, [&](uint32_t c, uint64_t) { return c >= p.keep; });
+    first_bin(0, [&](const Mass<FINE>& x) { return count_of(a, x) >= p.keep; });
     __syncthreads();
     p.k = s.found[0];
-    p.partly = s.count[p.k] > p.keep;
+    p.partly = count_of(a, upto<FINE>(s, p.k)) > p.keep;
     // the sum of the first top_k lies between lo and hi
-    double lo = (double)(p.partly ? before(s, p.k) : s.sum[p.k]), hi = (double)s.sum[p.k];
+    double lo = sum_of(a, p.partly ? before<FINE>(s, p.k) : upto<FINE>(s, p.k)), hi = sum_of(a, upto<FINE>(s, p.k));
     uint32_t l0 = p.k, l1 = p.k;  // the last kept token's bins
     p.p0 = p.p1 = p.m0 = p.m1 = kNone;
     if (r.top_p < 1.0f) {
         const double want0 = r.top_p * lo, want1 = r.top_p * hi;
-        first_bin(1, [&](uint32_t, uint64_t w) { return (double)w >= want0; });
-        first_bin(2, [&](uint32_t, uint64_t w) { return (double)w >= want1; });
+        first_bin(1, [&](const Mass<FINE>& x) { return sum_of(a, x) >= want0; });
+        first_bin(2, [&](const Mass<FINE>& x) { return sum_of(a, x) >= want1; });
         __syncthreads();
         l0 = p.p0 = min(s.found[1], p.k);
         l1 = p.p1 = min(s.found[2], p.k);
@@ -328,11 +374,11 @@ __device__ __forceinline__ Plan plan_of(const GhSampleArgs& a, const Row& r, uin
         l1 = min(l1, p.m1);
     }
     // the kept sum lies between lo and hi
-    if (p.partly || p.p0 != kNone || p.m0 != kNone) lo = (double)before(s, l0);
-    hi = (double)s.sum[l1];
+    if (p.partly || p.p0 != kNone || p.m0 != kNone) lo = sum_of(a, before<FINE>(s, l0));
+    hi = sum_of(a, upto<FINE>(s, l1));
     const double want0 = r.u * lo, want1 = r.u * hi;
-    first_bin(3, [&](uint32_t, uint64_t w) { return (double)w > want0; });
-    first_bin(4, [&](uint32_t, uint64_t w) { return (double)w > want1; });
+    first_bin(3, [&](const Mass<FINE>& x) { return sum_of(a, x) > want0; });
+    first_bin(4, [&](const Mass<FINE>& x) { return sum_of(a, x) > want1; });
     __syncthreads();
     p.d0 = min(s.found[3], l1);
     p.d1 = min(s.found[4], l1);
@@ -351,16 +397,15 @@ __device__ __forceinline__ Plan plan_of(const GhSampleArgs& a, const Row& r, uin
 }
 }  // namespace
 
-// Grid (chunks, rows), 256 threads. A block's tokens are counted first, so that it asks for its places in the list once.
-GH_KERNEL __launch_bounds__(256) void gh_sample_collect(GhSampleArgs a) {
-    __shared__ PlanLds s;
-    __shared__ uint32_t need[kBins / 32], places[5];
+namespace {
+template <bool FINE>
+__device__ __forceinline__ void sample_collect(const GhSampleArgs& a, PlanLds& s, uint32_t* need, uint32_t* places) {
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, row = blockIdx.y, first = blockIdx.x * a.per, end = min(a.vocab, first + a.per);
     float4 v[kLoads];
     load_block<256>(a, row, first, end, v);
     const Row r = row_of(a, row);
     if (r.greedy) return;
-    const Plan p = plan_of<256, 256>(a, r, row, s);
+    const Plan p = plan_of<FINE, 256, 256>(a, r, row, s);
     if (p.listed > kList) return;
 #pragma unroll
     for (uint32_t j = 0; j < kBins / 256; ++j) {
@@ -369,7 +414,7 @@ GH_KERNEL __launch_bounds__(256) void gh_sample_collect(GhSampleArgs a) {
     }
     __syncthreads();
     const uint64_t list = a.list + (uint64_t)row * kList * 8;
-    uint32_t* length = (uint32_t*)(a.bins + (uint64_t)row * GH_SAMPLE_BIN_BYTES + kBins * 12);
+    uint32_t* length = (uint32_t*)(a.bins + (uint64_t)(row + 1) * a.bin_bytes - 16);
     for (uint32_t block = first;;) {
         uint32_t mine = 0, bit = 1;  // which of the thread's 32 are wanted
         each_of<256>(v, block, [&](float l, uint32_t) __attribute__((always_inline)) {
@@ -377,14 +422,14 @@ GH_KERNEL __launch_bounds__(256) void gh_sample_collect(GhSampleArgs a) {
             if (finite(l) && (need[b >> 5] >> (b & 31u) & 1u)) mine |= bit;
             bit <<= 1;
         });
-        const uint32_t n = __popc(mine), upto = (uint32_t)gh_scan64(n);
-        if (lane == 63) places[wave] = upto;
+        const uint32_t n = __popc(mine), mine_upto = (uint32_t)gh_scan64(n);
+        if (lane == 63) places[wave] = mine_upto;
         __syncthreads();
         const uint32_t all = places[0] + places[1] + places[2] + places[3];
         if (all) {  // of the whole workgroup
             if (tid == 0) places[4] = atomicAdd(length, all);
             __syncthreads();
-            uint32_t at = places[4] + upto - n;
+            uint32_t at = places[4] + mine_upto - n;
             for (uint32_t w = 0; w < wave; ++w) at += places[w];
             bit = 1;
             each_of<256>(v, block, [&](float l, uint32_t i) __attribute__((always_inline)) {
@@ -401,24 +446,33 @@ GH_KERNEL __launch_bounds__(256) void gh_sample_collect(GhSampleArgs a) {
         __syncthreads();
     }
 }
+}  // namespace
+
+// Grid (chunks, rows), 256 threads. A block's tokens are counted first, so that it asks for its places in the list once.
+GH_KERNEL __launch_bounds__(256) void gh_sample_collect(GhSampleArgs a) {
+    __shared__ PlanLds s;
+    __shared__ uint32_t need[kBins / 32], places[5];
+    if (a.fine) sample_collect<true>(a, s, need, places);
+    else sample_collect<false>(a, s, need, places);
+}
 
 namespace {
 // Threads, their waves; those that look at bins, their waves, bins of each.
 constexpr uint32_t kPick = GH_SAMPLE_PICK, kPickWaves = kPick / 64, kLook = 512, kLookWaves = kLook / 64, kLookBins = kBins / kLook;
-// A token found by its running values: its key, and the count and sum up to and with it.
+// A token found by its running values: its key, and the mass up to and with it.
+template <bool FINE>
 struct Hit {
-    uint64_t key, sum;
-    uint32_t count;
+    uint64_t key;
+    Mass<FINE> mass;
 };
 struct PickLds {
     uint64_t list[kList];
     uint64_t few[64];       // the tokens among which a search ends
-    uint64_t sum[kBins];    // of a range of keys, in equal parts
-    uint32_t count[kBins];
-    uint64_t lo[16], hi[16], wave_sum[16];
-    uint32_t wave_count[16];
+    uint64_t whole[kBins], rest[kBins];  // of a range of keys, in equal parts
+    uint64_t lo[16], hi[16];
+    uint64_t wave_whole[16], wave_rest[16];
+    uint64_t hit_key, hit_whole, hit_rest;
     uint32_t found, fill;
-    Hit hit;
 };
 
 // The tokens of the list, or of the row, by key.
@@ -445,28 +499,29 @@ struct Whole {
     }
 };
 
-// The first token in rank order up to which count and sum satisfy `is`, which some token's do and stays true once it is. Its bin
+// The first token in rank order up to which the mass satisfies `is`, which some token's do and stays true once it is. Its bin
 // by the running values of the bins; then, while there are more than 64 tokens, in which 1024th of them it is, first by the next ten
 // bits of their distance, then by parts of the range of their keys; then among these, by one wave.
-template <class S, class F>
-__device__ __forceinline__ Hit search(const GhSampleArgs& a, const Row& r, const double* table, const PlanLds& s, PickLds& q, const S& source, F is) {
+template <bool FINE, class S, class F>
+__device__ __forceinline__ Hit<FINE> search(const GhSampleArgs& a, const Row& r, const double* table, const PlanLds& s, PickLds& q, const S& source, F is) {
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
     __syncthreads();
     if (tid == 0) q.found = kBins - 1;
     __syncthreads();
     const bool looks = tid < kLook;
     const uint32_t mine = tid * kLookBins;  // the thread's bins, or parts of a range
-    if (looks && is(s.count[mine + kLookBins - 1], s.sum[mine + kLookBins - 1]) && (tid == 0 || !is(s.count[mine - 1], s.sum[mine - 1]))) {
+    if (looks && is(upto<FINE>(s, mine + kLookBins - 1)) && (tid == 0 || !is(upto<FINE>(s, mine - 1)))) {
         uint32_t b = mine;
 #pragma unroll
-        for (uint32_t j = 0; j + 1 < kLookBins; ++j) b += b == mine + j && !is(s.count[b], s.sum[b]);
+        for (uint32_t j = 0; j + 1 < kLookBins; ++j) b += b == mine + j && !is(upto<FINE>(s, b));
         q.found = b;
     }
     __syncthreads();
     const uint32_t bin = q.found;
     __syncthreads();  // all have read it: the first round below writes it again
-    uint64_t sum = before(s, bin), lo = 0, hi = ~0ull;
-    uint32_t count = count_before(s, bin), n = s.count[bin] - count;
+    Mass<FINE> base = before<FINE>(s, bin);
+    uint64_t lo = 0, hi = ~0ull;
+    uint32_t n = count_of(a, upto<FINE>(s, bin) - base);
     // (the first and the last bin hold distances of any exponent)
     bool bits = bin && bin < kBins - 1;
     uint32_t tenth = kNone;  // the distance's ten bits, once known
@@ -477,10 +532,7 @@ __device__ __forceinline__ Hit search(const GhSampleArgs& a, const Row& r, const
     // (eight rounds narrow any range of keys to one: a bound for logits that another stream changes meanwhile)
     for (uint32_t round = 0; n > 64 && round < 8; ++round) {
         uint32_t shift = 0;
-        for (uint32_t i = tid; i < kBins; i += kPick) {
-            q.sum[i] = 0;
-            q.count[i] = 0;
-        }
+        for (uint32_t i = tid; i < kBins; i += kPick) put_mass(q.whole, q.rest, i, Mass<FINE>{0, 0});
         if (tid == 0) q.found = kBins - 1;
         if (!bits) {
             uint64_t least = ~0ull, most = 0;
@@ -510,51 +562,41 @@ __device__ __forceinline__ Hit search(const GhSampleArgs& a, const Row& r, const
         source.each([&](uint64_t key) __attribute__((always_inline)) {
             if (!inside(key)) return;
             const uint32_t part = bits ? ten(key) : (uint32_t)((key - lo) >> shift);
-            atomicAdd(&q.count[part], 1u);
-            atomicAdd((unsigned long long*)&q.sum[part], (unsigned long long)fixed(a, r, table, value_of(key)));
+            add_mass(q.whole, q.rest, part, fixed<FINE>(a, r, table, value_of(key)));
         });
         __syncthreads();
-        uint64_t ws[kLookBins], wall = 0, w = 0;
-        uint32_t cs[kLookBins], call = 0, c = 0;
+        Mass<FINE> ms[kLookBins], all = {0, 0}, m = {0, 0};
         if (looks) {
 #pragma unroll
             for (uint32_t j = 0; j < kLookBins; ++j) {
-                wall += ws[j] = q.sum[mine + j];
-                call += cs[j] = q.count[mine + j];
+                ms[j] = mass_at<FINE>(q.whole, q.rest, mine + j);
+                all = all + ms[j];
             }
-            w = gh_scan64(wall);
-            c = (uint32_t)gh_scan64(call);
-            if (lane == 63) {
-                q.wave_sum[wave] = w;
-                q.wave_count[wave] = c;
-            }
+            m = scan_mass(all);
+            if (lane == 63) put_mass(q.wave_whole, q.wave_rest, wave, m);
         }
         __syncthreads();
         if (looks) {
-            uint64_t w0 = sum + w - wall;
-            uint32_t c0 = count + c - call;
+            Mass<FINE> m0 = base + m - all;
 #pragma unroll
-            for (uint32_t i = 0; i + 1 < kLookWaves; ++i) {
-                w0 += i < wave ? q.wave_sum[i] : 0;
-                c0 += i < wave ? q.wave_count[i] : 0;
-            }
+            for (uint32_t i = 0; i + 1 < kLookWaves; ++i)
+                if (i < wave) m0 = m0 + mass_at<FINE>(q.wave_whole, q.wave_rest, i);
             // one part: the first of those that hold a token and end where `is` is true
+            const uint32_t none = count_of(a, base);
 #pragma unroll
             for (uint32_t j = 0; j < kLookBins; ++j) {
-                if (cs[j] && is(c0 + cs[j], w0 + ws[j]) && !(c0 > count && is(c0, w0))) {
+                const Mass<FINE> next = m0 + ms[j];
+                if (count_of(a, ms[j]) && is(next) && !(count_of(a, m0) > none && is(m0))) {
                     q.found = mine + j;
-                    q.hit.sum = w0;
-                    q.hit.count = c0;
+                    put_mass(&q.hit_whole, &q.hit_rest, 0, m0);
                 }
-                w0 += ws[j];
-                c0 += cs[j];
+                m0 = next;
             }
         }
         __syncthreads();
         const uint32_t part = q.found;
-        sum = q.hit.sum;
-        count = q.hit.count;
-        n = q.count[part];
+        base = mass_at<FINE>(&q.hit_whole, &q.hit_rest, 0);
+        n = count_of(a, mass_at<FINE>(q.whole, q.rest, part));
         if (bits) {
             tenth = part;
             bits = false;
@@ -575,80 +617,67 @@ __device__ __forceinline__ Hit search(const GhSampleArgs& a, const Row& r, const
     if (wave == 0) {
         // each lane's token against all of them, which are few
         const uint32_t all = min(q.fill, 64u);
-        const uint64_t key = lane < all ? q.few[lane] : ~0ull, w = lane < all ? fixed(a, r, table, value_of(key)) : 0;
-        uint64_t upto = sum;
-        uint32_t rank = count;
+        const uint64_t key = lane < all ? q.few[lane] : ~0ull;
+        Mass<FINE> own = {0, 0}, m = base;
+        if (lane < all) own = fixed<FINE>(a, r, table, value_of(key));
         for (uint32_t i = 0; i < all; ++i) {
             const bool first = gh_lane64(key, i) <= key;
-            const uint64_t wi = gh_lane64(w, i);
-            upto += first ? wi : 0;
-            rank += first;
+            const Mass<FINE> mi = lane_mass(own, i);
+            if (first) m = m + mi;
         }
-        const bool ends = is(rank, upto) && (rank == count + 1 || !is(rank - 1, upto - w));
-        const uint64_t good = __ballot(lane < all && ends), last = __ballot(lane < all && rank == count + all);
-        if (lane == (uint32_t)__builtin_ctzll(good ? good : last | 1ull << 63)) q.hit = Hit{key, upto, rank};
+        const uint32_t rank = count_of(a, m) - count_of(a, base);
+        const bool ends = is(m) && (rank == 1 || !is(m - own));
+        const uint64_t good = __ballot(lane < all && ends), last = __ballot(lane < all && rank == all);
+        if (lane == (uint32_t)__builtin_ctzll(good ? good : last | 1ull << 63)) {
+            q.hit_key = key;
+            put_mass(&q.hit_whole, &q.hit_rest, 0, m);
+        }
     }
     __syncthreads();
-    return q.hit;
+    return Hit<FINE>{q.hit_key, mass_at<FINE>(&q.hit_whole, &q.hit_rest, 0)};
 }
 
 // The row's token; its share of the kept sum in *prob.
-template <class S>
+template <bool FINE, class S>
 __device__ __forceinline__ uint32_t pick_by_search(const GhSampleArgs& a, const Row& r, const double* table, const Plan& p, const PlanLds& s,
                                                    PickLds& q, const S& source, double* prob) {
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
     uint32_t keep = p.keep;
-    uint64_t sum = s.sum[p.k];
-    if (p.partly) sum = search(a, r, table, s, q, source, [&](uint32_t c, uint64_t) { return c >= keep; }).sum;
+    Mass<FINE> mass = upto<FINE>(s, p.k);
+    if (p.partly) mass = search<FINE>(a, r, table, s, q, source, [&](const Mass<FINE>& x) { return count_of(a, x) >= keep; }).mass;
     if (p.p0 != kNone) {
-        const double want = r.top_p * (double)sum;
-        const Hit h = search(a, r, table, s, q, source, [&](uint32_t, uint64_t w) { return (double)w >= want; });
-        if (h.count < keep) {
-            keep = h.count;
-            sum = h.sum;
+        const double want = r.top_p * sum_of(a, mass);
+        const Hit<FINE> h = search<FINE>(a, r, table, s, q, source, [&](const Mass<FINE>& x) { return sum_of(a, x) >= want; });
+        if (count_of(a, h.mass) < keep) {
+            keep = count_of(a, h.mass);
+            mass = h.mass;
         }
     }
     if (p.m0 != kNone) {
-        uint64_t w = 0, c = 0;
+        Mass<FINE> in = {0, 0};
         source.each([&](uint64_t key) __attribute__((always_inline)) {
             const float l = value_of(key);
             const uint32_t b = bin_of(r.top - l);
-            if (p.m0 <= b && b <= p.m1 && weight(r, table, l) >= (double)r.min_p) {
-                ++c;
-                w += fixed(a, r, table, l);
-            }
+            if (p.m0 <= b && b <= p.m1 && weight(r, table, l) >= (double)r.min_p) in = in + fixed<FINE>(a, r, table, l);
         });
-        w = gh_scan64(w);
-        c = gh_scan64(c);
+        in = scan_mass(in);
         __syncthreads();
-        if (lane == 63) {
-            q.wave_sum[wave] = w;
-            q.wave_count[wave] = (uint32_t)c;
-        }
+        if (lane == 63) put_mass(q.wave_whole, q.wave_rest, wave, in);
         __syncthreads();
-        uint64_t to = before(s, p.m0);
-        uint32_t rank = count_before(s, p.m0);
-        for (uint32_t i = 0; i < kPickWaves; ++i) {
-            to += q.wave_sum[i];
-            rank += q.wave_count[i];
-        }
-        if (rank == 0) {
-            rank = 1;
-            to = fixed(a, r, table, r.top);
-        }
-        if (rank < keep) {
-            keep = rank;
-            sum = to;
-        }
+        Mass<FINE> to = before<FINE>(s, p.m0);
+        for (uint32_t i = 0; i < kPickWaves; ++i) to = to + mass_at<FINE>(q.wave_whole, q.wave_rest, i);
+        if (count_of(a, to) == 0) to = fixed<FINE>(a, r, table, r.top);
+        if (count_of(a, to) < keep) mass = to;
     }
-    const double want = r.u * (double)sum;
-    const Hit h = search(a, r, table, s, q, source, [&](uint32_t, uint64_t w) { return (double)w > want; });
-    *prob = weight(r, table, value_of(h.key)) * a.scale / (double)sum;
+    const double want = r.u * sum_of(a, mass);
+    const Hit<FINE> h = search<FINE>(a, r, table, s, q, source, [&](const Mass<FINE>& x) { return sum_of(a, x) > want; });
+    *prob = weight(r, table, value_of(h.key)) * a.scale / sum_of(a, mass);
     return (uint32_t)h.key;
 }
 
-// The same by one wave that has all of the list, at most 64 tokens: lane i the i-th in rank order, with the count and sum of the
+// The same by one wave that has all of the list, at most 64 tokens: lane i the i-th in rank order, with the mass of the
 // row's tokens up to it.
+template <bool FINE>
 __device__ __forceinline__ uint32_t pick_by_wave(const GhSampleArgs& a, const Row& r, const double* table, const Plan& p, const PlanLds& s,
                                                  uint64_t key, double* prob) {
     const uint32_t lane = threadIdx.x & 63u, n = p.listed;
@@ -656,57 +685,51 @@ __device__ __forceinline__ uint32_t pick_by_wave(const GhSampleArgs& a, const Ro
     const bool there = lane < n;
     const float l = value_of(key);
     const uint32_t bin = there ? bin_of(r.top - l) : kNone;
-    const uint64_t own = there ? fixed(a, r, table, l) : 0, upto = gh_scan64(own);
+    Mass<FINE> own = {0, 0};
+    if (there) own = fixed<FINE>(a, r, table, l);
+    const Mass<FINE> run = scan_mass(own), ahead = run - own;
     // the first lane of the token's bin: what is before it in the list is not what is before it in the row
     const uint32_t left = (uint32_t)__shfl_up((int)bin, 1, 64);
     const uint64_t heads = __ballot(lane == 0 || bin != left);
     const uint32_t head = 63 - (uint32_t)__clzll((long long)(heads & (~0ull >> (63 - lane))));
-    const uint64_t skip = __shfl((unsigned long long)(upto - own), (int)head, 64);
-    const uint64_t w = there ? before(s, bin) + upto - skip : 0;
-    const uint32_t c = there ? count_before(s, bin) + lane - head + 1 : 0;
+    Mass<FINE> skip;
+    skip.whole = __shfl((unsigned long long)ahead.whole, (int)head, 64);
+    if constexpr (FINE) skip.rest = __shfl((unsigned long long)ahead.rest, (int)head, 64);
+    else skip.rest = head;
+    Mass<FINE> m = {0, 0};
+    if (there) m = before<FINE>(s, bin) + run - skip;
+    const double w = sum_of(a, m);
     auto first = [&](bool is) __attribute__((always_inline)) {
         const uint64_t good = __ballot(there && is);
         return good ? (uint32_t)__builtin_ctzll(good) : 64u;
     };
     uint32_t keep = p.keep;
-    uint64_t sum = s.sum[p.k];
+    Mass<FINE> mass = upto<FINE>(s, p.k);
     if (p.partly) {
-        const uint32_t i = min(first(c >= keep), n - 1);
-        sum = gh_lane64(w, i);
+        const uint32_t i = min(first(count_of(a, m) >= keep), n - 1);
+        mass = lane_mass(m, i);
     }
     if (p.p0 != kNone) {
-        const uint32_t i = first((double)w >= r.top_p * (double)sum && bin >= p.p0);
-        const uint32_t ci = (uint32_t)__builtin_amdgcn_readlane(c, i & 63u);
-        if (i < n && ci < keep) {
-            keep = ci;
-            sum = gh_lane64(w, i);
+        const uint32_t i = first(w >= r.top_p * sum_of(a, mass) && bin >= p.p0);
+        const Mass<FINE> mi = lane_mass(m, i & 63u);
+        if (i < n && count_of(a, mi) < keep) {
+            keep = count_of(a, mi);
+            mass = mi;
         }
     }
     if (p.m0 != kNone) {
         const bool in = there && p.m0 <= bin && bin <= p.m1 && weight(r, table, l) >= (double)r.min_p;
-        uint32_t rank = count_before(s, p.m0) + (uint32_t)__popcll(__ballot(in));
-        uint64_t to = before(s, p.m0) + gh_lane64(gh_scan64(in ? own : 0), 63);
-        if (rank == 0) {
-            rank = 1;
-            to = fixed(a, r, table, r.top);
-        }
-        if (rank < keep) {
-            keep = rank;
-            sum = to;
-        }
+        Mass<FINE> to = before<FINE>(s, p.m0) + lane_mass(scan_mass(in ? own : Mass<FINE>{0, 0}), 63);
+        if (count_of(a, to) == 0) to = fixed<FINE>(a, r, table, r.top);
+        if (count_of(a, to) < keep) mass = to;
     }
-    const uint32_t i = min(first((double)w > r.u * (double)sum && bin >= p.d0), n - 1);
+    const uint32_t i = min(first(w > r.u * sum_of(a, mass) && bin >= p.d0), n - 1);
     const uint64_t hit = gh_lane64(key, i);
-    *prob = weight(r, table, value_of(hit)) * a.scale / (double)sum;
+    *prob = weight(r, table, value_of(hit)) * a.scale / sum_of(a, mass);
     return (uint32_t)hit;
 }
-}  // namespace
-
-// Grid (rows), kPick threads.
-GH_KERNEL __launch_bounds__(kPick) void gh_sample_pick(GhSampleArgs a) {
-    __shared__ PlanLds s;
-    __shared__ PickLds q;
-    __shared__ double table[64];
+template <bool FINE>
+__device__ __forceinline__ void sample_pick(const GhSampleArgs& a, PlanLds& s, PickLds& q, double* table) {
     const uint32_t tid = threadIdx.x, row = blockIdx.x;
     const Row r = row_of(a, row);
     auto done = [&](uint32_t token, double prob) __attribute__((always_inline)) {
@@ -721,17 +744,27 @@ GH_KERNEL __launch_bounds__(kPick) void gh_sample_pick(GhSampleArgs a) {
     const uint64_t list = a.list + (uint64_t)row * kList * 8;
     uint64_t key = ~0ull;
     if (tid < 64) key = gh_gp<uint64_t>(list)[tid];  // on its way while the plan is made
-    const Plan p = plan_of<kLook, kPick>(a, r, row, s);
+    const Plan p = plan_of<FINE, kLook, kPick>(a, r, row, s);
     double prob;
     uint32_t token;
     if (p.listed <= 64) {
         if (tid >= 64) return;
-        token = pick_by_wave(a, r, table, p, s, tid < p.listed ? key : ~0ull, &prob);
+        token = pick_by_wave<FINE>(a, r, table, p, s, tid < p.listed ? key : ~0ull, &prob);
     } else if (p.listed <= kList) {
         for (uint32_t i = tid; i < p.listed; i += kPick) q.list[i] = gh_gp<uint64_t>(list)[i];
-        token = pick_by_search(a, r, table, p, s, q, Listed{q.list, p.listed}, &prob);
+        token = pick_by_search<FINE>(a, r, table, p, s, q, Listed{q.list, p.listed}, &prob);
     } else {
-        token = pick_by_search(a, r, table, p, s, q, Whole{a, row}, &prob);
+        token = pick_by_search<FINE>(a, r, table, p, s, q, Whole{a, row}, &prob);
     }
     if (tid == 0) done(token, prob);
+}
+}  // namespace
+
+// Grid (rows), kPick threads.
+GH_KERNEL __launch_bounds__(kPick) void gh_sample_pick(GhSampleArgs a) {
+    __shared__ PlanLds s;
+    __shared__ PickLds q;
+    __shared__ double table[64];
+    if (a.fine) sample_pick<true>(a, s, q, table);
+    else sample_pick<false>(a, s, q, table);
 }

@@ -7,6 +7,7 @@ import subprocess
 import numpy as np
 import pytest
 
+import flat_tail
 from graph_horizon_amd import _ffi as F
 from sampled import sample
 
@@ -66,3 +67,12 @@ def test_waves_in_any_order(lib, order, params):
     for vocab, spread in ((3000, 2.0), (3000, 0.0005), (9000, 0.0005)):
         logits = (7 + spread * rng.standard_normal((2, vocab))).astype(np.float32)
         check(lib, logits, [params] * 2, rng.random(2).astype(np.float32), order)
+
+
+@pytest.mark.parametrize("vocab,distance", [(50000, 24.0), ((1 << 17) + 1, 23.5)])
+def test_a_flat_far_tail_keeps_its_mass(lib, vocab, distance):
+    """What many tiny weights sum up to, next to one of 1: the tail's share is 1e-5 or less and drawn from as such."""
+    def by_row(logits, want, us):
+        got = [run(lib, logits[i % len(us)][None], [c[0]], [c[1]], order=1) for i, c in enumerate(want)]
+        return [int(t[0]) for t, _ in got], [float(p[0]) for _, p in got]
+    flat_tail.check(by_row, vocab, distance)
