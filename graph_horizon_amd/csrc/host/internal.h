@@ -196,7 +196,7 @@ struct gh_backend {
     // pinned host word in which the paged kernels leave what they found wrong (GH_PAGED_*), 0: nothing
     volatile uint32_t* paged_fault = nullptr;
     size_t ws_bytes = 0;
-    // the least scratch that a paged operator could not have (0: none so far, or much was freed since), and how
+    // the least scratch that an operator over rows could not have (0: none so far, or much was freed since), and how
     // many calls did with less without asking
     uint64_t ws_short = 0;
     uint32_t ws_did_with_less = 0;
@@ -292,6 +292,25 @@ inline int growing_scratch(gh_backend* b, uint64_t bytes, char** at) {
         b->err.clear();
     }
     return ask(bytes);
+}
+// Scratch of `fixed` bytes and `per` bytes for each of *step rows, or of fewer where there is no memory for all: they take turns then.
+// Where memory was short (ws_short), the scratch that there is holds half or more of what could be had then, and rows take turns in
+// it: a refusal costs two allocations, two frees and a wait, and moves what recorded graphs hold. Every 256th such call asks for all
+// again, as others may have freed memory. Where it holds not one row, as many are tried as were not refused.
+inline int scratch_for_rows(gh_backend* b, uint64_t fixed, uint64_t per, uint32_t* step, char** at) {
+    if (b->ws_short && fixed + per * *step > workspace_room(b)) {
+        auto rows_in = [&](uint64_t bytes) { return bytes > fixed ? (uint32_t)std::min<uint64_t>((bytes - fixed) / per, *step) : 0; };
+        const uint32_t now = rows_in(workspace_room(b)), untried = rows_in(b->ws_short - 1);
+        if (++b->ws_did_with_less % 256 == 0) b->ws_short = 0;
+        else if (now || untried) *step = now ? now : untried;
+    }
+    int rc = GH_OK;
+    while ((rc = growing_scratch(b, fixed + per * *step, at)) == GH_E_OOM && *step > 1) {
+        *step = (*step + 1) / 2;
+        b->err.clear();
+    }
+    if (rc) b->ws_short = 0;
+    return rc;
 }
 // Workgroups of `block` threads and `shmem` bytes of LDS resident on the whole device at once.
 uint32_t resident_wgs(gh_backend* b, GhKernel k, uint32_t block, uint32_t shmem);

@@ -278,24 +278,9 @@ int attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv_pag
     const uint64_t room = std::min<uint64_t>((512ull << 20) / per, (1u << 30) / tiles1);  // tiles count in 32 bits
     uint32_t step = (uint32_t)std::min<uint64_t>(std::min(kv->rows, kPagedRows), std::max<uint64_t>(1, room));
     auto parts = [&] { return split ? (uint64_t)a.chunks * step : (uint64_t)a.chunks + step; };
-    auto need = [&] { return layout + (acc + ml) * parts() + raw * step; };
-    // Where memory was short (ws_short), the scratch that there is holds half or more of what could be had then, and rows take
-    // turns in it: a refusal costs two allocations, two frees and a wait. Every 256th such call asks for all again, as others
-    // may have freed memory. Where it holds not one row, as many are tried as were not refused.
-    if (b->ws_short && need() > workspace_room(b)) {
-        const uint64_t fixed = layout + (split ? 0 : (acc + ml) * a.chunks);
-        auto rows_in = [&](uint64_t bytes) { return bytes > fixed ? (uint32_t)std::min<uint64_t>((bytes - fixed) / per, step) : 0; };
-        const uint32_t now = rows_in(workspace_room(b)), untried = rows_in(b->ws_short - 1);
-        if (++b->ws_did_with_less % 256 == 0) b->ws_short = 0;
-        else if (now || untried) step = now ? now : untried;
-    }
     char* ws = nullptr;
-    int rc = GH_OK;
-    while ((rc = growing_scratch(b, need(), &ws)) == GH_E_OOM && step > 1) {
-        step = (step + 1) / 2;
-        b->err.clear();
-    }
-    if (rc) return b->ws_short = 0, rc;
+    int rc = scratch_for_rows(b, layout + (split ? 0 : (acc + ml) * a.chunks), per, &step, &ws);
+    if (rc) return rc;
     a.layout = split ? 0 : (uint64_t)ws;
     a.part_acc = (uint64_t)ws + layout;
     a.raw = scored ? a.part_acc + acc * parts() : 0;

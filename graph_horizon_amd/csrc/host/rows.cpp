@@ -100,13 +100,8 @@ int gh_sample_rows(gh_backend* b, gh_encoder* enc, const gh_buf* tokens, const g
         }
         uint32_t step = std::min<uint32_t>(rows, kSampleScratch / GH_SAMPLE_ROW_BYTES);
         char* ws = nullptr;
-        int rc = GH_OK;
-        // without memory for all rows they take turns in what there is
-        while ((rc = growing_scratch(b, (uint64_t)step * GH_SAMPLE_ROW_BYTES, &ws)) == GH_E_OOM && step > 1) {
-            step = (step + 1) / 2;
-            b->err.clear();
-        }
-        if (rc) return b->ws_short = 0, rc;
+        int rc = scratch_for_rows(b, 0, GH_SAMPLE_ROW_BYTES, &step, &ws);
+        if (rc) return rc;
         // about four workgroups per CU; a chunk is a whole number of a workgroup's rounds of 2048
         const uint32_t rounds = ceil_div(vocab, 2048);
         a.chunks = std::min({std::max(1u, 4 * b->cus / step), rounds, 64u});

@@ -29,12 +29,13 @@ def lib(tmp_path_factory):
     h.gh_sample_rows.argtypes = F.SIGNATURES["gh_sample_rows"][1]
     h.wave_backend.restype = h.wave_encoder.restype = C.c_void_p
     h.wave_encoder.argtypes = h.wave_error.argtypes = [C.c_void_p]
+    h.wave_limit.argtypes = [C.c_uint64]
     h.wave_error.restype = C.c_char_p
     h.backend = h.wave_backend(256)
     return h
 
 
-def run(lib, logits, params, u, order=0):
+def run(lib, logits, params, u, order=0, backend=None):
     rows, vocab = logits.shape
     logits = np.ascontiguousarray(logits)
     params, u = np.array(params, PARAMS), np.asarray(u, np.float32)
@@ -44,9 +45,10 @@ def run(lib, logits, params, u, order=0):
     tokens, probs = np.full(rows, 77, np.uint32), np.full(rows, 77, np.float32)
     bufs = [F.GhBuf(x.ctypes.data, x.nbytes) for x in (tokens, probs, logits, room[off:off + 4 * rows], u)]
     lib.wave_order(order)
-    rc = lib.gh_sample_rows(lib.backend, lib.wave_encoder(lib.backend), C.byref(bufs[0]), C.byref(bufs[1]), C.byref(bufs[2]), rows, vocab,
+    backend = backend or lib.backend
+    rc = lib.gh_sample_rows(backend, lib.wave_encoder(backend), C.byref(bufs[0]), C.byref(bufs[1]), C.byref(bufs[2]), rows, vocab,
                             vocab, C.byref(bufs[3]), C.byref(bufs[4]))
-    assert rc == 0, lib.wave_error(lib.backend)
+    assert rc == 0, lib.wave_error(backend)
     return tokens, probs
 
 
@@ -76,3 +78,22 @@ def test_a_flat_far_tail_keeps_its_mass(lib, vocab, distance):
         got = [run(lib, logits[i % len(us)][None], [c[0]], [c[1]], order=1) for i, c in enumerate(want)]
         return [int(t[0]) for t, _ in got], [float(p[0]) for _, p in got]
     flat_tail.check(by_row, vocab, distance)
+
+
+def test_short_of_memory_it_is_not_asked_for_at_every_call(lib):
+    """Scratch for three rows of ten, and no more to be had: later calls take turns in it at once."""
+    rng = np.random.default_rng(6)
+    logits, params, u = rng.standard_normal((10, 50)).astype(np.float32), [(1.0, 0.9, 0, 0.0)] * 10, rng.random(10).astype(np.float32)
+    want = run(lib, logits, params, u)
+    backend = lib.wave_backend(256)
+    lib.wave_limit(3 * 79000)
+    asked = []
+    for _ in range(4):
+        got = run(lib, logits, params, u, backend=backend)
+        assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+        asked.append(lib.wave_limit(3 * 79000))
+    assert asked[0] > 1 and asked[1:] == [0, 0, 0], asked
+    lib.wave_limit(0)  # memory is there again: asked for in the 256th call that did with less at the latest
+    for _ in range(260):
+        run(lib, logits, params, u, order=0xFFFFFFFF, backend=backend)
+    assert lib.wave_limit(0) >= 1
