@@ -53,7 +53,9 @@ __device__ __forceinline__ float quad_max(float v) {
 }
 
 // The lane's 8 of 32 values as codes; returns them, step and minimum in *dm. The step is cut off to FP16, so that
-// m + 15 d stays in the values' range. (x - m) / d is a true quotient (a product with 1 / d, corrected by what it leaves):
+// m + 15 d stays in the values' range where m is the minimum itself. Keys that were turned or normed have one between FP16 numbers,
+// and m may lie above it by half an FP16 step: where m + 15 d would reach 65520, which FP16 rounds to infinity, the step is
+// a fifteenth of what is left above m. (x - m) / d is a true quotient (a product with 1 / d, corrected by what it leaves):
 // FP16 values lie on ties that the product alone would miss. Values that FP16 does not hold as finite make the group NaN.
 __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], uint32_t* dm) {
     float lo = x[0], hi = x[0], odd = 0.0f;
@@ -67,7 +69,9 @@ __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], uint32_t* dm) 
     hi = quad_max(hi);
     odd = gh_quad_sum(odd);
     const uint32_t m16 = gh_f2h(lo);
-    const uint32_t d16 = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz((hi - lo) / 15.0f, 0.0f)) & 0xFFFFu;
+    uint32_t d16 = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz((hi - lo) / 15.0f, 0.0f)) & 0xFFFFu;
+    if (__builtin_fmaf(15.0f, gh_h2f(d16), gh_h2f(m16)) >= 65520.0f)
+        d16 = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz((hi - gh_h2f(m16)) / 15.0f, 0.0f)) & 0xFFFFu;
     if (odd != 0.0f || fmaxf(-lo, hi) >= 65520.0f) {  // (odd: a NaN)
         *dm = 0x7E007E00u;
         return 0u;

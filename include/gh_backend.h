@@ -79,7 +79,8 @@ typedef struct gh_yarn {
 enum gh_rope_role { GH_ROPE_QUERY = 0, GH_ROPE_KEY = 1 }; /* backend/rope.rs:23-27 */
 /* F16 and INT8: kv_cache/scheme.rs. Q4 has no counterpart in the reference: a vector of 128 values takes 80 bytes, 64 of
  * codes (dims 2 i and 2 i + 1 in the low and high half of byte i), then for each 32 dims a step d and a minimum m in FP16. Code c
- * stands for m + d c. Of 32 values, m is the least in FP16, d a fifteenth of their range cut off to FP16, and the
+ * stands for m + d c. Of 32 values, m is the least in FP16, d a fifteenth of their range cut off to FP16 (where m + 15 d would then
+ * reach 65520, FP16's infinity, a fifteenth of the largest less m), and the
  * code (x - m) / d as the nearest whole number, ties to even, 0 to 15 (0 where d is 0); 32 values of which FP16 holds
  * not all as finite stand for NaN. */
 enum gh_kv_scheme { GH_KV_F16 = 0, GH_KV_INT8 = 1, GH_KV_Q4 = 2 };

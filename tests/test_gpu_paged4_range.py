@@ -2,9 +2,10 @@
 import numpy as np
 import pytest
 
+from graph_horizon_amd import Yarn
 from paged import D, attend
 from paged4 import Paged4, pack, parts, values
-from test_gpu_paged4 import run_attention
+from test_gpu_paged4 import run_attention, turned
 
 pytestmark = pytest.mark.gpu
 
@@ -55,4 +56,43 @@ def test_attention_of_small_and_large_queries(hip, rng, q_size, k_size, lengths,
                 bound = wb.sum(0) + (group + 1) * 2.0 ** -24 * np.abs(total)
                 err = np.abs(after[0, r, h, :n] - total)
                 assert np.all(err <= bound), (r, h, float((err / bound).max()))
+    p.free()
+
+
+def test_keys_next_to_the_end_of_fp16_stay_finite(hip, rng):
+    """Rotated keys up to 65520, which FP16 rounds to 65504: the minimum of 32 may be rounded up, and no code may stand for more than
+    the largest. A step: the values' range over 15, or, where that would reach 65520, what is left above the minimum."""
+    tokens, heads = 3000, 4
+    yarn = Yarn(128, 16384, 1e6, 16.0, 32.0, 1.0, 1.0, 0.1)
+    p = Paged4(hip, rng, [tokens], 64, heads)
+    k = rng.uniform(60000, 65504, (1, tokens, heads, D)).astype(np.float16)
+    k[..., :64] = rng.standard_normal((1, tokens, heads, 64))  # pairs that turn further
+    kb, pb, qb = hip.from_host(k), hip.from_host(np.zeros(1, np.uint32)), hip.from_host(np.zeros((1, tokens, 1, D), np.float16))
+    out = [hip.alloc_buffer(k.nbytes) for _ in range(2)]
+    hip.rope_kv_write_paged(p.handle(), qb, qb, kb, kb, 1, pb, tokens, tokens, yarn, 0)
+    hip.kv_read_paged(out[0], out[1], p.handle(), tokens, 0)
+    back = hip.download(out[0], np.float16, k.size).reshape(k.shape)[0]
+    b = p.read("k")[0, p.cells(0, tokens)]
+    want, bound = turned(k[0].astype(np.float64), yarn, np.arange(tokens), False)
+    c, d, m = parts(b)
+    g, e = want.reshape(c.shape), bound.reshape(c.shape).max(-1)
+    low, high = g.min(-1), g.max(-1)
+    fits, past = high + e < 65520, high - e >= 65520  # (between: either)
+    assert np.isnan(m[past]).all() and np.isfinite(m[fits]).all()
+    most = m[fits] + 15 * d[fits]
+    assert np.all(most < 65520)
+    assert np.all(most <= high[fits] + e[fits] + 2.0 ** -11 * np.abs(low[fits]))
+    # m by its rounding, d at least the cut-off fifteenth of what is left
+    assert np.all(np.abs(m - low)[fits] <= (e + 2.0 ** -11 * np.abs(low))[fits])
+    left = np.minimum(high - low, high - m)[fits] - 2 * e[fits]
+    assert np.all(d[fits] >= left / 15 * (1 - 2.0 ** -10) - 2.0 ** -23)
+    err = np.abs(m[..., None] + d[..., None] * c - g).max(-1)
+    assert np.all(err[fits] <= (d / 2 + e + 2.0 ** -11 * np.abs(low))[fits] + 2.0 ** -20)
+    assert np.isfinite(back.reshape(c.shape)[fits]).all()
+    # cases of each kind are there: the plain step would have reached 65520, and would not
+    plain = np.floor((high - low) / 15 * 4) / 4  # steps of 256 to 511 are multiples of a quarter
+    over = (low.astype(np.float16).astype(np.float64) + 15 * plain > 65520 + 1) & fits & (plain >= 256)
+    assert over.sum() >= 20 and (fits & ~over).sum() >= 1000, (over.sum(), fits.sum())
+    for x in (kb, pb, qb, *out):
+        hip.free_buffer(x)
     p.free()
