@@ -279,14 +279,15 @@ int gh_kv_evict_paged(gh_backend* b, gh_encoder* enc, const gh_kv_paged* dst, co
                       const gh_buf* kept, uint32_t budget, uint32_t recent);
 
 /* ---- sampling of a batch (no counterpart in the reference, which samples one row on the host) ---- */
-typedef struct gh_sample_params { /* one row's; the fields of gh_sampling */
+typedef struct gh_sample_params { /* one row's; of the fields of gh_sampling all but repeat_penalty and seed */
     float temperature; /* <= 0 or NaN: greedy argmax */
     float top_p;       /* 1: off */
     uint32_t top_k;    /* 0: off */
     float min_p;       /* 0: off */
 } gh_sample_params;
 /* The next token of each row of logits, FP32 [rows][stride] of which the first vocab count, with settings and a
- * uniform random number in [0, 1) per row, all on the device (params on 16 bytes): the token that gh_sample draws, with
+ * uniform random number in [0, 1) per row, all on the device (params on 16 bytes): the token that gh_sample draws at a
+ * repeat_penalty of 1 (a caller with another one applies it to the row's logits first, or samples that row on the host), with
  * weights, sums and comparisons in 64 bits where gh_sample has FP32 (a sum of weights is off by at most 2^-29 of the largest one up to
  * 131072 tokens, and vocab·2^-54 of it beyond). Tokens with a finite logit, ranked by (logit descending
  * by f32 total order, index ascending), have weights exp((logit - largest) / temperature). Kept are the first top_k; of these
