@@ -261,6 +261,9 @@ int entry(gh_backend* b, gh_encoder* enc, F body) {
     return latch(enc, rc);
 }
 
+// The eps of a norm as the kernels' reciprocal root takes it, which reads numbers below FP32's least normal one as 0: no FP16 head
+// that is not all zeros has a mean square near that, and one of zeros stays 0.
+inline float norm_eps(float eps) { return eps > 0.0f ? std::max(eps, 0x1p-126f) : eps; }
 int check_attention(gh_backend* b, const gh_buf* out, const gh_buf* q, const gh_kv* kv,
                     uint32_t q_heads, uint32_t last_pos, uint32_t rows, uint32_t layer);
 // Resolves this device's address of the no-allocation scratch array (at gh_create).

@@ -394,7 +394,7 @@ int gh_norm_rope_kv_write_paged(gh_backend* b, gh_encoder* enc, const gh_kv_page
         if (rc) return rc;
         a.q_norm = q_norm->addr;
         a.k_norm = k_norm->addr;
-        a.eps = eps;
+        a.eps = norm_eps(eps);
         return rope_write(b, kv, q_out, q, k, v, q_heads, positions, tokens, max_pos, yarn, layer, a, what);
     });
 }

@@ -61,7 +61,7 @@ int gh_norm_rope_batched(gh_backend* b, gh_encoder* enc, const gh_buf* q, const 
         a.pairs = yarn->rope_dim / 2;
         a.base = base;
         a.rows = rows;
-        a.eps = eps;
+        a.eps = norm_eps(eps);
         return launch(b, K_NORM_ROPE, rows * a.groups, 1, 1, 256, &a);
     });
 }

@@ -96,3 +96,29 @@ def test_keys_next_to_the_end_of_fp16_stay_finite(hip, rng):
     for x in (kb, pb, qb, *out):
         hip.free_buffer(x)
     p.free()
+
+
+@pytest.mark.parametrize("eps", [1e-45, 1e-40, 1.2e-38, 1e-20])
+def test_a_head_of_zeros_stays_zero_with_any_eps(hip, rng, eps):
+    """0 over the root of eps is 0, with an eps below FP32's least normal number too; other heads are as with none."""
+    q = rng.standard_normal((1, 2, D)).astype(np.float16)
+    q[0, 0] = 0
+    wb = hip.from_host(np.ones(D, np.float16))
+    qb, kb, pb, zb = hip.from_host(q), hip.from_host(q), hip.from_host(np.zeros(1, np.uint32)), hip.from_host(q)
+    yarn = Yarn(128, 16384, 1e6, 16.0, 32.0, 1.0, 1.0, 0.1)
+    hip.norm_rope_batched(zb, kb, 2, 2, D, 0, 1, wb, wb, 0.0, yarn)
+    plain = hip.download(zb, np.float16, q.size).reshape(q.shape)
+    hip.upload(kb, q)
+    hip.norm_rope_batched(qb, kb, 2, 2, D, 0, 1, wb, wb, eps, yarn)
+    for b in (qb, kb):
+        got = hip.download(b, np.float16, q.size).reshape(q.shape)
+        assert not got[0, 0].view(np.uint16).any() and np.array_equal(got[0, 1], plain[0, 1])
+    p = Paged4(hip, rng, [1], 16, 2)
+    hip.upload(qb, q)
+    hip.upload(kb, q)
+    hip.norm_rope_kv_write_paged(p.handle(), qb, qb, kb, kb, 2, wb, wb, eps, pb, 1, 0, yarn, 0)
+    assert not hip.download(qb, np.uint16, D).any()
+    assert not p.read("k")[0, p.cells(0, 1)[0], 0].any()
+    for b in (wb, qb, kb, pb, zb):
+        hip.free_buffer(b)
+    p.free()
