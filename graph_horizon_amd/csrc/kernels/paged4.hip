@@ -40,8 +40,8 @@ __device__ __forceinline__ uint32_t highs(uint32_t x0, uint32_t x1) { return __b
 // As gh_paged_write: thread = 8 values of one head of one token, query heads first; a head is 16 lanes, a DPP row, and
 // 32 dims are a quad of them. With norms, queries and keys are divided by the root of their mean square over the head
 // and multiplied by the weight, in FP32, before the rotation, and rounded once at the end. All loads but the table's are asked for
-// at once: with few tokens a launch is a chain of their latencies. 32 query and 8 kv heads with norms, 1 / 256 rows: 2.9 / 4.6 us (6 MB);
-// a prompt of 2000, 11 MB: 6.0.
+// at once: with few tokens a launch is a chain of their latencies. 32 query and 8 kv heads with norms, 1 / 256 rows: 3.1 / 4.4 us (6 MB), with
+// the rotation alone 3.0 / 4.2, with norms into FP16 pools 2.9 / 4.2; a prompt of 2000, 11 MB, without either: 5.6.
 namespace {
 __device__ __forceinline__ float quad_min(float v) {
     v = fminf(v, GH_DPP(v, 0xB1, 0xF));
@@ -153,7 +153,7 @@ GH_KERNEL __launch_bounds__(256) void gh_paged_norm_write(GhPagedWriteArgs a) {
 
 // ---- read-back ---------------------------------------------------------------------------------
 // Thread = 8 values of one head of one position, key heads first: 8 bytes in (the step and minimum are read by four), 16 out.
-// 8 heads, 1 / 256 rows of one position 1.7 / 2.8 us, 2000 positions (11 MB) 4.5.
+// 8 heads, 1 / 256 rows of one position 1.8 / 2.8 us, 2000 positions (11 MB) 4.4; of FP16 pools 1.7 / 2.7 and, 16 MB, 4.8.
 namespace {
 template <bool Q4>
 __device__ __forceinline__ void paged_read(const GhPagedReadArgs& a) {

@@ -10,15 +10,17 @@
 // The second word costs 0.8 us of 22.2 for 1 row of 131072 and 4 of 47.4 for 64, so smaller ones do without.
 //
 // Four launches; a row's logits are read three times, from memory once (us of 1 / 8 / 64 rows of 131072):
-//   gh_sample_max     the largest logit of each chunk of a row (3.8 / 4.2 / 10.2; 34 MB of 64 rows);
+//   gh_sample_max     the largest logit of each chunk of a row (3.8 / 4.3 / 10.3: 34 MB of 64 rows at half the rate of a
+//                     long read, for a workgroup has one round of loads and ends);
 //   gh_sample_bins    counts and sums over 1024 bins of the distance d = M - l, 64 per octave from 2^-9 to 2^7, so
-//                     that a bin holds at most 3 % of any smooth distribution whatever its spread (5.6 / 6.9 / 13.9: three
+//                     that a bin holds at most 3 % of any smooth distribution whatever its spread (5.6 / 6.9 / 13.7: three
 //                     LDS operations a token, two of them atomic; a cheaper exponential, or fewer and larger workgroups, change nothing);
 //   gh_sample_collect the tokens of the bins in which a search can end: the running sums up to the bins are known, and
-//                     bound the top-k sum, then the kept sum, then the draw's target (7.5 / 8.5 / 11.6);
+//                     bound the top-k sum, then the kept sum, then the draw's target (7.5 / 8.5 / 11.9);
 //   gh_sample_pick    searches these tokens, or, where they are more than the list takes, the row itself: one wave where they
-//                     are 64 or fewer, else a workgroup of 16 waves, half of which look at the bins (4.8 / 12.8 / 10.9; all of
-//                     them 5.6 / 14.0 / 12.3, 8 waves in all 4.7 / 14.9 / 12.6; from memory without gh_sample_collect, 1 row: 23.3).
+//                     are 64 or fewer, else a workgroup of 16 waves, half of which look at the bins (4.8 / 12.8 / 11.7; all of
+//                     them, before Mass, 5.6 / 14.0 / 12.3, 8 waves in all 4.7 / 14.9 / 12.6). The row itself is read four times or more by
+//                     one workgroup: 131072 tokens within one bin 302 / 309 / 315.
 // Chains of dependent loads and barriers bound the launches of few rows.
 // What the device cannot trust is only the settings: any bits give a token of the row.
 #include <type_traits>

@@ -288,8 +288,8 @@ typedef struct gh_sample_params { /* one row's; of the fields of gh_sampling all
 /* The next token of each row of logits, FP32 [rows][stride] of which the first vocab count, with settings and a
  * uniform random number in [0, 1) per row, all on the device (params on 16 bytes): the token that gh_sample draws at a
  * repeat_penalty of 1 (a caller with another one applies it to the row's logits first, or samples that row on the host), with
- * weights, sums and comparisons in 64 bits where gh_sample has FP32 (a sum of weights is off by at most 2^-29 of the largest one up to
- * 131072 tokens, and vocab·2^-54 of it beyond). Tokens with a finite logit, ranked by (logit descending
+ * weights, sums and comparisons in 64 bits where gh_sample has FP32 (besides its exponentials' last bits a sum of weights is off by
+ * at most 2^-29 of the largest one up to 131072 tokens, and vocab·2^-54 of it beyond). Tokens with a finite logit, ranked by (logit descending
  * by f32 total order, index ascending), have weights exp((logit - largest) / temperature). Kept are the first top_k; of these
  * the fewest whose sum reaches top_p of theirs; of these the ones of at least min_p of the largest (always one). The draw
  * is the first at which the running sum passes uniform (below 0 or NaN: 0; from 1 on: the last number below it) times
