@@ -7,7 +7,7 @@
 // running counts and sums. Sums are of whole numbers, w in fixed point: the same in any order. One word must leave room for
 // `vocab` weights of 1: at a vocabulary of 2^17 a weight is off by 2^-46 at most, and a sum by 2^-29 of the largest weight. Larger
 // vocabularies, where that grows with their square, take two words (Mass<true>): a sum is off by vocab 2^-54 at most, as in FP64.
-// The second word costs 0.8 us of 22.2 for 1 row of 131072 and 4 of 47.4 for 64, so smaller ones do without.
+// The second word costs 1 us of 22 for 1 row of 131072 and 5 of 47 for 64, so smaller ones do without.
 //
 // Four launches; a row's logits are read three times, from memory once (us of 1 / 8 / 64 rows of 131072):
 //   gh_sample_max     the largest logit of each chunk of a row (3.8 / 4.3 / 10.3: 34 MB of 64 rows at half the rate of a
@@ -18,7 +18,7 @@
 //   gh_sample_collect the tokens of the bins in which a search can end: the running sums up to the bins are known, and
 //                     bound the top-k sum, then the kept sum, then the draw's target (7.5 / 8.5 / 11.9);
 //   gh_sample_pick    searches these tokens, or, where they are more than the list takes, the row itself: one wave where they
-//                     are 64 or fewer, else a workgroup of 16 waves, half of which look at the bins (4.8 / 12.8 / 11.7; all of
+//                     are 64 or fewer, else a workgroup of 16 waves, half of which look at the bins (4.8 / 12.6 / 11.2; all of
 //                     them, before Mass, 5.6 / 14.0 / 12.3, 8 waves in all 4.7 / 14.9 / 12.6). The row itself is read four times or more by
 //                     one workgroup: 131072 tokens within one bin 302 / 309 / 315.
 // Chains of dependent loads and barriers bound the launches of few rows.
@@ -145,6 +145,7 @@ __device__ __forceinline__ Mass<FINE> fixed(const GhSampleArgs& a, const Row& r,
 // The kernels have both forms, the one for two words behind the other, and an empty asm at its start keeps the compiler from drawing
 // the first instructions of both together ahead of the branch (gh_sample_pick of 8 / 64 rows otherwise 13.0 / 11.7 us instead of
 // 12.6 / 11.2: what is asked for there at once was waited for in turn).
+
 // Masses of the bins, or of parts of one: 64 bits each for `rest`, or the first half of them 32.
 template <bool FINE>
 __device__ __forceinline__ Mass<FINE> mass_at(const uint64_t* whole, const uint64_t* rest, uint32_t i) {
